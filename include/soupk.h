@@ -25,13 +25,16 @@
 extern "C" {
 #endif
 
-/* ABI version of this header; soupk_abi_version() returns the library's.  5 adds soupk_gemm_nn,
+/* ABI version of this header; soupk_abi_version() returns the library's.  6 adds
+   soupk_token_logprobs_fwd, soupk_token_logprobs_bwd, soupk_token_logprobs_workspace,
+   soupk_qk_norm_rope_fwd, soupk_qk_norm_rope_bwd, soupk_dropout, soupk_embedding_fwd,
+   soupk_embedding_bwd and soupk_embedding_bwd_workspace to version 5's; 5 added soupk_gemm_nn,
    soupk_gemm_nn_workspace, soupk_head_plan, soupk_head_stats_grad_planned, soupk_head_finish,
    soupk_head_dh and soupk_attention_wide to version 4's entry points, which had added
    soupk_lora_rope_fwd, soupk_gemm_nn_nf4, soupk_gemm_tn_nf4_split, soupk_gemm_nn_nf4_split,
    soupk_gemm_lt, soupk_gemm_lt_index, soupk_layer_fwd, soupk_layer_bwd (with the layer's
    products on NF4 weights: SoupkLayerNf4) and soupk_init_device to version 3's. */
-#define SOUPK_ABI_VERSION 5
+#define SOUPK_ABI_VERSION 6
 
 /* Status of soupk_lora_bwd_params_noalloc for a problem beyond its static scratch (no launch). */
 #define SOUPK_STATUS_SCRATCH_LIMIT 20001
@@ -170,9 +173,11 @@ int soupk_rmsnorm_bwd(const float* s, const float* rstd, const float* w, const u
                       const float* dypad, const int64_t* pad_idx, const float* ds, float* dx,
                       uint16_t* ddelta, int64_t rows, int64_t pad_rows, int32_t H, void* stream);
 
-/* LoRA-delta element types for soupk_rope_pack_fwd. */
+/* Element types: LoRA deltas of soupk_rope_pack_fwd (F16, F32), tensors of the entry points that
+   take several types. */
 #define SOUPK_DTYPE_F16 0
 #define SOUPK_DTYPE_F32 1
+#define SOUPK_DTYPE_BF16 2
 
 /*
  * LoRA add + RoPE + QKV pack forward (replaces rope_pack_fwd_kernel, solution/rope.py:24-75,
@@ -701,6 +706,103 @@ int soupk_gemm_nn(const uint16_t* a, int64_t lda, const uint16_t* b, int64_t ldb
                   int64_t ldo, int64_t M, int32_t N, int32_t K, const int32_t* rows,
                   float* workspace, int64_t workspace_floats, void* stream);
 int soupk_gemm_nn_workspace(int64_t M, int32_t N, int32_t K, int64_t* floats);
+
+/*
+ * Log probabilities of given tokens, the entropy of each row and its top_k alternatives (widening
+ * beyond the reference's kernel set, next to soupk_head_stats_grad; the reference takes the loss and
+ * the entropy only, solution/head.py:34-76).  logits: `rows` rows of V elements (dtype F16, BF16 or
+ * F32), row r at (r / inner) * stride_outer + (r % inner) * stride_inner elements.  Over
+ * d = (z - max z) / temperature, S = sum exp(d):
+ *   logprob = d[token] - ln S (0 for token -100; NaN for any other token outside [0, V))
+ *   entropy = ln S - sum(exp(d) d) / S;  row_max = max z, row_sum = S (kept for the backward)
+ *   top_id[r, k], top_lp[r, k] = d[top_id] - ln S: the top_k (0 .. 32, <= V) largest logits in
+ *   decreasing order, equal ones by the lower column; a NaN ranks with -inf
+ * NaN or +inf in a row, or a row of -inf alone, makes its numbers NaN.  top_lp and top_id are
+ * unused for top_k 0.  workspace: soupk_token_logprobs_workspace bytes, 16-byte aligned.
+ */
+int soupk_token_logprobs_workspace(int64_t rows, int64_t V, int32_t top_k, int32_t dtype,
+                                   int64_t* bytes);
+int soupk_token_logprobs_fwd(const void* logits, int32_t dtype, const int64_t* tokens, int64_t rows,
+                             int64_t inner, int64_t stride_outer, int64_t stride_inner, int64_t V,
+                             float temperature, int32_t top_k, float* logprob, float* entropy,
+                             float* row_max, float* row_sum, float* top_lp, int64_t* top_id,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Its backward: dlogits [rows, V] (contiguous, dtype as the logits) =
+ *   (g_lp (onehot(token) - p) + sum_k g_top[k] (onehot(top_id[k]) - p)
+ *    - g_ent p (ln p + entropy)) / temperature
+ * with g_lp, g_ent [rows] and g_top [rows, top_k] fp32, each nullable (zero).  g_lp counts only for
+ * a token in [0, V).  A row whose gradients are all zero gets zeros.
+ */
+int soupk_token_logprobs_bwd(const void* logits, int32_t dtype, const int64_t* tokens, int64_t rows,
+                             int64_t inner, int64_t stride_outer, int64_t stride_inner, int64_t V,
+                             float temperature, int32_t top_k, const float* row_max,
+                             const float* row_sum, const float* entropy, const int64_t* top_id,
+                             const float* g_lp, const float* g_ent, const float* g_top,
+                             void* dlogits, void* stream);
+
+/*
+ * RMS norm of every query and key head, then the rotation, into the token-major rows of
+ * soupk_attention_varlen_fwd (widening: soupk_rope_pack_tokens for models that normalise queries
+ * and keys).  qkv, out: [rows, (NH + 2*NKV) * D] of dtype F16 or BF16; D a multiple of 16, <= 256.
+ *   x = qkv (+ lora_q [rows, NH*D] for queries), n = x / sqrt(mean(x^2) + eps), y = n * w
+ *   q, k = (y1*c1 - y2*s1, y2*c2 + y1*s2);  v = qkv (+ lora_v [rows, NKV*D])
+ * wq, wk: fp32 [D]; cos, sin, pos, B, T as soupk_rope_pack_tokens; lora_dtype F32 or dtype.  A
+ * token whose pos lies outside [0, B*T) gets a row of zeros.
+ */
+int soupk_qk_norm_rope_fwd(const void* qkv, const void* lora_q, const void* lora_v,
+                           int32_t lora_dtype, const float* wq, const float* wk, const float* cos,
+                           const float* sin, const int64_t* pos, void* out, int32_t dtype,
+                           int64_t rows, int32_t B, int32_t T, int32_t NH, int32_t NKV, int32_t D,
+                           float eps, void* stream);
+
+/*
+ * Its backward: dqkv [rows, (NH + 2*NKV) * D] (its q and v columns are also the gradients of lora_q
+ * and lora_v) and, where not NULL, dwq, dwk [D] fp32, summed in a fixed order.  A token whose pos
+ * lies outside [0, B*T) gets zeros and adds nothing to dwq, dwk.  workspace (only for dwq, dwk):
+ * SOUPK_QK_NORM_BLOCKS * 2 * D floats suffice.
+ */
+#define SOUPK_QK_NORM_BLOCKS 1024
+int soupk_qk_norm_rope_bwd(const void* dout, const void* qkv, const void* lora_q,
+                           int32_t lora_dtype, const float* wq, const float* wk, const float* cos,
+                           const float* sin, const int64_t* pos, void* dqkv, float* dwq, float* dwk,
+                           float* workspace, int64_t workspace_floats, int32_t dtype, int64_t rows,
+                           int32_t B, int32_t T, int32_t NH, int32_t NKV, int32_t D, float eps,
+                           void* stream);
+
+/*
+ * Dropout drawn from a counter (widening: the reference calls peft's dropout modules,
+ * solution/model.py:195-206).  x, out [R, C]; residual [R, C] of out's type, nullable:
+ *   out = residual + (word >= limit ? x * scale : 0)
+ * word: element c % 4 of Philox4x32-10 at counter (c / 4, row, call low, call high), row =
+ * rows[r] (int64, its low 32 bits) or r, key (seed low, seed high); seed_dev, where not NULL, holds
+ * the seed in device memory instead.  0 <= limit <= 2^32 (2^32 drops everything).  The types are
+ * equal, or one of them is F32.  The backward is the same call on the gradient without a residual.
+ */
+int soupk_dropout(const void* x, int32_t x_dtype, const void* residual, void* out,
+                  int32_t out_dtype, const int64_t* rows, const int64_t* seed_dev, int64_t seed,
+                  int64_t call, int64_t limit, float scale, int64_t R, int64_t C, void* stream);
+
+/*
+ * Embedding lookup (the torch embedding and fp32 cast at the start of the reference's
+ * fused_forward, solution/model.py:209-279, in one launch): out[i] = table[ids[i]] * scale, table [V, H] of dtype, out [M, H] of out_dtype (dtype or F32).  An id
+ * outside [0, V) gives zeros.
+ */
+int soupk_embedding_fwd(const void* table, int32_t dtype, const int64_t* ids, void* out,
+                        int32_t out_dtype, float scale, int64_t M, int64_t V, int64_t H,
+                        void* stream);
+
+/*
+ * Its backward: dtable [V, H] of dtype, written whole: scale times the sum of dout's rows (grad_dtype
+ * dtype or F32) over each id's tokens in their order, fp32 sums rounded once; zeros for every
+ * other row and for padding_idx (-1: none).  Ids outside [0, V) are skipped.  workspace:
+ * soupk_embedding_bwd_workspace(M, H) bytes, 16-byte aligned.
+ */
+int soupk_embedding_bwd_workspace(int64_t M, int64_t H, int64_t* bytes);
+int soupk_embedding_bwd(const void* dout, int32_t grad_dtype, const int64_t* ids, void* dtable,
+                        int32_t dtype, float scale, int64_t padding_idx, void* workspace,
+                        int64_t workspace_bytes, int64_t M, int64_t V, int64_t H, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,170 @@
+"""dropout.dropout against the generator in Python integers: the mask exactly, the values within one
+rounding.  The scale is exact to fp32's half step (2^-24), the product and the sum with the residual each
+round once in fp32 and the result once in its type: eps / 2 |out| + 4 * 2^-24 (|x| scale + |residual|)."""
+
+import pytest
+import torch
+
+from oracle.dropout import keep_mask
+from testt_amd import dropout, workloads
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+U = 2.0 ** -24
+H, B, F = torch.float16, torch.bfloat16, torch.float32
+
+CASES = [  # shape, x type, residual type, p, seed, call
+    ((37, 64), H, None, 0.1, 0, 0),
+    ((5, 1536), H, None, 0.05, (1 << 64) - 1, 7),
+    ((3, 7, 20), B, B, 0.5, 1 << 40, (1 << 64) - 1),
+    ((9, 13), F, F, 0.3, 12345, 1 << 33),
+    ((9, 13), H, F, 0.3, 12345, 1 << 33),
+    ((4, 1001), B, F, 0.9, 77, 3),
+    ((2, 3), H, H, 0.25, 8, 1),
+    ((50,), H, None, 0.4, 9, 2),
+    ((7, 1), F, None, 0.5, 10, 2),
+    ((6, 40), H, None, 0.0, 11, 0),
+    ((6, 40), H, H, 1.0, 11, 0),
+    ((0, 8), H, None, 0.5, 1, 0),
+    ((4, 0), H, None, 0.5, 1, 0),
+]
+
+
+def expected(x, residual, keep, p):
+    limit = round(p * 2 ** 32)
+    scale = 2 ** 32 / (2 ** 32 - limit) if limit < 2 ** 32 else 0.0
+    y = torch.where(keep, x.double() * scale, 0)
+    return y if residual is None else y + residual.double()
+
+
+def within(got, want, size, dtype):
+    half = torch.finfo(dtype).eps / 2
+    tol = half * want.abs() + 4 * U * size + torch.finfo(dtype).smallest_normal * half * 2
+    assert got.dtype == dtype and got.shape == want.shape
+    assert ((got.double().cpu() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("shape,dtype,res,p,seed,call", CASES)
+def test_values_and_gradient(shape, dtype, res, p, seed, call):
+    print(f"dropout {shape} {dtype} residual {res} p {p}", flush=True)
+    g = torch.Generator().manual_seed(len(shape) + shape[0])
+    x = torch.randn(*shape, generator=g).to(dtype)
+    x[x == 0] = 1
+    r = None if res is None else torch.randn(*shape, generator=g).to(res)
+    leaf = x.to(DEV).requires_grad_(True)
+    rl = None if r is None else r.to(DEV).requires_grad_(True)
+    out = dropout.dropout(leaf, p, seed, call, residual=rl)
+    up = torch.randn(*shape, generator=g).to(out.dtype)
+    out.backward(up.to(DEV))
+    if x.numel() == 0:
+        assert out.shape == x.shape and leaf.grad.shape == x.shape
+        return
+    rows = x.numel() // shape[-1]
+    keep = torch.from_numpy(keep_mask(range(rows), shape[-1], p, seed, call)).view(shape)
+    if r is None:
+        assert torch.equal(out.detach().cpu() != 0, keep)
+    size = expected(x.abs(), None, keep, p) + (0 if r is None else r.double().abs())
+    within(out.detach(), expected(x, r, keep, p), size, res or dtype)
+    within(leaf.grad, expected(up, None, keep, p), expected(up.abs(), None, keep, p), dtype)
+    if rl is not None:
+        assert torch.equal(rl.grad.cpu(), up)
+
+
+def test_rows_draw_at_their_positions():
+    """Real tokens alone draw what the padded batch draws; the number of columns changes no draw."""
+    pos = workloads.ragged_positions((5, 9, 2), 12).to(DEV)
+    x = torch.randn(3, 12, 200, device=DEV)
+    padded = dropout.dropout(x, 0.3, 5, 2).view(36, 200)
+    real = dropout.dropout(x.view(36, 200)[pos].contiguous(), 0.3, 5, 2, rows=pos)
+    assert torch.equal(padded[pos], real)
+    narrow = dropout.dropout(x.view(36, 200)[:, :101].contiguous(), 0.3, 5, 2)
+    assert torch.equal(narrow, padded[:, :101])
+    big = torch.tensor([(1 << 32) - 1], device=DEV)
+    out = dropout.dropout(torch.ones(1, 64, device=DEV), 0.5, 5, 2, rows=big)
+    keep = torch.from_numpy(keep_mask([(1 << 32) - 1], 64, 0.5, 5, 2))
+    assert torch.equal(out.cpu() != 0, keep)
+
+
+def test_dropped_values_leave_nothing():
+    x = torch.full((4, 64), float("nan"), device=DEV, dtype=H)
+    x[1] = float("inf")
+    out = dropout.dropout(x, 0.5, 3)
+    keep = torch.from_numpy(keep_mask(range(4), 64, 0.5, 3, 0)).to(DEV)
+    assert out[~keep].eq(0).all() and not torch.isfinite(out[keep]).any()
+    res = torch.randn(4, 64, device=DEV, dtype=H)
+    assert torch.equal(dropout.dropout(x, 1.0, 3, residual=res), res)
+
+
+def test_strided_and_misaligned_inputs():
+    x = torch.randn(40, 130, device=DEV, dtype=H)
+    for view in (x.t(), x[:, 1:], x[::2, :65]):
+        assert torch.equal(dropout.dropout(view, 0.2, 4),
+                           dropout.dropout(view.contiguous(), 0.2, 4))
+    flat = torch.randn(1 + 30 * 24, device=DEV, dtype=H)
+    odd = flat[1:].view(30, 24)                  # contiguous, 2 bytes off alignment
+    assert torch.equal(dropout.dropout(odd, 0.2, 4), dropout.dropout(odd.clone(), 0.2, 4))
+    y = torch.randn(8, 16, device=DEV, requires_grad=True)
+    dropout.dropout(y, 0.2, 4).sum().backward()  # an expanded gradient
+    assert torch.equal(y.grad, dropout.dropout(torch.ones_like(y), 0.2, 4).detach())
+
+
+def test_seed_on_the_device_under_a_graph():
+    """A captured forward and backward reads the seed on each replay."""
+    x = torch.randn(300, 512, device=DEV, dtype=H)
+    seed = torch.tensor([11], dtype=torch.int64, device=DEV)
+
+    def step():
+        leaf = x.detach().requires_grad_(True)
+        y = dropout.dropout(leaf, 0.4, seed, 6)
+        g, = torch.autograd.grad(y, leaf, x)
+        return y.detach(), g
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for s in (11, 12, 1 << 62, 12):
+        seed.fill_(s)
+        graph.replay()
+        y = dropout.dropout(x, 0.4, s, 6)
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], y) and torch.equal(outs[1], y)   # (x is its own gradient here)
+
+
+def test_changed_seed_before_the_backward_raises():
+    x = torch.randn(4, 8, device=DEV, requires_grad=True)
+    seed = torch.tensor([1], device=DEV)
+    y = dropout.dropout(x, 0.5, seed)
+    seed.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def test_module():
+    m = dropout.CounterDropout(0.3, seed=21)
+    x = torch.randn(2, 6, 32, device=DEV)
+    a, b = m(x), m(x)
+    assert m.call == 2 and not torch.equal(a, b)
+    assert torch.equal(a, dropout.dropout(x, 0.3, 21, 0))
+    m.call = 0
+    pos = torch.tensor([1, 4, 11], device=DEV)
+    assert torch.equal(m.rows(x.view(12, 32)[pos], pos), a.view(12, 32)[pos])
+    assert m.eval()(x) is x
+
+
+def test_refusals():
+    x = torch.randn(4, 8, device=DEV)
+    for kw, error in ((dict(p=1.1), ValueError), (dict(seed=-1), ValueError),
+                      (dict(seed=1.0), TypeError), (dict(call=1 << 64), ValueError),
+                      (dict(seed=torch.tensor([1])), ValueError),
+                      (dict(rows=torch.zeros(3, dtype=torch.int64, device=DEV)), ValueError),
+                      (dict(rows=torch.zeros(4, device=DEV)), TypeError),
+                      (dict(residual=x[:2]), ValueError), (dict(residual=x.half()), TypeError)):
+        with pytest.raises(error):
+            dropout.dropout(**{**dict(x=x, p=0.1, seed=1), **kw})
+    with pytest.raises(TypeError):
+        dropout.dropout(x.double(), 0.1, 1)

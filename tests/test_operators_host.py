@@ -1,0 +1,136 @@
+"""Refusals of the operators around the layer, on the CPU: Python arguments before a launch, and the C
+entry points' own checks."""
+
+import ctypes
+
+import pytest
+import torch
+
+from testt_amd import _ext, attention, dropout, embedding, head, rope
+
+H = torch.float16
+
+
+def test_cpu_tensors_are_refused():
+    z = torch.zeros(2, 8, dtype=H)
+    tok = torch.zeros(2, dtype=torch.int64)
+    with pytest.raises(ValueError, match="no CPU path"):
+        head.token_logprobs(z, tok)
+    with pytest.raises(ValueError, match="no CPU path"):
+        head.fused_token_logprobs(z, z, tok)
+    with pytest.raises(ValueError, match="no CPU path"):
+        dropout.dropout(z, 0.1, 1)
+    with pytest.raises(ValueError, match="no CPU path"):
+        embedding.embedding(tok, z)
+    with pytest.raises(ValueError, match="no CPU path"):
+        rope.qk_norm_rope(z, None, None, z[0], z[0], z, z, tok, 1, 2, 1, 0, 16)
+    with pytest.raises(ValueError, match="HIP device"):
+        attention.norm_rope_attention(z, None, None, z[0], z[0], z, z, tok, tok, 1, 2, 1, 1)
+
+
+@pytest.mark.parametrize("p", [-0.1, 1.5, float("nan")])
+def test_dropout_probability(p):
+    with pytest.raises(ValueError, match="probability"):
+        dropout.CounterDropout(p)
+
+
+@pytest.mark.parametrize("seed", [-1, 1 << 64])
+def test_dropout_seed(seed):
+    with pytest.raises(ValueError, match="seed"):
+        dropout.CounterDropout(0.1, seed)
+    with pytest.raises(TypeError):
+        dropout.CounterDropout(0.1, 1.5)
+
+
+def test_counter_dropout_leaves_eval_alone():
+    m = dropout.CounterDropout(0.5, 3).eval()
+    x = torch.ones(3)
+    assert m(x) is x and m.call == 0 and isinstance(m, torch.nn.Dropout)
+
+
+A = 4096       # an aligned address that is never read: every call below is refused before a launch
+BAD = [
+    # logits: dtype, columns, temperature, top_k, missing outputs, a missing or short workspace
+    ("soupk_token_logprobs_fwd", (A, 9, A, 4, 4, 0, 8, 8, 1.0, 0, A, A, A, A, None, None, None, 0,
+                                  None)),
+    ("soupk_token_logprobs_fwd", (A, 0, A, 4, 4, 0, 8, 0, 1.0, 0, A, A, A, A, None, None, None, 0,
+                                  None)),
+    ("soupk_token_logprobs_fwd", (A, 0, A, 4, 4, 0, 8, 8, 0.0, 0, A, A, A, A, None, None, None, 0,
+                                  None)),
+    ("soupk_token_logprobs_fwd", (A, 0, A, 4, 4, 0, 8, 8, 1.0, 9, A, A, A, A, A, A, None, 0, None)),
+    ("soupk_token_logprobs_fwd", (A, 0, A, 4, 4, 0, 99, 99, 1.0, 33, A, A, A, A, A, A, None, 0,
+                                  None)),
+    ("soupk_token_logprobs_fwd", (A, 0, A, 4, 4, 0, 8, 8, 1.0, 2, A, A, A, A, None, A, None, 0,
+                                  None)),
+    ("soupk_token_logprobs_fwd", (A + 1, 0, A, 4, 4, 0, 8, 8, 1.0, 0, A, A, A, A, None, None, None,
+                                  0, None)),
+    ("soupk_token_logprobs_fwd", (A, 0, A, 1, 1, 0, 151936, 151936, 1.0, 2, A, A, A, A, A, A, A, 64,
+                                  None)),
+    ("soupk_token_logprobs_bwd", (A, 0, A, 4, 4, 0, 8, 8, 1.0, 0, A, A, A, None, A, None, A, A,
+                                  None)),                                 # g_top without top_k
+    ("soupk_token_logprobs_bwd", (A, 0, A, 4, 4, 0, 8, 8, 1.0, 0, None, A, A, None, A, None, None,
+                                  A, None)),
+    # q/k norm: fp32 rows, head dims, eps, the delta's type, positions, a short workspace
+    ("soupk_qk_norm_rope_fwd", (A, None, None, 0, A, A, A, A, A, A, 1, 4, 1, 4, 2, 1, 128, 1e-6,
+                                None)),
+    ("soupk_qk_norm_rope_fwd", (A, None, None, 0, A, A, A, A, A, A, 0, 4, 1, 4, 2, 1, 72, 1e-6,
+                                None)),
+    ("soupk_qk_norm_rope_fwd", (A, None, None, 0, A, A, A, A, A, A, 0, 4, 1, 4, 2, 1, 272, 1e-6,
+                                None)),
+    ("soupk_qk_norm_rope_fwd", (A, None, None, 0, A, A, A, A, A, A, 0, 4, 1, 4, 2, 1, 128,
+                                float("nan"), None)),
+    ("soupk_qk_norm_rope_fwd", (A, A, None, 2, A, A, A, A, A, A, 0, 4, 1, 4, 2, 1, 128, 1e-6, None)),
+    ("soupk_qk_norm_rope_fwd", (A, None, None, 0, A, A, A, A, None, A, 0, 4, 1, 4, 2, 1, 128, 1e-6,
+                                None)),
+    ("soupk_qk_norm_rope_bwd", (A, A, None, 0, A, A, A, A, A, A, A, A, A, 255, 0, 4, 1, 4, 2, 1, 128,
+                                1e-6, None)),
+    # dropout: limit, two half types, misaligned rows
+    ("soupk_dropout", (A, 0, None, A, 0, None, None, 1, 0, -1, 1.0, 4, 4, None)),
+    ("soupk_dropout", (A, 0, None, A, 0, None, None, 1, 0, (1 << 32) + 1, 1.0, 4, 4, None)),
+    ("soupk_dropout", (A, 0, None, A, 2, None, None, 1, 0, 5, 1.0, 4, 4, None)),
+    ("soupk_dropout", (A, 0, None, A, 0, A + 4, None, 1, 0, 5, 1.0, 4, 4, None)),
+    ("soupk_dropout", (A, 0, None, A, 0, None, None, 1, 0, 5, 1.0, -4, 4, None)),
+    # embedding: types, sizes, missing workspace
+    ("soupk_embedding_fwd", (A, 1, A, A, 0, 1.0, 4, 8, 8, None)),
+    ("soupk_embedding_fwd", (A, 0, A, A, 0, 1.0, 4, 1 << 31, 8, None)),
+    ("soupk_embedding_fwd", (None, 0, A, A, 0, 1.0, 4, 8, 8, None)),
+    ("soupk_embedding_bwd", (A, 0, A, A, 0, 1.0, -1, None, 0, 4, 8, 8, None)),
+    ("soupk_embedding_bwd", (A, 0, A, A, 0, 1.0, -1, A, 100, 4, 8, 8, None)),
+    ("soupk_embedding_bwd", (A, 2, A, A, 0, 1.0, -1, A, 1 << 30, 4, 8, 8, None)),
+    ("soupk_embedding_bwd_workspace", (-1, 8, A)),
+    ("soupk_token_logprobs_workspace", (4, 8, 0, 0, None)),
+]
+
+
+@pytest.mark.parametrize("name,args", BAD)
+def test_entry_points_refuse(name, args):
+    with pytest.raises(_ext.SoupkError, match="status 1"):
+        _ext.call(name, *args)
+
+
+@pytest.mark.parametrize("name,args", [
+    ("soupk_token_logprobs_fwd", (None, 0, None, 0, 1, 0, 8, 8, 1.0, 2, *(None,) * 7, 0, None)),
+    ("soupk_token_logprobs_bwd", (None, 0, None, 0, 1, 0, 8, 8, 1.0, 2, *(None,) * 8, None)),
+    ("soupk_qk_norm_rope_fwd", (None,) * 3 + (0,) + (None,) * 6 + (0, 0, 1, 4, 2, 1, 128, 1e-6,
+                                                                   None)),
+    ("soupk_dropout", (None, 0, None, None, 0, None, None, 1, 0, 5, 1.0, 0, 4, None)),
+    ("soupk_embedding_fwd", (None, 0, None, None, 0, 1.0, 0, 8, 8, None)),
+    ("soupk_embedding_bwd", (None, 0, None, None, 0, 1.0, -1, None, 0, 4, 0, 8, None)),
+])
+def test_no_work_is_a_no_op(name, args):
+    _ext.call(name, *args)
+
+
+def test_workspaces_grow_with_the_work():
+    need = ctypes.c_int64()
+
+    def size(name, *args):
+        _ext.call(name, *args, ctypes.addressof(need))
+        return need.value
+
+    assert size("soupk_embedding_bwd_workspace", 0, 1536) >= 0
+    assert size("soupk_embedding_bwd_workspace", 100, 1536) >= 4 * 4 * 100 + 7 * 2 * 1536 * 4
+    assert size("soupk_token_logprobs_workspace", 1, 151936, 20, 0) > 0
+    # a part without alternatives keeps its statistics alone
+    assert size("soupk_token_logprobs_workspace", 1, 151936, 0, 0) < \
+        size("soupk_token_logprobs_workspace", 1, 151936, 20, 0)

@@ -17,11 +17,13 @@ _lock = threading.Lock()
 _lib = None
 _host = None     # the CPython extension (csrc/host_ops.cpp), bound to the library's entry points
 
-ABI_VERSION = 5
+ABI_VERSION = 6
 STATUS_SCRATCH_LIMIT = 20001          # SOUPK_STATUS_SCRATCH_LIMIT
 LORA_SCRATCH_FLOATS = 4 << 20         # SOUPK_LORA_SCRATCH_FLOATS
 DTYPE_F16 = 0
 DTYPE_F32 = 1
+DTYPE_BF16 = 2
+QK_NORM_BLOCKS = 1024                 # SOUPK_QK_NORM_BLOCKS
 
 _p = ctypes.c_void_p
 _i32 = ctypes.c_int32
@@ -88,6 +90,19 @@ SIGNATURES = {
                             _i32, _i32, _i32, _i32, _i32, _i64],
     "soupk_gemm_nn": [_p, _i64, _p, _i64, _p, _i64, _i64, _i32, _i32, _p, _p, _i64, _p],
     "soupk_gemm_nn_workspace": [_i64, _i32, _i32, _p],
+    "soupk_token_logprobs_workspace": [_i64, _i64, _i32, _i32, _p],
+    "soupk_token_logprobs_fwd": [_p, _i32, _p, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _p, _p,
+                                 _p, _p, _p, _p, _p, _i64, _p],
+    "soupk_token_logprobs_bwd": [_p, _i32, _p, _i64, _i64, _i64, _i64, _i64, _f32, _i32, _p, _p,
+                                 _p, _p, _p, _p, _p, _p, _p],
+    "soupk_qk_norm_rope_fwd": [_p, _p, _p, _i32, _p, _p, _p, _p, _p, _p, _i32, _i64, _i32, _i32,
+                               _i32, _i32, _i32, _f32, _p],
+    "soupk_qk_norm_rope_bwd": [_p, _p, _p, _i32, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i32,
+                               _i64, _i32, _i32, _i32, _i32, _i32, _f32, _p],
+    "soupk_dropout": [_p, _i32, _p, _p, _i32, _p, _p, _i64, _i64, _i64, _f32, _i64, _i64, _p],
+    "soupk_embedding_fwd": [_p, _i32, _p, _p, _i32, _f32, _i64, _i64, _i64, _p],
+    "soupk_embedding_bwd_workspace": [_i64, _i64, _p],
+    "soupk_embedding_bwd": [_p, _i32, _p, _p, _i32, _f32, _i64, _p, _i64, _i64, _i64, _i64, _p],
     "soupk_layer_fwd": [_p, _p, _p],
     "soupk_layer_bwd": [_p, _p, _p],
 }
@@ -184,6 +199,27 @@ def call(name, *args):
         text = lib().soupk_status_string(status)
         text = text.decode() if text else "?"
         raise SoupkError(f"{name} failed with status {status}: {text}")
+
+
+def call_on(tensor, name, *args):
+    """call(name, *args) with the tensor's device current (its stream is the last argument): a
+    launch on another device's stream needs that device."""
+    index = tensor.device.index
+    if index == torch.cuda.current_device():
+        return call(name, *args)
+    with torch.cuda.device(index):
+        return call(name, *args)
+
+
+DTYPES = {torch.float16: DTYPE_F16, torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
+
+
+def dtype_code(tensor, name, allowed=(torch.float16, torch.bfloat16, torch.float32)):
+    """The SOUPK_DTYPE_* code of a tensor of one of the allowed types."""
+    if tensor.dtype not in allowed:
+        raise TypeError(f"{name} must be one of {', '.join(str(d) for d in allowed)}, got "
+                        f"{tensor.dtype}")
+    return DTYPES[tensor.dtype]
 
 
 def ptr(tensor):

@@ -163,6 +163,43 @@ def rope_attention(qkv, lora_q, lora_v, cos, sin, pos_idx, cu_seqlens, batch, se
                                cos, sin, pos_idx, cu_seqlens, batch, seq, n_heads, n_kv, scale)
 
 
+class VarlenAttention(torch.autograd.Function):
+    """out [M, NH*D] = causal GQA attention of the token-major rows qkv_r as they are (rotated by the
+    caller); the gradient of qkv_r."""
+
+    @staticmethod
+    def forward(ctx, qkv_r, cu_seqlens, n_heads, n_kv, scale):
+        out, lse = attention_varlen_fwd(qkv_r, cu_seqlens, n_heads, n_kv, scale)
+        ctx.save_for_backward(qkv_r, cu_seqlens, out, lse)
+        ctx.dims = (n_heads, n_kv, scale)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        qkv_r, cu, out, lse = ctx.saved_tensors
+        n_heads, n_kv, scale = ctx.dims
+        dqkv = attention_varlen_bwd(qkv_r, cu, out, lse, dout, scale, n_heads, n_kv)
+        return dqkv, None, None, None, None
+
+
+def norm_rope_attention(qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx, cu_seqlens,
+                        batch, seq, n_heads, n_kv, eps=1e-6, scale=None):
+    """rope_attention for models that normalise queries and keys per head (rope.qk_norm_rope, then
+    the varlen attention over its rows): out [M, NH*D] fp16, differentiable in qkv, the LoRA deltas
+    and the two norm weights.  fp16 rows, head dim 128."""
+    from .rope import qk_norm_rope
+
+    if not varlen_supported(qkv, HEAD_DIM, n_heads, n_kv):
+        raise ValueError(f"norm_rope_attention takes fp16 [M, W] rows on a HIP device and query "
+                         f"heads that are a multiple of the key heads, got {tuple(qkv.shape)} "
+                         f"{qkv.dtype} on {qkv.device} with {n_heads} and {n_kv} heads")
+    rows = qk_norm_rope(qkv.contiguous(), lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx,
+                        batch, seq, n_heads, n_kv, HEAD_DIM, eps)
+    scale = 1.0 / math.sqrt(HEAD_DIM) if scale is None else float(scale)
+    return VarlenAttention.apply(rows, cu_seqlens, n_heads, n_kv, scale)
+
+
 def supported(q, k, v):
     return (q.is_cuda and q.dtype == torch.float16 and q.dim() == 4 and q.shape[-1] == HEAD_DIM
             and k.shape[1] > 0 and q.shape[1] % k.shape[1] == 0)

@@ -47,7 +47,9 @@ using at::Tensor;
   X(soupk_lora_bwd_rows) X(soupk_lora_bwd_params) X(soupk_lora_bwd_params_noalloc)                \
   X(soupk_gemm_tn) X(soupk_gemm_nn_nf4) X(soupk_gemm_tn_nf4) X(soupk_gemm_tn_nf4_split)           \
   X(soupk_gemm_nn_nf4_split) X(soupk_gemm_lt) X(soupk_gemm_nn) X(soupk_gemm_nn_workspace)         \
-  X(soupk_layer_fwd) X(soupk_layer_bwd)
+  X(soupk_token_logprobs_fwd) X(soupk_token_logprobs_bwd) X(soupk_token_logprobs_workspace)      \
+  X(soupk_qk_norm_rope_fwd) X(soupk_qk_norm_rope_bwd) X(soupk_dropout) X(soupk_embedding_fwd)     \
+  X(soupk_embedding_bwd) X(soupk_embedding_bwd_workspace) X(soupk_layer_fwd) X(soupk_layer_bwd)
 
 #define X(name) decltype(&name) p_##name = nullptr;
 SOUPK_ENTRIES(X)

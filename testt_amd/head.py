@@ -31,7 +31,9 @@ Every row's statistics and gradient are computed from that row alone: on the chu
 nothing but the order of dh's fp32 sums (the cut of the contraction follows from the rows).
 """
 
+import ctypes
 import math
+from collections import namedtuple
 
 import torch
 
@@ -369,3 +371,196 @@ def fused_head_loss(hidden16, weight16, targets, denominator):
     if not hidden16.is_cuda:
         raise ValueError("fused_head_loss: hidden16 must be a HIP device tensor (no CPU path)")
     return FusedHeadLoss.apply(hidden16.contiguous(), weight16, targets.contiguous(), denominator)
+
+
+# --------------------------------------------------------------------------------------------
+# Log probabilities of given tokens, entropy and top alternatives (csrc/token_logprobs.hip)
+
+MAX_TOP = 32      # most alternatives per row
+
+TokenLogprobs = namedtuple("TokenLogprobs", "logprob entropy top_logprobs top_ids")
+
+
+def _check_logprobs(top_k, temperature, vocab):
+    """(top_k, temperature) as numbers the kernels take, or an error."""
+    if isinstance(top_k, bool) or not isinstance(top_k, int):
+        raise TypeError(f"top_k must be an int, got {type(top_k).__name__}")
+    if not 0 <= top_k <= min(MAX_TOP, vocab):
+        raise ValueError(f"top_k must lie in [0, {min(MAX_TOP, vocab)}], got {top_k}")
+    temperature = float(temperature)
+    # (an fp32 value with an fp32 reciprocal)
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"temperature must lie in [1e-30, 1e30], got {temperature}")
+    return top_k, temperature
+
+
+def _logit_rows(logits, tokens):
+    """(logits with unit column stride, flat tokens, rows, inner, stride_outer, stride_inner)."""
+    if logits.stride(-1) != 1 and logits.shape[-1] != 1:
+        logits = logits.contiguous()
+    tokens = tokens.contiguous().view(-1)
+    rows = tokens.numel()
+    if logits.dim() == 2:
+        return logits, tokens, rows, max(rows, 1), 0, logits.stride(0)
+    return logits, tokens, rows, max(logits.shape[1], 1), logits.stride(0), logits.stride(1)
+
+
+def _logprobs_fwd(logits, tokens, top_k, temperature, outs=None):
+    """(logprob, entropy, row_max, row_sum, top_logprobs, top_ids) of checked arguments; `outs`:
+    buffers to fill instead of new ones (contiguous, of the rows' number)."""
+    z, tok, rows, inner, so, si = _logit_rows(logits, tokens)
+    vocab, dev = logits.shape[-1], logits.device
+    if outs is None:
+        shape = tokens.shape
+        outs = [torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(4)]
+        outs += [torch.empty((*shape, top_k), dtype=torch.float32, device=dev),
+                 torch.empty((*shape, top_k), dtype=torch.int64, device=dev)]
+    if rows:
+        code = _ext.DTYPES[z.dtype]
+        need = ctypes.c_int64()
+        _ext.call_on(z, "soupk_token_logprobs_workspace", rows, vocab, top_k, code,
+                     ctypes.addressof(need))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
+        _ext.call_on(z, "soupk_token_logprobs_fwd", z.data_ptr(), code, tok.data_ptr(), rows,
+                     inner, so, si, vocab, temperature, top_k, *(o.data_ptr() for o in outs),
+                     _ext.ptr(ws), need.value, _ext.stream_of(z))
+    return outs
+
+
+def _logprobs_bwd(logits, tokens, stats, top_ids, grads, top_k, temperature, dlogits):
+    """Fills dlogits (contiguous) from the forward's (row_max, row_sum, entropy) and the gradients
+    of logprob, entropy and top_logprobs (None: zero)."""
+    z, tok, rows, inner, so, si = _logit_rows(logits, tokens)
+    grads = [None if g is None else g.to(torch.float32).contiguous() for g in grads]
+    if top_k == 0:
+        grads[2] = None
+    if rows:
+        _ext.call_on(z, "soupk_token_logprobs_bwd", z.data_ptr(), _ext.DTYPES[z.dtype],
+                     tok.data_ptr(), rows, inner, so, si, logits.shape[-1], temperature, top_k,
+                     *(t.data_ptr() for t in stats), _ext.ptr(top_ids),
+                     *(_ext.ptr(g) for g in grads), dlogits.data_ptr(), _ext.stream_of(z))
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, top_k, temperature):
+        lp, ent, row_max, row_sum, top_lp, top_ids = _logprobs_fwd(logits, tokens, top_k,
+                                                                   temperature)
+        ctx.save_for_backward(logits, tokens, row_max, row_sum, ent, top_ids)
+        ctx.args = (top_k, temperature)
+        ctx.mark_non_differentiable(top_ids)
+        ctx.set_materialize_grads(False)
+        return lp, ent, top_lp, top_ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_lp, g_ent, g_top, _ids):
+        if not ctx.needs_input_grad[0] or (g_lp is None and g_ent is None and g_top is None):
+            return None, None, None, None
+        logits, tokens, row_max, row_sum, ent, top_ids = ctx.saved_tensors
+        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        _logprobs_bwd(logits, tokens, (row_max, row_sum, ent), top_ids, [g_lp, g_ent, g_top],
+                      *ctx.args, dlogits)
+        return dlogits, None, None, None
+
+
+def token_logprobs(logits, tokens, top_k=0, temperature=1.0):
+    """TokenLogprobs(logprob, entropy, top_logprobs, top_ids) of the distributions
+    softmax(logits / temperature), differentiable in `logits`.
+
+    logits: fp16, bf16 or fp32 [rows, V] or [batch, seq, V] on a HIP device, any row strides (a
+    view shifted by one position is read where it is); tokens: int64 of the leading shape.
+    logprob, entropy: fp32 of that shape; top_logprobs fp32 and top_ids int64 [..., top_k]: the
+    top_k (0 to 32) largest logits, equal ones by the lower id.  A token of IGNORE_INDEX has log
+    probability 0 and passes no gradient on, any other token outside the vocabulary NaN (and no
+    gradient).  Masked logits may be -inf or the type's lowest value; a NaN or +inf in a row, or a
+    row of -inf alone, makes the row's numbers NaN (its NaN logits rank with -inf among the
+    alternatives).  A row without upstream gradient gets zeros."""
+    if not isinstance(logits, torch.Tensor) or not isinstance(tokens, torch.Tensor):
+        raise TypeError("logits and tokens must be tensors")
+    if not logits.is_cuda:
+        raise ValueError(f"logits must be a HIP device tensor (got device {logits.device}); the "
+                         "soupk kernels have no CPU path")
+    _ext.dtype_code(logits, "logits")
+    if logits.dim() not in (2, 3) or logits.shape[-1] == 0:
+        raise ValueError(f"logits must be [rows, V] or [batch, seq, V] with V > 0, got "
+                         f"{tuple(logits.shape)}")
+    if tokens.dtype != torch.int64:
+        raise TypeError(f"tokens must be torch.int64, got {tokens.dtype}")
+    if tokens.device != logits.device or tokens.shape != logits.shape[:-1]:
+        raise ValueError(f"tokens {tuple(tokens.shape)} on {tokens.device} do not fit logits "
+                         f"{tuple(logits.shape)} on {logits.device}")
+    top_k, temperature = _check_logprobs(top_k, temperature, logits.shape[-1])
+    return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, top_k, temperature))
+
+
+class _HiddenLogprobs(torch.autograd.Function):
+    """token_logprobs(hidden @ weight^T, ...) in chunks of CHUNK_ROWS rows, for a frozen head: no
+    chunk's logits outlive it.  The backward forms them again."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, tokens, top_k, temperature):
+        rows, dev = hidden.shape[0], hidden.device
+        outs = [torch.empty(rows, dtype=torch.float32, device=dev) for _ in range(4)]
+        outs += [torch.empty((rows, top_k), dtype=torch.float32, device=dev),
+                 torch.empty((rows, top_k), dtype=torch.int64, device=dev)]
+        for start in range(0, rows, CHUNK_ROWS):
+            part = slice(start, min(rows, start + CHUNK_ROWS))
+            logits = _blas.linear(hidden[part], weight)
+            _logprobs_fwd(logits, tokens[part], top_k, temperature, [o[part] for o in outs])
+            del logits
+        lp, ent, row_max, row_sum, top_lp, top_ids = outs
+        ctx.save_for_backward(hidden, weight, tokens, row_max, row_sum, ent, top_ids)
+        ctx.args = (top_k, temperature)
+        ctx.mark_non_differentiable(top_ids)
+        ctx.set_materialize_grads(False)
+        return lp, ent, top_lp, top_ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g_lp, g_ent, g_top, _ids):
+        grads = [g_lp, g_ent, g_top]
+        if not ctx.needs_input_grad[0] or all(g is None for g in grads):
+            return None, None, None, None, None
+        hidden, weight, tokens, row_max, row_sum, ent, top_ids = ctx.saved_tensors
+        # The fp16 gradient of the logits is held at a power of two that brings the largest upstream
+        # gradient to 32 .. 64 (as _grad_unit does for the loss): most of its entries are p * g, far
+        # below fp16's range otherwise.  Scaling by a power of two is exact.
+        tops = [g.detach().to(torch.float32).abs().amax().reshape(1) for g in grads
+                if g is not None and g.numel()]
+        top = torch.cat(tops).amax() if tops else hidden.new_ones((), dtype=torch.float32)
+        _, exponent = torch.frexp(torch.where(top > 0, top, 1.0))
+        exponent = exponent.clamp(-100, 100)
+        unit = torch.ldexp(torch.ones_like(top), 6 - exponent)
+        grads = [None if g is None else g.to(torch.float32) * unit for g in grads]
+        rows, width = hidden.shape
+        vocab = weight.shape[0]
+        dh = torch.empty_like(hidden)
+        for start in range(0, rows, CHUNK_ROWS):
+            part = slice(start, min(rows, start + CHUNK_ROWS))
+            logits = _blas.linear(hidden[part], weight)
+            g = torch.empty_like(logits)
+            _logprobs_bwd(logits, tokens[part], [t[part] for t in (row_max, row_sum, ent)],
+                          top_ids[part], [None if x is None else x[part] for x in grads],
+                          *ctx.args, g)
+            del logits
+            _hidden_grad(g, weight, dh[part])
+            del g
+        return (dh.to(torch.float32) / unit).to(torch.float16), None, None, None, None
+
+
+def fused_token_logprobs(hidden16, weight16, tokens, top_k=0, temperature=1.0):
+    """token_logprobs of the frozen head's logits hidden16 [rows, H] @ weight16 [V, H]^T without
+    the full logits (chunks of CHUNK_ROWS rows), differentiable in hidden16: the log probabilities
+    a policy-gradient or preference loss takes, where fused_head_loss gives the cross-entropy.
+    The logits are fp16, as there."""
+    _ext.require(hidden16, "hidden16", dtype=torch.float16, ndim=2)
+    _ext.require(weight16, "weight16", dtype=torch.float16, ndim=2, device=hidden16.device)
+    _ext.require(tokens, "tokens", dtype=torch.int64, ndim=1, device=hidden16.device)
+    if weight16.shape[1] != hidden16.shape[1] or weight16.shape[0] == 0:
+        raise ValueError(f"weight16 {tuple(weight16.shape)} does not fit hidden16 "
+                         f"{tuple(hidden16.shape)}")
+    if tokens.numel() != hidden16.shape[0]:
+        raise ValueError(f"{tokens.numel()} tokens for {hidden16.shape[0]} rows")
+    top_k, temperature = _check_logprobs(top_k, temperature, weight16.shape[0])
+    return TokenLogprobs(*_HiddenLogprobs.apply(hidden16, weight16, tokens, top_k, temperature))

@@ -164,3 +164,103 @@ def rope_pack_tokens(qkv, lora_q, lora_v, cos, sin, pos_idx, batch, seq, n_heads
                   _ext.ptr(lv), code, _ext.ptr(cos32), _ext.ptr(sin32), _ext.ptr(pos),
                   _ext.ptr(out), rows, batch, seq, n_heads, n_kv, head_dim, _ext.stream_of(out))
     return out, cos32, sin32, pos
+
+
+class QkNormRope(torch.autograd.Function):
+    """Rows [M, W] of normalised and rotated queries and keys (csrc/qk_norm_rope.hip); gradients for
+    qkv, the LoRA deltas (views of qkv's gradient, as RopePack's) and the two weights."""
+
+    @staticmethod
+    def forward(ctx, qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos, batch, seq, n_heads,
+                n_kv, head_dim, eps):
+        rows, dev = qkv.shape[0], qkv.device
+        lq, lv, code = lora_q, lora_v, _ext.DTYPES[qkv.dtype]
+        if any(t is not None and t.dtype == torch.float32 for t in (lq, lv)):
+            lq, lv = (None if t is None else t.detach().float() for t in (lq, lv))
+            code = _ext.DTYPE_F32
+        out = torch.empty_like(qkv)
+        if rows:
+            _ext.call_on(qkv, "soupk_qk_norm_rope_fwd", _ext.ptr(qkv), _ext.ptr(lq), _ext.ptr(lv),
+                         code, _ext.ptr(q_weight), _ext.ptr(k_weight), _ext.ptr(cos),
+                         _ext.ptr(sin), _ext.ptr(pos), _ext.ptr(out), _ext.DTYPES[qkv.dtype], rows,
+                         batch, seq, n_heads, n_kv, head_dim, eps, _ext.stream_of(qkv))
+        ctx.save_for_backward(qkv, lq, q_weight, k_weight, cos, sin, pos)
+        ctx.dims = (batch, seq, n_heads, n_kv, head_dim, eps, code)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        qkv, lq, q_weight, k_weight, cos, sin, pos = ctx.saved_tensors
+        batch, seq, n_heads, n_kv, head_dim, eps, code = ctx.dims
+        need = ctx.needs_input_grad
+        none = (None,) * 9
+        if not any(need[:5]):
+            return (None,) * 5 + none
+        rows, dev = qkv.shape[0], qkv.device
+        dout = dout.to(qkv.dtype).contiguous()
+        dqkv = torch.empty_like(qkv)
+        dwq, dwk = (torch.empty(head_dim, dtype=torch.float32, device=dev) if n else None
+                    for n in need[3:5])
+        ws = None
+        if need[3] or need[4]:
+            ws = torch.empty(_ext.QK_NORM_BLOCKS * 2 * head_dim, dtype=torch.float32, device=dev)
+        _ext.call_on(qkv, "soupk_qk_norm_rope_bwd", _ext.ptr(dout), _ext.ptr(qkv), _ext.ptr(lq),
+                     code, _ext.ptr(q_weight), _ext.ptr(k_weight), _ext.ptr(cos), _ext.ptr(sin),
+                     _ext.ptr(pos), _ext.ptr(dqkv), _ext.ptr(dwq), _ext.ptr(dwk), _ext.ptr(ws),
+                     0 if ws is None else ws.numel(), _ext.DTYPES[qkv.dtype], rows, batch, seq,
+                     n_heads, n_kv, head_dim, eps, _ext.stream_of(qkv))
+        v_start = (n_heads + n_kv) * head_dim
+        return ((dqkv if need[0] else None),
+                (dqkv[:, :n_heads * head_dim] if need[1] else None),
+                (dqkv[:, v_start:] if need[2] else None), dwq, dwk) + none
+
+
+def qk_norm_rope(qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx, batch, seq, n_heads,
+                 n_kv, head_dim, eps=1e-6):
+    """rope_pack_tokens for models that normalise queries and keys per head: the q|k|v rows
+    [M, (n_heads + 2*n_kv) * head_dim] with every query and key head (after its LoRA delta)
+    RMS-normalised over head_dim, multiplied by q_weight or k_weight [head_dim] and rotated, the
+    value heads with their delta; in the rows' type (fp16 or bf16), fp32 inside with one rounding.
+    Differentiable in qkv, the deltas and the weights.
+
+    lora_q [M, n_heads*head_dim] / lora_v [M, n_kv*head_dim]: None, the rows' type or fp32.  cos,
+    sin, pos_idx, batch, seq as rope_pack_tokens; head_dim a multiple of 16 up to 256.  A token
+    whose position lies outside [0, batch*seq) gets a row of zeros (and passes no gradient)."""
+    _ext.require(qkv, "qkv", ndim=2)
+    _ext.dtype_code(qkv, "qkv", (torch.float16, torch.bfloat16))
+    rows, dev = qkv.shape[0], qkv.device
+    if n_heads <= 0 or n_kv < 0 or head_dim <= 0 or head_dim % 16 or head_dim > 256:
+        raise ValueError(f"qk_norm_rope takes head dims that are multiples of 16 up to 256 and at "
+                         f"least one query head, got {n_heads}, {n_kv} heads of {head_dim}")
+    width = (n_heads + 2 * n_kv) * head_dim
+    if qkv.shape[1] != width:
+        raise ValueError(f"qkv width {qkv.shape[1]} != (n_heads + 2*n_kv) * head_dim = {width}")
+    deltas = []
+    for t, name, heads in ((lora_q, "lora_q", n_heads), (lora_v, "lora_v", n_kv)):
+        if t is not None:
+            if not isinstance(t, torch.Tensor) or t.device != dev:
+                raise ValueError(f"{name} must be a tensor on {dev}")
+            if t.dtype not in (qkv.dtype, torch.float32):
+                raise TypeError(f"{name} must be {qkv.dtype} or torch.float32, got {t.dtype}")
+            if tuple(t.shape) != (rows, heads * head_dim):
+                raise ValueError(f"{name} shape {tuple(t.shape)} != {(rows, heads * head_dim)}")
+            t = t.contiguous()
+        deltas.append(t)
+    weights = []
+    for t, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if not isinstance(t, torch.Tensor) or t.device != dev or tuple(t.shape) != (head_dim,) or \
+                not t.dtype.is_floating_point:
+            raise ValueError(f"{name} must be a floating-point tensor of {head_dim} on {dev}")
+        weights.append(t.float().contiguous())
+    if not isinstance(pos_idx, torch.Tensor) or pos_idx.device != dev or pos_idx.dim() != 1 or \
+            pos_idx.numel() != rows or pos_idx.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"pos_idx must be {rows} integer positions on {dev}")
+    if batch < 0 or seq < 0 or batch * seq >= 1 << 31:
+        raise ValueError(f"batch ({batch}) and seq ({seq}) must span fewer than 2^31 positions")
+    eps = float(eps)
+    if not 0.0 <= eps <= 3e38:
+        raise ValueError(f"eps must be a non-negative number, got {eps}")
+    return QkNormRope.apply(qkv, *deltas, *weights, _table(cos, seq, head_dim, "cos", dev),
+                            _table(sin, seq, head_dim, "sin", dev), as_index(pos_idx), batch, seq,
+                            n_heads, n_kv, head_dim, eps)
