@@ -222,6 +222,13 @@ def dtype_code(tensor, name, allowed=(torch.float16, torch.bfloat16, torch.float
     return DTYPES[tensor.dtype]
 
 
+def checked(result):
+    """The result of a native operator (host()) for arguments that the caller has checked."""
+    if result is None:
+        raise SoupkError("the host extension does not take checked arguments")
+    return result
+
+
 def ptr(tensor):
     """Device address of a tensor (None for None)."""
     return None if tensor is None else tensor.data_ptr()

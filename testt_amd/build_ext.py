@@ -18,7 +18,7 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB_NAME = "libsoupk.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
-HOST_SRC = os.path.join(CSRC, "host_ops.cpp")
+HOST_SRCS = [os.path.join(CSRC, f) for f in ("host_ops.cpp", "host_autograd.cpp")]
 HOST_NAME = "_soupk_host.so"       # the CPython extension of the operators' host side
 HOST_PATH = os.path.join(HERE, HOST_NAME)
 ARCH = "gfx950"
@@ -68,7 +68,7 @@ def _build_host(hipcc, build_dir):
     import torch
 
     root = os.path.dirname(os.path.abspath(torch.__file__))
-    obj = os.path.join(build_dir, "host_ops.o")
+    objs = [os.path.join(build_dir, os.path.basename(src)[:-4] + ".o") for src in HOST_SRCS]
     # NDEBUG: without it the headers bring a thread-local debug counter, and a library with
     # thread-local storage loaded last sends every such access of the libraries before it (HIP
     # makes several per launch) through the slow path of glibc before 2.39: the 64-token layer took
@@ -80,12 +80,17 @@ def _build_host(hipcc, build_dir):
              f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include",
              f"-I{sysconfig.get_paths()['include']}", "-I/opt/rocm/include"]
     tmp = HOST_PATH + ".tmp"
-    for cmd in ([hipcc, *flags, "-c", HOST_SRC, "-o", obj],
-                [hipcc, "-shared", obj, "-o", tmp, f"-L{root}/lib", "-ltorch_python", "-ltorch",
-                 "-ltorch_cpu", "-lc10", "-lc10_hip"]):
+
+    def run(cmd):
         proc = subprocess.run(cmd, capture_output=True, text=True)
         if proc.returncode != 0:
             raise RuntimeError(f"building {HOST_NAME} failed:\n{proc.stderr}")
+
+    with ThreadPoolExecutor(len(objs)) as pool:
+        list(pool.map(lambda so: run([hipcc, *flags, "-c", so[0], "-o", so[1]]),
+                      zip(HOST_SRCS, objs)))
+    run([hipcc, "-shared", *objs, "-o", tmp, f"-L{root}/lib", "-ltorch_python", "-ltorch",
+         "-ltorch_cpu", "-lc10", "-lc10_hip"])
     return tmp
 
 

@@ -258,8 +258,10 @@ __device__ __forceinline__ float write_row(const RowOut& o, int64_t r, const Sta
   else if (tok >= 0 && tok < V)
     lp = (Elem<T>::load1(row + tok * Elem<T>::kBytes) - st.m) * inv_t - lse;
   o.logprob[r] = lp;
-  o.row_max[r] = st.m;
-  o.row_sum[r] = st.s;
+  if (o.row_max != nullptr) {
+    o.row_max[r] = st.m;
+    o.row_sum[r] = st.s;
+  }
   return lse;
 }
 
@@ -587,7 +589,8 @@ extern "C" __attribute__((visibility("default"))) int soupk_token_logprobs_fwd(
   if (bad_lp(dtype, rows, inner, V, temperature)) return kInvalid;
   if (top_k < 0 || top_k > kMaxTop || top_k > V) return kInvalid;
   if (rows == 0) return kOk;
-  if (bad_elem_ptr(logits, dtype) || !tokens || !logprob || !entropy || !row_max || !row_sum)
+  if (bad_elem_ptr(logits, dtype) || !tokens || !logprob || !entropy ||
+      (row_max == nullptr) != (row_sum == nullptr))
     return kInvalid;
   if (top_k > 0 && (!top_lp || !top_id)) return kInvalid;
   int64_t need = 0;

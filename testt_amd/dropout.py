@@ -15,53 +15,6 @@ import torch
 
 from . import _ext
 
-_ONE = 1 << 32
-
-
-class _Dropout(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, p, seed, call, rows):
-        out_dtype = x.dtype if residual is None else residual.dtype
-        out = _launch(x, residual, out_dtype, p, seed, call, rows)
-        on_device = isinstance(seed, torch.Tensor)
-        # (a seed tensor changed before the backward raises there, as any saved tensor does)
-        ctx.save_for_backward(seed if on_device else None, rows)
-        ctx.args = (p, None if on_device else seed, call, x.dtype)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        seed, rows = ctx.saved_tensors
-        p, host_seed, call, dtype = ctx.args
-        dx = None
-        if ctx.needs_input_grad[0]:
-            dx = _launch(grad.contiguous(), None, dtype, p, host_seed if seed is None else seed,
-                         call, rows)
-        return dx, (grad if ctx.needs_input_grad[1] else None), None, None, None, None
-
-
-def _launch(x, residual, out_dtype, p, seed, call, rows):
-    out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    limit = round(p * _ONE)
-    scale = _ONE / (_ONE - limit) if limit < _ONE else 0.0
-    cols = x.shape[-1] if x.dim() else 1
-    n = x.numel()
-    if n:
-        on_device = isinstance(seed, torch.Tensor)
-        _ext.call_on(x, "soupk_dropout", x.data_ptr(), _ext.DTYPES[x.dtype], _ext.ptr(residual),
-                     out.data_ptr(), _ext.DTYPES[out_dtype], _ext.ptr(rows),
-                     seed.data_ptr() if on_device else None,
-                     0 if on_device else _signed(seed), _signed(call), limit, scale, n // cols,
-                     cols, _ext.stream_of(x))
-    return out
-
-
-def _signed(v):
-    """The 64 bits of 0 <= v < 2^64 as a signed integer."""
-    return v - (1 << 64) if v >> 63 else v
-
-
 def _check_p(p):
     p = float(p)
     if not 0.0 <= p <= 1.0:
@@ -95,6 +48,9 @@ def dropout(x, p, seed, call=0, rows=None, residual=None):
     step's or layer's number); rows: int64, the row number in [0, 2^32) that each row draws as;
     residual: x's shape, x's type or fp32.  The sum is rounded once.  p = 1 gives the residual (or
     zeros) exactly, whatever x holds."""
+    done = _ext.host().dropout(x, p, seed, call, rows, residual)
+    if done is not None:
+        return done
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"x must be a tensor, got {type(x).__name__}")
     if not x.is_cuda:
@@ -119,7 +75,7 @@ def dropout(x, p, seed, call=0, rows=None, residual=None):
         if residual.dtype not in (x.dtype, torch.float32):
             raise TypeError(f"residual must be {x.dtype} or torch.float32, got {residual.dtype}")
         residual = residual.contiguous()
-    return _Dropout.apply(x.contiguous(), residual, p, seed, call, rows)
+    return _ext.checked(_ext.host().dropout(x.contiguous(), p, seed, call, rows, residual))
 
 
 class CounterDropout(torch.nn.Dropout):

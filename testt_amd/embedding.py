@@ -8,51 +8,9 @@ an fp16 table: what the model path takes).  The table's gradient is dense, in th
 tokens are sorted by id, stably, and every row's gradient is summed over its tokens in their order
 in fp32 and rounded once -- the same bits every time, unlike sums by atomics."""
 
-import ctypes
-
 import torch
 
 from . import _ext
-
-
-class _Embedding(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, ids, table, scale, out_dtype, padding_idx):
-        vocab, width = table.shape
-        out = torch.empty((*ids.shape, width), dtype=out_dtype, device=table.device)
-        if out.numel():
-            _ext.call_on(table, "soupk_embedding_fwd", table.data_ptr(), _ext.DTYPES[table.dtype],
-                         ids.data_ptr(), out.data_ptr(), _ext.DTYPES[out_dtype], scale,
-                         ids.numel(), vocab, width, _ext.stream_of(table))
-        ctx.save_for_backward(ids)
-        ctx.args = (table.shape, table.dtype, scale, out_dtype, padding_idx)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        if not ctx.needs_input_grad[1]:
-            return None, None, None, None, None
-        ids, = ctx.saved_tensors
-        shape, dtype, scale, out_dtype, padding_idx = ctx.args
-        return None, _table_grad(grad.contiguous(), ids, shape, dtype, scale, padding_idx), None, \
-            None, None
-
-
-def _table_grad(grad, ids, shape, dtype, scale, padding_idx):
-    vocab, width = shape
-    dtable = torch.empty(shape, dtype=dtype, device=grad.device)
-    if dtable.numel() == 0:
-        return dtable
-    tokens = ids.numel()
-    need = ctypes.c_int64()
-    _ext.call("soupk_embedding_bwd_workspace", tokens, width, ctypes.addressof(need))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=grad.device)
-    _ext.call_on(grad, "soupk_embedding_bwd", grad.data_ptr(), _ext.DTYPES[grad.dtype],
-                 ids.data_ptr(), dtable.data_ptr(), _ext.DTYPES[dtype], scale,
-                 -1 if padding_idx is None else padding_idx, ws.data_ptr(), ws.numel(), tokens,
-                 vocab, width, _ext.stream_of(grad))
-    return dtable
 
 
 def embedding(ids, table, scale=1.0, out_dtype=None, padding_idx=None):
@@ -62,6 +20,10 @@ def embedding(ids, table, scale=1.0, out_dtype=None, padding_idx=None):
     ids: int64 or int32 of any shape; an id outside [0, V) gives a row of zeros and no gradient.
     table: contiguous fp16, bf16 or fp32 [V, H].  padding_idx: a row that gets no gradient (its
     values are looked up like any other's), as torch's."""
+    if padding_idx is None and (out_dtype is None or out_dtype is torch.float32):
+        done = _ext.host().embedding(ids, table, scale, out_dtype is torch.float32, -1)
+        if done is not None:
+            return done
     _ext.require(table, "table", ndim=2)
     _ext.dtype_code(table, "table")
     if not isinstance(ids, torch.Tensor):
@@ -78,8 +40,9 @@ def embedding(ids, table, scale=1.0, out_dtype=None, padding_idx=None):
             raise ValueError(f"padding_idx {padding_idx} lies outside the table of "
                              f"{table.shape[0]} rows")
         padding_idx = int(padding_idx) % table.shape[0]
-    scale = float(scale)
-    return _Embedding.apply(ids.to(torch.int64).contiguous(), table, scale, out_dtype, padding_idx)
+    return _ext.checked(_ext.host().embedding(
+        ids.to(torch.int64).contiguous(), table, float(scale), out_dtype is torch.float32,
+        -1 if padding_idx is None else padding_idx))
 
 
 def supported(table):

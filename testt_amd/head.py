@@ -394,74 +394,28 @@ def _check_logprobs(top_k, temperature, vocab):
     return top_k, temperature
 
 
-def _logit_rows(logits, tokens):
-    """(logits with unit column stride, flat tokens, rows, inner, stride_outer, stride_inner)."""
-    if logits.stride(-1) != 1 and logits.shape[-1] != 1:
-        logits = logits.contiguous()
-    tokens = tokens.contiguous().view(-1)
-    rows = tokens.numel()
-    if logits.dim() == 2:
-        return logits, tokens, rows, max(rows, 1), 0, logits.stride(0)
-    return logits, tokens, rows, max(logits.shape[1], 1), logits.stride(0), logits.stride(1)
+def _chunk_logprobs(logits, tokens, top_k, temperature, outs):
+    """Fills `outs` (logprob, entropy, row_max, row_sum, top_logprobs, top_ids) from a chunk's
+    contiguous logits [rows, V]."""
+    rows, vocab = logits.shape
+    code = _ext.DTYPES[logits.dtype]
+    need = ctypes.c_int64()
+    _ext.call("soupk_token_logprobs_workspace", rows, vocab, top_k, code, ctypes.addressof(need))
+    ws = torch.empty(need.value, dtype=torch.uint8, device=logits.device)
+    _ext.call_on(logits, "soupk_token_logprobs_fwd", logits.data_ptr(), code, tokens.data_ptr(),
+                 rows, rows, 0, vocab, vocab, temperature, top_k, *(o.data_ptr() for o in outs),
+                 ws.data_ptr(), need.value, _ext.stream_of(logits))
 
 
-def _logprobs_fwd(logits, tokens, top_k, temperature, outs=None):
-    """(logprob, entropy, row_max, row_sum, top_logprobs, top_ids) of checked arguments; `outs`:
-    buffers to fill instead of new ones (contiguous, of the rows' number)."""
-    z, tok, rows, inner, so, si = _logit_rows(logits, tokens)
-    vocab, dev = logits.shape[-1], logits.device
-    if outs is None:
-        shape = tokens.shape
-        outs = [torch.empty(shape, dtype=torch.float32, device=dev) for _ in range(4)]
-        outs += [torch.empty((*shape, top_k), dtype=torch.float32, device=dev),
-                 torch.empty((*shape, top_k), dtype=torch.int64, device=dev)]
-    if rows:
-        code = _ext.DTYPES[z.dtype]
-        need = ctypes.c_int64()
-        _ext.call_on(z, "soupk_token_logprobs_workspace", rows, vocab, top_k, code,
-                     ctypes.addressof(need))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=dev) if need.value else None
-        _ext.call_on(z, "soupk_token_logprobs_fwd", z.data_ptr(), code, tok.data_ptr(), rows,
-                     inner, so, si, vocab, temperature, top_k, *(o.data_ptr() for o in outs),
-                     _ext.ptr(ws), need.value, _ext.stream_of(z))
-    return outs
-
-
-def _logprobs_bwd(logits, tokens, stats, top_ids, grads, top_k, temperature, dlogits):
-    """Fills dlogits (contiguous) from the forward's (row_max, row_sum, entropy) and the gradients
-    of logprob, entropy and top_logprobs (None: zero)."""
-    z, tok, rows, inner, so, si = _logit_rows(logits, tokens)
-    grads = [None if g is None else g.to(torch.float32).contiguous() for g in grads]
-    if top_k == 0:
-        grads[2] = None
-    if rows:
-        _ext.call_on(z, "soupk_token_logprobs_bwd", z.data_ptr(), _ext.DTYPES[z.dtype],
-                     tok.data_ptr(), rows, inner, so, si, logits.shape[-1], temperature, top_k,
-                     *(t.data_ptr() for t in stats), _ext.ptr(top_ids),
-                     *(_ext.ptr(g) for g in grads), dlogits.data_ptr(), _ext.stream_of(z))
-
-
-class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, tokens, top_k, temperature):
-        lp, ent, row_max, row_sum, top_lp, top_ids = _logprobs_fwd(logits, tokens, top_k,
-                                                                   temperature)
-        ctx.save_for_backward(logits, tokens, row_max, row_sum, ent, top_ids)
-        ctx.args = (top_k, temperature)
-        ctx.mark_non_differentiable(top_ids)
-        ctx.set_materialize_grads(False)
-        return lp, ent, top_lp, top_ids
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g_lp, g_ent, g_top, _ids):
-        if not ctx.needs_input_grad[0] or (g_lp is None and g_ent is None and g_top is None):
-            return None, None, None, None
-        logits, tokens, row_max, row_sum, ent, top_ids = ctx.saved_tensors
-        dlogits = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        _logprobs_bwd(logits, tokens, (row_max, row_sum, ent), top_ids, [g_lp, g_ent, g_top],
-                      *ctx.args, dlogits)
-        return dlogits, None, None, None
+def _chunk_logprobs_grad(logits, tokens, stats, top_ids, grads, top_k, temperature, dlogits):
+    """Fills dlogits from a chunk's (row_max, row_sum, entropy) and the gradients of logprob, entropy
+    and top_logprobs (fp32, contiguous; None: zero)."""
+    rows, vocab = logits.shape
+    _ext.call_on(logits, "soupk_token_logprobs_bwd", logits.data_ptr(), _ext.DTYPES[logits.dtype],
+                 tokens.data_ptr(), rows, rows, 0, vocab, vocab, temperature, top_k,
+                 *(t.data_ptr() for t in stats), top_ids.data_ptr(),
+                 *(_ext.ptr(g) for g in grads[:2]), _ext.ptr(grads[2]) if top_k else None,
+                 dlogits.data_ptr(), _ext.stream_of(logits))
 
 
 def token_logprobs(logits, tokens, top_k=0, temperature=1.0):
@@ -476,6 +430,9 @@ def token_logprobs(logits, tokens, top_k=0, temperature=1.0):
     gradient).  Masked logits may be -inf or the type's lowest value; a NaN or +inf in a row, or a
     row of -inf alone, makes the row's numbers NaN (its NaN logits rank with -inf among the
     alternatives).  A row without upstream gradient gets zeros."""
+    done = _ext.host().token_logprobs(logits, tokens, top_k, temperature)
+    if done is not None:
+        return TokenLogprobs(*done)
     if not isinstance(logits, torch.Tensor) or not isinstance(tokens, torch.Tensor):
         raise TypeError("logits and tokens must be tensors")
     if not logits.is_cuda:
@@ -491,7 +448,10 @@ def token_logprobs(logits, tokens, top_k=0, temperature=1.0):
         raise ValueError(f"tokens {tuple(tokens.shape)} on {tokens.device} do not fit logits "
                          f"{tuple(logits.shape)} on {logits.device}")
     top_k, temperature = _check_logprobs(top_k, temperature, logits.shape[-1])
-    return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, top_k, temperature))
+    if logits.stride(-1) != 1 and logits.shape[-1] != 1:
+        logits = logits.contiguous()
+    return TokenLogprobs(*_ext.checked(
+        _ext.host().token_logprobs(logits, tokens.contiguous(), top_k, temperature)))
 
 
 class _HiddenLogprobs(torch.autograd.Function):
@@ -507,7 +467,7 @@ class _HiddenLogprobs(torch.autograd.Function):
         for start in range(0, rows, CHUNK_ROWS):
             part = slice(start, min(rows, start + CHUNK_ROWS))
             logits = _blas.linear(hidden[part], weight)
-            _logprobs_fwd(logits, tokens[part], top_k, temperature, [o[part] for o in outs])
+            _chunk_logprobs(logits, tokens[part], top_k, temperature, [o[part] for o in outs])
             del logits
         lp, ent, row_max, row_sum, top_lp, top_ids = outs
         ctx.save_for_backward(hidden, weight, tokens, row_max, row_sum, ent, top_ids)
@@ -532,7 +492,7 @@ class _HiddenLogprobs(torch.autograd.Function):
         _, exponent = torch.frexp(torch.where(top > 0, top, 1.0))
         exponent = exponent.clamp(-100, 100)
         unit = torch.ldexp(torch.ones_like(top), 6 - exponent)
-        grads = [None if g is None else g.to(torch.float32) * unit for g in grads]
+        grads = [None if g is None else (g.to(torch.float32) * unit).contiguous() for g in grads]
         rows, width = hidden.shape
         vocab = weight.shape[0]
         dh = torch.empty_like(hidden)
@@ -540,9 +500,9 @@ class _HiddenLogprobs(torch.autograd.Function):
             part = slice(start, min(rows, start + CHUNK_ROWS))
             logits = _blas.linear(hidden[part], weight)
             g = torch.empty_like(logits)
-            _logprobs_bwd(logits, tokens[part], [t[part] for t in (row_max, row_sum, ent)],
-                          top_ids[part], [None if x is None else x[part] for x in grads],
-                          *ctx.args, g)
+            _chunk_logprobs_grad(logits, tokens[part], [t[part] for t in (row_max, row_sum, ent)],
+                                 top_ids[part], [None if x is None else x[part] for x in grads],
+                                 *ctx.args, g)
             del logits
             _hidden_grad(g, weight, dh[part])
             del g

@@ -166,56 +166,6 @@ def rope_pack_tokens(qkv, lora_q, lora_v, cos, sin, pos_idx, batch, seq, n_heads
     return out, cos32, sin32, pos
 
 
-class QkNormRope(torch.autograd.Function):
-    """Rows [M, W] of normalised and rotated queries and keys (csrc/qk_norm_rope.hip); gradients for
-    qkv, the LoRA deltas (views of qkv's gradient, as RopePack's) and the two weights."""
-
-    @staticmethod
-    def forward(ctx, qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos, batch, seq, n_heads,
-                n_kv, head_dim, eps):
-        rows, dev = qkv.shape[0], qkv.device
-        lq, lv, code = lora_q, lora_v, _ext.DTYPES[qkv.dtype]
-        if any(t is not None and t.dtype == torch.float32 for t in (lq, lv)):
-            lq, lv = (None if t is None else t.detach().float() for t in (lq, lv))
-            code = _ext.DTYPE_F32
-        out = torch.empty_like(qkv)
-        if rows:
-            _ext.call_on(qkv, "soupk_qk_norm_rope_fwd", _ext.ptr(qkv), _ext.ptr(lq), _ext.ptr(lv),
-                         code, _ext.ptr(q_weight), _ext.ptr(k_weight), _ext.ptr(cos),
-                         _ext.ptr(sin), _ext.ptr(pos), _ext.ptr(out), _ext.DTYPES[qkv.dtype], rows,
-                         batch, seq, n_heads, n_kv, head_dim, eps, _ext.stream_of(qkv))
-        ctx.save_for_backward(qkv, lq, q_weight, k_weight, cos, sin, pos)
-        ctx.dims = (batch, seq, n_heads, n_kv, head_dim, eps, code)
-        return out
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
-        qkv, lq, q_weight, k_weight, cos, sin, pos = ctx.saved_tensors
-        batch, seq, n_heads, n_kv, head_dim, eps, code = ctx.dims
-        need = ctx.needs_input_grad
-        none = (None,) * 9
-        if not any(need[:5]):
-            return (None,) * 5 + none
-        rows, dev = qkv.shape[0], qkv.device
-        dout = dout.to(qkv.dtype).contiguous()
-        dqkv = torch.empty_like(qkv)
-        dwq, dwk = (torch.empty(head_dim, dtype=torch.float32, device=dev) if n else None
-                    for n in need[3:5])
-        ws = None
-        if need[3] or need[4]:
-            ws = torch.empty(_ext.QK_NORM_BLOCKS * 2 * head_dim, dtype=torch.float32, device=dev)
-        _ext.call_on(qkv, "soupk_qk_norm_rope_bwd", _ext.ptr(dout), _ext.ptr(qkv), _ext.ptr(lq),
-                     code, _ext.ptr(q_weight), _ext.ptr(k_weight), _ext.ptr(cos), _ext.ptr(sin),
-                     _ext.ptr(pos), _ext.ptr(dqkv), _ext.ptr(dwq), _ext.ptr(dwk), _ext.ptr(ws),
-                     0 if ws is None else ws.numel(), _ext.DTYPES[qkv.dtype], rows, batch, seq,
-                     n_heads, n_kv, head_dim, eps, _ext.stream_of(qkv))
-        v_start = (n_heads + n_kv) * head_dim
-        return ((dqkv if need[0] else None),
-                (dqkv[:, :n_heads * head_dim] if need[1] else None),
-                (dqkv[:, v_start:] if need[2] else None), dwq, dwk) + none
-
-
 def qk_norm_rope(qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx, batch, seq, n_heads,
                  n_kv, head_dim, eps=1e-6):
     """rope_pack_tokens for models that normalise queries and keys per head: the q|k|v rows
@@ -227,6 +177,10 @@ def qk_norm_rope(qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx, bat
     lora_q [M, n_heads*head_dim] / lora_v [M, n_kv*head_dim]: None, the rows' type or fp32.  cos,
     sin, pos_idx, batch, seq as rope_pack_tokens; head_dim a multiple of 16 up to 256.  A token
     whose position lies outside [0, batch*seq) gets a row of zeros (and passes no gradient)."""
+    done = _ext.host().qk_norm_rope(qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx, batch,
+                                    seq, n_heads, n_kv, head_dim, eps)
+    if done is not None:
+        return done
     _ext.require(qkv, "qkv", ndim=2)
     _ext.dtype_code(qkv, "qkv", (torch.float16, torch.bfloat16))
     rows, dev = qkv.shape[0], qkv.device
@@ -247,6 +201,8 @@ def qk_norm_rope(qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx, bat
                 raise ValueError(f"{name} shape {tuple(t.shape)} != {(rows, heads * head_dim)}")
             t = t.contiguous()
         deltas.append(t)
+    if any(t is not None and t.dtype == torch.float32 for t in deltas):
+        deltas = [None if t is None else t.float() for t in deltas]     # (one type for both)
     weights = []
     for t, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
         if not isinstance(t, torch.Tensor) or t.device != dev or tuple(t.shape) != (head_dim,) or \
@@ -261,6 +217,7 @@ def qk_norm_rope(qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx, bat
     eps = float(eps)
     if not 0.0 <= eps <= 3e38:
         raise ValueError(f"eps must be a non-negative number, got {eps}")
-    return QkNormRope.apply(qkv, *deltas, *weights, _table(cos, seq, head_dim, "cos", dev),
-                            _table(sin, seq, head_dim, "sin", dev), as_index(pos_idx), batch, seq,
-                            n_heads, n_kv, head_dim, eps)
+    return _ext.checked(_ext.host().qk_norm_rope(
+        qkv, *deltas, *weights, _table(cos, seq, head_dim, "cos", dev),
+        _table(sin, seq, head_dim, "sin", dev), as_index(pos_idx), batch, seq, n_heads, n_kv,
+        head_dim, eps))
