@@ -762,7 +762,7 @@ int soupk_qk_norm_rope_fwd(const void* qkv, const void* lora_q, const void* lora
  * Its backward: dqkv [rows, (NH + 2*NKV) * D] (its q and v columns are also the gradients of lora_q
  * and lora_v) and, where not NULL, dwq, dwk [D] fp32, summed in a fixed order.  A token whose pos
  * lies outside [0, B*T) gets zeros and adds nothing to dwq, dwk.  workspace (only for dwq, dwk):
- * SOUPK_QK_NORM_BLOCKS * 2 * D floats suffice.
+ * SOUPK_QK_NORM_BLOCKS * D floats suffice.
  */
 #define SOUPK_QK_NORM_BLOCKS 1024
 int soupk_qk_norm_rope_bwd(const void* dout, const void* qkv, const void* lora_q,
@@ -798,9 +798,9 @@ int soupk_embedding_fwd(const void* table, int32_t dtype, const int64_t* ids, vo
  * Its backward: dtable [V, H] of dtype, written whole: scale times the sum of dout's rows (grad_dtype
  * dtype or F32) over each id's tokens in their order, fp32 sums rounded once; zeros for every
  * other row and for padding_idx (-1: none).  Ids outside [0, V) are skipped.  workspace:
- * soupk_embedding_bwd_workspace(M, H) bytes, 16-byte aligned.
+ * soupk_embedding_bwd_workspace(M, V, H) bytes, 16-byte aligned.
  */
-int soupk_embedding_bwd_workspace(int64_t M, int64_t H, int64_t* bytes);
+int soupk_embedding_bwd_workspace(int64_t M, int64_t V, int64_t H, int64_t* bytes);
 int soupk_embedding_bwd(const void* dout, int32_t grad_dtype, const int64_t* ids, void* dtable,
                         int32_t dtype, float scale, int64_t padding_idx, void* workspace,
                         int64_t workspace_bytes, int64_t M, int64_t V, int64_t H, void* stream);

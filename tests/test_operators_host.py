@@ -82,7 +82,7 @@ BAD = [
     ("soupk_qk_norm_rope_fwd", (A, A, None, 2, A, A, A, A, A, A, 0, 4, 1, 4, 2, 1, 128, 1e-6, None)),
     ("soupk_qk_norm_rope_fwd", (A, None, None, 0, A, A, A, A, None, A, 0, 4, 1, 4, 2, 1, 128, 1e-6,
                                 None)),
-    ("soupk_qk_norm_rope_bwd", (A, A, None, 0, A, A, A, A, A, A, A, A, A, 255, 0, 4, 1, 4, 2, 1, 128,
+    ("soupk_qk_norm_rope_bwd", (A, A, None, 0, A, A, A, A, A, A, A, A, A, 127, 0, 4, 1, 4, 2, 1, 128,
                                 1e-6, None)),
     # dropout: limit, two half types, misaligned rows
     ("soupk_dropout", (A, 0, None, A, 0, None, None, 1, 0, -1, 1.0, 4, 4, None)),
@@ -97,7 +97,7 @@ BAD = [
     ("soupk_embedding_bwd", (A, 0, A, A, 0, 1.0, -1, None, 0, 4, 8, 8, None)),
     ("soupk_embedding_bwd", (A, 0, A, A, 0, 1.0, -1, A, 100, 4, 8, 8, None)),
     ("soupk_embedding_bwd", (A, 2, A, A, 0, 1.0, -1, A, 1 << 30, 4, 8, 8, None)),
-    ("soupk_embedding_bwd_workspace", (-1, 8, A)),
+    ("soupk_embedding_bwd_workspace", (-1, 8, 8, A)),
     ("soupk_token_logprobs_workspace", (4, 8, 0, 0, None)),
 ]
 
@@ -128,8 +128,8 @@ def test_workspaces_grow_with_the_work():
         _ext.call(name, *args, ctypes.addressof(need))
         return need.value
 
-    assert size("soupk_embedding_bwd_workspace", 0, 1536) >= 0
-    assert size("soupk_embedding_bwd_workspace", 100, 1536) >= 4 * 4 * 100 + 7 * 2 * 1536 * 4
+    assert size("soupk_embedding_bwd_workspace", 0, 10, 1536) >= 0
+    assert size("soupk_embedding_bwd_workspace", 100, 10, 1536) >= 4 * 4 * 100 + 7 * 2 * 1536 * 4
     assert size("soupk_token_logprobs_workspace", 1, 151936, 20, 0) > 0
     # a part without alternatives keeps its statistics alone
     assert size("soupk_token_logprobs_workspace", 1, 151936, 0, 0) < \

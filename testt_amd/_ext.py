@@ -101,7 +101,7 @@ SIGNATURES = {
                                _i64, _i32, _i32, _i32, _i32, _i32, _f32, _p],
     "soupk_dropout": [_p, _i32, _p, _p, _i32, _p, _p, _i64, _i64, _i64, _f32, _i64, _i64, _p],
     "soupk_embedding_fwd": [_p, _i32, _p, _p, _i32, _f32, _i64, _i64, _i64, _p],
-    "soupk_embedding_bwd_workspace": [_i64, _i64, _p],
+    "soupk_embedding_bwd_workspace": [_i64, _i64, _i64, _p],
     "soupk_embedding_bwd": [_p, _i32, _p, _p, _i32, _f32, _i64, _p, _i64, _i64, _i64, _i64, _p],
     "soupk_layer_fwd": [_p, _p, _p],
     "soupk_layer_bwd": [_p, _p, _p],

@@ -13,7 +13,20 @@ namespace soupk {
 typedef __bf16 bf16;
 
 typedef u32x4 u32x4_a2 __attribute__((aligned(2)));
-typedef f32x4 f32x4_a4 __attribute__((aligned(4)));
+
+// 16 bytes at any even address.
+template <bool NT>
+__device__ __forceinline__ u32x4 ld16(const void* p) {
+  const u32x4_a2* q = static_cast<const u32x4_a2*>(p);
+  if constexpr (NT) return __builtin_nontemporal_load(q);
+  else return *q;
+}
+template <bool NT>
+__device__ __forceinline__ void st16(void* p, u32x4 v) {
+  u32x4_a2* q = static_cast<u32x4_a2*>(p);
+  if constexpr (NT) __builtin_nontemporal_store(v, q);
+  else *q = v;
+}
 
 __device__ __forceinline__ float bf2f(uint32_t bits16) {
   return __builtin_bit_cast(float, bits16 << 16);
@@ -41,7 +54,7 @@ struct Elem16 {
   };
   template <bool NT>
   static __device__ __forceinline__ Raw8 load8(const void* p) {
-    return {ld<NT>(static_cast<const u32x4_a2*>(p))};
+    return {ld16<NT>(p)};
   }
 };
 
@@ -56,7 +69,7 @@ struct Elem<f16> : Elem16<f16> {
   static __device__ __forceinline__ void store8(void* p, const float* v) {
     const u32x4 w = {pack_h2(v[0], v[1]), pack_h2(v[2], v[3]), pack_h2(v[4], v[5]),
                      pack_h2(v[6], v[7])};
-    st<NT>(static_cast<u32x4_a2*>(p), static_cast<u32x4_a2>(w));
+    st16<NT>(p, w);
   }
   static __device__ __forceinline__ float load1(const void* p) {
     return h2f(*static_cast<const uint16_t*>(p));
@@ -79,7 +92,7 @@ struct Elem<bf16> : Elem16<bf16> {
   static __device__ __forceinline__ void store8(void* p, const float* v) {
     const u32x4 w = {pack_b2(v[0], v[1]), pack_b2(v[2], v[3]), pack_b2(v[4], v[5]),
                      pack_b2(v[6], v[7])};
-    st<NT>(static_cast<u32x4_a2*>(p), static_cast<u32x4_a2>(w));
+    st16<NT>(p, w);
   }
   static __device__ __forceinline__ float load1(const void* p) {
     return bf2f(*static_cast<const uint16_t*>(p));
@@ -97,8 +110,8 @@ struct Elem<float> {
   };
   template <bool NT>
   static __device__ __forceinline__ Raw8 load8(const void* p) {
-    const f32x4_a4* q = static_cast<const f32x4_a4*>(p);
-    return {ld<NT>(q), ld<NT>(q + 1)};
+    const char* q = static_cast<const char*>(p);
+    return {__builtin_bit_cast(f32x4, ld16<NT>(q)), __builtin_bit_cast(f32x4, ld16<NT>(q + 16))};
   }
   static __device__ __forceinline__ void unpack8(const Raw8& r, float* v) {
     v[0] = r.a.x; v[1] = r.a.y; v[2] = r.a.z; v[3] = r.a.w;
@@ -106,9 +119,9 @@ struct Elem<float> {
   }
   template <bool NT>
   static __device__ __forceinline__ void store8(void* p, const float* v) {
-    f32x4_a4* q = static_cast<f32x4_a4*>(p);
-    st<NT>(q, static_cast<f32x4_a4>(f32x4{v[0], v[1], v[2], v[3]}));
-    st<NT>(q + 1, static_cast<f32x4_a4>(f32x4{v[4], v[5], v[6], v[7]}));
+    char* q = static_cast<char*>(p);
+    st16<NT>(q, __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]}));
+    st16<NT>(q + 16, __builtin_bit_cast(u32x4, f32x4{v[4], v[5], v[6], v[7]}));
   }
   static __device__ __forceinline__ float load1(const void* p) {
     return *static_cast<const float*>(p);

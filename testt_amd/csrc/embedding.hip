@@ -10,15 +10,20 @@
 //
 //   sort    least-significant-digit radix sort of (id, token) by 9-bit digits, ranks from wavefront
 //           ballots.  Up to kOneBlock tokens are sorted by one workgroup in one launch; more tokens
-//           by up to kMaxBlocks workgroups, a histogram and a scatter launch per digit.
-//   sums    the sorted tokens are cut every kRun positions.  A workgroup adds the rows of its run, in
-//           order, and writes a table row for each id that lies within the run; an id that continues
-//           past an end of the run leaves a partial fp32 row instead.
+//           by up to kMaxBlocks workgroups, a histogram and a scatter launch per digit.  The last pass
+//           also notes, per id, the sorted place of one of its tokens.
+//   write   the sorted tokens are cut into runs.  A workgroup adds the rows of its run, in order, and
+//           writes a table row for each id that lies within the run; an id that continues past an end
+//           of the run leaves a partial fp32 row instead.  All other workgroups write zeros, 16 bytes
+//           a thread, to the rows that no token names.
 //   join    the partial rows of an id that spans runs are added in run order and written.
 //
 // The whole table gradient has to be written once (467 MB of fp16 at 151936 x 1536), which is by far
-// the largest part of the traffic: the launches of the sort carry workgroups that write its zeros,
-// and only the rows of the ids that occur are written again by the sums.
+// the largest part of the traffic.  Whether a row is named needs no cleared flags: the noted place is
+// looked up, whatever the memory holds, and counts only if the sorted id there is the row.  The sort's
+// launches, which leave the chip idle, carry zeros for the first rows of the table.
+// Zeros go out as one 16-byte store per thread: 467 MB took 70 us that way on MI355X, 84 us with four
+// stores a thread, 95 - 115 us from a grid of resident workgroups.
 
 #include <algorithm>
 #include <type_traits>
@@ -66,26 +71,19 @@ constexpr int kDigitBits = 9;
 constexpr int kDigits = 1 << kDigitBits;
 constexpr int kMaxBlocks = 64;
 constexpr int64_t kOneBlock = 4096;    // tokens that one workgroup sorts alone
-constexpr int kRun = 16;               // sorted positions that one workgroup adds
+constexpr int64_t kHidden = 48 << 20;  // bytes of zeros that a launch of the sort carries
 
-struct Zeros {         // the table gradient, cleared in pieces by extra workgroups
+// Sorted positions that one workgroup adds: few when there are few tokens, so that the chip is filled.
+__host__ __device__ constexpr int run_length(int64_t M) { return M <= kOneBlock ? 8 : 32; }
+
+struct Zeros {         // 16-byte words of the table gradient, cleared by extra workgroups
   char* base;
-  int64_t bytes;       // this launch's piece: [first, first + count) 16-byte words, then the tail
-  int64_t first, count;
-  bool tail;           // also the bytes past the last whole word
+  int64_t count;
 };
 
-__device__ __forceinline__ void write_zeros(const Zeros& z, int64_t block, int64_t blocks) {
-  const u32x4 zero = {0u, 0u, 0u, 0u};
-  u32x4_a2* p = reinterpret_cast<u32x4_a2*>(z.base) + z.first;
-  const int64_t step = blocks * kSortThreads;
-  for (int64_t i = block * kSortThreads + threadIdx.x; i < z.count; i += step)
-    st<true>(p + i, static_cast<u32x4_a2>(zero));
-  if (z.tail && block == 0) {
-    const int64_t done = z.bytes & ~int64_t{15};
-    if (threadIdx.x < (z.bytes - done) / 2)
-      *reinterpret_cast<uint16_t*>(z.base + done + 2 * threadIdx.x) = 0;
-  }
+__device__ __forceinline__ void write_zeros(const Zeros& z, int64_t block) {
+  const int64_t i = block * kSortThreads + threadIdx.x;
+  if (i < z.count) st16<true>(z.base + 16 * i, u32x4{0u, 0u, 0u, 0u});
 }
 
 // The id a token sorts by: V (behind every row) for an id that gets no gradient.
@@ -119,11 +117,12 @@ __device__ __forceinline__ void scan_digits(SortLds& s, uint32_t total) {
 }
 
 // Moves the tokens [t0, t1) to their places by the digit at `shift`; s.base holds, per digit, the
-// place of the workgroup's first token of it.  s.count is clear and left clear.
+// place of the workgroup's first token of it.  s.count is clear and left clear.  place: in the last
+// pass, where each id's place is noted.
 template <typename Load>
 __device__ __forceinline__ void scatter_tokens(SortLds& s, int64_t t0, int64_t t1, int shift,
                                                uint32_t* out_key, uint32_t* out_tok,
-                                               const Load& load) {
+                                               uint32_t* place, int64_t V, const Load& load) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   for (int64_t t = t0; t < t1; t += kSortThreads) {
     const int64_t i = t + threadIdx.x;
@@ -156,6 +155,8 @@ __device__ __forceinline__ void scatter_tokens(SortLds& s, int64_t t0, int64_t t
       const uint32_t to = s.count[w][digit] + rank;
       out_key[to] = key;
       out_tok[to] = tok;
+      // (any token's place will do: of an id's several writers any may win)
+      if (place != nullptr && key < static_cast<uint32_t>(V)) place[key] = to;
     }
     __syncthreads();
 #pragma unroll
@@ -177,9 +178,9 @@ __device__ __forceinline__ void clear_counts(SortLds& s) {
 // sorted pairs end in key[0] / tok[0] for an even number of passes, else in key[1] / tok[1].
 __global__ __launch_bounds__(kSortThreads) void embedding_sort_small_kernel(
     const int64_t* __restrict__ ids, int64_t M, int64_t V, int64_t padding, int passes,
-    uint32_t* key0, uint32_t* tok0, uint32_t* key1, uint32_t* tok1, Zeros z) {
+    uint32_t* key0, uint32_t* tok0, uint32_t* key1, uint32_t* tok1, uint32_t* place, Zeros z) {
   if (blockIdx.x > 0) {
-    write_zeros(z, blockIdx.x - 1, gridDim.x - 1);
+    write_zeros(z, blockIdx.x - 1);
     return;
   }
   __shared__ SortLds s;
@@ -207,7 +208,7 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_small_kernel(
     __syncthreads();
     if (threadIdx.x < kDigits) s.count[0][threadIdx.x] = 0;
     scan_digits(s, total);
-    scatter_tokens(s, 0, M, shift, ok, ot, load);
+    scatter_tokens(s, 0, M, shift, ok, ot, p == passes - 1 ? place : nullptr, V, load);
     __threadfence_block();
     __syncthreads();
   }
@@ -218,7 +219,7 @@ __global__ __launch_bounds__(kSortThreads) void embedding_hist_kernel(
     const int64_t* __restrict__ ids, const uint32_t* __restrict__ in_key, int64_t M, int64_t V,
     int64_t padding, int shift, int blocks, int64_t per, uint32_t* __restrict__ hist, Zeros z) {
   if (static_cast<int>(blockIdx.x) >= blocks) {
-    write_zeros(z, blockIdx.x - blocks, gridDim.x - blocks);
+    write_zeros(z, blockIdx.x - blocks);
     return;
   }
   __shared__ uint32_t count[kDigits];
@@ -238,9 +239,9 @@ __global__ __launch_bounds__(kSortThreads) void embedding_scatter_kernel(
     const int64_t* __restrict__ ids, const uint32_t* __restrict__ in_key,
     const uint32_t* __restrict__ in_tok, int64_t M, int64_t V, int64_t padding, int shift,
     int blocks, int64_t per, const uint32_t* __restrict__ hist, uint32_t* __restrict__ out_key,
-    uint32_t* __restrict__ out_tok, Zeros z) {
+    uint32_t* __restrict__ out_tok, uint32_t* __restrict__ place, Zeros z) {
   if (static_cast<int>(blockIdx.x) >= blocks) {
-    write_zeros(z, blockIdx.x - blocks, gridDim.x - blocks);
+    write_zeros(z, blockIdx.x - blocks);
     return;
   }
   __shared__ SortLds s;
@@ -257,7 +258,8 @@ __global__ __launch_bounds__(kSortThreads) void embedding_scatter_kernel(
   __syncthreads();
   scan_digits(s, total);
   const int64_t t0 = blockIdx.x * per, t1 = min(M, t0 + per);
-  scatter_tokens(s, t0, t1, shift, out_key, out_tok, [&](int64_t i, uint32_t& k, uint32_t& t) {
+  scatter_tokens(s, t0, t1, shift, out_key, out_tok, place, V,
+                 [&](int64_t i, uint32_t& k, uint32_t& t) {
     if (in_key == nullptr) {
       k = sort_key(ids[i], V, padding);
       t = static_cast<uint32_t>(i);
@@ -295,18 +297,59 @@ __device__ __forceinline__ void store_row(char* dst, int n, const float* v, floa
   }
 }
 
-// Workgroup (run, column block): the kRun sorted positions from run * kRun on.  partial holds two
-// rows of H8 floats per run: of the id that entered the run, and of the id that leaves it (an id that
-// does both leaves its sum in the first).
+// The first `sums` workgroups: (run, column block), the run's sorted positions; the others: zeros.
+// partial holds two rows of H8 floats per run: of the id that entered the run, and of the id that
+// leaves it (an id that does both leaves its sum in the first).
+struct Cut {
+  int run;                    // positions per run
+  int64_t sums;               // workgroups that add
+  int col_blocks;             // per run
+  int64_t zero_row0;          // rows before it were cleared with the sort
+  uint32_t zero_items;        // 16-byte items (of a row) of this launch
+  FastDiv per_row;            // items of a row
+};
+
+template <typename E>
+__device__ __forceinline__ void zero_rows(char* dtable, const uint32_t* key, const uint32_t* place,
+                                          int64_t M, int64_t H, const Cut& cut) {
+  constexpr int N = 16 / Elem<E>::kBytes;
+  const uint32_t i =
+      static_cast<uint32_t>(blockIdx.x - cut.sums) * kEmbThreads + threadIdx.x;
+  if (i >= cut.zero_items) return;
+  const uint32_t r = cut.per_row.div(i);
+  const int64_t row = cut.zero_row0 + r;
+  const int64_t col = static_cast<int64_t>(i - r * cut.per_row.d) * N;
+  if (M > 0) {
+    const uint32_t p = place[row];
+    if (p < M && key[p] == static_cast<uint32_t>(row)) return;
+  }
+  char* const to = dtable + (row * H + col) * Elem<E>::kBytes;
+  if (col + N <= H) {
+    st16<true>(to, u32x4{0u, 0u, 0u, 0u});
+  } else {
+    for (int j = 0; j < H - col; ++j) Elem<E>::store1(to + j * Elem<E>::kBytes, 0.f);
+  }
+}
+
+constexpr int kSumAhead = 4;   // gradient rows in flight per thread
+
 template <typename G, typename E>
-__global__ __launch_bounds__(kEmbThreads) void embedding_sum_kernel(
+__global__ __launch_bounds__(kEmbThreads) void embedding_write_kernel(
     const char* __restrict__ dout, const uint32_t* __restrict__ key,
-    const uint32_t* __restrict__ tok, char* __restrict__ dtable, float* __restrict__ partial,
-    float scale, int64_t M, int64_t V, int64_t H, int64_t H8) {
-  const int64_t col = (static_cast<int64_t>(blockIdx.y) * kEmbThreads + threadIdx.x) * 8;
+    const uint32_t* __restrict__ tok, const uint32_t* __restrict__ place,
+    char* __restrict__ dtable, float* __restrict__ partial, float scale, int64_t M, int64_t V,
+    int64_t H, int64_t H8, Cut cut) {
+  if (static_cast<int64_t>(blockIdx.x) >= cut.sums) {
+    zero_rows<E>(dtable, key, place, M, H, cut);
+    return;
+  }
+  const int64_t run = blockIdx.x / static_cast<uint32_t>(cut.col_blocks);
+  const int64_t col =
+      (static_cast<int64_t>(blockIdx.x % static_cast<uint32_t>(cut.col_blocks)) * kEmbThreads +
+       threadIdx.x) * 8;
   if (col >= H) return;
   const int n = static_cast<int>(min(int64_t{8}, H - col));
-  const int64_t p0 = static_cast<int64_t>(blockIdx.x) * kRun, p1 = min(M, p0 + kRun);
+  const int64_t p0 = run * cut.run, p1 = min(M, p0 + cut.run);
   const uint32_t none = static_cast<uint32_t>(V);
   uint32_t id = key[p0];
   if (id == none) return;                        // (and all that follow)
@@ -314,7 +357,7 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_sum_kernel(
   float acc[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-  float* const mine = partial + static_cast<int64_t>(blockIdx.x) * 2 * H8 + col;
+  float* const mine = partial + run * 2 * H8 + col;
   auto put_partial = [&](float* to) {
     *reinterpret_cast<f32x4*>(to) = f32x4{acc[0], acc[1], acc[2], acc[3]};
     *reinterpret_cast<f32x4*>(to + 4) = f32x4{acc[4], acc[5], acc[6], acc[7]};
@@ -322,21 +365,30 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_sum_kernel(
   auto put_row = [&]() {
     store_row<E>(dtable + (static_cast<int64_t>(id) * H + col) * Elem<E>::kBytes, n, acc, scale);
   };
-  for (int64_t p = p0; p < p1; ++p) {
-    const uint32_t k = key[p];
-    if (k != id) {
-      if (entered) put_partial(mine);
-      else put_row();
-      id = k;
-      entered = false;
-      if (k == none) return;
+  for (int64_t p = p0; p < p1; p += kSumAhead) {
+    float v[kSumAhead][8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+    for (int u = 0; u < kSumAhead; ++u) {
+      // (past the run: its last row, unused)
+      const int64_t t = tok[min(p + u, p1 - 1)];
+      load_grad<G>(dout + (t * H + col) * Elem<G>::kBytes, n, v[u]);
     }
-    float v[8];
-    load_grad<G>(dout + (static_cast<int64_t>(tok[p]) * H + col) * Elem<G>::kBytes, n, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = acc[j] + v[j];
+    for (int u = 0; u < kSumAhead; ++u) {
+      if (p + u >= p1) break;
+      const uint32_t k = key[p + u];
+      if (k != id) {
+        if (entered) put_partial(mine);
+        else put_row();
+        id = k;
+        entered = false;
+        if (k == none) return;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] = acc[j] + v[u][j];
+    }
   }
   const bool leaves = p1 < M && key[p1] == id;
   if (entered) put_partial(mine);
@@ -344,18 +396,21 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_sum_kernel(
   else put_row();
 }
 
-// Workgroup (run, column block): the id that leaves the run, if it began in it: its partial rows in
-// run order.
+// Workgroup (run, column block of 64 x 8): the id that leaves the run, if it began in it.  Its partial
+// rows are added in run order by four groups, each a quarter of them, joined in their order.
+constexpr int kJoinCols = kWave * 8;
+constexpr int kJoinGroups = kEmbThreads / kWave;
 template <typename E>
 __global__ __launch_bounds__(kEmbThreads) void embedding_join_kernel(
     const uint32_t* __restrict__ key, const float* __restrict__ partial, char* __restrict__ dtable,
-    float scale, int64_t M, int64_t V, int64_t H, int64_t H8) {
-  const int64_t run = blockIdx.x;
-  const int64_t p0 = run * kRun, p1 = p0 + kRun;
+    float scale, int64_t M, int64_t V, int64_t H, int64_t H8, int run_len, int col_blocks) {
+  __shared__ float sum[kJoinGroups][kJoinCols];
+  const int64_t run = blockIdx.x / static_cast<uint32_t>(col_blocks);
+  const int64_t p0 = run * run_len, p1 = p0 + run_len;
   if (p1 >= M) return;
   const uint32_t id = key[p1 - 1];
   if (id == static_cast<uint32_t>(V) || key[p1] != id) return;
-  if (p0 > 0 && key[p0 - 1] == id) return;       // (began before: key is sorted)
+  if (p0 > 0 && key[p0 - 1] == id) return;       // (began before: the keys are sorted)
   // one past the last position of the id
   int64_t lo = p1, hi = M;
   while (lo < hi) {
@@ -363,35 +418,56 @@ __global__ __launch_bounds__(kEmbThreads) void embedding_join_kernel(
     if (key[mid] <= id) lo = mid + 1;
     else hi = mid;
   }
-  const int64_t last = (lo - 1) / kRun;
-  const int64_t col = (static_cast<int64_t>(blockIdx.y) * kEmbThreads + threadIdx.x) * 8;
-  if (col >= H) return;
-  const int n = static_cast<int>(min(int64_t{8}, H - col));
+  const int64_t last = (lo - 1) / run_len;
+  const int lane = threadIdx.x % kWave, group = threadIdx.x / kWave;
+  const int64_t col =
+      static_cast<int64_t>(blockIdx.x % static_cast<uint32_t>(col_blocks)) * kJoinCols + lane * 8;
+  const bool on = col < H;
+  const int64_t per = (last - run + kJoinGroups - 1) / kJoinGroups;
+  const int64_t r0 = run + 1 + group * per, r1 = min(last + 1, r0 + per);
   float acc[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[j] = 0.f;
+  if (on) {
+#pragma unroll 4
+    for (int64_t r = r0; r < r1; ++r) {
+      const f32x4* row = reinterpret_cast<const f32x4*>(partial + r * 2 * H8 + col);
+      const f32x4 a = row[0], b = row[1];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        acc[j] = acc[j] + a[j];
+        acc[4 + j] = acc[4 + j] + b[j];
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sum[group][lane * 8 + j] = acc[j];
+  __syncthreads();
+  if (group != 0 || !on) return;
   const float* first = partial + run * 2 * H8 + H8 + col;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) acc[j] = first[j];
-  for (int64_t r = run + 1; r <= last; ++r) {
-    const float* row = partial + r * 2 * H8 + col;
+  for (int j = 0; j < 8; ++j) {
+    acc[j] = first[j];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] = acc[j] + row[j];
+    for (int g = 0; g < kJoinGroups; ++g) acc[j] = acc[j] + sum[g][lane * 8 + j];
   }
-  store_row<E>(dtable + (static_cast<int64_t>(id) * H + col) * Elem<E>::kBytes, n, acc, scale);
+  store_row<E>(dtable + (static_cast<int64_t>(id) * H + col) * Elem<E>::kBytes,
+               static_cast<int>(min(int64_t{8}, H - col)), acc, scale);
 }
 
 int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
-// Workspace of a backward: sorted keys and tokens twice, the histograms, the partial rows.
+// Workspace of a backward: sorted keys and tokens twice, the histograms, the places, the partial rows.
 struct Layout {
-  int64_t pairs, hist, partial, bytes;   // byte offsets; the total
+  int64_t hist, place, partial, bytes;   // byte offsets; the total
 };
-Layout emb_layout(int64_t M, int64_t H) {
+Layout emb_layout(int64_t M, int64_t V, int64_t H) {
   Layout l;
-  l.pairs = 0;
-  const int64_t m4 = round_up(M * 4, 256);
-  l.hist = 4 * m4;
-  l.partial = l.hist + int64_t{kDigits} * kMaxBlocks * 4;
-  l.bytes = l.partial + (M + kRun - 1) / kRun * 2 * round_up(H, 8) * 4;
+  l.hist = 4 * round_up(M * 4, 256);
+  l.place = l.hist + int64_t{kDigits} * kMaxBlocks * 4;
+  l.partial = l.place + round_up(V * 4, 256);
+  const int run = run_length(M);
+  l.bytes = l.partial + (M + run - 1) / run * 2 * round_up(H, 8) * 4;
   return l;
 }
 
@@ -442,9 +518,9 @@ extern "C" __attribute__((visibility("default"))) int soupk_embedding_fwd(
 }
 
 extern "C" __attribute__((visibility("default"))) int soupk_embedding_bwd_workspace(
-    int64_t M, int64_t H, int64_t* bytes) {
-  if (bad_sizes(M, 0, H) || bytes == nullptr) return kInvalid;
-  *bytes = emb_layout(M, H).bytes;
+    int64_t M, int64_t V, int64_t H, int64_t* bytes) {
+  if (bad_sizes(M, V, H) || bytes == nullptr) return kInvalid;
+  *bytes = emb_layout(M, V, H).bytes;
   return kOk;
 }
 
@@ -456,7 +532,7 @@ extern "C" __attribute__((visibility("default"))) int soupk_embedding_bwd(
   if (dtype != grad_dtype && grad_dtype != SOUPK_DTYPE_F32) return kInvalid;
   if (V == 0 || H == 0) return kOk;
   if (bad_elem_ptr(dtable, dtype)) return kInvalid;
-  const Layout l = emb_layout(M, H);
+  const Layout l = emb_layout(M, V, H);
   if (M > 0) {
     if (bad_elem_ptr(dout, grad_dtype) || !ids || (reinterpret_cast<uintptr_t>(ids) & 7u))
       return kInvalid;
@@ -464,72 +540,91 @@ extern "C" __attribute__((visibility("default"))) int soupk_embedding_bwd(
       return kInvalid;
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int64_t table_bytes = V * H * (dtype == SOUPK_DTYPE_F32 ? 4 : 2);
-  const int64_t words = table_bytes / 16;
-  const int cus = device_cu_count();
-  // The launches that come before the sums, each with its share of the zeros.
+  const int64_t row_bytes = H * (dtype == SOUPK_DTYPE_F32 ? 4 : 2);
   int bits = 0;
   while ((V >> bits) != 0) ++bits;
   const int passes = (bits + kDigitBits - 1) / kDigitBits;
   const bool small = M <= kOneBlock;
-  const int launches = small ? 1 : 2 * passes;
+  const int launches = M == 0 ? 0 : small ? 1 : 2 * passes;
+  // The rows cleared with the sort: a multiple of 8 per launch (whole 16-byte words).
+  const int64_t hidden_rows =
+      launches ? std::min<int64_t>(kHidden / row_bytes, V / launches) / 8 * 8 : 0;
   auto zeros = [&](int k) {
-    const int64_t a = words * k / launches, b = words * (k + 1) / launches;
-    return Zeros{static_cast<char*>(dtable), table_bytes, a, b - a, k == 0};
+    return Zeros{static_cast<char*>(dtable) + k * hidden_rows * row_bytes,
+                 hidden_rows * row_bytes / 16};
   };
-  auto zero_blocks = [&](const Zeros& z) {
-    return static_cast<int>(std::max<int64_t>(
-        1, std::min<int64_t>((z.count + kSortThreads - 1) / kSortThreads, 4 * cus)));
-  };
+  const int zero_blocks =
+      static_cast<int>((hidden_rows * row_bytes / 16 + kSortThreads - 1) / kSortThreads);
   char* const ws = static_cast<char*>(workspace);
   const int64_t m4 = round_up(M * 4, 256);
   uint32_t* const key[2] = {reinterpret_cast<uint32_t*>(ws), reinterpret_cast<uint32_t*>(ws + m4)};
   uint32_t* const tok[2] = {reinterpret_cast<uint32_t*>(ws + 2 * m4),
                             reinterpret_cast<uint32_t*>(ws + 3 * m4)};
-  int rc;
-  if (small) {
-    const Zeros z = zeros(0);
-    rc = launch_kernel(embedding_sort_small_kernel, dim3(1 + zero_blocks(z)), dim3(kSortThreads), s,
-                       ids, M, V, padding_idx, M > 0 ? passes : 0, key[0], tok[0], key[1], tok[1],
-                       z);
+  uint32_t* const place = reinterpret_cast<uint32_t*>(ws + l.place);
+  if (M > 0 && small) {
+    const int rc = launch_kernel(embedding_sort_small_kernel, dim3(1 + zero_blocks),
+                                 dim3(kSortThreads), s, ids, M, V, padding_idx, passes, key[0],
+                                 tok[0], key[1], tok[1], place, zeros(0));
     if (rc != kOk) return rc;
-  } else {
+  } else if (M > 0) {
     const int64_t per = round_up((M + kMaxBlocks - 1) / kMaxBlocks, kSortThreads);
     const int blocks = static_cast<int>((M + per - 1) / per);
     uint32_t* const hist = reinterpret_cast<uint32_t*>(ws + l.hist);
     for (int p = 0; p < passes; ++p) {
       const uint32_t* const in_key = p ? key[p & 1] : nullptr;
       const uint32_t* const in_tok = p ? tok[p & 1] : nullptr;
-      const Zeros z0 = zeros(2 * p), z1 = zeros(2 * p + 1);
-      rc = launch_kernel(embedding_hist_kernel, dim3(blocks + zero_blocks(z0)), dim3(kSortThreads),
-                         s, ids, in_key, M, V, padding_idx, p * kDigitBits, blocks, per, hist, z0);
+      int rc = launch_kernel(embedding_hist_kernel, dim3(blocks + zero_blocks), dim3(kSortThreads),
+                             s, ids, in_key, M, V, padding_idx, p * kDigitBits, blocks, per, hist,
+                             zeros(2 * p));
       if (rc != kOk) return rc;
-      rc = launch_kernel(embedding_scatter_kernel, dim3(blocks + zero_blocks(z1)),
-                         dim3(kSortThreads), s, ids, in_key, in_tok, M, V, padding_idx,
-                         p * kDigitBits, blocks, per, static_cast<const uint32_t*>(hist),
-                         key[(p + 1) & 1], tok[(p + 1) & 1], z1);
+      rc = launch_kernel(embedding_scatter_kernel, dim3(blocks + zero_blocks), dim3(kSortThreads),
+                         s, ids, in_key, in_tok, M, V, padding_idx, p * kDigitBits, blocks, per,
+                         static_cast<const uint32_t*>(hist), key[(p + 1) & 1], tok[(p + 1) & 1],
+                         p == passes - 1 ? place : nullptr, zeros(2 * p + 1));
       if (rc != kOk) return rc;
     }
   }
-  if (M == 0) return kOk;
   const uint32_t* const skey = key[passes & 1];
   const uint32_t* const stok = tok[passes & 1];
   float* const partial = reinterpret_cast<float*>(ws + l.partial);
   const int64_t H8 = round_up(H, 8);
-  const dim3 grid(static_cast<unsigned>((M + kRun - 1) / kRun),
-                  static_cast<unsigned>((H8 / 8 + kEmbThreads - 1) / kEmbThreads));
+  const int run = run_length(M);
+  const int64_t runs = (M + run - 1) / run;
+  const int col_blocks = static_cast<int>((H8 / 8 + kEmbThreads - 1) / kEmbThreads);
+  if (runs * col_blocks > (int64_t{1} << 30)) return kInvalid;
+  const int64_t row_items = (row_bytes + 15) / 16;
+  const int64_t rows_per =
+      std::max<int64_t>(1, ((int64_t{1} << 30) - kEmbThreads) / row_items);
   return with_type(grad_dtype, [&](auto gt) {
     return with_type(dtype, [&](auto et) -> int {
       using G = typename decltype(gt)::type;
       using E = typename decltype(et)::type;
       if constexpr (std::is_same_v<G, E> || std::is_same_v<G, float>) {
-        int st = launch_kernel(embedding_sum_kernel<G, E>, grid, dim3(kEmbThreads), s,
-                               static_cast<const char*>(dout), skey, stok,
-                               static_cast<char*>(dtable), partial, scale, M, V, H, H8);
-        if (st != kOk) return st;
-        return launch_kernel(embedding_join_kernel<E>, grid, dim3(kEmbThreads), s, skey,
-                             static_cast<const float*>(partial), static_cast<char*>(dtable), scale,
-                             M, V, H, H8);
+        // (one launch, unless the table's items do not fit 32 bits)
+        int64_t row = launches * hidden_rows;
+        Cut cut{run, runs * col_blocks, col_blocks, 0, 0, FastDiv(static_cast<uint32_t>(row_items))};
+        do {
+          const int64_t n = std::min(rows_per, V - row);
+          cut.zero_row0 = row;
+          cut.zero_items = static_cast<uint32_t>(n * row_items);
+          const int64_t grid = cut.sums + (cut.zero_items + kEmbThreads - 1) / kEmbThreads;
+          if (grid > 0) {
+            const int st = launch_kernel(
+                embedding_write_kernel<G, E>, dim3(static_cast<unsigned>(grid)), dim3(kEmbThreads),
+                s, static_cast<const char*>(dout), skey, stok,
+                static_cast<const uint32_t*>(place), static_cast<char*>(dtable), partial, scale, M,
+                V, H, H8, cut);
+            if (st != kOk) return st;
+          }
+          row += n;
+          cut.sums = 0;
+        } while (row < V);
+        if (M == 0) return kOk;
+        const int join_blocks = static_cast<int>((H + kJoinCols - 1) / kJoinCols);
+        return launch_kernel(embedding_join_kernel<E>,
+                             dim3(static_cast<unsigned>(runs * join_blocks)), dim3(kEmbThreads), s,
+                             skey, static_cast<const float*>(partial), static_cast<char*>(dtable),
+                             scale, M, V, H, H8, run, join_blocks);
       } else {
         return kInvalid;
       }

@@ -260,7 +260,7 @@ struct QkNorm : Function<QkNorm> {
       Tensor dqkv = empty(qkv.sizes(), qkv.scalar_type(), dev), dwq, dwk, ws;
       if (n[7]) dwq = empty({hd}, at::kFloat, dev);
       if (n[8]) dwk = empty({hd}, at::kFloat, dev);
-      const int64_t floats = n[7] || n[8] ? int64_t{SOUPK_QK_NORM_BLOCKS} * 2 * hd : 0;
+      const int64_t floats = n[7] || n[8] ? int64_t{SOUPK_QK_NORM_BLOCKS} * hd : 0;
       if (floats > 0) ws = empty({floats}, at::kFloat, dev);
       const int32_t code = code_of(qkv.scalar_type());
       check("soupk_qk_norm_rope_bwd",
@@ -374,7 +374,7 @@ struct Embedding : Function<Embedding> {
       if (dtable.numel() > 0) {
         int64_t need = 0;
         check("soupk_embedding_bwd_workspace",
-              p_soupk_embedding_bwd_workspace(tokens, width, &need));
+              p_soupk_embedding_bwd_workspace(tokens, vocab, width, &need));
         Tensor ws = empty({need}, at::kByte, dout.device());
         check("soupk_embedding_bwd",
               p_soupk_embedding_bwd(address(dout), code_of(dout.scalar_type()),

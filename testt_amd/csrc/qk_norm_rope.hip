@@ -10,15 +10,16 @@
 // All in fp32, one rounding to the rows' type at the store; x and r are formed again in the
 // backward from the rows it has to read anyway, so nothing is kept of the forward.
 //
-// Mapping: a head is a group of G = 2^k lanes, each with 8 dims of the first half and the 8 dims of
+// Mapping (forward): a head is a group of G = 2^k lanes, each with 8 dims of the first half and the 8 dims of
 // the second half they rotate with, so the rotation is inside a lane and the mean of squares one
 // DPP reduction of at most 16 lanes.  A wavefront takes 64 / G neighbouring heads of one token (8
 // at D = 128): its loads and stores are whole rows of 2 KiB.  The token's cos / sin and the weight
 // come from the caches.
 //
-// The weights' gradients are sums over all tokens: every lane adds its dims over the heads that it
-// visits, a workgroup adds its lanes in LDS and writes one partial row, and a second launch adds the
-// partials in workgroup order (no atomics: the same result every time).
+// The weights' gradients are sums over all tokens: in the backward a workgroup keeps to query heads or
+// to key heads, every lane adds its dims over the heads that it visits, the workgroup adds its lanes
+// in LDS and writes one partial row, and a second launch adds the partials in workgroup order (no
+// atomics: the same result every time).
 
 #include <algorithm>
 #include <type_traits>
@@ -86,10 +87,7 @@ __device__ __forceinline__ Place place(uint32_t item, const NormDims& dm, const 
 }
 
 __device__ __forceinline__ void load8f(const float* p, float* v) {
-  const f32x4_a4* q = reinterpret_cast<const f32x4_a4*>(p);
-  const f32x4 a = q[0], b = q[1];
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  Elem<float>::unpack8(Elem<float>::load8<false>(p), v);
 }
 
 template <typename T>
@@ -163,45 +161,77 @@ __global__ __launch_bounds__(kNormThreads) void qk_norm_rope_fwd_kernel(
   Elem<T>::template store8<true>(out + (p.at + half) * Elem<T>::kBytes, b);
 }
 
+// Workgroups [0, q_blocks) take the query heads (tokens * NH of them in order, q_per each), the others
+// the key heads and, with each, the value head of the same number, whose gradient passes through.  So
+// a lane needs one weight's sums only, and the weight stays in registers.
+struct NormSplit {
+  int q_blocks;
+  uint32_t q_per, kv_per;      // heads of a workgroup
+  FastDiv by_q, by_kv;         // divide by NH, NKV
+};
+
 template <typename T, int G, bool DW>
 __global__ __launch_bounds__(kNormThreads) void qk_norm_rope_bwd_kernel(
     const char* __restrict__ dout, const char* __restrict__ qkv, const char* __restrict__ lora_q,
     bool lora_f32, const float* __restrict__ wq, const float* __restrict__ wk,
     const float* __restrict__ cos_t, const float* __restrict__ sin_t,
     const int64_t* __restrict__ pos, char* __restrict__ dqkv, float* __restrict__ partial,
-    float eps, NormDims dm, uint32_t items) {
+    float eps, NormDims dm, NormSplit sp) {
+  constexpr int kSlots = kNormThreads / G;               // heads at a time
   const int half = dm.D >> 1;
-  const int c = (threadIdx.x & 63) % G;
-  float acc[32];     // [q: first half, second half | k: first half, second half]
-  if constexpr (DW) {
+  const int c = threadIdx.x % G, slot = threadIdx.x / G;
+  const bool is_q = static_cast<int>(blockIdx.x) < sp.q_blocks;
+  const FastDiv by = is_q ? sp.by_q : sp.by_kv;
+  const uint32_t per = is_q ? sp.q_per : sp.kv_per;
+  const uint32_t start = (is_q ? blockIdx.x : blockIdx.x - sp.q_blocks) * per;
+  const uint32_t total = static_cast<uint32_t>(dm.rows) * by.d;
+  const uint32_t end = min(total, start + per);
+  const int heads = dm.NH + 2 * dm.NKV;
+  const bool dims = 16 * c < dm.D;
+  const float inv_d = static_cast<float>(dm.D);
+  float w1[8], w2[8], acc1[8], acc2[8];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) acc[j] = 0.f;
+  for (int j = 0; j < 8; ++j) w1[j] = w2[j] = acc1[j] = acc2[j] = 0.f;
+  if (dims) {
+    load8f((is_q ? wq : wk) + 8 * c, w1);
+    load8f((is_q ? wq : wk) + 8 * c + half, w2);
   }
-  const uint32_t stride = gridDim.x * kNormWaves;
-  for (uint32_t item = blockIdx.x * kNormWaves + (threadIdx.x >> 6); item < items;
-       item += stride) {
-    const Place p = place<G>(item, dm, cos_t, sin_t, pos);
+  for (uint32_t i0 = start; i0 < end; i0 += kSlots) {
+    const uint32_t i = i0 + slot;
+    const bool live = i < end && dims;
+    const uint32_t tok = by.div(live ? i : i0);
+    const int h = static_cast<int>((live ? i : i0) - tok * by.d);
+    const int64_t ps = pos[tok];
+    const bool known = ps >= 0 && ps < dm.slots;
+    const uint32_t pu = known ? static_cast<uint32_t>(ps) : 0u;
+    const uint32_t t = pu - dm.per_seq.div(pu) * dm.per_seq.d;
+    const int64_t at =
+        (static_cast<int64_t>(tok) * heads + (is_q ? h : dm.NH + h)) * dm.D + 8 * c;
+    const int64_t at_v = at + static_cast<int64_t>(dm.NKV) * dm.D;
     float a[8], b[8], g1[8], g2[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) a[j] = b[j] = g1[j] = g2[j] = 0.f;
-    const bool norm = p.live && p.known && !p.is_v;
-    if (p.live && p.known) load16<T>(dout, p.at, half, g1, g2);
-    if (norm) {
-      load16<T>(qkv, p.at, half, a, b);
-      if (p.is_q && lora_q != nullptr) add_lora<T>(lora_q, lora_f32, p.at_lora, half, a, b);
+    typename Elem<T>::Raw8 v1{}, v2{};
+    if (live && known) {
+      load16<T>(dout, at, half, g1, g2);
+      load16<T>(qkv, at, half, a, b);
+      if (!is_q) {
+        v1 = Elem<T>::template load8<true>(dout + at_v * Elem<T>::kBytes);
+        v2 = Elem<T>::template load8<true>(dout + (at_v + half) * Elem<T>::kBytes);
+      }
+      if (is_q && lora_q != nullptr)
+        add_lora<T>(lora_q, lora_f32, (static_cast<int64_t>(tok) * dm.NH + h) * dm.D + 8 * c, half,
+                    a, b);
     }
-    const float r =
-        1.0f / sqrtf(group_sum<G>(sum_squares(a, b)) / static_cast<float>(dm.D) + eps);
+    const float r = 1.0f / sqrtf(group_sum<G>(sum_squares(a, b)) / inv_d + eps);
     float dot = 0.f;
-    if (norm) {
-      const float* w = (p.is_q ? wq : wk) + 8 * c;
-      float w1[8], w2[8], c1[8], c2[8], s1[8], s2[8];
-      load8f(w, w1);
-      load8f(w + half, w2);
-      load8f(p.cos, c1);
-      load8f(p.cos + half, c2);
-      load8f(p.sin, s1);
-      load8f(p.sin + half, s2);
+    if (live && known) {
+      const int64_t row = static_cast<int64_t>(t) * dm.D + 8 * c;
+      float c1[8], c2[8], s1[8], s2[8];
+      load8f(cos_t + row, c1);
+      load8f(cos_t + row + half, c2);
+      load8f(sin_t + row, s1);
+      load8f(sin_t + row + half, s2);
       float d1 = 0.f, d2 = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -209,12 +239,9 @@ __global__ __launch_bounds__(kNormThreads) void qk_norm_rope_bwd_kernel(
         const float y2 = g2[j] * c2[j] - g1[j] * s1[j];
         a[j] = a[j] * r;
         b[j] = b[j] * r;
-        const float t1 = y1 * a[j], t2 = y2 * b[j];
         if constexpr (DW) {
-          acc[j] = acc[j] + (p.is_q ? t1 : 0.f);
-          acc[8 + j] = acc[8 + j] + (p.is_q ? t2 : 0.f);
-          acc[16 + j] = acc[16 + j] + (p.is_q ? 0.f : t1);
-          acc[24 + j] = acc[24 + j] + (p.is_q ? 0.f : t2);
+          acc1[j] = acc1[j] + y1 * a[j];
+          acc2[j] = acc2[j] + y2 * b[j];
         }
         g1[j] = y1 * w1[j];
         g2[j] = y2 * w2[j];
@@ -223,62 +250,68 @@ __global__ __launch_bounds__(kNormThreads) void qk_norm_rope_bwd_kernel(
       }
       dot = d1 + d2;
     }
-    dot = group_sum<G>(dot) / static_cast<float>(dm.D);
-    if (!p.live) continue;
-    if (norm) {
+    dot = group_sum<G>(dot) / inv_d;
+    if (live) {
+      if (known) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        g1[j] = r * (g1[j] - a[j] * dot);
-        g2[j] = r * (g2[j] - b[j] * dot);
+        for (int j = 0; j < 8; ++j) {
+          g1[j] = r * (g1[j] - a[j] * dot);
+          g2[j] = r * (g2[j] - b[j] * dot);
+        }
+      }
+      Elem<T>::template store8<true>(dqkv + at * Elem<T>::kBytes, g1);
+      Elem<T>::template store8<true>(dqkv + (at + half) * Elem<T>::kBytes, g2);
+      if (!is_q) {
+        st16<true>(dqkv + at_v * Elem<T>::kBytes, v1.w);
+        st16<true>(dqkv + (at_v + half) * Elem<T>::kBytes, v2.w);
       }
     }
-    Elem<T>::template store8<true>(dqkv + p.at * Elem<T>::kBytes, g1);
-    Elem<T>::template store8<true>(dqkv + (p.at + half) * Elem<T>::kBytes, g2);
   }
   if constexpr (DW) {
-    // The lanes of one c hold the same dims: they are added in the order of the thread index.
-    constexpr int kPer = kNormThreads / G;               // lanes per c
-    __shared__ float sum[kNormThreads * 8 + 8];
-    const int who = threadIdx.x / G;
-    float* const row = partial + static_cast<int64_t>(blockIdx.x) * 2 * dm.D;
-    for (int part = 0; part < 4; ++part) {
+    // The slots' sums of a dim are added in slot order.
+    __shared__ float sum[kNormThreads * 8];
+    float* const row = partial + static_cast<int64_t>(blockIdx.x) * dm.D;
+#pragma unroll
+    for (int part = 0; part < 2; ++part) {
       __syncthreads();
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float v = part == 0 ? acc[j] : part == 1 ? acc[8 + j] : part == 2 ? acc[16 + j]
-                                                                            : acc[24 + j];
-        sum[who * (G * 8) + c * 8 + j] = v;
-      }
+      for (int j = 0; j < 8; ++j)
+        sum[slot * (G * 8) + c * 8 + j] = part == 0 ? acc1[j] : acc2[j];
       __syncthreads();
       if (static_cast<int>(threadIdx.x) < half) {          // (half <= G * 8)
         float s = 0.f;
-        for (int k = 0; k < kPer; ++k) s = s + sum[k * (G * 8) + threadIdx.x];
-        row[(part >> 1) * dm.D + (part & 1) * half + threadIdx.x] = s;
+#pragma unroll 8
+        for (int k = 0; k < kSlots; ++k) s = s + sum[k * (G * 8) + threadIdx.x];
+        row[part * half + threadIdx.x] = s;
       }
     }
   }
 }
 
-// dw = sum of the partial rows in workgroup order: 16 threads per column, each a stretch of the
-// rows, joined in stretch order.
-constexpr int kSumCols = 16, kSumParts = 16;
-__global__ __launch_bounds__(kSumCols* kSumParts) void qk_norm_dw_kernel(
-    const float* __restrict__ partial, int blocks, int D, float* __restrict__ dwq,
+// dw = sum of the workgroups' rows in their order: per column 64 threads, each a stretch of the
+// rows, joined in stretch order.  Columns [0, D) are the query weight's, [D, 2D) the key weight's.
+constexpr int kSumCols = 4, kSumParts = kNormThreads / kSumCols;
+__global__ __launch_bounds__(kNormThreads) void qk_norm_dw_kernel(
+    const float* __restrict__ partial, int q_blocks, int blocks, int D, float* __restrict__ dwq,
     float* __restrict__ dwk) {
   __shared__ float s[kSumParts][kSumCols];
   const int col = threadIdx.x % kSumCols, part = threadIdx.x / kSumCols;
-  const int x = blockIdx.x * kSumCols + col;
-  const int per = (blocks + kSumParts - 1) / kSumParts;
+  const int x = blockIdx.x * kSumCols + col;               // (D is a multiple of 16)
+  const bool is_q = x < D;
+  const int b0 = is_q ? 0 : q_blocks, n = is_q ? q_blocks : blocks - q_blocks;
+  const int per = (n + kSumParts - 1) / kSumParts;
+  const float* const from = partial + static_cast<int64_t>(b0) * D + (is_q ? x : x - D);
   float v = 0.f;
-  if (x < 2 * D)
-    for (int b = part * per; b < min(blocks, (part + 1) * per); ++b)
-      v = v + partial[static_cast<int64_t>(b) * 2 * D + x];
+  const int last = min(n, (part + 1) * per);
+#pragma unroll 8
+  for (int b = part * per; b < last; ++b) v = v + from[static_cast<int64_t>(b) * D];
   s[part][col] = v;
   __syncthreads();
-  if (part != 0 || x >= 2 * D) return;
+  if (part != 0) return;
+#pragma unroll 16
   for (int k = 1; k < kSumParts; ++k) v = v + s[k][col];
-  float* const to = x < D ? dwq : dwk;
-  if (to != nullptr) to[x < D ? x : x - D] = v;
+  float* const to = is_q ? dwq : dwk;
+  if (to != nullptr) to[is_q ? x : x - D] = v;
 }
 
 // Calls f(integral constant G) with the lanes of a head of D dims.
@@ -308,7 +341,8 @@ int norm_dims(int64_t rows, int32_t B, int32_t T, int32_t NH, int32_t NKV, int32
     return kInvalid;
   const int64_t heads = NH + 2 * static_cast<int64_t>(NKV);
   const int groups = static_cast<int>((heads * group_of(D) + kWave - 1) / kWave);
-  if (rows > ((int64_t{1} << 31) - 1 - kNormWaves * kNormBlocks) / groups) return kInvalid;
+  // (32-bit indices of heads, with room for a last round)
+  if (rows > ((int64_t{1} << 31) - 1 - (1 << 16)) / std::max<int64_t>(groups, heads)) return kInvalid;
   items = rows * groups;
   dm = NormDims{rows, static_cast<int64_t>(B) * T, T,  NH, NKV, D, groups,
                 FastDiv(static_cast<uint32_t>(groups)),
@@ -368,8 +402,26 @@ extern "C" __attribute__((visibility("default"))) int soupk_qk_norm_rope_bwd(
   if (dtype != SOUPK_DTYPE_F16 && dtype != SOUPK_DTYPE_BF16) return kInvalid;
   if (lora_q && lora_dtype != dtype && lora_dtype != SOUPK_DTYPE_F32) return kInvalid;
   const bool want_dw = dwq != nullptr || dwk != nullptr;
-  const int64_t blocks =
-      std::min<int64_t>(kNormBlocks, (items + kNormWaves - 1) / kNormWaves);
+  // Workgroups for the query heads and for the key and value heads, in proportion to what they
+  // move; with weight gradients at most kNormBlocks in all (their partial rows).
+  const int64_t slots = kNormThreads / group_of(D);
+  const int64_t q_heads = rows * NH, kv_heads = rows * NKV;
+  const int64_t q_need = (q_heads + slots - 1) / slots, kv_need = (kv_heads + slots - 1) / slots;
+  const int64_t most = want_dw ? kNormBlocks : int64_t{1} << 30;
+  int64_t q_blocks = q_need, kv_blocks = kv_need;
+  if (q_need + kv_need > most) {
+    kv_blocks = std::min<int64_t>(kv_need, most * 5 * NKV / (3 * NH + 5 * NKV));
+    if (NKV > 0) kv_blocks = std::max<int64_t>(kv_blocks, 1);
+    q_blocks = std::min<int64_t>(q_need, most - kv_blocks);
+  }
+  auto share = [&](int64_t heads, int64_t blocks) {      // heads per workgroup, whole rounds
+    return blocks > 0 ? ((heads + blocks - 1) / blocks + slots - 1) / slots * slots : slots;
+  };
+  const NormSplit sp{static_cast<int>(q_blocks), static_cast<uint32_t>(share(q_heads, q_blocks)),
+                     static_cast<uint32_t>(share(kv_heads, kv_blocks)),
+                     FastDiv(static_cast<uint32_t>(NH)),
+                     FastDiv(static_cast<uint32_t>(std::max(NKV, 1)))};
+  const int64_t blocks = q_blocks + kv_blocks;
   if (rows > 0) {
     if (bad_elem_ptr(dout, dtype) || bad_elem_ptr(qkv, dtype) || bad_elem_ptr(dqkv, dtype) ||
         bad4(wq) || bad4(wk))
@@ -379,7 +431,7 @@ extern "C" __attribute__((visibility("default"))) int soupk_qk_norm_rope_bwd(
     if (lora_q && bad_elem_ptr(lora_q, lora_dtype)) return kInvalid;
   }
   if ((dwq && bad4(dwq)) || (dwk && bad4(dwk))) return kInvalid;
-  if (want_dw && blocks > 0 && (bad4(workspace) || workspace_floats < blocks * 2 * D))
+  if (want_dw && blocks > 0 && (bad4(workspace) || workspace_floats < blocks * D))
     return kInvalid;
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (rows > 0) {
@@ -390,23 +442,22 @@ extern "C" __attribute__((visibility("default"))) int soupk_qk_norm_rope_bwd(
       } else {
         return with_group(D, [&](auto g) {
           constexpr int G = decltype(g)::value;
-          auto run = [&](auto kernel, int64_t n) {
-            return launch_kernel(kernel, dim3(static_cast<unsigned>(n)), dim3(kNormThreads), s,
+          auto run = [&](auto kernel) {
+            return launch_kernel(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kNormThreads), s,
                                  static_cast<const char*>(dout), static_cast<const char*>(qkv),
                                  static_cast<const char*>(lora_q), lora_dtype == SOUPK_DTYPE_F32,
                                  wq, wk, cos, sin, pos, static_cast<char*>(dqkv), workspace, eps,
-                                 dm, static_cast<uint32_t>(items));
+                                 dm, sp);
           };
-          return want_dw ? run(qk_norm_rope_bwd_kernel<E, G, true>, blocks)
-                         : run(qk_norm_rope_bwd_kernel<E, G, false>,
-                               (items + kNormWaves - 1) / kNormWaves);
+          return want_dw ? run(qk_norm_rope_bwd_kernel<E, G, true>)
+                         : run(qk_norm_rope_bwd_kernel<E, G, false>);
         });
       }
     });
     if (rc != kOk) return rc;
   }
   if (!want_dw) return kOk;
-  return launch_kernel(qk_norm_dw_kernel, dim3((2 * D + kSumCols - 1) / kSumCols),
-                       dim3(kSumCols * kSumParts), s, static_cast<const float*>(workspace),
+  return launch_kernel(qk_norm_dw_kernel, dim3(2 * D / kSumCols), dim3(kNormThreads), s,
+                       static_cast<const float*>(workspace), static_cast<int>(q_blocks),
                        static_cast<int>(blocks), static_cast<int>(D), dwq, dwk);
 }

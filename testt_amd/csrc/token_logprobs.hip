@@ -16,11 +16,12 @@
 // The alternatives come out of the same pass.  Each thread knows the largest value it has seen; the K-th
 // largest of 64 groups' maxima is a bound: K columns at least as large have been seen, all of them
 // further left than what is still to come, so from there on only a value strictly above the bound can be
-// among the K, and goes into a short list in LDS.  The bound is raised after 1, 2, 8, 32, ... steps,
-// so the list stays at some ten times K entries whatever the row's length.  Columns of the first step are
-// listed by the bound found from it, equal ones only as far as they can count (by their order).  At the
-// end the list is ranked.  A row that rises so steadily that the list overflows (no such row comes from
-// a model) is ranked by K searches over the row instead.
+// among the K, and its chunk's number goes into a short list in LDS.  The bound is raised after 1, 4,
+// 16, 64 ... steps, so the list stays at some ten times K entries whatever the row's length.  Of the first
+// step's columns, those equal to its bound are listed by themselves, only as far as they can count (by
+// their order).  At the end the listed chunks that reach the last bound are read again, and their
+// columns ranked.  A row that rises so steadily that a list overflows (no such row comes from a model)
+// is ranked by K searches over the row instead.
 //
 // Few rows are cut into parts, whose statistics and alternatives a second launch joins.
 
@@ -32,10 +33,21 @@
 namespace soupk {
 namespace {
 
-constexpr int kLpThreads = 256;
+#ifndef SOUPK_LP_THREADS
+#define SOUPK_LP_THREADS 256
+#endif
+constexpr int kLpThreads = SOUPK_LP_THREADS;
 constexpr int kLpWaves = kLpThreads / kWave;
-constexpr int kLpUnroll = 4;          // chunk loads in flight per thread
+constexpr int kGroup = kLpThreads / 64;   // neighbouring threads whose largest value bounds the list
+#ifndef SOUPK_LP_UNROLL
+#define SOUPK_LP_UNROLL 4
+#endif
+constexpr int kLpUnroll = SOUPK_LP_UNROLL;          // chunk loads in flight per thread
 constexpr int kMaxTop = 32;
+#ifndef SOUPK_LP_FILL
+#define SOUPK_LP_FILL 4
+#endif
+constexpr int kLpFill = SOUPK_LP_FILL;   // workgroups per CU below which rows are cut into parts
 constexpr int kListCap = 1024;        // candidates of a part
 constexpr int kMaxParts = 64;
 constexpr int64_t kIgnored = -100;
@@ -43,20 +55,23 @@ constexpr float kFloor = -200.f;      // below 2^kFloor an exponential is zero i
 
 // Rows of the logits: row r is (r / inner, r % inner) with its two strides (elements).
 struct LpRows {
-  int64_t inner, stride_outer, stride_inner, V;
+  int64_t inner, stride_outer, stride_inner, V, count;
   __device__ __forceinline__ int64_t at(int64_t r) const {
     const int64_t o = r / inner;
     return o * stride_outer + (r - o * inner) * stride_inner;
   }
 };
 
-// A 16-byte chunk as floats: 8 half-size or 4 fp32 columns.
+// A 16-byte chunk: 8 half-size or 4 fp32 columns, and the order of its type's values as integers
+// (kBits of them; a NaN as -inf, -0 as 0).
 template <typename T>
 struct Chunk {
   static constexpr int N = 16 / Elem<T>::kBytes;
+  static constexpr int kBits = 8 * Elem<T>::kBytes;
   u32x4 w;
-  __device__ __forceinline__ void load(const char* p) {
-    w = ld<true>(reinterpret_cast<const u32x4_a2*>(p));
+  // base: uniform; off: bytes
+  __device__ __forceinline__ void load(const char* base, uint32_t off) {
+    w = ld16<true>(base + off);
   }
   __device__ __forceinline__ void unpack(float* v) const {
     if constexpr (std::is_same_v<T, float>) {
@@ -66,66 +81,113 @@ struct Chunk {
       Elem<T>::unpack8(typename Elem<T>::Raw8{w}, v);
     }
   }
+  // Columns of -inf.
+  __device__ __forceinline__ void clear() {
+    const uint32_t inf = kBits == 32 ? 0xff800000u
+                                     : std::is_same_v<T, f16> ? 0xfc00fc00u : 0xff80ff80u;
+    w = u32x4{inf, inf, inf, inf};
+  }
+  // The largest column, NaN passed over (v: the columns unpacked).
+  __device__ __forceinline__ float max(const float* v) const {
+    if constexpr (std::is_same_v<T, f16>) {
+      const f16x2 m = __builtin_elementwise_max(
+          __builtin_elementwise_max(as_h2(w.x), as_h2(w.y)),
+          __builtin_elementwise_max(as_h2(w.z), as_h2(w.w)));
+      return static_cast<float>(__builtin_elementwise_max(m[0], m[1]));
+    } else {
+      float m = v[0];
+#pragma unroll
+      for (int j = 1; j < N; ++j) m = fmaxf(m, v[j]);
+      return m;
+    }
+  }
   static __device__ __forceinline__ void store(char* p, const float* v) {
     if constexpr (std::is_same_v<T, float>)
-      st<true>(reinterpret_cast<f32x4_a4*>(p), static_cast<f32x4_a4>(f32x4{v[0], v[1], v[2], v[3]}));
+      st16<true>(p, __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]}));
     else
       Elem<T>::template store8<true>(p, v);
   }
+  static __device__ __forceinline__ uint32_t key(float z) {
+    if (z != z) z = -INFINITY;
+    uint32_t b = z == 0.f ? 0u : __builtin_bit_cast(uint32_t, z);
+    if constexpr (std::is_same_v<T, f16>)
+      b = static_cast<uint32_t>(__builtin_bit_cast(uint16_t, static_cast<f16>(z == 0.f ? 0.f : z)))
+          << 16;
+    b = (b & 0x80000000u) ? ~b : b | 0x80000000u;
+    return b >> (32 - kBits);
+  }
+  static __device__ __forceinline__ float value(uint32_t k) {
+    uint32_t b = k << (32 - kBits);
+    b = (b & 0x80000000u) ? b & 0x7fffffffu : ~b;
+    if constexpr (std::is_same_v<T, f16>) return h2f(b >> 16);
+    else if constexpr (std::is_same_v<T, bf16>) return bf2f(b >> 16);
+    else return __builtin_bit_cast(float, b);
+  }
 };
 
-// Running statistics: the maximum, S = sum 2^x and A = sum 2^x x with x = (z - m) * c, c = log2(e) / T.
+// Running statistics: the maximum m, S = sum 2^x and A = sum 2^x x over x = z c - m c, c = log2(e) / T.
+// x is one fused multiply-add with the rounded m c, which every column of a row shares: its rounding
+// shifts all x alike and drops out of what is computed from them.  Where m c is out of that form's
+// range (rows of -inf, of the lowest value, with +inf) x is (z - m) c.
 struct Stats {
   float m, s, a;
 };
 
-__device__ __forceinline__ float shifted(float z, float m, float c) {
-  return (z - (m == -INFINITY ? 0.f : m)) * c;      // (a part of -inf alone: 2^-inf = 0)
+__device__ __forceinline__ bool plain_form(float mc) { return fabsf(mc) < 1e30f; }
+__device__ __forceinline__ float exponent(float z, float m, float mc, float c) {
+  return plain_form(mc) ? __builtin_fmaf(z, c, -mc) : (m == -INFINITY ? z : z - m) * c;
 }
 
 // The statistics relative to another maximum m >= st.m.
 __device__ __forceinline__ void move_max(Stats& st, float m, float c) {
   if (st.m == m) return;
-  const float x = fmaxf((st.m - m) * c, kFloor);    // (st.m = -inf: s and a are 0)
-  const float f = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x);
-  st.a = f * (st.a + x * st.s);
+  const float from = st.m * c, to = m * c;
+  float x = plain_form(from) && plain_form(to) ? from - to : (st.m - m) * c;
+  x = fmaxf(x, kFloor);
+  const float f = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x);   // (then s and a are 0)
+  st.a = f * __builtin_fmaf(x, st.s, st.a);
   st.s = f * st.s;
   st.m = m;
 }
 
+// Folds N columns with maximum bm into the statistics; the whole wavefront calls it.  odd: a lane's
+// maximum is out of the plain form's range (kept across calls).  A column of -inf makes the sum A NaN
+// (0 * -inf): then A is formed again with the exponents bounded.
 template <int N>
-__device__ __forceinline__ void absorb(Stats& st, const float* z, float bm, float c) {
-  if (bm > st.m) move_max(st, bm, c);
-  const float m = st.m == -INFINITY ? 0.f : st.m;
-  float e[N], x[N];
-#pragma unroll
-  for (int j = 0; j < N; ++j) {
-    x[j] = (z[j] - m) * c;
-    e[j] = __builtin_amdgcn_exp2f(x[j]);
+__device__ __forceinline__ void absorb(Stats& st, float& mc, bool& odd, const float* z, float bm,
+                                       float c) {
+  if (__any(bm > st.m)) {
+    if (bm > st.m) move_max(st, bm, c);
+    mc = st.m * c;
+    odd = __any(!plain_form(mc));
   }
-  float s = 0.f, a = 0.f;
+  float e[N], x[N];
+  if (!odd) {
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
+    for (int j = 0; j < N; ++j) x[j] = __builtin_fmaf(z[j], c, -mc);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = exponent(z[j], st.m, mc, c);
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j) e[j] = __builtin_amdgcn_exp2f(x[j]);
+  float s = e[0], a = e[0] * x[0];
+#pragma unroll
+  for (int j = 1; j < N; ++j) {
     s = s + e[j];
-    a = __builtin_fmaf(e[j], fmaxf(x[j], kFloor), a);
+    a = __builtin_fmaf(e[j], x[j], a);
+  }
+  if (a != a) {
+    a = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) a = __builtin_fmaf(e[j], fmaxf(x[j], kFloor), a);
   }
   st.s = st.s + s;
   st.a = st.a + a;
 }
 
-// fp32 bits in an order that integers compare; NaN as -inf, -0 as 0.
-__device__ __forceinline__ uint32_t sort_bits(float z) {
-  if (z != z) z = -INFINITY;
-  if (z == 0.f) z = 0.f;
-  const uint32_t b = __builtin_bit_cast(uint32_t, z);
-  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float unsort_bits(uint32_t k) {
-  return __builtin_bit_cast(float, (k & 0x80000000u) ? k & 0x7fffffffu : ~k);
-}
-
 struct Cand {
-  uint32_t key;   // sort_bits of the value
+  uint32_t key;   // Chunk<T>::key of the value
   uint32_t col;
 };
 __device__ __forceinline__ bool ahead(const Cand& a, const Cand& b) {
@@ -144,37 +206,64 @@ struct RowOut {
 };
 
 struct ListLds {
-  Cand list[kListCap];
-  Cand keep[kListCap];
+  // Lower half: chunks (the key of their largest column, their number in the part); upper half: the
+  // columns that are ranked at the end.  (The join ranks from the whole.)
+  Cand list[2 * kListCap];
+  Cand tie[kMaxTop];            // columns of the first step that equal its bound
   uint32_t group_max[64];
-  int count, kept;
+  int count, kept, ties;
   int wave_n[kLpWaves];
   Cand best[kLpWaves];
+  Cand top[kMaxTop];
 };
 
-// The K-th largest of the 64 groups' maxima (a group: 4 neighbouring threads); every thread of the
-// workgroup calls it and gets it.
-__device__ __forceinline__ uint32_t raise_bound(ListLds& s, float tmax, int K) {
+// The K-th largest of the 64 groups' largest keys, by two bits a step; every thread of the workgroup calls it and gets it.
+template <int BITS>
+__device__ __forceinline__ uint32_t raise_bound(ListLds& s, uint32_t k, int K) {
   const int lane = threadIdx.x & 63;
-  uint32_t k = sort_bits(tmax);
   k = max(k, static_cast<uint32_t>(dpp_i<kDppQuad1032>(static_cast<int>(k))));
   k = max(k, static_cast<uint32_t>(dpp_i<kDppQuad2301>(static_cast<int>(k))));
+  if constexpr (kGroup >= 8)
+    k = max(k, static_cast<uint32_t>(dpp_i<kDppHalfMirror>(static_cast<int>(k))));
+  if constexpr (kGroup >= 16)
+    k = max(k, static_cast<uint32_t>(dpp_i<kDppMirror>(static_cast<int>(k))));
   __syncthreads();                               // (group_max of the last call has been read)
-  if ((threadIdx.x & 3) == 0) s.group_max[threadIdx.x >> 2] = k;
+  if (threadIdx.x % kGroup == 0) s.group_max[threadIdx.x / kGroup] = k;
   __syncthreads();
   const uint32_t mine = s.group_max[lane];
   uint32_t bound = 0;
 #pragma unroll
-  for (int b = 31; b >= 0; --b) {
-    const uint32_t cand = bound | (1u << b);
-    if (__popcll(__ballot(mine >= cand)) >= K) bound = cand;
+  for (int b = BITS - 2; b >= 0; b -= 2) {
+    const uint32_t c1 = bound | (1u << b), c2 = bound | (2u << b), c3 = bound | (3u << b);
+    const int n1 = __popcll(__ballot(mine >= c1)), n2 = __popcll(__ballot(mine >= c2)),
+              n3 = __popcll(__ballot(mine >= c3));
+    bound = n3 >= K ? c3 : n2 >= K ? c2 : n1 >= K ? c1 : bound;
   }
   return bound;
 }
 
-__device__ __forceinline__ void push(ListLds& s, uint32_t key, uint32_t col) {
+__device__ __forceinline__ void push(ListLds& s, uint32_t key, uint32_t chunk) {
   const int at = atomicAdd(&s.count, 1);
-  if (at < kListCap) s.list[at] = Cand{key, col};
+  if (at < kListCap) s.list[at] = Cand{key, chunk};
+}
+__device__ __forceinline__ void keep(ListLds& s, uint32_t key, uint32_t col) {
+  const int at = atomicAdd(&s.kept, 1);
+  if (at < kListCap) s.list[kListCap + at] = Cand{key, col};
+}
+
+// Sum of the lanes up to and including this one.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);   // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);   // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);   // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);   // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);   // row_bcast:15
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);   // row_bcast:31
+  return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = row16_max(v);
+  return fmaxf(fmaxf(lanef(v, 0), lanef(v, 16)), fmaxf(lanef(v, 32), lanef(v, 48)));
 }
 
 // Writes the K best of n candidates in order (entries past the last one have column kNoCol); every
@@ -191,15 +280,14 @@ __device__ __forceinline__ void rank_list(const Cand* list, int n, int K, Cand* 
 
 // The K best columns of [col0, col1) by K searches, each for the best one behind the last.
 template <typename T>
-__device__ void search_top(ListLds& s, const char* row, int64_t col0, int64_t col1, int K,
-                           Cand* out) {
+__device__ void search_top(ListLds& s, const char* row, int64_t col0, int64_t col1, int K) {
   Cand last{0xffffffffu, 0};
   bool any = true;
   for (int k = 0; k < K; ++k) {
     Cand best{0, kNoCol};
     if (any)
       for (int64_t i = col0 + threadIdx.x; i < col1; i += kLpThreads) {
-        const Cand c{sort_bits(Elem<T>::load1(row + i * Elem<T>::kBytes)),
+        const Cand c{Chunk<T>::key(Elem<T>::load1(row + i * Elem<T>::kBytes)),
                      static_cast<uint32_t>(i)};
         if ((k == 0 || ahead(last, c)) && ahead(c, best)) best = c;
       }
@@ -213,23 +301,18 @@ __device__ void search_top(ListLds& s, const char* row, int64_t col0, int64_t co
 #pragma unroll
     for (int w = 1; w < kLpWaves; ++w)
       if (ahead(s.best[w], best)) best = s.best[w];
-    if (threadIdx.x == 0) out[k] = best;
+    if (threadIdx.x == 0) s.top[k] = best;
     any = best.col != kNoCol;
     last = best;
     __syncthreads();
   }
 }
 
-// Statistics of the workgroup, in every thread of its first wavefront.
+// Statistics of the workgroup, in every thread.
 __device__ __forceinline__ Stats merge_stats(Stats* lds, Stats st, float c) {
-  auto across = [&](float v, auto f) {
-    for (int d = 32; d > 0; d >>= 1) v = f(v, __shfl_xor(v, d));
-    return v;
-  };
-  const float m = across(st.m, [](float a, float b) { return fmaxf(a, b); });
-  move_max(st, m, c);
-  st.s = across(st.s, [](float a, float b) { return a + b; });
-  st.a = across(st.a, [](float a, float b) { return a + b; });
+  move_max(st, wave_max(st.m), c);
+  st.s = wave_sum(st.s);
+  st.a = wave_sum(st.a);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = st;
   __syncthreads();
   float mx = lds[0].m;
@@ -246,30 +329,44 @@ __device__ __forceinline__ Stats merge_stats(Stats* lds, Stats st, float c) {
   return r;
 }
 
+// ln S of a row relative to its maximum: the sum's logarithm without the rounding of m c that the
+// exponents share (NaN for a row of -inf alone, as the formula gives); a column's log probability.
+__device__ __forceinline__ float log_sum(const Stats& st, float c) {
+  if (!(st.m > -INFINITY)) return NAN;
+  const float mc = st.m * c;
+  const float shift = plain_form(mc) ? __builtin_fmaf(st.m, c, -mc) : 0.f;
+  return logf(st.s) - kLn2 * shift;
+}
+template <typename T>
+__device__ __forceinline__ float column_lp(const char* row, int64_t col, const Stats& st,
+                                           float inv_t, float lse) {
+  const float z = Elem<T>::load1(row + col * Elem<T>::kBytes);
+  return (z - st.m) * inv_t - lse;
+}
+
 // The numbers of a row from its statistics (one thread).
 template <typename T>
-__device__ __forceinline__ float write_row(const RowOut& o, int64_t r, const Stats& st,
-                                           const char* row, int64_t V, int64_t tok, float inv_t) {
-  // (a row without a finite maximum: NaN, as the formula gives)
-  const float lse = st.m > -INFINITY ? logf(st.s) : NAN;
-  o.entropy[r] = lse - kLn2 * (st.a / st.s);
+__device__ __forceinline__ void write_row(const RowOut& o, int64_t r, const Stats& st,
+                                          const char* row, int64_t V, int64_t tok, float inv_t,
+                                          float lse) {
+  // (the exponents' shared rounding is in both terms)
+  o.entropy[r] = (st.m > -INFINITY ? logf(st.s) : NAN) - kLn2 * (st.a / st.s);
   float lp = NAN;
   if (tok == kIgnored) lp = 0.f;
-  else if (tok >= 0 && tok < V)
-    lp = (Elem<T>::load1(row + tok * Elem<T>::kBytes) - st.m) * inv_t - lse;
+  else if (tok >= 0 && tok < V) lp = column_lp<T>(row, tok, st, inv_t, lse);
   o.logprob[r] = lp;
   if (o.row_max != nullptr) {
     o.row_max[r] = st.m;
     o.row_sum[r] = st.s;
   }
-  return lse;
 }
 
 template <typename T, bool TOP>
 __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(
     const char* __restrict__ logits, const int64_t* __restrict__ tokens, LpRows rows, float c,
     float inv_t, int K, int parts, int64_t part_chunks, PartOut part, RowOut out) {
-  constexpr int N = Chunk<T>::N;
+  using C = Chunk<T>;
+  constexpr int N = C::N;
   constexpr int kSize = Elem<T>::kBytes;
   __shared__ Stats stat_lds[kLpWaves];
   __shared__ std::conditional_t<TOP, ListLds, int> lds;
@@ -281,174 +378,184 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(
   const int64_t last = min(chunks, first + part_chunks);
   const int tid = threadIdx.x;
   Stats st{-INFINITY, 0.f, 0.f};
+  float mc = -INFINITY;
+  bool odd = true;
   float tmax = -INFINITY;        // this thread's largest value so far (never NaN)
-  uint32_t bound_key = 0;
   float bound = -INFINITY;
+  uint32_t first_key = 0;        // the first step's bound
   if constexpr (TOP) {
-    if (tid == 0) lds.count = lds.kept = 0;
+    if (tid == 0) lds.count = lds.kept = lds.ties = 0;
     __syncthreads();
   }
-  const char* const p0 = row + (first + tid) * 16;
-  const int64_t n = last - first - tid;          // chunks of this thread: every 256th
-  const int64_t steps = (last - first + kLpThreads - 1) / kLpThreads;
-  int64_t next_raise = 2;
-  for (int64_t step = 0; step < steps; step += kLpUnroll) {
-    Chunk<T> w[kLpUnroll];
+  // Offsets within the part fit 32 bits (the host cuts longer rows).
+  const char* const base = row + first * 16;
+  const int n = static_cast<int>(last - first);          // (<= 0: an empty last part)
+  const int steps = n > 0 ? (n + kLpThreads - 1) / kLpThreads : 0;
+  const uint32_t col_base = static_cast<uint32_t>(first) * N;
+  int next_raise = kLpUnroll;
+  for (int step = 0; step < steps; step += kLpUnroll) {
+    C w[kLpUnroll];
+    const int i0 = step * kLpThreads + tid;
 #pragma unroll
     for (int u = 0; u < kLpUnroll; ++u) {
-      // (past the part's end: its first chunk, unused, so that no load waits for a branch)
-      const int64_t i = (step + u) * kLpThreads;
-      w[u].load(i < n ? p0 + i * 16 : row + first * 16);
+      // (past the part's end: its first chunk, so that no load waits for a branch ...)
+      const int i = i0 + u * kLpThreads;
+      w[u].load(base, i < n ? static_cast<uint32_t>(i) * 16u : 0u);
+    }
+    if constexpr (TOP) {
+      if (step == next_raise) {
+        next_raise *= 4;
+        bound = C::value(raise_bound<C::kBits>(lds, C::key(tmax), K));
+      }
+    }
+    if ((step + kLpUnroll) * kLpThreads > n) {
+      // (... and counted as -inf)
+#pragma unroll
+      for (int u = 0; u < kLpUnroll; ++u)
+        if (i0 + u * kLpThreads >= n) w[u].clear();
     }
 #pragma unroll
     for (int u = 0; u < kLpUnroll; ++u) {
-      if constexpr (TOP) {
-        if (step + u == next_raise && step + u < steps) {
-          next_raise *= 4;
-          bound_key = raise_bound(lds, tmax, K);
-          bound = unsort_bits(bound_key);
-        }
-      }
-      const int64_t i = (step + u) * kLpThreads;
-      const bool on = i < n;
+      const int i = i0 + u * kLpThreads;
       float z[N];
-      if (on) {
-        w[u].unpack(z);
-        float bm = z[0];
-#pragma unroll
-        for (int j = 1; j < N; ++j) bm = fmaxf(bm, z[j]);
-        absorb<N>(st, z, bm, c);
-        if constexpr (TOP) {
-          tmax = fmaxf(tmax, bm);
-          if (step + u > 0 && bm > bound) {
-            const uint32_t col = static_cast<uint32_t>((first + tid + i) * N);
-#pragma unroll
-            for (int j = 0; j < N; ++j)
-              if (z[j] > bound) push(lds, sort_bits(z[j]), col + j);
-          }
-        }
-      }
+      w[u].unpack(z);
+      const float bm = w[u].max(z);
+      absorb<N>(st, mc, odd, z, bm, c);
       if constexpr (TOP) {
-        if (step + u == 0) {
-          // The first step's columns against the bound that they give: those above it, and as many of
-          // the equal ones, from the left, as the K can still take.
-          bound_key = raise_bound(lds, tmax, K);
-          uint32_t key[N];
-          int above = 0, equal = 0;
-          if (on) {
+        tmax = fmaxf(tmax, bm);
+        if (u == 0 && step == 0) {
+          // The first step's columns against the bound that they give: the chunks with one above it,
+          // and as many of the equal ones, from the left, as the K can still take.
+          first_key = raise_bound<C::kBits>(lds, C::key(tmax), K);
+          bound = C::value(first_key);
+          int equal = 0;
+          if (i < n) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-              key[j] = sort_bits(z[j]);
-              above += key[j] > bound_key ? 1 : 0;
-              equal += key[j] == bound_key ? 1 : 0;
-            }
+            for (int j = 0; j < N; ++j) equal += C::key(z[j]) == first_key ? 1 : 0;
           }
-          // equal columns left of this thread's, by a scan over the workgroup
-          int upto = equal;
-          for (int d = 1; d < kWave; d <<= 1) {
-            const int v = __shfl_up(upto, d);
-            if ((tid & 63) >= d) upto += v;
-          }
+          const int upto = wave_scan(equal);     // equal columns left of and in this thread's
           if ((tid & 63) == 63) lds.wave_n[tid >> 6] = upto;
           __syncthreads();
           int left = upto - equal;
           for (int k = 0; k < (tid >> 6); ++k) left += lds.wave_n[k];
-          if (on && (above > 0 || (equal > 0 && left < K))) {
-            const uint32_t col = static_cast<uint32_t>((first + tid) * N);
+          if (equal > 0 && left < K) {
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-              if (key[j] > bound_key) push(lds, key[j], col + j);
-              if (key[j] == bound_key) {
-                if (left < K) push(lds, key[j], col + j);
+            for (int j = 0; j < N; ++j)
+              if (C::key(z[j]) == first_key) {
+                if (left < K) {
+                  lds.tie[left] = Cand{first_key, col_base + static_cast<uint32_t>(tid) * N + j};
+                  atomicAdd(&lds.ties, 1);
+                }
                 ++left;
               }
-            }
           }
-          bound = unsort_bits(bound_key);
         }
+        if (bm > bound) push(lds, C::key(bm), static_cast<uint32_t>(i));
       }
     }
   }
   // The columns past the last whole chunk, in the last part.
-  const bool has_tail = last == chunks && which == parts - 1;
+  const bool has_tail = which == parts - 1;
   const int64_t tail0 = chunks * N;
-  if (has_tail && tail0 + tid < rows.V) {
-    const float z = Elem<T>::load1(row + (tail0 + tid) * kSize);
-    absorb<1>(st, &z, z, c);
-    if constexpr (TOP) push(lds, sort_bits(z), static_cast<uint32_t>(tail0 + tid));
+  float tail = -INFINITY;
+  if (has_tail) {                                // (whole wavefronts: the others add nothing)
+    if (tail0 + tid < rows.V) tail = Elem<T>::load1(row + (tail0 + tid) * kSize);
+    if (tid < kWave) absorb<1>(st, mc, odd, &tail, tail, c);
   }
   const Stats total = merge_stats(stat_lds, st, c);
   const int64_t at = blockIdx.x;
-  float lse = 0.f;
-  if (parts > 1) {
-    if (tid == 0) part.stats[at] = total;
-  } else if (tid < 64) {
-    lse = total.m > -INFINITY ? logf(total.s) : NAN;
-    if (tid == 0) write_row<T>(out, r, total, row, rows.V, tokens[r], inv_t);
+  const float lse = log_sum(total, c);
+  if (tid == 0) {
+    if (parts > 1) part.stats[at] = total;
+    else write_row<T>(out, r, total, row, rows.V, tokens[r], inv_t, lse);
   }
   if constexpr (TOP) {
-    // (merge_stats synchronised the workgroup: the list is complete)
-    __shared__ Cand top[kMaxTop];
+    // The chunks that reach the bound of all whole chunks, column by column; the first step's equal
+    // columns, if that bound is still theirs; the tail.  (merge_stats synchronised the workgroup: the
+    // lists are complete.)
     const int count = lds.count;
-    if (count > kListCap) {
-      search_top<T>(lds, row, first * N, has_tail ? rows.V : last * N, K, top);
-    } else {
-      bound_key = raise_bound(lds, tmax, K);     // of all whole chunks: what is below it is out
-      for (int i = tid; i < count; i += kLpThreads)
-        if (lds.list[i].key >= bound_key) lds.keep[atomicAdd(&lds.kept, 1)] = lds.list[i];
-      __syncthreads();
-      rank_list(lds.keep, lds.kept, K, top);
+    const uint32_t key = steps > 0 ? raise_bound<C::kBits>(lds, C::key(tmax), K) : 0u;
+    for (int i = tid; i < min(count, kListCap); i += kLpThreads) {
+      const Cand e = lds.list[i];
+      if (e.key < key) continue;
+      C w;
+      w.load(base, e.col * 16u);
+      float z[N];
+      w.unpack(z);
+      const bool ties_apart = e.col < kLpThreads;          // a chunk of the first step
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const uint32_t k = C::key(z[j]);
+        if (k >= key && !(ties_apart && k == first_key)) keep(lds, k, col_base + e.col * N + j);
+      }
     }
+    if (first_key == key && tid < lds.ties) keep(lds, lds.tie[tid].key, lds.tie[tid].col);
+    if (has_tail && tail0 + tid < rows.V) keep(lds, C::key(tail), static_cast<uint32_t>(tail0 + tid));
+    __syncthreads();
+    if (count > kListCap || lds.kept > kListCap)
+      search_top<T>(lds, row, min(first, chunks) * N, has_tail ? rows.V : last * N, K);
+    else
+      rank_list(lds.list + kListCap, lds.kept, K, lds.top);
     __syncthreads();
     if (tid < K) {
-      const Cand e = top[tid];
+      const Cand e = lds.top[tid];
       if (parts > 1) {
         part.cand[at * K + tid] = e;
       } else {
-        const float z = Elem<T>::load1(row + static_cast<int64_t>(e.col) * kSize);
         out.top_id[r * K + tid] = e.col;
-        out.top_lp[r * K + tid] = (z - total.m) * inv_t - lse;
+        out.top_lp[r * K + tid] = column_lp<T>(row, e.col, total, inv_t, lse);
       }
     }
   }
 }
 
-// One wavefront per row: lane l holds part l.  The alternatives are merged by K rounds over the heads
-// of the parts' lists.
-template <typename T>
-__global__ __launch_bounds__(kWave) void token_logprobs_join_kernel(
+// The rows of several parts: lane l of every wavefront holds part l's statistics.  The K best of all
+// parts' alternatives are found as in the parts: a bound, the list of what reaches it, ranks.
+template <typename T, bool TOP>
+__global__ __launch_bounds__(kLpThreads) void token_logprobs_join_kernel(
     const char* __restrict__ logits, const int64_t* __restrict__ tokens, LpRows rows, float c,
     float inv_t, int K, int parts, PartOut part, RowOut out) {
-  const int64_t r = blockIdx.x;
+  using C = Chunk<T>;
+  __shared__ std::conditional_t<TOP, ListLds, int> lds;
+  // Without alternatives a wavefront takes a row.
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t r = TOP ? static_cast<int64_t>(blockIdx.x)
+                        : static_cast<int64_t>(blockIdx.x) * kLpWaves + wave;
+  if (r >= rows.count) return;
   const char* const row = logits + rows.at(r) * Elem<T>::kBytes;
-  const int lane = threadIdx.x;
   Stats st{-INFINITY, 0.f, 0.f};
   if (lane < parts) st = part.stats[r * parts + lane];
-  float m = st.m;
-  for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-  move_max(st, m, c);
-  for (int d = 32; d > 0; d >>= 1) {
-    st.s = st.s + __shfl_xor(st.s, d);
-    st.a = st.a + __shfl_xor(st.a, d);
-  }
-  const float lse = st.m > -INFINITY ? logf(st.s) : NAN;
-  if (lane == 0) write_row<T>(out, r, st, row, rows.V, tokens[r], inv_t);
-  if (K == 0) return;
-  const Cand* const mine = part.cand + (r * parts + lane) * K;
-  int at = 0;
-  Cand head = lane < parts ? mine[0] : Cand{0, kNoCol};
-  for (int k = 0; k < K; ++k) {
-    Cand best = head;
-    for (int d = 32; d > 0; d >>= 1) {
-      const Cand o{__shfl_xor(best.key, d), __shfl_xor(best.col, d)};
-      if (ahead(o, best)) best = o;
+  move_max(st, wave_max(st.m), c);
+  st.s = wave_sum(st.s);
+  st.a = wave_sum(st.a);
+  const float lse = log_sum(st, c);
+  if (lane == 0 && (!TOP || wave == 0)) write_row<T>(out, r, st, row, rows.V, tokens[r], inv_t, lse);
+  if constexpr (TOP) {
+    const int tid = threadIdx.x;
+    const Cand* const all = part.cand + r * parts * K;
+    const int n = parts * K;                       // <= 64 * 32
+    if (tid == 0) lds.kept = 0;
+    uint32_t best = 0;
+    Cand mine[kMaxParts * kMaxTop / kLpThreads];
+#pragma unroll
+    for (int u = 0; u < kMaxParts * kMaxTop / kLpThreads; ++u) {
+      const int i = u * kLpThreads + tid;
+      mine[u] = i < n ? all[i] : Cand{0, kNoCol};
+      if (mine[u].col != kNoCol) best = max(best, mine[u].key);
     }
-    if (head.col == best.col && head.col != kNoCol) {
-      const float z = Elem<T>::load1(row + static_cast<int64_t>(best.col) * Elem<T>::kBytes);
-      out.top_id[r * K + k] = best.col;
-      out.top_lp[r * K + k] = (z - m) * inv_t - lse;
-      ++at;
-      head = at < K ? mine[at] : Cand{0, kNoCol};
+    const uint32_t bound_key = raise_bound<C::kBits>(lds, best, K);
+    static_assert(kMaxParts * kMaxTop <= 2 * kListCap, "the list holds every candidate");
+#pragma unroll
+    for (int u = 0; u < kMaxParts * kMaxTop / kLpThreads; ++u)
+      if (mine[u].col != kNoCol && mine[u].key >= bound_key)
+        lds.list[atomicAdd(&lds.kept, 1)] = mine[u];
+    __syncthreads();
+    rank_list(lds.list, lds.kept, K, lds.top);
+    __syncthreads();
+    if (tid < K) {
+      const Cand e = lds.top[tid];
+      out.top_id[r * K + tid] = e.col;
+      out.top_lp[r * K + tid] = column_lp<T>(row, e.col, st, inv_t, lse);
     }
   }
 }
@@ -461,7 +568,7 @@ struct LpGrads {
   const int64_t* top_id;
 };
 
-// Workgroup (block of chunks, row).  dz = 2^x (k0 + k1 x) with x = (z - m) c and the row's factors k0,
+// Workgroup (block of chunks, row).  dz = 2^x (k0 + k1 x), x as in the forward and the row's factors k0,
 // k1; then the few columns with a gradient of their own are written again by the thread that wrote them.
 template <typename T>
 __global__ __launch_bounds__(kLpThreads) void token_logprobs_bwd_kernel(
@@ -499,11 +606,13 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_bwd_kernel(
 #pragma unroll
     for (int u = 0; u < kLpUnroll; ++u) {
       const int64_t i = first + u * kLpThreads;
-      if (i < chunks) w[u].load(row + i * 16);
+      if (i < chunks) w[u].load(row + i * 16, 0);
     }
   }
+  const float mc = m * c;
+  const bool plain = plain_form(mc);
   auto dense = [&](float z) {
-    const float x = (z - m) * c;
+    const float x = plain ? __builtin_fmaf(z, c, -mc) : exponent(z, m, mc, c);
     return __builtin_amdgcn_exp2f(x) * __builtin_fmaf(k1, fmaxf(x, kFloor), k0);
   };
 #pragma unroll
@@ -552,8 +661,10 @@ int64_t lp_align(int64_t v) { return (v + 255) / 256 * 256; }
 int lp_parts(int64_t rows, int64_t V, int32_t dtype) {
   const int64_t chunks = V / (dtype == SOUPK_DTYPE_F32 ? 4 : 8);
   const int64_t steps = (chunks + kLpThreads - 1) / kLpThreads;
-  const int64_t want = rows > 0 ? (int64_t{4} * device_cu_count() + rows - 1) / rows : 1;
-  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({want, steps / 2, kMaxParts})));
+  const int64_t want = rows > 0 ? (int64_t{kLpFill} * device_cu_count() + rows - 1) / rows : 1;
+  const int64_t least = steps * kLpThreads / (int64_t{1} << 27) + 1;   // (32-bit offsets in a part)
+  return static_cast<int>(
+      std::max<int64_t>(least, std::min<int64_t>({want, steps / 2, kMaxParts})));
 }
 
 bool bad_dtype(int32_t d) {
@@ -601,7 +712,7 @@ extern "C" __attribute__((visibility("default"))) int soupk_token_logprobs_fwd(
   const int parts = lp_parts(rows, V, dtype);
   const float inv_t = 1.0f / temperature;
   const float c = static_cast<float>(1.4426950408889634 / static_cast<double>(temperature));
-  const LpRows lr{inner, stride_outer, stride_inner, V};
+  const LpRows lr{inner, stride_outer, stride_inner, V, rows};
   const PartOut po{static_cast<Stats*>(workspace),
                    reinterpret_cast<Cand*>(static_cast<char*>(workspace) +
                                            lp_align(rows * parts *
@@ -620,9 +731,13 @@ extern "C" __attribute__((visibility("default"))) int soupk_token_logprobs_fwd(
     int rc = top_k > 0 ? run(token_logprobs_kernel<T, true>)
                        : run(token_logprobs_kernel<T, false>);
     if (rc != kOk || parts == 1) return rc;
-    return launch_kernel(token_logprobs_join_kernel<T>, dim3(static_cast<unsigned>(rows)),
-                         dim3(kWave), s, static_cast<const char*>(logits), tokens, lr, c, inv_t,
-                         static_cast<int>(top_k), parts, po, ro);
+    auto join = [&](auto kernel, int64_t blocks) {
+      return launch_kernel(kernel, dim3(static_cast<unsigned>(blocks)), dim3(kLpThreads), s,
+                           static_cast<const char*>(logits), tokens, lr, c, inv_t,
+                           static_cast<int>(top_k), parts, po, ro);
+    };
+    return top_k > 0 ? join(token_logprobs_join_kernel<T, true>, rows)
+                     : join(token_logprobs_join_kernel<T, false>, (rows + kLpWaves - 1) / kLpWaves);
   });
 }
 
@@ -640,7 +755,7 @@ extern "C" __attribute__((visibility("default"))) int soupk_token_logprobs_bwd(
   if (g_top != nullptr && (top_k == 0 || !top_id)) return kInvalid;
   const float inv_t = 1.0f / temperature;
   const float c = static_cast<float>(1.4426950408889634 / static_cast<double>(temperature));
-  const LpRows lr{inner, stride_outer, stride_inner, V};
+  const LpRows lr{inner, stride_outer, stride_inner, V, rows};
   return with_type(dtype, [&](auto tag) -> int {
     using T = typename decltype(tag)::type;
     constexpr int64_t kPer = kLpThreads * kLpUnroll;
