@@ -71,7 +71,10 @@ constexpr int kDigitBits = 9;
 constexpr int kDigits = 1 << kDigitBits;
 constexpr int kMaxBlocks = 64;
 constexpr int64_t kOneBlock = 4096;    // tokens that one workgroup sorts alone
-constexpr int64_t kHidden = 48 << 20;  // bytes of zeros that a launch of the sort carries
+// Bytes of zeros that a launch of the sort carries: what the chip writes in its time (one workgroup's
+// sort about 11 us, a histogram or scatter 9).  467 MB at 888 tokens 88 us without, 84 with 48 MB, 82
+// with 64; at 32768 tokens 138 without, 129 with 32 MB each, 127 with 48, 132 with 80.
+constexpr int64_t hidden_bytes(bool small) { return int64_t{small ? 64 : 48} << 20; }
 
 // Sorted positions that one workgroup adds: few when there are few tokens, so that the chip is filled.
 __host__ __device__ constexpr int run_length(int64_t M) { return M <= kOneBlock ? 8 : 32; }
@@ -117,12 +120,11 @@ __device__ __forceinline__ void scan_digits(SortLds& s, uint32_t total) {
 }
 
 // Moves the tokens [t0, t1) to their places by the digit at `shift`; s.base holds, per digit, the
-// place of the workgroup's first token of it.  s.count is clear and left clear.  place: in the last
-// pass, where each id's place is noted.
-template <typename Load>
+// place of the workgroup's first token of it.  s.count is clear.  store(place, key, token) is called
+// once per token.
+template <typename Load, typename Store>
 __device__ __forceinline__ void scatter_tokens(SortLds& s, int64_t t0, int64_t t1, int shift,
-                                               uint32_t* out_key, uint32_t* out_tok,
-                                               uint32_t* place, int64_t V, const Load& load) {
+                                               const Load& load, const Store& store) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   for (int64_t t = t0; t < t1; t += kSortThreads) {
     const int64_t i = t + threadIdx.x;
@@ -151,13 +153,8 @@ __device__ __forceinline__ void scatter_tokens(SortLds& s, int64_t t0, int64_t t
       s.base[threadIdx.x] = at;
     }
     __syncthreads();
-    if (on) {
-      const uint32_t to = s.count[w][digit] + rank;
-      out_key[to] = key;
-      out_tok[to] = tok;
-      // (any token's place will do: of an id's several writers any may win)
-      if (place != nullptr && key < static_cast<uint32_t>(V)) place[key] = to;
-    }
+    if (on) store(s.count[w][digit] + rank, key, tok);
+    if (t + kSortThreads >= t1) break;
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < kSortWaves * kDigits / kSortThreads; ++k)
@@ -208,7 +205,13 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_small_kernel(
     __syncthreads();
     if (threadIdx.x < kDigits) s.count[0][threadIdx.x] = 0;
     scan_digits(s, total);
-    scatter_tokens(s, 0, M, shift, ok, ot, p == passes - 1 ? place : nullptr, V, load);
+    const bool last = p == passes - 1;
+    scatter_tokens(s, 0, M, shift, load, [&](uint32_t to, uint32_t key, uint32_t tok) {
+      ok[to] = key;
+      ot[to] = tok;
+      // (any token's place will do: of an id's several writers any may win)
+      if (last && key < static_cast<uint32_t>(V)) place[key] = to;
+    });
     __threadfence_block();
     __syncthreads();
   }
@@ -248,26 +251,40 @@ __global__ __launch_bounds__(kSortThreads) void embedding_scatter_kernel(
   clear_counts(s);
   uint32_t total = 0, before = 0;
   if (threadIdx.x < kDigits) {
-    for (int b = 0; b < blocks; ++b) {
-      const uint32_t n = hist[threadIdx.x * kMaxBlocks + b];
-      before += b < static_cast<int>(blockIdx.x) ? n : 0u;
-      total += n;
-    }
+    // (four workgroups' counts a load, all loads in flight; those past the last workgroup are not used)
+    const u32x4* const row = reinterpret_cast<const u32x4*>(hist + threadIdx.x * kMaxBlocks);
+    u32x4 n[kMaxBlocks / 4];
+#pragma unroll
+    for (int q = 0; q < kMaxBlocks / 4; ++q) n[q] = 4 * q < blocks ? row[q] : u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int q = 0; q < kMaxBlocks / 4; ++q)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int b = 4 * q + e;
+        before += b < static_cast<int>(blockIdx.x) ? n[q][e] : 0u;
+        total += b < blocks ? n[q][e] : 0u;
+      }
     s.base[threadIdx.x] = before;
   }
   __syncthreads();
   scan_digits(s, total);
   const int64_t t0 = blockIdx.x * per, t1 = min(M, t0 + per);
-  scatter_tokens(s, t0, t1, shift, out_key, out_tok, place, V,
-                 [&](int64_t i, uint32_t& k, uint32_t& t) {
-    if (in_key == nullptr) {
-      k = sort_key(ids[i], V, padding);
-      t = static_cast<uint32_t>(i);
-    } else {
-      k = in_key[i];
-      t = in_tok[i];
-    }
-  });
+  scatter_tokens(
+      s, t0, t1, shift,
+      [&](int64_t i, uint32_t& k, uint32_t& t) {
+        if (in_key == nullptr) {
+          k = sort_key(ids[i], V, padding);
+          t = static_cast<uint32_t>(i);
+        } else {
+          k = in_key[i];
+          t = in_tok[i];
+        }
+      },
+      [&](uint32_t to, uint32_t key, uint32_t tok) {
+        out_key[to] = key;
+        out_tok[to] = tok;
+        if (place != nullptr && key < static_cast<uint32_t>(V)) place[key] = to;
+      });
 }
 
 // ---- sums ---------------------------------------------------------------------------------------
@@ -548,7 +565,7 @@ extern "C" __attribute__((visibility("default"))) int soupk_embedding_bwd(
   const int launches = M == 0 ? 0 : small ? 1 : 2 * passes;
   // The rows cleared with the sort: a multiple of 8 per launch (whole 16-byte words).
   const int64_t hidden_rows =
-      launches ? std::min<int64_t>(kHidden / row_bytes, V / launches) / 8 * 8 : 0;
+      launches ? std::min<int64_t>(hidden_bytes(small) / row_bytes, V / launches) / 8 * 8 : 0;
   auto zeros = [&](int k) {
     return Zeros{static_cast<char*>(dtable) + k * hidden_rows * row_bytes,
                  hidden_rows * row_bytes / 16};

@@ -43,6 +43,13 @@ constexpr int kGroup = kLpThreads / 64;   // neighbouring threads whose largest 
 #define SOUPK_LP_UNROLL 4
 #endif
 constexpr int kLpUnroll = SOUPK_LP_UNROLL;          // chunk loads in flight per thread
+#ifndef SOUPK_GRAD_UNROLL
+#define SOUPK_GRAD_UNROLL 4
+#endif
+#ifndef SOUPK_GRAD_THREADS
+#define SOUPK_GRAD_THREADS 256
+#endif
+constexpr int kGradThreads = SOUPK_GRAD_THREADS, kGradUnroll = SOUPK_GRAD_UNROLL;
 constexpr int kMaxTop = 32;
 #ifndef SOUPK_LP_FILL
 #define SOUPK_LP_FILL 4
@@ -571,7 +578,7 @@ struct LpGrads {
 // Workgroup (block of chunks, row).  dz = 2^x (k0 + k1 x), x as in the forward and the row's factors k0,
 // k1; then the few columns with a gradient of their own are written again by the thread that wrote them.
 template <typename T>
-__global__ __launch_bounds__(kLpThreads) void token_logprobs_bwd_kernel(
+__global__ __launch_bounds__(kGradThreads) void token_logprobs_bwd_kernel(
     const char* __restrict__ logits, const int64_t* __restrict__ tokens, LpRows rows, float c,
     float inv_t, int K, int64_t r0, int blocks, LpGrads g, char* __restrict__ dlogits) {
   constexpr int N = Chunk<T>::N;
@@ -600,12 +607,12 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_bwd_kernel(
   const float k1 = none ? 0.f : -inv_t * inv_s * (g_ent * kLn2);
   const float k0 = none ? 0.f : -inv_t * inv_s * (weight + g_ent * (g.entropy[r] - lse));
   const int64_t chunks = rows.V / N;
-  const int64_t first = static_cast<int64_t>(which) * (kLpThreads * kLpUnroll) + tid;
-  Chunk<T> w[kLpUnroll];
+  const int64_t first = static_cast<int64_t>(which) * (kGradThreads * kGradUnroll) + tid;
+  Chunk<T> w[kGradUnroll];
   if (!none) {
 #pragma unroll
-    for (int u = 0; u < kLpUnroll; ++u) {
-      const int64_t i = first + u * kLpThreads;
+    for (int u = 0; u < kGradUnroll; ++u) {
+      const int64_t i = first + u * kGradThreads;
       if (i < chunks) w[u].load(row + i * 16, 0);
     }
   }
@@ -616,8 +623,8 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_bwd_kernel(
     return __builtin_amdgcn_exp2f(x) * __builtin_fmaf(k1, fmaxf(x, kFloor), k0);
   };
 #pragma unroll
-  for (int u = 0; u < kLpUnroll; ++u) {
-    const int64_t i = first + u * kLpThreads;
+  for (int u = 0; u < kGradUnroll; ++u) {
+    const int64_t i = first + u * kGradThreads;
     if (i >= chunks) continue;
     float z[N];
     if (none) {
@@ -642,8 +649,8 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_bwd_kernel(
     const int64_t col = k < 0 ? tok : g.top_id[r * K + k];
     if (col < 0 || col >= rows.V) continue;
     const int64_t i = col / N;
-    const bool own = i < chunks ? i % kLpThreads == tid &&
-                                      i / (kLpThreads * kLpUnroll) == which
+    const bool own = i < chunks ? i % kGradThreads == tid &&
+                                      i / (kGradThreads * kGradUnroll) == which
                                 : has_tail && col - chunks * N == tid;
     if (!own) continue;
     float add = 0.f;
@@ -758,13 +765,13 @@ extern "C" __attribute__((visibility("default"))) int soupk_token_logprobs_bwd(
   const LpRows lr{inner, stride_outer, stride_inner, V, rows};
   return with_type(dtype, [&](auto tag) -> int {
     using T = typename decltype(tag)::type;
-    constexpr int64_t kPer = kLpThreads * kLpUnroll;
+    constexpr int64_t kPer = kGradThreads * kGradUnroll;
     const int64_t blocks = std::max<int64_t>(1, (V / Chunk<T>::N + kPer - 1) / kPer);
     const int64_t most = 0x7fffffff / blocks;        // rows of one launch
     for (int64_t r0 = 0; r0 < rows; r0 += most) {
       const int64_t n = std::min(most, rows - r0);
       const int rc = launch_kernel(
-          token_logprobs_bwd_kernel<T>, dim3(static_cast<unsigned>(n * blocks)), dim3(kLpThreads),
+          token_logprobs_bwd_kernel<T>, dim3(static_cast<unsigned>(n * blocks)), dim3(kGradThreads),
           static_cast<hipStream_t>(stream), static_cast<const char*>(logits), tokens, lr, c, inv_t,
           static_cast<int>(top_k), r0, static_cast<int>(blocks),
           LpGrads{row_max, row_sum, entropy, g_lp, g_ent, g_top, top_id},
