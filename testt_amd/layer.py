@@ -26,7 +26,10 @@ projection GEMM reads (the norm kernel rounds the same fp32 value into both), so
 runs the projection and both LoRA branches on y in one autograd node: A_q|A_v as one skinny
 GEMM, no padded fp32 copy, gather, casts or scatter-add, and in backward the LoRA input
 gradient accumulated into the projection's input-gradient GEMM.  The norm then writes no padded
-output at all.  With dropout the reference's path is kept (the padded layout fixes the draws).
+output at all.  With dropout the reference's path is kept (the padded layout fixes the draws),
+unless the dropout is a dropout.CounterDropout, whose draws do not depend on the layout
+(counter_lora_branch).  With q_norm / k_norm the query and key heads are RMS-normalised in the pass
+that rotates them (rope.qk_norm_rope).
 """
 
 import math
@@ -39,12 +42,13 @@ from . import blas as _blas
 from . import layer_native as _native
 from . import lora as _lora
 from . import workloads
+from .dropout import CounterDropout
 from .mlp import FusedNF4MLP, fused_mlp
 from .nf4 import (FrozenNF4Linear, frozen_linear, fused_grad_input, fused_linear,
                   keep_for_backward, unpack_concat, unpack_groups,
                   unpack_groups_lora, unpacked_for_backward)
 from .rmsnorm import AddRMSNorm, RMSNormNoAdd, add_rmsnorm
-from .rope import rope_pack
+from .rope import qk_norm_rope, rope_pack
 
 
 @dataclass
@@ -71,6 +75,9 @@ class LayerWeights:
     scaling_v: float = None         # LoRA scaling of v when it differs from q's
     lora_dropout: tuple = None      # (q, v) dropout modules to call (peft's), instead of dropout
     attn_scale: float = None        # attention softmax scale (None: 1/sqrt(head_dim))
+    q_norm: torch.Tensor = None     # [head_dim]: RMS norm of every query head before the rotation
+    k_norm: torch.Tensor = None     # [head_dim]: the same of the key heads (both or neither)
+    qk_eps: float = None            # their eps (None: eps)
 
 
 def synthetic_layer(device, hidden=workloads.HIDDEN, inter=workloads.INTER,
@@ -326,6 +333,22 @@ def lora_branch(y_pad, ab, scaling, dropout, batch, seq, pos_idx):
     return (rows @ a.to(torch.float16).t()) @ b.to(torch.float16).t() * scaling
 
 
+def counter_lora_branch(y, ab, scaling, dropout, pos_idx):
+    """lora_branch for a dropout.CounterDropout: its draws belong to the padded positions whatever
+    rows are there, so it runs on the real rows of the fp16 norm output y, and the norm writes no
+    padded copy."""
+    a, b = ab
+    rows = dropout.rows(y, pos_idx)
+    return (rows @ a.to(torch.float16).t()) @ b.to(torch.float16).t() * scaling
+
+
+def padded_heads(rows, pos_idx, batch, seq, n_heads, n_kv, head_dim):
+    """q [B, NH, T, D] and k, v [B, NKV, T, D] of token-major q|k|v rows, zeros at the padding."""
+    full = rows.new_zeros((batch * seq, rows.shape[1])).index_copy(0, pos_idx, rows)
+    full = full.view(batch, seq, n_heads + 2 * n_kv, head_dim).transpose(1, 2)
+    return tuple(t.contiguous() for t in full.split((n_heads, n_kv, n_kv), dim=1))
+
+
 def attention(q, k, v, key_valid, scale=None):
     """Causal GQA attention of the padded [B, heads, T, D] layout -> token-major [B*T, NH*D].
 
@@ -472,6 +495,9 @@ def decoder_layer(s, delta, w, pos_idx, batch, seq, cos, sin, key_valid):
     padded."""
     padded = batch * seq
     nh, nkv, hd = w.n_heads, w.n_kv, w.head_dim
+    normed = w.q_norm is not None
+    if normed != (w.k_norm is not None):
+        raise ValueError("q_norm and k_norm go together")
     plain = lora_without_dropout(w)
     params = (w.lora_q[0], w.lora_v[0], w.lora_q[1], w.lora_v[1]) if plain else None
     w_qkv = w_o = w_gu = w_d = staged = None
@@ -484,7 +510,7 @@ def decoder_layer(s, delta, w, pos_idx, batch, seq, cos, sin, key_valid):
                 groups, s.device, tuple(p.detach() for p in params))
         else:
             w_qkv, w_o, w_gu, w_d = unpack_groups(groups, s.device)
-    if plain and FUSE_LORA_ROPE and USE_FUSED_LORA and USE_VARLEN_ATTENTION and \
+    if plain and not normed and FUSE_LORA_ROPE and USE_FUSED_LORA and USE_VARLEN_ATTENTION and \
             hd == _attention.HEAD_DIM and nkv > 0 and nh % nkv == 0 and \
             w.lora_q[1].shape[0] == nh * hd and w.lora_v[1].shape[0] == nkv * hd and \
             _lora.params_supported(*params, s.device):
@@ -522,19 +548,38 @@ def decoder_layer(s, delta, w, pos_idx, batch, seq, cos, sin, key_valid):
                                     (w.q, w.k, w.v), w_qkv, staged)
     else:
         any_lora = w.lora_q is not None or w.lora_v is not None
-        if any_lora:
+        drops = w.lora_dropout if w.lora_dropout is not None else (w.dropout, w.dropout)
+        scales = (w.scaling, w.scaling if w.scaling_v is None else w.scaling_v)
+        counted = any_lora and all(ab is None or isinstance(dr, CounterDropout)
+                                   for ab, dr in zip((w.lora_q, w.lora_v), drops))
+        y_pad = None
+        if any_lora and not counted:
             s, y, y_pad = add_rmsnorm(s, delta, w.input_norm, w.eps, pos_idx, padded)
         else:
             s, y, _ = add_rmsnorm(s, delta, w.input_norm, w.eps)
         qkv = frozen_linear(y, (w.q, w.k, w.v), w.qkv_bias, w_qkv)
-        drops = w.lora_dropout if w.lora_dropout is not None else (w.dropout, w.dropout)
-        scales = (w.scaling, w.scaling if w.scaling_v is None else w.scaling_v)
         lq, lv = (None if ab is None else
+                  counter_lora_branch(y, ab, sc, dr, pos_idx) if counted else
                   lora_branch(y_pad, ab, sc, dr, batch, seq, pos_idx)
                   for ab, sc, dr in zip((w.lora_q, w.lora_v), scales, drops))
-        if any_lora:
-            del y_pad
-    if USE_VARLEN_ATTENTION and _attention.varlen_supported(qkv, hd, nh, nkv):
+        del y_pad
+    if normed:
+        eps = w.eps if w.qk_eps is None else w.qk_eps
+        if USE_VARLEN_ATTENTION and _attention.varlen_supported(qkv, hd, nh, nkv):
+            cu = _attention.cu_seqlens_of(pos_idx, batch, seq)
+            a = _attention.norm_rope_attention(qkv, lq, lv, w.q_norm, w.k_norm, cos, sin, pos_idx,
+                                               cu, batch, seq, nh, nkv, eps, w.attn_scale)
+        else:
+            rows = qk_norm_rope(qkv, lq, lv, w.q_norm, w.k_norm, cos, sin, pos_idx, batch, seq, nh,
+                                nkv, hd, eps)
+            q, k, v = padded_heads(rows, pos_idx, batch, seq, nh, nkv, hd)
+            del rows
+            a = attention(q, k, v, key_valid, w.attn_scale)
+            del q, k, v
+            if pos_idx.numel() != padded:
+                a = a.index_select(0, pos_idx)
+        del qkv, lq, lv, w_qkv
+    elif USE_VARLEN_ATTENTION and _attention.varlen_supported(qkv, hd, nh, nkv):
         # the real tokens only: rows of batch row b are cu[b] .. cu[b+1] of the sorted pos_idx
         cu = _attention.cu_seqlens_of(pos_idx, batch, seq)
         a = _attention.rope_attention(qkv, lq, lv, cos, sin, pos_idx, cu, batch, seq, nh, nkv,

@@ -42,6 +42,7 @@ from dataclasses import dataclass, field
 
 import torch
 
+from . import embedding as _embedding
 from . import layer as _layer
 from ._common import kernels_ok
 from .head import IGNORE_INDEX, fused_head_loss
@@ -165,7 +166,7 @@ class LayerPlan:
     LoRA state is read on every forward."""
 
     __slots__ = ("layer", "attn", "q", "k", "v", "o", "gate", "up", "down", "qkv_bias",
-                 "o_bias", "lora_modules")
+                 "o_bias", "lora_modules", "q_norm", "k_norm")
 
     def __init__(self, layer):
         self.layer = layer
@@ -193,6 +194,18 @@ class LayerPlan:
         for m in (attn.k_proj, attn.o_proj, mlp.gate_proj, mlp.up_proj, mlp.down_proj):
             if _lora_parts(m) is not None:
                 raise ValueError("LoRA outside q_proj/v_proj")
+        # Per-head norms of queries and keys, where the attention has them: RMS norms over the head
+        # dim that carry their eps as the layer's own norms do.
+        self.q_norm, self.k_norm = getattr(attn, "q_norm", None), getattr(attn, "k_norm", None)
+        if (self.q_norm is None) != (self.k_norm is None):
+            raise ValueError("a norm on only one of queries and keys")
+        if self.q_norm is not None:
+            for n in (self.q_norm, self.k_norm):
+                if getattr(n, "variance_epsilon", None) is None or n.weight.dim() != 1 or \
+                        getattr(n, "bias", None) is not None:
+                    raise ValueError("a query or key norm that is not a plain RMS norm")
+            if self.q_norm.variance_epsilon != self.k_norm.variance_epsilon:
+                raise ValueError("the query and key norms have different eps")
 
 
 class ModelPlan:
@@ -217,6 +230,11 @@ class ModelPlan:
         if self.head_dim % 2:
             raise ValueError("odd head_dim")
         self.layers = [LayerPlan(lyr) for lyr in inner.layers[:cfg.num_hidden_layers]]
+        for lp in self.layers:
+            if lp.q_norm is not None and (
+                    self.head_dim % 16 or self.head_dim > 256 or
+                    any(n.weight.numel() != self.head_dim for n in (lp.q_norm, lp.k_norm))):
+                raise ValueError("query and key norms that are not per head of 16 to 256 dims")
         self.embed = inner.embed_tokens
         self.head = causal_lm.lm_head
         self.norm = inner.norm
@@ -247,7 +265,10 @@ class ModelPlan:
             n_heads=self.n_heads, n_kv=self.n_kv, head_dim=self.head_dim, eps=eps_in,
             dropout=max(_dropout_p(d) for d in drop if d is not None) if any(
                 d is not None for d in drop) else 0.0,
-            lora_dropout=tuple(drop), attn_scale=getattr(lp.attn, "scaling", None))
+            lora_dropout=tuple(drop), attn_scale=getattr(lp.attn, "scaling", None),
+            **({} if lp.q_norm is None else dict(
+                q_norm=lp.q_norm.weight, k_norm=lp.k_norm.weight,
+                qk_eps=lp.q_norm.variance_epsilon)))
 
 
 def model_plan(causal_lm):
@@ -375,7 +396,10 @@ def _forward(model, cos, sin, input_ids, attention_mask, labels, num_items_in_ba
     pos_idx = attention_mask.reshape(-1).nonzero().squeeze(1)
 
     ids = input_ids.reshape(-1).index_select(0, pos_idx)
-    s = torch.nn.functional.embedding(ids, model.embed).float()
+    if _embedding.supported(model.embed):     # (the fp32 residual stream in one launch)
+        s = _embedding.embedding(ids, model.embed, out_dtype=torch.float32)
+    else:
+        s = torch.nn.functional.embedding(ids, model.embed).float()
     key_valid = _layer.key_valid_of(attention_mask)
 
     delta = None
