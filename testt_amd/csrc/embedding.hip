@@ -608,7 +608,8 @@ extern "C" __attribute__((visibility("default"))) int soupk_embedding_bwd(
   const int run = run_length(M);
   const int64_t runs = (M + run - 1) / run;
   const int col_blocks = static_cast<int>((H8 / 8 + kEmbThreads - 1) / kEmbThreads);
-  if (runs * col_blocks > (int64_t{1} << 30)) return kInvalid;
+  const int join_blocks = static_cast<int>((H + kJoinCols - 1) / kJoinCols);
+  if (runs * join_blocks > (int64_t{1} << 30)) return kInvalid;     // (>= runs * col_blocks)
   const int64_t row_items = (row_bytes + 15) / 16;
   const int64_t rows_per =
       std::max<int64_t>(1, ((int64_t{1} << 30) - kEmbThreads) / row_items);
@@ -637,7 +638,6 @@ extern "C" __attribute__((visibility("default"))) int soupk_embedding_bwd(
           cut.sums = 0;
         } while (row < V);
         if (M == 0) return kOk;
-        const int join_blocks = static_cast<int>((H + kJoinCols - 1) / kJoinCols);
         return launch_kernel(embedding_join_kernel<E>,
                              dim3(static_cast<unsigned>(runs * join_blocks)), dim3(kEmbThreads), s,
                              skey, static_cast<const float*>(partial), static_cast<char*>(dtable),

@@ -33,23 +33,11 @@
 namespace soupk {
 namespace {
 
-#ifndef SOUPK_LP_THREADS
-#define SOUPK_LP_THREADS 256
-#endif
-constexpr int kLpThreads = SOUPK_LP_THREADS;
+constexpr int kLpThreads = 256;
 constexpr int kLpWaves = kLpThreads / kWave;
 constexpr int kGroup = kLpThreads / 64;   // neighbouring threads whose largest value bounds the list
-#ifndef SOUPK_LP_UNROLL
-#define SOUPK_LP_UNROLL 4
-#endif
-constexpr int kLpUnroll = SOUPK_LP_UNROLL;          // chunk loads in flight per thread
-#ifndef SOUPK_GRAD_UNROLL
-#define SOUPK_GRAD_UNROLL 4
-#endif
-#ifndef SOUPK_GRAD_THREADS
-#define SOUPK_GRAD_THREADS 256
-#endif
-constexpr int kGradThreads = SOUPK_GRAD_THREADS, kGradUnroll = SOUPK_GRAD_UNROLL;
+constexpr int kLpUnroll = 4;          // chunk loads in flight per thread
+constexpr int kGradThreads = 256, kGradUnroll = 4;
 constexpr int kMaxTop = 32;
 #ifndef SOUPK_LP_FILL
 #define SOUPK_LP_FILL 4
@@ -588,18 +576,24 @@ __global__ __launch_bounds__(kGradThreads) void token_logprobs_bwd_kernel(
   const char* const row = logits + rows.at(r) * kSize;
   char* const drow = dlogits + r * rows.V * kSize;
   const int tid = threadIdx.x;
+  // The columns with a gradient of their own, one a lane in every wavefront: the alternatives' in lanes
+  // 0 .. K - 1, the token's in lane 63.
+  const int lane = tid & 63;
   const int64_t tok = tokens[r];
   const bool has_tok = g.g_lp != nullptr && tok >= 0 && tok < rows.V;
-  const float g_tok = has_tok ? g.g_lp[r] : 0.f;
+  int64_t col = -1;
+  float g_col = 0.f;
+  if (lane == 63 && has_tok) {
+    col = tok;
+    g_col = g.g_lp[r];
+  }
+  if (g.g_top != nullptr && lane < K) {
+    col = g.top_id[r * K + lane];
+    g_col = g.g_top[r * K + lane];
+  }
   const float g_ent = g.g_ent != nullptr ? g.g_ent[r] : 0.f;
-  float weight = g_tok;
-  bool none = g_tok == 0.f && g_ent == 0.f;
-  if (g.g_top != nullptr)
-    for (int k = 0; k < K; ++k) {
-      const float v = g.g_top[r * K + k];
-      weight = weight + v;
-      none = none && v == 0.f;
-    }
+  const float weight = wave_sum(g_col);
+  const bool none = g_ent == 0.f && !__any(g_col != 0.f);
   const float m = g.row_max[r], sum = g.row_sum[r];
   const float inv_s = 1.0f / sum;
   const float lse = logf(sum);
@@ -643,22 +637,22 @@ __global__ __launch_bounds__(kGradThreads) void token_logprobs_bwd_kernel(
     Elem<T>::store1(drow + tail * kSize,
                     none ? 0.f : dense(Elem<T>::load1(row + tail * kSize)));
   if (none) return;
-  // The token's column and the alternatives': -1 stands for the token.
-  const int tops = g.g_top != nullptr ? K : 0;
-  for (int k = has_tok ? -1 : 0; k < tops; ++k) {
-    const int64_t col = k < 0 ? tok : g.top_id[r * K + k];
-    if (col < 0 || col >= rows.V) continue;
-    const int64_t i = col / N;
-    const bool own = i < chunks ? i % kGradThreads == tid &&
-                                      i / (kGradThreads * kGradUnroll) == which
-                                : has_tail && col - chunks * N == tid;
-    if (!own) continue;
-    float add = 0.f;
-    for (int q = has_tok ? -1 : 0; q < tops; ++q)
-      if ((q < 0 ? tok : g.top_id[r * K + q]) == col)
-        add = add + (q < 0 ? g_tok : g.g_top[r * K + q]);
-    const float z = Elem<T>::load1(row + col * kSize);
-    Elem<T>::store1(drow + col * kSize, dense(z) + add * inv_t);
+  // Those of them that lie in this workgroup's columns are written again, each by the thread that wrote
+  // it before (its stores to one address stay in order), with the gradients of all its mentions.
+  const int64_t at = col / N;
+  const bool here = col >= 0 && col < rows.V &&
+                    (at < chunks ? at / (kGradThreads * kGradUnroll) == which : has_tail);
+  for (uint64_t left = __ballot(here); left != 0; left &= left - 1) {
+    const int k = __builtin_ctzll(left);
+    const int64_t one =
+        static_cast<int64_t>(static_cast<uint32_t>(
+            __builtin_amdgcn_readlane(static_cast<int>(col), k)));   // (a column: below 2^31)
+    const float add = wave_sum(col == one ? g_col : 0.f);
+    const int64_t chunk = one / N;
+    const int owner = static_cast<int>(chunk < chunks ? chunk % kGradThreads : one - chunks * N);
+    if (owner != tid) continue;
+    const float z = Elem<T>::load1(row + one * kSize);
+    Elem<T>::store1(drow + one * kSize, dense(z) + add * inv_t);
   }
 }
 

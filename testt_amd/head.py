@@ -400,7 +400,8 @@ def _chunk_logprobs(logits, tokens, top_k, temperature, outs):
     rows, vocab = logits.shape
     code = _ext.DTYPES[logits.dtype]
     need = ctypes.c_int64()
-    _ext.call("soupk_token_logprobs_workspace", rows, vocab, top_k, code, ctypes.addressof(need))
+    _ext.call_on(logits, "soupk_token_logprobs_workspace", rows, vocab, top_k, code,
+                 ctypes.addressof(need))
     ws = torch.empty(need.value, dtype=torch.uint8, device=logits.device)
     _ext.call_on(logits, "soupk_token_logprobs_fwd", logits.data_ptr(), code, tokens.data_ptr(),
                  rows, rows, 0, vocab, vocab, temperature, top_k, *(o.data_ptr() for o in outs),
@@ -454,6 +455,12 @@ def token_logprobs(logits, tokens, top_k=0, temperature=1.0):
         _ext.host().token_logprobs(logits, tokens.contiguous(), top_k, temperature)))
 
 
+def _head_logits(hidden, weight):
+    """hidden @ weight^T in fp16, whatever autocast is set to."""
+    with torch.autocast("cuda", enabled=False):
+        return _blas.linear(hidden, weight)
+
+
 class _HiddenLogprobs(torch.autograd.Function):
     """token_logprobs(hidden @ weight^T, ...) in chunks of CHUNK_ROWS rows, for a frozen head: no
     chunk's logits outlive it.  The backward forms them again."""
@@ -466,7 +473,7 @@ class _HiddenLogprobs(torch.autograd.Function):
                  torch.empty((rows, top_k), dtype=torch.int64, device=dev)]
         for start in range(0, rows, CHUNK_ROWS):
             part = slice(start, min(rows, start + CHUNK_ROWS))
-            logits = _blas.linear(hidden[part], weight)
+            logits = _head_logits(hidden[part], weight)
             _chunk_logprobs(logits, tokens[part], top_k, temperature, [o[part] for o in outs])
             del logits
         lp, ent, row_max, row_sum, top_lp, top_ids = outs
@@ -484,12 +491,12 @@ class _HiddenLogprobs(torch.autograd.Function):
             return None, None, None, None, None
         hidden, weight, tokens, row_max, row_sum, ent, top_ids = ctx.saved_tensors
         # The fp16 gradient of the logits is held at a power of two that brings the largest upstream
-        # gradient to 32 .. 64 (as _grad_unit does for the loss): most of its entries are p * g, far
+        # gradient, over the temperature, to 32 .. 64 (as _grad_unit does for the loss): most of its entries are p * g, far
         # below fp16's range otherwise.  Scaling by a power of two is exact.
         tops = [g.detach().to(torch.float32).abs().amax().reshape(1) for g in grads
                 if g is not None and g.numel()]
         top = torch.cat(tops).amax() if tops else hidden.new_ones((), dtype=torch.float32)
-        _, exponent = torch.frexp(torch.where(top > 0, top, 1.0))
+        _, exponent = torch.frexp(torch.where(top > 0, top / ctx.args[1], 1.0))
         exponent = exponent.clamp(-100, 100)
         unit = torch.ldexp(torch.ones_like(top), 6 - exponent)
         grads = [None if g is None else (g.to(torch.float32) * unit).contiguous() for g in grads]
@@ -498,7 +505,7 @@ class _HiddenLogprobs(torch.autograd.Function):
         dh = torch.empty_like(hidden)
         for start in range(0, rows, CHUNK_ROWS):
             part = slice(start, min(rows, start + CHUNK_ROWS))
-            logits = _blas.linear(hidden[part], weight)
+            logits = _head_logits(hidden[part], weight)
             g = torch.empty_like(logits)
             _chunk_logprobs_grad(logits, tokens[part], [t[part] for t in (row_max, row_sum, ent)],
                                  top_ids[part], [None if x is None else x[part] for x in grads],
