@@ -125,6 +125,36 @@ def test_masked_rows(rows, vocab, dtype):
     compare(z, tok, 32, 0.5, seed=2)
 
 
+@pytest.mark.parametrize("vocab", [7000, 8192, 40000, 40007])
+@pytest.mark.parametrize("dtype,top_k", [(torch.float16, 32), (torch.float32, 32),
+                                         (torch.float32, 3), (torch.bfloat16, 8)])
+def test_rising_rows(vocab, dtype, top_k):
+    """Rows that rise from left to right, whole (enough of them not to be cut into parts): the lists of
+    candidates overflow and the row is searched.  Others among them fall, or rise in a few wide steps
+    of equal columns."""
+    print(f"rising {vocab} {dtype} top {top_k}", flush=True)
+    rows = 1030
+    z, tok = logits_of(8, vocab, dtype, vocab)
+    ramp = torch.linspace(-8, 8, vocab)
+    z[0], z[1] = ramp.to(dtype), ramp.flip(0).to(dtype)
+    z[2] = (ramp * 0.5).floor().to(dtype)
+    z[3] = (ramp * 4).floor().to(dtype)
+    z[4, : vocab // 2] = float("-inf")
+    z[4, vocab // 2:] = ramp[vocab // 2:].to(dtype)
+    z[5] = float("-inf")
+    z[5, vocab // 3: vocab // 3 + 20] = 1.0
+    many = z.repeat(rows // 8 + 1, 1)[:rows]
+    got = head.token_logprobs(many.to(DEV), tok.repeat(rows // 8 + 1)[:rows].to(DEV), top_k)
+    want = reference(z.double(), tok, top_k)
+    ids = want[3].repeat(rows // 8 + 1, 1)[:rows]
+    assert torch.equal(got.top_ids.cpu(), ids)
+    lp = want[2].repeat(rows // 8 + 1, 1)[:rows]
+    rel, _, x, _ = bounds(z.double(), 1.0)
+    tol = (rel[:, None] + 4 * U * (x.gather(-1, want[3]).abs().nan_to_num(posinf=0.0) + 1)).repeat(
+        rows // 8 + 1, 1)[:rows]
+    check(got.top_logprobs, lp, tol, "top")
+
+
 def test_rows_without_a_distribution():
     """A row of -inf alone, one with NaN, one with +inf: NaN numbers, ordered ids; other rows
     unharmed, and a row without upstream gradient keeps a zero gradient."""
