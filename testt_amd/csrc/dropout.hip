@@ -15,10 +15,12 @@
 // and once more to the output's type.  A dropped element is replaced, not multiplied by zero, so an
 // infinity or NaN under the mask does not survive.
 //
-// Bound: memory.  A thread takes 8 consecutive columns of one row: two 16-byte (fp32: four) vector
-// accesses beside two generator calls.  On MI355X a copy of 147 MB of fp16 runs at 5.87 TB/s and
-// with the draws at 5.79 (16 bits per element would give 5.93: the multiplies hide under the
-// traffic, so every element gets the full word).
+// Bound: memory.  On MI355X a copy of 147 MB of fp16 runs at 5.87 TB/s and with the draws at 5.79 (16
+// bits per element would give 5.93: the multiplies hide under the traffic, so every element gets the
+// full word).  What a thread takes follows the result's type, so that each store of a wavefront fills
+// whole lines: 8 columns for 16-bit results, 4 and 4 more 256 items on for fp32 ones.  8192 x 8960 fp16
+// into an fp32 residual 128 -> 114 us (6.4 TB/s) against 8 columns in two stores; 16-bit results in 4
+// columns take 147 instead of 115 us (forward and backward).
 
 #include <algorithm>
 #include <type_traits>
@@ -30,6 +32,17 @@ namespace soupk {
 namespace {
 
 constexpr int kDropThreads = 256;
+
+// Columns of an item, and items of a thread: a wavefront's store covers whole lines.  An fp32 result
+// goes out as 16 bytes of 4 columns (two items a thread), a 16-bit one as 16 bytes of 8.
+template <typename Out>
+constexpr int item_cols() {
+  return Elem<Out>::kBytes == 4 ? 4 : 8;
+}
+template <typename Out>
+constexpr int thread_items() {
+  return Elem<Out>::kBytes == 4 ? 2 : 1;
+}
 
 struct Draw {
   uint32_t key0, key1, call0, call1;
@@ -58,48 +71,58 @@ __global__ __launch_bounds__(kDropThreads) void dropout_kernel(
     const char* __restrict__ x, const char* __restrict__ residual, char* __restrict__ out,
     const int64_t* __restrict__ rows, const int64_t* __restrict__ seed, Draw d, float scale,
     uint32_t items, int64_t row0, int64_t C, FastDiv per_row) {
-  const uint32_t i = blockIdx.x * kDropThreads + threadIdx.x;
-  if (i >= items) return;
-  const uint32_t r = per_row.div(i);
-  const uint32_t c8 = i - r * per_row.d;
-  const int64_t row = row0 + r;
-  const int64_t at = row * C + static_cast<int64_t>(c8) * 8;
-  const int n = static_cast<int>(min(int64_t{8}, C - static_cast<int64_t>(c8) * 8));
+  constexpr int N = item_cols<Out>(), U = thread_items<Out>();
   if (seed != nullptr) {
     const uint64_t s = static_cast<uint64_t>(*seed);
     d.key0 = static_cast<uint32_t>(s);
     d.key1 = static_cast<uint32_t>(s >> 32);
   }
-  const uint32_t R = static_cast<uint32_t>(rows != nullptr ? rows[row] : row);
-  float v[8], e[8];
-  if (n == 8) {
-    const auto raw = Elem<In>::template load8<true>(x + at * Elem<In>::kBytes);
-    if constexpr (RES) {
-      const auto rr = Elem<Out>::template load8<true>(residual + at * Elem<Out>::kBytes);
-      Elem<Out>::unpack8(rr, e);
-    }
-    Elem<In>::unpack8(raw, v);
-  } else {
+  const uint32_t i0 = blockIdx.x * (kDropThreads * U) + threadIdx.x;
+  float v[U][N], e[U][N];
+  uint32_t block[U], drawn[U];
+  int64_t at[U];
+  int n[U];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[j] = j < n ? Elem<In>::load1(x + (at + j) * Elem<In>::kBytes) : 0.f;
-      if constexpr (RES)
-        e[j] = j < n ? Elem<Out>::load1(residual + (at + j) * Elem<Out>::kBytes) : 0.f;
+  for (int u = 0; u < U; ++u) {
+    const uint32_t i = min(i0 + u * kDropThreads, items - 1);   // (past the end: the last item, unused)
+    const uint32_t r = per_row.div(i);
+    block[u] = i - r * per_row.d;
+    const int64_t row = row0 + r, col = static_cast<int64_t>(block[u]) * N;
+    at[u] = row * C + col;
+    n[u] = static_cast<int>(min(int64_t{N}, C - col));
+    drawn[u] = static_cast<uint32_t>(rows != nullptr ? rows[row] : row);
+    if (n[u] == N) {
+      load_n<In, N, true>(x + at[u] * Elem<In>::kBytes, v[u]);
+      if constexpr (RES) load_n<Out, N, true>(residual + at[u] * Elem<Out>::kBytes, e[u]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        v[u][j] = j < n[u] ? Elem<In>::load1(x + (at[u] + j) * Elem<In>::kBytes) : 0.f;
+        if constexpr (RES)
+          e[u][j] = j < n[u] ? Elem<Out>::load1(residual + (at[u] + j) * Elem<Out>::kBytes) : 0.f;
+      }
     }
   }
-  const u32x4 lo = philox(2 * c8, R, d), hi = philox(2 * c8 + 1, R, d);
-  const uint32_t w[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    v[j] = (w[j] >= d.limit && !d.drop_all) ? v[j] * scale : 0.f;
-    if constexpr (RES) v[j] = e[j] + v[j];
-  }
-  if (n == 8) {
-    Elem<Out>::template store8<true>(out + at * Elem<Out>::kBytes, v);
-  } else {
+  for (int u = 0; u < U; ++u) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j < n) Elem<Out>::store1(out + (at + j) * Elem<Out>::kBytes, v[j]);
+    for (int q = 0; q < N / 4; ++q) {
+      const u32x4 w = philox(block[u] * (N / 4) + q, drawn[u], d);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float& y = v[u][4 * q + j];
+        y = (w[j] >= d.limit && !d.drop_all) ? y * scale : 0.f;
+        if constexpr (RES) y = e[u][4 * q + j] + y;
+      }
+    }
+    if (i0 + u * kDropThreads >= items) return;
+    if (n[u] == N) {
+      store_n<Out, N, true>(out + at[u] * Elem<Out>::kBytes, v[u]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (j < n[u]) Elem<Out>::store1(out + (at[u] + j) * Elem<Out>::kBytes, v[u][j]);
+    }
   }
 }
 
@@ -113,7 +136,7 @@ extern "C" __attribute__((visibility("default"))) int soupk_dropout(
     const int64_t* rows, const int64_t* seed_dev, int64_t seed, int64_t call, int64_t limit,
     float scale, int64_t R, int64_t C, void* stream) {
   if (R < 0 || C < 0 || limit < 0 || limit > (int64_t{1} << 32)) return kInvalid;
-  if (C > (int64_t{1} << 33) || (C > 0 && R > (int64_t{1} << 62) / C)) return kInvalid;
+  if (C > (int64_t{1} << 32) || (C > 0 && R > (int64_t{1} << 62) / C)) return kInvalid;
   if (x_dtype != out_dtype && x_dtype != SOUPK_DTYPE_F32 && out_dtype != SOUPK_DTYPE_F32)
     return kInvalid;
   if (R == 0 || C == 0) return kOk;
@@ -126,18 +149,19 @@ extern "C" __attribute__((visibility("default"))) int soupk_dropout(
   const Draw d{static_cast<uint32_t>(key), static_cast<uint32_t>(key >> 32),
                static_cast<uint32_t>(off), static_cast<uint32_t>(off >> 32),
                all ? 0xffffffffu : static_cast<uint32_t>(limit), all};
-  const int64_t per_row = (C + 7) / 8;                     // <= 2^30: a row fits one launch
-  const int64_t rows_per = std::max<int64_t>(1, ((int64_t{1} << 31) - 1 - kDropThreads) / per_row);
-  const FastDiv div(static_cast<uint32_t>(per_row));
   return with_type(x_dtype, [&](auto in) {
     return with_type(out_dtype, [&](auto o) -> int {
       using In = typename decltype(in)::type;
       using Out = typename decltype(o)::type;
       if constexpr (std::is_same_v<In, Out> || std::is_same_v<In, float> ||
                     std::is_same_v<Out, float>) {
+        constexpr int64_t kCols = item_cols<Out>(), kPer = kDropThreads * thread_items<Out>();
+        const int64_t per_row = (C + kCols - 1) / kCols;      // (<= 2^30: a row fits one launch)
+        const int64_t rows_per = std::max<int64_t>(1, ((int64_t{1} << 31) - 1 - kPer) / per_row);
+        const FastDiv div(static_cast<uint32_t>(per_row));
         for (int64_t r0 = 0; r0 < R; r0 += rows_per) {
           const uint32_t items = static_cast<uint32_t>(std::min(rows_per, R - r0) * per_row);
-          const dim3 grid((items + kDropThreads - 1) / kDropThreads), block(kDropThreads);
+          const dim3 grid(static_cast<unsigned>((items + kPer - 1) / kPer)), block(kDropThreads);
           hipStream_t s = static_cast<hipStream_t>(stream);
           auto run = [&](auto kernel) {
             return launch_kernel(kernel, grid, block, s, static_cast<const char*>(x),

@@ -6,6 +6,8 @@
 // the compiler that it may not assume more than the element's own alignment).
 #pragma once
 
+#include <type_traits>
+
 #include "soupk_common.hpp"
 
 namespace soupk {
@@ -39,6 +41,22 @@ __device__ __forceinline__ uint32_t pack_b2(float a, float b) {
   typedef bf16 bf16x2 __attribute__((ext_vector_type(2)));
   bf16x2 v = {static_cast<bf16>(a), static_cast<bf16>(b)};
   return __builtin_bit_cast(uint32_t, v);
+}
+
+typedef u32x2 u32x2_a2 __attribute__((aligned(2)));
+
+// 8 bytes at any even address.
+template <bool NT>
+__device__ __forceinline__ u32x2 ld8(const void* p) {
+  const u32x2_a2* q = static_cast<const u32x2_a2*>(p);
+  if constexpr (NT) return __builtin_nontemporal_load(q);
+  else return *q;
+}
+template <bool NT>
+__device__ __forceinline__ void st8(void* p, u32x2 v) {
+  u32x2_a2* q = static_cast<u32x2_a2*>(p);
+  if constexpr (NT) __builtin_nontemporal_store(v, q);
+  else *q = v;
 }
 
 // Elem<T>: T is the element as stored (f16, bf16, float).  kBytes of one element; Raw8, eight
@@ -128,6 +146,38 @@ struct Elem<float> {
   }
   static __device__ __forceinline__ void store1(void* p, float v) { *static_cast<float*>(p) = v; }
 };
+
+// N = 4 or 8 consecutive elements to and from fp32.
+template <typename T, int N, bool NT>
+__device__ __forceinline__ void load_n(const char* p, float* v) {
+  static_assert(N == 4 || N == 8, "");
+  if constexpr (N == 8) {
+    Elem<T>::unpack8(Elem<T>::template load8<NT>(p), v);
+  } else if constexpr (std::is_same_v<T, float>) {
+    const f32x4 f = __builtin_bit_cast(f32x4, ld16<NT>(p));
+    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+  } else {
+    const u32x2 w = ld8<NT>(p);
+    if constexpr (std::is_same_v<T, f16>) {
+      v[0] = lo_h(w.x); v[1] = hi_h(w.x); v[2] = lo_h(w.y); v[3] = hi_h(w.y);
+    } else {
+      v[0] = bf2f(w.x & 0xffffu); v[1] = bf2f(w.x >> 16);
+      v[2] = bf2f(w.y & 0xffffu); v[3] = bf2f(w.y >> 16);
+    }
+  }
+}
+template <typename T, int N, bool NT>
+__device__ __forceinline__ void store_n(char* p, const float* v) {
+  static_assert(N == 4 || N == 8, "");
+  if constexpr (N == 8)
+    Elem<T>::template store8<NT>(p, v);
+  else if constexpr (std::is_same_v<T, float>)
+    st16<NT>(p, __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]}));
+  else if constexpr (std::is_same_v<T, f16>)
+    st8<NT>(p, u32x2{pack_h2(v[0], v[1]), pack_h2(v[2], v[3])});
+  else
+    st8<NT>(p, u32x2{pack_b2(v[0], v[1]), pack_b2(v[2], v[3])});
+}
 
 // Host: calls f(Elem type tag) for a SOUPK_DTYPE_* code; kInvalid for any other code.
 template <typename T>

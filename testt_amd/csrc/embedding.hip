@@ -1,7 +1,7 @@
 // Embedding lookup with a scale, and the gradient of the table.
 //
 // Forward:  out[i] = table[ids[i]] * scale, in fp32, rounded once to the output's type; an id outside
-// [0, V) gives a row of zeros.  One thread per 8 columns; bound by the rows it copies.
+// [0, V) gives a row of zeros.  Bound by the rows it copies.
 //
 // Gradient:  dtable[v] = scale * sum of dout[i] over the tokens i with ids[i] = v, zero for the rows
 // that no token names (nor for padding_idx).  The tokens are sorted by id, stably, so each row's sum
@@ -36,26 +36,33 @@ namespace {
 
 constexpr int kEmbThreads = 256;
 
+// A thread takes 16 bytes of the result: a wavefront's store fills whole lines.
+template <typename Out>
+constexpr int lookup_cols() {
+  return 16 / Elem<Out>::kBytes;
+}
+
 template <typename In, typename Out>
 __global__ __launch_bounds__(kEmbThreads) void embedding_fwd_kernel(
     const char* __restrict__ table, const int64_t* __restrict__ ids, char* __restrict__ out,
     float scale, int64_t V, int64_t H, uint32_t items, int64_t row0, FastDiv per_row) {
+  constexpr int N = lookup_cols<Out>();
   const uint32_t i = blockIdx.x * kEmbThreads + threadIdx.x;
   if (i >= items) return;
   const uint32_t r = per_row.div(i);
-  const int64_t col = static_cast<int64_t>(i - r * per_row.d) * 8;
+  const int64_t col = static_cast<int64_t>(i - r * per_row.d) * N;
   const int64_t row = row0 + r;
-  const int n = static_cast<int>(min(int64_t{8}, H - col));
+  const int n = static_cast<int>(min(int64_t{N}, H - col));
   const int64_t id = ids[row];
   const bool known = id >= 0 && id < V;
   const char* src = table + ((known ? id : 0) * H + col) * Elem<In>::kBytes;
   char* dst = out + (row * H + col) * Elem<Out>::kBytes;
-  float v[8];
-  if (n == 8) {
-    Elem<In>::unpack8(Elem<In>::template load8<false>(src), v);
+  float v[N];
+  if (n == N) {
+    load_n<In, N, false>(src, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = known ? v[j] * scale : 0.f;
-    Elem<Out>::template store8<true>(dst, v);
+    for (int j = 0; j < N; ++j) v[j] = known ? v[j] * scale : 0.f;
+    store_n<Out, N, true>(dst, v);
   } else {
     for (int j = 0; j < n; ++j)
       Elem<Out>::store1(dst + j * Elem<Out>::kBytes,
@@ -507,14 +514,14 @@ extern "C" __attribute__((visibility("default"))) int soupk_embedding_fwd(
   if (bad_elem_ptr(out, out_dtype) || !ids || (reinterpret_cast<uintptr_t>(ids) & 7u))
     return kInvalid;
   if (V > 0 && bad_elem_ptr(table, dtype)) return kInvalid;
-  const int64_t per_row = (H + 7) / 8;
-  const int64_t rows_per = ((int64_t{1} << 31) - 1 - kEmbThreads) / per_row;
-  const FastDiv div(static_cast<uint32_t>(per_row));
   return with_type(dtype, [&](auto in) {
     return with_type(out_dtype, [&](auto o) -> int {
       using In = typename decltype(in)::type;
       using Out = typename decltype(o)::type;
       if constexpr (std::is_same_v<In, Out> || std::is_same_v<Out, float>) {
+        const int64_t per_row = (H + lookup_cols<Out>() - 1) / lookup_cols<Out>();
+        const int64_t rows_per = ((int64_t{1} << 31) - 1 - kEmbThreads) / per_row;
+        const FastDiv div(static_cast<uint32_t>(per_row));
         for (int64_t r0 = 0; r0 < M; r0 += rows_per) {
           const uint32_t items = static_cast<uint32_t>(std::min(rows_per, M - r0) * per_row);
           const int rc = launch_kernel(

@@ -479,7 +479,7 @@ OP(dropout) {
   const at::Device dev = x->device();
   const int64_t cols = x->dim() ? x->size(-1) : 1;
   if (!(d.p >= 0.0 && d.p <= 1.0) || code_of(x->scalar_type()) < 0 || !x->is_cuda() ||
-      !on(*x, dev) || !x->is_contiguous() || cols > (int64_t{1} << 33) ||
+      !on(*x, dev) || !x->is_contiguous() || cols > (int64_t{1} << 32) ||
       (seed.defined() && (!on(seed, dev) || seed.scalar_type() != at::kLong || seed.numel() != 1)))
     ELSE_PYTHON;
   int64_t n_rows = 1;

@@ -60,8 +60,8 @@ def dropout(x, p, seed, call=0, rows=None, residual=None):
     p = _check_p(p)
     _check_seed(seed, x.device)
     _check_word(call, "call")
-    if x.dim() and x.shape[-1] > 1 << 33:
-        raise ValueError(f"x has {x.shape[-1]} columns, at most 2^33 are drawn for")
+    if x.dim() and x.shape[-1] > 1 << 32:
+        raise ValueError(f"x has {x.shape[-1]} columns, at most 2^32 are drawn for")
     if rows is not None:
         _ext.require(rows, "rows", dtype=torch.int64, device=x.device)
         n_rows = x.shape[:-1].numel() if x.dim() else 1
