@@ -7,8 +7,8 @@
 // Backward, with g the gradient of out:
 //   gy1 = g1 c1 + g2 s2, gy2 = g2 c2 - g1 s1;  dw = sum over tokens and heads of gy * n
 //   dx = r * (gy w - n * mean(gy w n));        a value head's gradient passes through
-// All in fp32, one rounding to the rows' type at the store; x and r are formed again in the
-// backward from the rows it has to read anyway, so nothing is kept of the forward.
+// All in fp32 with fused multiply-adds, one rounding to the rows' type at the store; x and r are formed
+// again in the backward from the rows it has to read anyway, so nothing is kept of the forward.
 //
 // Mapping (forward): a head is a group of G = 2^k lanes, each with 8 dims of the first half and the 8 dims of
 // the second half they rotate with, so the rotation is inside a lane and the mean of squares one
@@ -38,6 +38,7 @@ constexpr int kNormBlocks = SOUPK_QK_NORM_BLOCKS;   // most workgroups (partial 
 struct NormDims {
   int64_t rows, slots;  // tokens; B * T
   int T, NH, NKV, D;
+  float inv_d;          // 1 / D
   int groups;           // wavefront items per token: ceil((NH + 2 NKV) * G / 64)
   FastDiv per_tok;      // divides by groups
   FastDiv per_seq;      // divides by T
@@ -81,10 +82,18 @@ __device__ __forceinline__ void add_lora(const char* lora, bool f32, int64_t at,
 }
 
 __device__ __forceinline__ float sum_squares(const float* a, const float* b) {
-  float s[8];
+  float s = a[0] * a[0], t = b[0] * b[0];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) s[j] = a[j] * a[j] + b[j] * b[j];
-  return ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+  for (int j = 1; j < 8; ++j) {
+    s = __builtin_fmaf(a[j], a[j], s);
+    t = __builtin_fmaf(b[j], b[j], t);
+  }
+  return s + t;
+}
+
+// 1 / sqrt(mean + eps) by the hardware's reciprocal root (1 ulp).
+__device__ __forceinline__ float inv_rms(float sum, float inv_d, float eps) {
+  return __builtin_amdgcn_rsqf(__builtin_fmaf(sum, inv_d, eps));
 }
 
 // A wavefront takes PER neighbouring groups of 64 / G heads of one token (per_tok: such items per token).
@@ -141,7 +150,7 @@ __global__ __launch_bounds__(kNormThreads) void qk_norm_rope_fwd_kernel(
     const float ss = group_sum<G>(sum_squares(a[u], b[u]));
     if (h < heads && 16 * c < dm.D) {
       if (known && h < dm.NH + dm.NKV) {
-        const float r = 1.0f / sqrtf(ss / static_cast<float>(dm.D) + eps);
+        const float r = inv_rms(ss, dm.inv_d, eps);
         const float* w = (h < dm.NH ? wq : wk) + 8 * c;
         float w1[8], w2[8];
         load8f(w, w1);
@@ -149,8 +158,8 @@ __global__ __launch_bounds__(kNormThreads) void qk_norm_rope_fwd_kernel(
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float y1 = a[u][j] * r * w1[j], y2 = b[u][j] * r * w2[j];
-          a[u][j] = y1 * c1[j] - y2 * s1[j];
-          b[u][j] = y2 * c2[j] + y1 * s2[j];
+          a[u][j] = __builtin_fmaf(y1, c1[j], -(y2 * s1[j]));
+          b[u][j] = __builtin_fmaf(y2, c2[j], y1 * s2[j]);
         }
       }
       Elem<T>::template store8<true>(out + (at0 + u * step) * Elem<T>::kBytes, a[u]);
@@ -186,7 +195,6 @@ __global__ __launch_bounds__(kNormThreads) void qk_norm_rope_bwd_kernel(
   const uint32_t end = min(total, start + per);
   const int heads = dm.NH + 2 * dm.NKV;
   const bool dims = 16 * c < dm.D;
-  const float inv_d = static_cast<float>(dm.D);
   float w1[8], w2[8], acc1[8], acc2[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) w1[j] = w2[j] = acc1[j] = acc2[j] = 0.f;
@@ -221,7 +229,7 @@ __global__ __launch_bounds__(kNormThreads) void qk_norm_rope_bwd_kernel(
         add_lora<T>(lora_q, lora_f32, (static_cast<int64_t>(tok) * dm.NH + h) * dm.D + 8 * c, half,
                     a, b);
     }
-    const float r = 1.0f / sqrtf(group_sum<G>(sum_squares(a, b)) / inv_d + eps);
+    const float r = inv_rms(group_sum<G>(sum_squares(a, b)), dm.inv_d, eps);
     float dot = 0.f;
     if (live && known) {
       const int64_t row = static_cast<int64_t>(t) * dm.D + 8 * c;
@@ -233,28 +241,28 @@ __global__ __launch_bounds__(kNormThreads) void qk_norm_rope_bwd_kernel(
       float d1 = 0.f, d2 = 0.f;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float y1 = g1[j] * c1[j] + g2[j] * s2[j];
-        const float y2 = g2[j] * c2[j] - g1[j] * s1[j];
+        const float y1 = __builtin_fmaf(g1[j], c1[j], g2[j] * s2[j]);
+        const float y2 = __builtin_fmaf(g2[j], c2[j], -(g1[j] * s1[j]));
         a[j] = a[j] * r;
         b[j] = b[j] * r;
         if constexpr (DW) {
-          acc1[j] = acc1[j] + y1 * a[j];
-          acc2[j] = acc2[j] + y2 * b[j];
+          acc1[j] = __builtin_fmaf(y1, a[j], acc1[j]);
+          acc2[j] = __builtin_fmaf(y2, b[j], acc2[j]);
         }
         g1[j] = y1 * w1[j];
         g2[j] = y2 * w2[j];
-        d1 = d1 + g1[j] * a[j];
-        d2 = d2 + g2[j] * b[j];
+        d1 = __builtin_fmaf(g1[j], a[j], d1);
+        d2 = __builtin_fmaf(g2[j], b[j], d2);
       }
       dot = d1 + d2;
     }
-    dot = group_sum<G>(dot) / inv_d;
+    dot = group_sum<G>(dot) * dm.inv_d;
     if (live) {
       if (known) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          g1[j] = r * (g1[j] - a[j] * dot);
-          g2[j] = r * (g2[j] - b[j] * dot);
+          g1[j] = r * __builtin_fmaf(-a[j], dot, g1[j]);
+          g2[j] = r * __builtin_fmaf(-b[j], dot, g2[j]);
         }
       }
       Elem<T>::template store8<true>(dqkv + at * Elem<T>::kBytes, g1);
@@ -342,7 +350,7 @@ int norm_dims(int64_t rows, int32_t B, int32_t T, int32_t NH, int32_t NKV, int32
   // (32-bit indices of heads, with room for a last round)
   if (rows > ((int64_t{1} << 31) - 1 - (1 << 16)) / std::max<int64_t>(groups, heads)) return kInvalid;
   items = rows * groups;
-  dm = NormDims{rows, static_cast<int64_t>(B) * T, T,  NH, NKV, D, groups,
+  dm = NormDims{rows, static_cast<int64_t>(B) * T, T, NH, NKV, D, 1.0f / static_cast<float>(D), groups,
                 FastDiv(static_cast<uint32_t>(groups)),
                 FastDiv(static_cast<uint32_t>(std::max(T, 1)))};
   return kOk;
@@ -392,7 +400,8 @@ extern "C" __attribute__((visibility("default"))) int soupk_qk_norm_rope_fwd(
         };
         // Two groups a wavefront share the token's cos / sin loads, one a wavefront fills the chip
         // with fewer tokens: 8192 tokens of 48 heads 43.8 -> 40.1 us with two, 2048 of 16 heads
-        // 5.9 -> 5.7, 888 of 16 heads 5.6 -> 6.5 (so not there).
+        // 5.9 -> 5.7, 888 of 16 heads 5.6 -> 6.5 (so not there).  (Fused multiply-adds and the
+        // hardware's reciprocal root took the first from 40.1 to 38.5.)
         if (items >= kTwoGroups) return run(qk_norm_rope_fwd_kernel<E, G, 2>, 2);
         return run(qk_norm_rope_fwd_kernel<E, G, 1>, 1);
       });

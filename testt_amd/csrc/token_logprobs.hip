@@ -39,10 +39,10 @@ constexpr int kGroup = kLpThreads / 64;   // neighbouring threads whose largest 
 constexpr int kLpUnroll = 4;          // chunk loads in flight per thread
 constexpr int kGradThreads = 256, kGradUnroll = 4;
 constexpr int kMaxTop = 32;
-#ifndef SOUPK_LP_FILL
-#define SOUPK_LP_FILL 4
-#endif
-constexpr int kLpFill = SOUPK_LP_FILL;   // workgroups per CU below which rows are cut into parts
+// Workgroups per CU below which rows are cut into parts: 888 rows of 151936 without alternatives 54.2 us
+// with 4, 56.0 with 2 (one part a row); 333 rows of 32003 with five alternatives, where a part costs
+// its bounds and lists, 25.0 with 4, 23.5 with 2.
+constexpr int kLpFill = 4, kLpFillTop = 2;
 constexpr int kListCap = 1024;        // candidates of a part
 constexpr int kMaxParts = 64;
 constexpr int64_t kIgnored = -100;
@@ -658,11 +658,12 @@ __global__ __launch_bounds__(kGradThreads) void token_logprobs_bwd_kernel(
 
 int64_t lp_align(int64_t v) { return (v + 255) / 256 * 256; }
 
-// Parts per row: enough workgroups to fill the chip, each with at least kMinSteps steps.
-int lp_parts(int64_t rows, int64_t V, int32_t dtype) {
+// Parts per row: enough workgroups to fill the chip, each with two steps at least.
+int lp_parts(int64_t rows, int64_t V, int32_t dtype, int32_t top_k) {
   const int64_t chunks = V / (dtype == SOUPK_DTYPE_F32 ? 4 : 8);
   const int64_t steps = (chunks + kLpThreads - 1) / kLpThreads;
-  const int64_t want = rows > 0 ? (int64_t{kLpFill} * device_cu_count() + rows - 1) / rows : 1;
+  const int64_t fill = int64_t{top_k > 0 ? kLpFillTop : kLpFill} * device_cu_count();
+  const int64_t want = rows > 0 ? (fill + rows - 1) / rows : 1;
   const int64_t least = steps * kLpThreads / (int64_t{1} << 27) + 1;   // (32-bit offsets in a part)
   return static_cast<int>(
       std::max<int64_t>(least, std::min<int64_t>({want, steps / 2, kMaxParts})));
@@ -686,7 +687,7 @@ extern "C" __attribute__((visibility("default"))) int soupk_token_logprobs_works
     int64_t rows, int64_t V, int32_t top_k, int32_t dtype, int64_t* bytes) {
   if (bad_lp(dtype, rows, 1, V, 1.f) || top_k < 0 || top_k > kMaxTop || bytes == nullptr)
     return kInvalid;
-  const int parts = lp_parts(rows, V, dtype);
+  const int parts = lp_parts(rows, V, dtype, top_k);
   *bytes = parts == 1 ? 0
                       : lp_align(rows * parts * static_cast<int64_t>(sizeof(Stats))) +
                             rows * parts * top_k * static_cast<int64_t>(sizeof(Cand));
@@ -710,7 +711,7 @@ extern "C" __attribute__((visibility("default"))) int soupk_token_logprobs_fwd(
   if (need > 0 && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) ||
                    workspace_bytes < need))
     return kInvalid;
-  const int parts = lp_parts(rows, V, dtype);
+  const int parts = lp_parts(rows, V, dtype, top_k);
   const float inv_t = 1.0f / temperature;
   const float c = static_cast<float>(1.4426950408889634 / static_cast<double>(temperature));
   const LpRows lr{inner, stride_outer, stride_inner, V, rows};
