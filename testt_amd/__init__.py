@@ -5,10 +5,14 @@ functions, autograd.Function signatures and constants):
 
 - nf4.py      NF4 double-quant unpack + frozen 4-bit linear (hipBLASLt GEMM)
 - rmsnorm.py  residual add + RMSNorm, forward and backward
-- rope.py     LoRA add + rotary + scatter of q/k/v to the attention's layout, fwd and bwd
+- rope.py     LoRA add + rotary + scatter of q/k/v to the attention's layout, fwd and bwd; the same
+              with per-head norms of queries and keys
 - attention.py causal GQA flash attention (head dim 128), forward and backward
 - mlp.py      gate/up GEMM + SwiGLU in fp16, gate/up kept (or recomputed) for backward
-- head.py     fused head + loss + entropy + accuracy + per-row loss, no full logits
+- head.py     fused head + loss + entropy + accuracy + per-row loss, no full logits; log
+              probabilities of given tokens with entropy and top alternatives
+- dropout.py  dropout drawn from a counter, with no mask stored
+- embedding.py scaled lookup and its gradient by sorted tokens
 - warmup.py   start/wait hooks (the kernels are prebuilt, nothing compiles at run time)
 
 The kernels are hand-written HIP in testt_amd/csrc, built into libsoupk.so behind the C ABI of
@@ -17,7 +21,7 @@ current stream.  There is no CPU or Triton path.
 """
 
 __all__ = ["apply", "configure_backward", "nf4", "rmsnorm", "rope", "attention", "mlp", "head",
-           "warmup"]
+           "dropout", "embedding", "warmup"]
 
 # One process drives one GPU here, so autograd's per-device worker thread adds no parallelism,
 # and handing every backward to it costs host time: on the MI355X boxes one decoder layer's
