@@ -155,6 +155,35 @@ def test_rising_rows(vocab, dtype, top_k):
     check(got.top_logprobs, lp, tol, "top")
 
 
+@pytest.mark.parametrize("dtype,top_k", [(torch.float32, 32), (torch.float32, 2),
+                                         (torch.float16, 32), (torch.bfloat16, 8)])
+@pytest.mark.parametrize("vocab", [40007, 151936])
+def test_rows_that_rise_with_noise(vocab, dtype, top_k):
+    """Rows whose candidates overflow the lists in each of their ways: noise on a rise; a rise of which
+    long runs are equal; and the large columns in a few threads' places (K - 1 of them, so that the
+    bound of the threads' largest lies below them all), rising and random."""
+    print(f"noisy rise {vocab} {dtype} top {top_k}", flush=True)
+    rows = 1030 if vocab < 100000 else 600
+    z, tok = logits_of(6, vocab, dtype, vocab + 1)
+    ramp = torch.linspace(-8, 8, vocab)
+    noise = torch.randn(6, vocab, generator=torch.Generator().manual_seed(vocab))
+    cols = 16 // z.element_size()
+    place = (torch.arange(vocab) // cols) % 256
+    comb = torch.where(place < top_k - 1, 20.0, 0.0)
+    z[0] = (ramp + noise[0]).to(dtype)
+    z[1] = (ramp * 8).floor().to(dtype)
+    z[2] = (comb + ramp).to(dtype)
+    z[3] = (comb + noise[3]).to(dtype)
+    z[4] = comb.to(dtype)
+    reps = rows // 6 + 1
+    got = head.token_logprobs(z.repeat(reps, 1)[:rows].to(DEV), tok.repeat(reps)[:rows].to(DEV), top_k)
+    want = reference(z.double(), tok, top_k)
+    assert torch.equal(got.top_ids.cpu(), want[3].repeat(reps, 1)[:rows])
+    rel, _, x, _ = bounds(z.double(), 1.0)
+    tol = rel[:, None] + 4 * U * (x.gather(-1, want[3]).abs().nan_to_num(posinf=0.0) + 1)
+    check(got.top_logprobs, want[2].repeat(reps, 1)[:rows], tol.repeat(reps, 1)[:rows], "top")
+
+
 def test_rows_without_a_distribution():
     """A row of -inf alone, one with NaN, one with +inf: NaN numbers, ordered ids; other rows
     unharmed, and a row without upstream gradient keeps a zero gradient."""
