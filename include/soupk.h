@@ -797,8 +797,8 @@ int soupk_embedding_fwd(const void* table, int32_t dtype, const int64_t* ids, vo
 /*
  * Its backward: dtable [V, H] of dtype, written whole: scale times the sum of dout's rows (grad_dtype
  * dtype or F32) over each id's tokens in their order, fp32 sums rounded once; zeros for every
- * other row and for padding_idx (-1: none).  Ids outside [0, V) are skipped.  workspace:
- * soupk_embedding_bwd_workspace(M, V, H) bytes, 16-byte aligned.
+ * other row and for padding_idx (-1: none).  Ids outside [0, V) are skipped.  M * ceil(H / 512) at
+ * most 2^28.  workspace: soupk_embedding_bwd_workspace(M, V, H) bytes, 16-byte aligned.
  */
 int soupk_embedding_bwd_workspace(int64_t M, int64_t V, int64_t H, int64_t* bytes);
 int soupk_embedding_bwd(const void* dout, int32_t grad_dtype, const int64_t* ids, void* dtable,

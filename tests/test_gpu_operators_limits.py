@@ -85,6 +85,36 @@ def test_dropout_and_norm_past_two_to_the_31_elements():
     assert torch.equal(out.detach()[-100:], alone.detach()) and torch.equal(g[-100:], ga)
 
 
+def test_more_rows_than_a_launch_takes():
+    """A grid spans fewer than 2^32 threads: more rows than that gives workgroups for are launched in turn."""
+    rows, vocab = (1 << 24) + 77, 5
+    z = fill(rows, vocab).requires_grad_(True)
+    tok = torch.arange(rows, device=DEV) % vocab
+    out = head.token_logprobs(z, tok, 2)
+    g, = torch.autograd.grad(out.logprob, z, torch.ones(rows, device=DEV))
+    for at in (0, (1 << 23) - 50, (1 << 24) - 50, rows - 100):
+        part = slice(at, at + 100)
+        zp = z.detach()[part].clone().requires_grad_(True)
+        alone = head.token_logprobs(zp, tok[part], 2)
+        ga, = torch.autograd.grad(alone.logprob, zp, torch.ones(100, device=DEV))
+        assert all(torch.equal(a, o[part]) for a, o in zip(alone, out))
+        assert torch.equal(ga, g[part])
+    del z, tok, out, g
+    m, d = (1 << 26) + 77, 16
+    qkv = fill(m, d).requires_grad_(True)
+    pos = torch.arange(m, device=DEV) % 64
+    cos, sin = (t.to(DEV) for t in workloads.rope_tables(64, d))
+    w = torch.ones(d, device=DEV)
+    y = rope.qk_norm_rope(qkv, None, None, w, w, cos, sin, pos, 1, 64, 1, 0, d)
+    g, = torch.autograd.grad(y, qkv, y.detach())
+    for at in (0, (1 << 25) - 50, (1 << 26) - 50, m - 100):
+        part = slice(at, at + 100)
+        qp = qkv.detach()[part].clone().requires_grad_(True)
+        alone = rope.qk_norm_rope(qp, None, None, w, w, cos, sin, pos[part].clone(), 1, 64, 1, 0, d)
+        ga, = torch.autograd.grad(alone, qp, alone.detach())
+        assert torch.equal(y.detach()[part], alone.detach()) and torch.equal(ga, g[part])
+
+
 def steps(seed):
     """One forward and backward of each operator on its own data: a function that runs them."""
     g = torch.Generator(device=DEV).manual_seed(seed)

@@ -97,6 +97,8 @@ BAD = [
     ("soupk_embedding_bwd", (A, 0, A, A, 0, 1.0, -1, None, 0, 4, 8, 8, None)),
     ("soupk_embedding_bwd", (A, 0, A, A, 0, 1.0, -1, A, 100, 4, 8, 8, None)),
     ("soupk_embedding_bwd", (A, 2, A, A, 0, 1.0, -1, A, 1 << 30, 4, 8, 8, None)),
+    ("soupk_embedding_bwd", (A, 0, A, A, 0, 1.0, -1, A, 1 << 50, (1 << 28) + 1, 8, 512, None)),
+    ("soupk_embedding_bwd", (A, 0, A, A, 0, 1.0, -1, A, 1 << 50, 1 << 28, 8, 513, None)),
     ("soupk_embedding_bwd_workspace", (-1, 8, 8, A)),
     ("soupk_token_logprobs_workspace", (4, 8, 0, 0, None)),
 ]

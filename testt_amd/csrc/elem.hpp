@@ -179,6 +179,10 @@ __device__ __forceinline__ void store_n(char* p, const float* v) {
     st8<NT>(p, u32x2{pack_b2(v[0], v[1]), pack_b2(v[2], v[3])});
 }
 
+// Most workgroups of a launch: HIP takes at most 2^32 - 1 threads along a grid's axis, and these kernels have
+// up to 256 a workgroup (this leaves half of that for a launch of two kinds of them).
+constexpr int64_t kMaxGrid = int64_t{1} << 23;
+
 // Host: calls f(Elem type tag) for a SOUPK_DTYPE_* code; kInvalid for any other code.
 template <typename T>
 struct TypeTag {

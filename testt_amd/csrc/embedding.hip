@@ -563,6 +563,12 @@ extern "C" __attribute__((visibility("default"))) int soupk_embedding_bwd(
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) || workspace_bytes < l.bytes)
       return kInvalid;
   }
+  const int64_t H8 = round_up(H, 8);
+  const int run = run_length(M);
+  const int64_t runs = (M + run - 1) / run;
+  const int col_blocks = static_cast<int>((H8 / 8 + kEmbThreads - 1) / kEmbThreads);
+  const int join_blocks = static_cast<int>((H + kJoinCols - 1) / kJoinCols);
+  if (runs * join_blocks > kMaxGrid) return kInvalid;               // (>= runs * col_blocks)
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t row_bytes = H * (dtype == SOUPK_DTYPE_F32 ? 4 : 2);
   int bits = 0;
@@ -611,12 +617,6 @@ extern "C" __attribute__((visibility("default"))) int soupk_embedding_bwd(
   const uint32_t* const skey = key[passes & 1];
   const uint32_t* const stok = tok[passes & 1];
   float* const partial = reinterpret_cast<float*>(ws + l.partial);
-  const int64_t H8 = round_up(H, 8);
-  const int run = run_length(M);
-  const int64_t runs = (M + run - 1) / run;
-  const int col_blocks = static_cast<int>((H8 / 8 + kEmbThreads - 1) / kEmbThreads);
-  const int join_blocks = static_cast<int>((H + kJoinCols - 1) / kJoinCols);
-  if (runs * join_blocks > (int64_t{1} << 30)) return kInvalid;     // (>= runs * col_blocks)
   const int64_t row_items = (row_bytes + 15) / 16;
   const int64_t rows_per =
       std::max<int64_t>(1, ((int64_t{1} << 30) - kEmbThreads) / row_items);

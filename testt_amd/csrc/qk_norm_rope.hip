@@ -103,10 +103,10 @@ __global__ __launch_bounds__(kNormThreads) void qk_norm_rope_fwd_kernel(
     const char* __restrict__ qkv, const char* __restrict__ lora_q, const char* __restrict__ lora_v,
     bool lora_f32, const float* __restrict__ wq, const float* __restrict__ wk,
     const float* __restrict__ cos_t, const float* __restrict__ sin_t,
-    const int64_t* __restrict__ pos, char* __restrict__ out, float eps, NormDims dm,
+    const int64_t* __restrict__ pos, char* __restrict__ out, float eps, NormDims dm, uint32_t item0,
     uint32_t items) {
   constexpr int kSlots = kWave / G;                       // heads of a group
-  const uint32_t item = blockIdx.x * kNormWaves + (threadIdx.x >> 6);
+  const uint32_t item = item0 + blockIdx.x * kNormWaves + (threadIdx.x >> 6);
   if (item >= items) return;
   const int lane = threadIdx.x & 63, c = lane % G;
   const int heads = dm.NH + 2 * dm.NKV, half = dm.D >> 1;
@@ -392,12 +392,18 @@ extern "C" __attribute__((visibility("default"))) int soupk_qk_norm_rope_fwd(
           NormDims d = dm;
           d.per_tok = FastDiv(static_cast<uint32_t>(per_tok));
           const int64_t n = rows * per_tok;
-          return launch_kernel(kernel, dim3(static_cast<unsigned>((n + kNormWaves - 1) / kNormWaves)),
-                               dim3(kNormThreads), static_cast<hipStream_t>(stream),
-                               static_cast<const char*>(qkv), static_cast<const char*>(lora_q),
-                               static_cast<const char*>(lora_v), lora_dtype == SOUPK_DTYPE_F32, wq,
-                               wk, cos, sin, pos, static_cast<char*>(out), eps, d,
-                               static_cast<uint32_t>(n));
+          constexpr int64_t kMost = kMaxGrid * kNormWaves;      // of one launch
+          for (int64_t i0 = 0; i0 < n; i0 += kMost) {
+            const int64_t blocks = (std::min(kMost, n - i0) + kNormWaves - 1) / kNormWaves;
+            const int rc = launch_kernel(
+                kernel, dim3(static_cast<unsigned>(blocks)), dim3(kNormThreads),
+                static_cast<hipStream_t>(stream), static_cast<const char*>(qkv),
+                static_cast<const char*>(lora_q), static_cast<const char*>(lora_v),
+                lora_dtype == SOUPK_DTYPE_F32, wq, wk, cos, sin, pos, static_cast<char*>(out), eps, d,
+                static_cast<uint32_t>(i0), static_cast<uint32_t>(n));
+            if (rc != kOk) return rc;
+          }
+          return static_cast<int>(kOk);
         };
         // Two groups a wavefront share the token's cos / sin loads, one a wavefront fills the chip
         // with fewer tokens: 8192 tokens of 48 heads 43.8 -> 40.1 us with two, 2048 of 16 heads
@@ -426,7 +432,7 @@ extern "C" __attribute__((visibility("default"))) int soupk_qk_norm_rope_bwd(
   const int64_t slots = kNormThreads / group_of(D);
   const int64_t q_heads = rows * NH, kv_heads = rows * NKV;
   const int64_t q_need = (q_heads + slots - 1) / slots, kv_need = (kv_heads + slots - 1) / slots;
-  const int64_t most = want_dw ? kNormBlocks : int64_t{1} << 30;
+  const int64_t most = want_dw ? kNormBlocks : kMaxGrid / 2;    // (head numbers below 2^32)
   int64_t q_blocks = q_need, kv_blocks = kv_need;
   if (q_need + kv_need > most) {
     kv_blocks = std::min<int64_t>(kv_need, most * 5 * NKV / (3 * NH + 5 * NKV));

@@ -432,13 +432,13 @@ __device__ __forceinline__ void write_row(const RowOut& o, int64_t r, const Stat
 template <typename T, bool TOP, bool KEEP>
 __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(
     const char* __restrict__ logits, const int64_t* __restrict__ tokens, LpRows rows, float c,
-    float inv_t, int K, int parts, int64_t part_chunks, PartOut part, RowOut out) {
+    float inv_t, int K, int parts, int64_t part_chunks, int64_t r0, PartOut part, RowOut out) {
   using C = Chunk<T>;
   constexpr int N = C::N;
   constexpr int kSize = Elem<T>::kBytes;
   __shared__ Stats stat_lds[kLpWaves];
   __shared__ std::conditional_t<TOP, ListLds, int> lds;
-  const int64_t r = blockIdx.x / static_cast<uint32_t>(parts);
+  const int64_t r = r0 + blockIdx.x / static_cast<uint32_t>(parts);
   const int which = static_cast<int>(blockIdx.x % static_cast<uint32_t>(parts));
   const char* const row = logits + rows.at(r) * kSize;
   const int64_t chunks = rows.V / N;
@@ -511,7 +511,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(
     if (tid < kWave) absorb<1>(st, mc, odd, &tail, tail, c);
   }
   const Stats total = merge_stats(stat_lds, st, c);
-  const int64_t at = blockIdx.x;
+  const int64_t at = r * parts + which;
   const float lse = log_sum(total, c);
   if (tid == 0) {
     if (parts > 1) part.stats[at] = total;
@@ -785,9 +785,15 @@ extern "C" __attribute__((visibility("default"))) int soupk_token_logprobs_fwd(
     const int64_t part_chunks = (chunks + parts - 1) / parts;
     const RowOut ro{logprob, entropy, row_max, row_sum, top_lp, top_id};
     auto run = [&](auto kernel) {
-      return launch_kernel(kernel, dim3(static_cast<unsigned>(rows * parts)), dim3(kLpThreads), s,
-                           static_cast<const char*>(logits), tokens, lr, c, inv_t,
-                           static_cast<int>(top_k), parts, part_chunks, po, ro);
+      const int64_t most = kMaxGrid / parts;         // rows of one launch
+      for (int64_t r0 = 0; r0 < rows; r0 += most) {
+        const int64_t n = std::min(most, rows - r0);
+        const int rc = launch_kernel(kernel, dim3(static_cast<unsigned>(n * parts)), dim3(kLpThreads),
+                                     s, static_cast<const char*>(logits), tokens, lr, c, inv_t,
+                                     static_cast<int>(top_k), parts, part_chunks, r0, po, ro);
+        if (rc != kOk) return rc;
+      }
+      return static_cast<int>(kOk);
     };
     const bool keep = row_max != nullptr;       // (asked for by a backward)
     const int rc = top_k > 0 ? keep ? run(token_logprobs_kernel<T, true, true>)
@@ -824,7 +830,7 @@ extern "C" __attribute__((visibility("default"))) int soupk_token_logprobs_bwd(
     using T = typename decltype(tag)::type;
     constexpr int64_t kPer = kGradThreads * kGradUnroll;
     const int64_t blocks = std::max<int64_t>(1, (V / Chunk<T>::N + kPer - 1) / kPer);
-    const int64_t most = 0x7fffffff / blocks;        // rows of one launch
+    const int64_t most = std::max<int64_t>(1, kMaxGrid / blocks);    // rows of one launch
     for (int64_t r0 = 0; r0 < rows; r0 += most) {
       const int64_t n = std::min(most, rows - r0);
       const int rc = launch_kernel(
