@@ -202,3 +202,25 @@ def test_attention_over_normalised_rows():
         f = lambda w: float((call(w).double() * up.half().double()).sum())
         slope = (f(x["wq"] + h * dirn) - f(x["wq"] - h * dirn)) / (2 * h)
     assert abs(slope - float(grads[3].norm())) < 0.05 * float(grads[3].norm())
+
+
+@pytest.mark.parametrize("rows,nh,nkv", [(1, 4, 2), (9, 4, 0), (9, 4, 2)])
+def test_gradients_of_leaves_share_no_memory(rows, nh, nkv):
+    """Two backwards add up in every leaf's .grad by themselves."""
+    d = 64
+    leaves = [torch.randn(rows, (nh + 2 * nkv) * d, device=DEV).half().requires_grad_(True),
+              torch.randn(rows, nh * d, device=DEV).half().requires_grad_(True),
+              torch.randn(rows, nkv * d, device=DEV).half().requires_grad_(True) if nkv else None]
+    w = torch.ones(d, device=DEV)
+    cos, sin = (t.to(DEV) for t in workloads.rope_tables(16, d))
+    pos = torch.arange(rows, device=DEV)
+    given = [t for t in leaves if t is not None]
+    up = torch.randn(rows, (nh + 2 * nkv) * d, device=DEV).half()
+    once = None
+    for _ in range(2):
+        rope.qk_norm_rope(*leaves, w, w, cos, sin, pos, 1, 16, nh, nkv, d).backward(up)
+        if once is None:
+            once = [t.grad.clone() for t in given]
+    assert len({t.grad.untyped_storage().data_ptr() for t in given}) == len(given)
+    for t, g in zip(given, once):
+        assert torch.equal(t.grad, (g.float() * 2).half())

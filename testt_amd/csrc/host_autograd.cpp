@@ -273,10 +273,16 @@ struct QkNorm : Function<QkNorm> {
                 static_cast<int32_t>(n[1]), static_cast<int32_t>(nh), static_cast<int32_t>(nkv),
                 static_cast<int32_t>(hd), static_cast<float>(ctx->saved_data["e"].toDouble()),
                 stream_of(qkv)));
-      // (the deltas' gradients are columns of qkv's)
+      // The deltas' gradients are columns of qkv's.  Where they are contiguous (one row, or query heads
+      // alone) they are copied: autograd would make such a view a leaf's .grad as it is, and adding to
+      // it later would change qkv's.
+      auto columns = [&](int64_t from, int64_t n_cols) {
+        const Tensor view = dqkv.narrow(1, from, n_cols);
+        return view.is_contiguous() ? view.clone() : view;
+      };
       Tensor dlq, dlv;
-      if (n[5]) dlq = dqkv.narrow(1, 0, nh * hd);
-      if (n[6]) dlv = dqkv.narrow(1, (nh + nkv) * hd, nkv * hd);
+      if (n[5]) dlq = columns(0, nh * hd);
+      if (n[6]) dlv = columns((nh + nkv) * hd, nkv * hd);
       return {dqkv, dlq, dlv, dwq, dwk, Tensor(), Tensor(), Tensor(), Tensor()};
     });
   }
