@@ -168,3 +168,21 @@ def test_refusals():
             dropout.dropout(**{**dict(x=x, p=0.1, seed=1), **kw})
     with pytest.raises(TypeError):
         dropout.dropout(x.double(), 0.1, 1)
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_checkpointed_forward(reentrant):
+    """A forward that runs again in the backward: the module refuses to draw anew, the function with
+    its call number given redraws the same."""
+    from torch.utils.checkpoint import checkpoint
+    x = torch.randn(40, 96, device=DEV).half().requires_grad_(True)
+    m = dropout.CounterDropout(0.4, seed=5)
+    y = checkpoint(lambda t: m(t) * t, x, use_reentrant=reentrant)     # (the product needs m(t) again)
+    with pytest.raises(RuntimeError, match="inside a backward"):
+        y.sum().backward()
+    x.grad = None
+    y = checkpoint(lambda t: dropout.dropout(t, 0.4, 5, 3) * t, x, use_reentrant=reentrant)
+    y.sum().backward()
+    z = x.detach().requires_grad_(True)
+    (dropout.dropout(z, 0.4, 5, 3) * z).sum().backward()
+    assert torch.equal(x.grad, z.grad)

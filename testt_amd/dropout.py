@@ -15,6 +15,7 @@ import torch
 
 from . import _ext
 
+
 def _check_p(p):
     p = float(p)
     if not 0.0 <= p <= 1.0:
@@ -82,7 +83,11 @@ class CounterDropout(torch.nn.Dropout):
     """dropout() as a module: in training mode each forward draws under `seed` with the next call
     number (`self.call`, which may be set, e.g. to repeat a step); in eval mode, or with p = 0, x
     itself.  As the LoRA dropout of a layer or model of this package (it is a torch.nn.Dropout) it
-    runs on the real tokens' rows alone and draws at their padded positions."""
+    runs on the real tokens' rows alone and draws at their padded positions.
+
+    Modules that are to draw independently (of two projections, of the layers) get seeds of their own.
+    A forward that is run again inside a backward (activation checkpointing) raises: it would draw with
+    another call number than the first run did; such a program calls dropout() with the step's number."""
 
     def __init__(self, p=0.5, seed=0):
         super().__init__(_check_p(p))
@@ -95,6 +100,10 @@ class CounterDropout(torch.nn.Dropout):
         """forward(x) for rows that stand at the positions `rows`."""
         if not self.training or self.p == 0.0:
             return x
+        if torch._C._current_graph_task_id() != -1:     # (this thread is inside a backward)
+            raise RuntimeError("CounterDropout was called inside a backward pass (a checkpointed "
+                               "forward?), where its call number is not the first run's; use "
+                               "dropout.dropout() with a call number of the program's own")
         out = dropout(x, self.p, self.seed, self.call, rows)
         self.call += 1
         return out
