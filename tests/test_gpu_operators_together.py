@@ -195,3 +195,24 @@ def test_model_with_counter_dropout():
         d.call = 0
     c, gc = step()
     assert torch.equal(a, c) and all(torch.equal(x, y) for x, y in zip(ga, gc))
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_tangents_are_refused(grad):
+    """No operator has a forward-mode derivative: a dual tensor raises, also without gradients."""
+    import torch.autograd.forward_ad as ad
+    from testt_amd import dropout, embedding, head, rope
+    z = torch.randn(4, 200, device=DEV)
+    tok = torch.arange(4, device=DEV)
+    qkv, w = torch.randn(4, 3 * 64, device=DEV).half(), torch.ones(64, device=DEV)
+    cos, sin = (t.to(DEV) for t in workloads.rope_tables(16, 64))
+    with torch.set_grad_enabled(grad), ad.dual_level():
+        dual = lambda t: ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: head.token_logprobs(dual(z), tok, 2),
+                     lambda: dropout.dropout(dual(z), 0.5, 1),
+                     lambda: dropout.dropout(z, 0.5, 1, residual=dual(z)),
+                     lambda: embedding.embedding(tok, dual(z)),
+                     lambda: rope.qk_norm_rope(qkv, None, None, dual(w), w, cos, sin, tok, 1, 16, 1, 1,
+                                               64)):
+            with pytest.raises(RuntimeError, match="jvp"):
+                call()

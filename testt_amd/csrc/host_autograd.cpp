@@ -75,10 +75,12 @@ variable_list once(const variable_list& grads, F&& f) {
   return out;
 }
 
+// (A tensor with a tangent goes through the node too, whatever the grad mode: it raises there, as no
+// forward-mode derivative is given.)
 bool wants_grad(std::initializer_list<const Tensor*> ts) {
-  if (!at::GradMode::is_enabled()) return false;
+  const bool grads = at::GradMode::is_enabled();
   for (const Tensor* t : ts)
-    if (t && t->defined() && t->requires_grad()) return true;
+    if (t && t->defined() && ((grads && t->requires_grad()) || t->_fw_grad(0).defined())) return true;
   return false;
 }
 
