@@ -48,8 +48,8 @@ constexpr int kGroup = kLpThreads / 64;   // neighbouring threads whose largest 
 constexpr int kLpUnroll = 4;              // chunk loads in flight per thread
 constexpr int kGradThreads = 256, kGradUnroll = 4;
 constexpr int kMaxTop = 32;
-// Workgroups per CU below which rows are cut into parts: 888 rows of 151936 without alternatives 54.2 us
-// with 4, 56.0 with 2 (one part a row); 333 rows of 32003 with five alternatives, where a part costs
+// Workgroups per CU below which rows are cut into parts: 888 rows of 151936 without alternatives 52.6 us
+// with 4, 55.8 with 2 (one part a row); 333 rows of 32003 with five alternatives, where a part costs
 // its bounds and lists, 25.0 with 4, 23.5 with 2.
 constexpr int kLpFill = 4, kLpFillTop = 2;
 constexpr int kListCap = 1024;        // chunks that a part lists
@@ -428,7 +428,7 @@ __device__ __forceinline__ void write_row(const RowOut& o, int64_t r, const Stat
 
 // KEEP: the rows are read through the caches, for the backward that comes back to them (888 rows of
 // 151936 forward + backward 148.5 -> 137.9 us, 200 rows 45.5 -> 41.7, 2048 rows 322 -> 313); without one
-// they stream past (the forward of 888 rows alone 54.2 us, through the caches 60.4).
+// they stream past (the forward of 888 rows alone 52.6 us, through the caches 59.1).
 template <typename T, bool TOP, bool KEEP>
 __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(
     const char* __restrict__ logits, const int64_t* __restrict__ tokens, LpRows rows, float c,
@@ -484,6 +484,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(
     }
 #pragma unroll
     for (int u = 0; u < kLpUnroll; ++u) {
+      if (step + u >= steps) break;              // (888 rows of 151936 fp16 54.2 -> 52.4 us)
       const int i = i0 + u * kLpThreads;
       float z[N];
       w[u].unpack(z);
