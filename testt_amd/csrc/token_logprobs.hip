@@ -156,15 +156,21 @@ __device__ __forceinline__ void move_max(Stats& st, float m, float c) {
   st.m = m;
 }
 
-// Folds N columns with maximum bm into the statistics; the whole wavefront calls it.  odd: a lane's
-// maximum is out of the plain form's range (kept across calls).  A column of -inf makes the sum A NaN
-// (0 * -inf): then A is formed again with the exponents bounded.
+// While a lane reads, its m may lag behind the largest value by kLag of x (2^8 in the terms): moving it
+// costs an exponential and a branch that some lane of 64 takes at nearly every chunk of a row of 40 or 80
+// chunks a lane.  The maximum itself is kept beside it, and the statistics are moved to it at the end.
+constexpr float kLag = 8.f;
+
+// Folds N columns with maximum bm into the statistics; the whole wavefront calls it.  limit: st.m and
+// the lag; odd: a lane's m is out of the plain form's range (both kept across calls).  A column of -inf
+// makes the sum A NaN (0 * -inf): then A is formed again with the exponents bounded.
 template <int N>
-__device__ __forceinline__ void absorb(Stats& st, float& mc, bool& odd, const float* z, float bm,
-                                       float c) {
-  if (__any(bm > st.m)) {
-    if (bm > st.m) move_max(st, bm, c);
+__device__ __forceinline__ void absorb(Stats& st, float& mc, float& limit, bool& odd, const float* z,
+                                       float bm, float c, float lag) {
+  if (__any(bm > limit)) {
+    if (bm > limit) move_max(st, bm, c);
     mc = st.m * c;
+    limit = st.m + lag;
     odd = __any(!plain_form(mc));
   }
   float e[N], x[N];
@@ -446,7 +452,8 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(
   const int64_t last = min(chunks, first + part_chunks);
   const int tid = threadIdx.x;
   Stats st{-INFINITY, 0.f, 0.f};
-  float mc = -INFINITY;
+  float mc = -INFINITY, limit = -INFINITY;
+  const float lag = kLag / c;
   bool odd = true;
   float tmax = -INFINITY;        // this thread's largest value so far (never NaN)
   float bound = -INFINITY;
@@ -489,9 +496,9 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(
       float z[N];
       w[u].unpack(z);
       const float bm = w[u].max(z);
-      absorb<N>(st, mc, odd, z, bm, c);
+      absorb<N>(st, mc, limit, odd, z, bm, c, lag);
+      tmax = fmaxf(tmax, bm);
       if constexpr (TOP) {
-        tmax = fmaxf(tmax, bm);
         if (u == 0 && step == 0) {
           // The first step's columns against the bound that they give: the chunks with one above it,
           // and as many of the equal ones, from the left, as the K can still take.
@@ -509,8 +516,9 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(
   float tail = -INFINITY;
   if (has_tail) {                                // (whole wavefronts: the others add nothing)
     if (tail0 + tid < rows.V) tail = Elem<T>::load1(row + (tail0 + tid) * kSize);
-    if (tid < kWave) absorb<1>(st, mc, odd, &tail, tail, c);
+    if (tid < kWave) absorb<1>(st, mc, limit, odd, &tail, tail, c, lag);
   }
+  move_max(st, fmaxf(tmax, tail), c);
   const Stats total = merge_stats(stat_lds, st, c);
   const int64_t at = r * parts + which;
   const float lse = log_sum(total, c);
