@@ -87,6 +87,23 @@ struct Chunk {
       Elem<T>::unpack8(typename Elem<T>::Raw8{w}, v);
     }
   }
+  // x = z c + add, fused.  (fp16 columns from the loaded words, which lets the instruction that widens
+  // one operand do it: 2048 rows of 151936 102.9 -> 99.7 us against the columns unpacked before.)
+  __device__ __forceinline__ void scale(float* x, float c, float add) const {
+    if constexpr (std::is_same_v<T, f16>) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f16x2 h = as_h2(w[q]);
+        x[2 * q] = __builtin_fmaf(static_cast<float>(h[0]), c, add);
+        x[2 * q + 1] = __builtin_fmaf(static_cast<float>(h[1]), c, add);
+      }
+    } else {
+      float v[N];
+      unpack(v);
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[j] = __builtin_fmaf(v[j], c, add);
+    }
+  }
   // Columns of -inf.
   __device__ __forceinline__ void clear() {
     const uint32_t inf = kBits == 32 ? 0xff800000u
@@ -162,11 +179,12 @@ __device__ __forceinline__ void move_max(Stats& st, float m, float c) {
 constexpr float kLag = 8.f;
 
 // Folds N columns with maximum bm into the statistics; the whole wavefront calls it.  limit: st.m and
-// the lag; odd: a lane's m is out of the plain form's range (both kept across calls).  A column of -inf
-// makes the sum A NaN (0 * -inf): then A is formed again with the exponents bounded.
-template <int N>
+// the lag; odd: a lane's m is out of the plain form's range (both kept across calls).  exponents(x, add):
+// x = z c + add.  A column of -inf makes the sum A NaN (0 * -inf): then A is formed again with the exponents
+// bounded.
+template <int N, typename F>
 __device__ __forceinline__ void absorb(Stats& st, float& mc, float& limit, bool& odd, const float* z,
-                                       float bm, float c, float lag) {
+                                       float bm, float c, float lag, const F& exponents) {
   if (__any(bm > limit)) {
     if (bm > limit) move_max(st, bm, c);
     mc = st.m * c;
@@ -175,8 +193,7 @@ __device__ __forceinline__ void absorb(Stats& st, float& mc, float& limit, bool&
   }
   float e[N], x[N];
   if (!odd) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = __builtin_fmaf(z[j], c, -mc);
+    exponents(x, -mc);
   } else {
 #pragma unroll
     for (int j = 0; j < N; ++j) x[j] = exponent(z[j], st.m, mc, c);
@@ -496,7 +513,8 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(
       float z[N];
       w[u].unpack(z);
       const float bm = w[u].max(z);
-      absorb<N>(st, mc, limit, odd, z, bm, c, lag);
+      absorb<N>(st, mc, limit, odd, z, bm, c, lag,
+                [&](float* x, float shift) { w[u].scale(x, c, shift); });
       tmax = fmaxf(tmax, bm);
       if constexpr (TOP) {
         if (u == 0 && step == 0) {
@@ -516,7 +534,9 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(
   float tail = -INFINITY;
   if (has_tail) {                                // (whole wavefronts: the others add nothing)
     if (tail0 + tid < rows.V) tail = Elem<T>::load1(row + (tail0 + tid) * kSize);
-    if (tid < kWave) absorb<1>(st, mc, limit, odd, &tail, tail, c, lag);
+    if (tid < kWave)
+      absorb<1>(st, mc, limit, odd, &tail, tail, c, lag,
+                [&](float* x, float shift) { *x = __builtin_fmaf(tail, c, shift); });
   }
   move_max(st, fmaxf(tmax, tail), c);
   const Stats total = merge_stats(stat_lds, st, c);
