@@ -184,6 +184,31 @@ def test_rows_that_rise_with_noise(vocab, dtype, top_k):
     check(got.top_logprobs, want[2].repeat(reps, 1)[:rows], tol.repeat(reps, 1)[:rows], "top")
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [33, 130, 257, 600, 1031])
+def test_few_columns(vocab, dtype):
+    """Rows of fewer chunks than the bound has groups: most columns reach it, and the list is thinned.
+    Random, rising, equal and nearly all masked rows."""
+    print(f"few columns {vocab} {dtype}", flush=True)
+    z, tok = logits_of(7, vocab, dtype, vocab)
+    z[1] = torch.linspace(-3, 3, vocab).to(dtype)
+    z[2] = 1.0
+    z[3] = (torch.arange(vocab) % 3).to(dtype)
+    z[4] = float("-inf")
+    z[4, 5:8] = 2.0
+    tok[4] = 6
+    compare(z, tok, 32, 1.0, grads=False)
+    compare(z[:1], tok[:1], 20, 1.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_equal_columns_in_every_part(dtype):
+    """One long row, cut into parts that all offer the same values: the join's list is thinned."""
+    z = torch.zeros(2, 151936, dtype=dtype)
+    z[1] = (torch.arange(151936) % 5 == 3).to(dtype)
+    compare(z, torch.tensor([7, 151935]), 32, 1.0, grads=False)
+
+
 def test_rows_without_a_distribution():
     """A row of -inf alone, one with NaN, one with +inf: NaN numbers, ordered ids; other rows
     unharmed, and a row without upstream gradient keeps a zero gradient."""

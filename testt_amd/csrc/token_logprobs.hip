@@ -48,12 +48,13 @@ constexpr int kGroup = kLpThreads / 64;   // neighbouring threads whose largest 
 constexpr int kLpUnroll = 4;              // chunk loads in flight per thread
 constexpr int kGradThreads = 256, kGradUnroll = 4;
 constexpr int kMaxTop = 32;
-// Workgroups per CU below which rows are cut into parts: 888 rows of 151936 without alternatives 52.6 us
-// with 4, 55.8 with 2 (one part a row); 333 rows of 32003 with five alternatives, where a part costs
-// its bounds and lists, 25.0 with 4, 23.5 with 2.
-constexpr int kLpFill = 4, kLpFillTop = 2;
+// Workgroups per CU that parts of rows are cut for, to the nearest whole number a row (151936 fp16 columns
+// without alternatives: 200 rows 16.9 us in 5 parts, 17.9 in 6; 888 rows 48.6 whole, 51.5 in 2).  With
+// alternatives, where a part costs its bounds and lists, three: 333 rows of 32003 fp32 columns with five
+// 23.8 us, 25.4 cut for four a CU; 300 rows of 151936 bf16 with eight 32.9, 35.0 cut for two.
+constexpr int kLpFill = 4, kLpFillTop = 3;
 constexpr int kListCap = 1024;        // chunks that a part lists
-constexpr int kKeepCap = 1536;        // columns that it ranks
+constexpr int kKeepCap = 1280;        // columns that it ranks
 constexpr int kMaxParts = 64;
 constexpr int64_t kIgnored = -100;
 constexpr float kFloor = -200.f;      // below 2^kFloor an exponential is zero in fp32
@@ -110,14 +111,16 @@ struct Chunk {
                                      : std::is_same_v<T, f16> ? 0xfc00fc00u : 0xff80ff80u;
     w = u32x4{inf, inf, inf, inf};
   }
-  // The largest column, NaN passed over (v: the columns unpacked).
-  __device__ __forceinline__ float max(const float* v) const {
+  // The largest column, NaN passed over.
+  __device__ __forceinline__ float max() const {
     if constexpr (std::is_same_v<T, f16>) {
       const f16x2 m = __builtin_elementwise_max(
           __builtin_elementwise_max(as_h2(w.x), as_h2(w.y)),
           __builtin_elementwise_max(as_h2(w.z), as_h2(w.w)));
       return static_cast<float>(__builtin_elementwise_max(m[0], m[1]));
     } else {
+      float v[N];
+      unpack(v);
       float m = v[0];
 #pragma unroll
       for (int j = 1; j < N; ++j) m = fmaxf(m, v[j]);
@@ -178,13 +181,23 @@ __device__ __forceinline__ void move_max(Stats& st, float m, float c) {
 // chunks a lane.  The maximum itself is kept beside it, and the statistics are moved to it at the end.
 constexpr float kLag = 8.f;
 
-// Folds N columns with maximum bm into the statistics; the whole wavefront calls it.  limit: st.m and
-// the lag; odd: a lane's m is out of the plain form's range (both kept across calls).  exponents(x, add):
-// x = z c + add.  A column of -inf makes the sum A NaN (0 * -inf): then A is formed again with the exponents
+// A column by itself, as absorb takes them.
+struct OneColumn {
+  static constexpr int N = 1;
+  float z;
+  __device__ __forceinline__ void unpack(float* v) const { *v = z; }
+  __device__ __forceinline__ void scale(float* x, float c, float add) const {
+    *x = __builtin_fmaf(z, c, add);
+  }
+};
+
+// Folds columns with maximum bm into the statistics; the whole wavefront calls it.  limit: st.m and
+// the lag; odd: a lane's m is out of the plain form's range (both kept across calls).  A column of -inf makes the sum A NaN (0 * -inf): then A is formed again with the exponents
 // bounded.
-template <int N, typename F>
-__device__ __forceinline__ void absorb(Stats& st, float& mc, float& limit, bool& odd, const float* z,
-                                       float bm, float c, float lag, const F& exponents) {
+template <typename W>
+__device__ __forceinline__ void absorb(Stats& st, float& mc, float& limit, bool& odd, const W& w,
+                                       float bm, float c, float lag) {
+  constexpr int N = W::N;
   if (__any(bm > limit)) {
     if (bm > limit) move_max(st, bm, c);
     mc = st.m * c;
@@ -193,10 +206,11 @@ __device__ __forceinline__ void absorb(Stats& st, float& mc, float& limit, bool&
   }
   float e[N], x[N];
   if (!odd) {
-    exponents(x, -mc);
+    w.scale(x, c, -mc);
   } else {
+    w.unpack(x);
 #pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = exponent(z[j], st.m, mc, c);
+    for (int j = 0; j < N; ++j) x[j] = exponent(x[j], st.m, mc, c);
   }
 #pragma unroll
   for (int j = 0; j < N; ++j) e[j] = __builtin_amdgcn_exp2f(x[j]);
@@ -240,6 +254,7 @@ struct ListLds {
   Cand list[kListCap + kKeepCap];
   Cand tie[kMaxTop];            // the leftmost columns that equal a bound
   uint32_t group_max[64];
+  unsigned long long group_best[64];
   int count, kept, ties;
   int wave_n[kLpWaves];
   Cand best[kLpWaves];
@@ -293,9 +308,47 @@ __device__ __forceinline__ float wave_max(float v) {
   return fmaxf(fmaxf(lanef(v, 0), lanef(v, 16)), fmaxf(lanef(v, 32), lanef(v, 48)));
 }
 
+// Lists longer than this are thinned before they are ranked, which takes a list's length squared: few
+// columns (64 rows of 600 fp16 with 20 alternatives 75.7 us ranked whole, 10.4 thinned), or many equal ones at the bound.
+constexpr int kRankAll = 128;
+
+// Leaves of n > kRankAll candidates those that are not behind the K-th best of the 64 groups' best ones, in
+// place; returns how many.  (With more than 128 entries 32 groups have one.)
+__device__ int thin_list(ListLds& s, Cand* list, int n, int K) {
+  const int tid = threadIdx.x;
+  auto order = [](const Cand& c) {
+    return static_cast<unsigned long long>(c.key) << 32 | static_cast<uint32_t>(~c.col);
+  };
+  unsigned long long best = 0;
+#pragma unroll 1
+  for (int i = tid; i < n; i += kLpThreads) best = max(best, order(list[i]));
+  best = max(best, __shfl_xor(best, 1));
+  best = max(best, __shfl_xor(best, 2));
+  __syncthreads();                               // (n, the list's count, has been read)
+  if (tid % kGroup == 0) s.group_best[tid / kGroup] = best;
+  if (tid == 0) s.kept = 0;
+  __syncthreads();
+  best = s.group_best[tid & 63];
+  int rank = 0;
+#pragma unroll 4
+  for (int j = 0; j < 64; ++j) rank += s.group_best[j] > best ? 1 : 0;
+  const int at = __builtin_ctzll(__ballot(rank == K - 1));       // (the groups' best ones differ)
+  const unsigned long long bound = s.group_best[at];
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += kLpThreads) {
+    const bool on = i0 + tid < n;
+    const Cand c = on ? list[i0 + tid] : Cand{0, kNoCol};
+    __syncthreads();                             // (the places up to here are free)
+    if (on && order(c) >= bound) list[atomicAdd(&s.kept, 1)] = c;
+  }
+  __syncthreads();
+  return s.kept;
+}
+
 // Writes the K best of n candidates in order (entries past the last one have column kNoCol); every
 // thread of the workgroup calls it.
-__device__ __forceinline__ void rank_list(const Cand* list, int n, int K, Cand* out) {
+__device__ __forceinline__ void rank_list(ListLds& s, Cand* list, int n, int K, Cand* out) {
+  if (n > kRankAll) n = thin_list(s, list, n, K);
   for (int i = threadIdx.x; i < n; i += kLpThreads) {
     const Cand mine = list[i];
     int rank = 0;
@@ -337,35 +390,31 @@ __device__ void search_top(ListLds& s, const char* row, int64_t col0, int64_t co
 
 // Lists the columns of a step that equal `bound`, as far as they are among the first K of them from the
 // left, `before` of them lying in earlier steps; returns how many the step holds.  The whole workgroup
-// calls it; on: the thread has a chunk, of columns z from col on.
+// calls it; on: the thread has a chunk, of columns from col on.
 template <typename T>
-__device__ __forceinline__ int list_ties(ListLds& s, const float* z, bool on, uint32_t col,
+__device__ __forceinline__ int list_ties(ListLds& s, const Chunk<T>& chunk, bool on, uint32_t col,
                                          uint32_t bound, int K, int before) {
   constexpr int N = Chunk<T>::N;
   const int wave = threadIdx.x >> 6;
-  int equal = 0;
+  uint32_t equal = 0;                            // a bit for each column
   if (on) {
+    float z[N];
+    chunk.unpack(z);
 #pragma unroll
-    for (int j = 0; j < N; ++j) equal += Chunk<T>::key(z[j]) == bound ? 1 : 0;
+    for (int j = 0; j < N; ++j) equal |= Chunk<T>::key(z[j]) == bound ? 1u << j : 0u;
   }
-  const int upto = wave_scan(equal);             // equal columns left of and in this thread's
+  const int own = __popc(equal);
+  const int upto = wave_scan(own);               // equal columns left of and in this thread's
   if ((threadIdx.x & 63) == 63) s.wave_n[wave] = upto;
   __syncthreads();
-  int left = before + upto - equal, total = 0;
+  int left = before + upto - own, total = 0;
   for (int k = 0; k < kLpWaves; ++k) {
     left += k < wave ? s.wave_n[k] : 0;
     total += s.wave_n[k];
   }
-  if (equal > 0 && left < K) {
-#pragma unroll
-    for (int j = 0; j < N; ++j)
-      if (Chunk<T>::key(z[j]) == bound) {
-        if (left < K) {
-          s.tie[left] = Cand{bound, col + j};
-          atomicAdd(&s.ties, 1);
-        }
-        ++left;
-      }
+  for (; equal != 0 && left < K; equal &= equal - 1, ++left) {
+    s.tie[left] = Cand{bound, col + static_cast<uint32_t>(__builtin_ctz(equal))};
+    atomicAdd(&s.ties, 1);
   }
   return total;
 }
@@ -385,12 +434,10 @@ __device__ void list_again(ListLds& s, const char* base, int n, uint32_t col_bas
     const bool on = i < n;
     C w;
     w.template load<false>(base, on ? static_cast<uint32_t>(i) * 16u : 0u);
-    float z[C::N];
-    w.unpack(z);
     __syncthreads();                             // (wave_n and the cleared counts)
     if (ties < K)
-      ties += list_ties<T>(s, z, on, col_base + static_cast<uint32_t>(i) * C::N, key, K, ties);
-    const float bm = w.max(z);
+      ties += list_ties<T>(s, w, on, col_base + static_cast<uint32_t>(i) * C::N, key, K, ties);
+    const float bm = w.max();
     if (on && bm > bound) push(s, C::key(bm), static_cast<uint32_t>(i));
   }
   __syncthreads();
@@ -452,8 +499,11 @@ __device__ __forceinline__ void write_row(const RowOut& o, int64_t r, const Stat
 // KEEP: the rows are read through the caches, for the backward that comes back to them (888 rows of
 // 151936 forward + backward 148.5 -> 137.9 us, 200 rows 45.5 -> 41.7, 2048 rows 322 -> 313); without one
 // they stream past (the forward of 888 rows alone 52.6 us, through the caches 59.1).
+// Eight workgroups a CU (registers by the launch bound, the lists below 20 KB): with the seven that fit
+// otherwise, eight alternatives of 1792 bf16 rows took 106.3 us instead of 95.6, of 2048 rows 113.8
+// instead of 106.4.
 template <typename T, bool TOP, bool KEEP>
-__global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(
+__global__ __launch_bounds__(kLpThreads, 8) void token_logprobs_kernel(
     const char* __restrict__ logits, const int64_t* __restrict__ tokens, LpRows rows, float c,
     float inv_t, int K, int parts, int64_t part_chunks, int64_t r0, PartOut part, RowOut out) {
   using C = Chunk<T>;
@@ -510,11 +560,8 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(
     for (int u = 0; u < kLpUnroll; ++u) {
       if (step + u >= steps) break;              // (888 rows of 151936 fp16 54.2 -> 52.4 us)
       const int i = i0 + u * kLpThreads;
-      float z[N];
-      w[u].unpack(z);
-      const float bm = w[u].max(z);
-      absorb<N>(st, mc, limit, odd, z, bm, c, lag,
-                [&](float* x, float shift) { w[u].scale(x, c, shift); });
+      const float bm = w[u].max();
+      absorb(st, mc, limit, odd, w[u], bm, c, lag);
       tmax = fmaxf(tmax, bm);
       if constexpr (TOP) {
         if (u == 0 && step == 0) {
@@ -522,7 +569,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(
           // and as many of the equal ones, from the left, as the K can still take.
           first_key = raise_bound<C::kBits>(lds, C::key(tmax), K);
           bound = C::value(first_key);
-          list_ties<T>(lds, z, i < n, col_base + static_cast<uint32_t>(tid) * N, first_key, K, 0);
+          list_ties<T>(lds, w[u], i < n, col_base + static_cast<uint32_t>(tid) * N, first_key, K, 0);
         }
         if (bm > bound) push(lds, C::key(bm), static_cast<uint32_t>(i));
       }
@@ -534,9 +581,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(
   float tail = -INFINITY;
   if (has_tail) {                                // (whole wavefronts: the others add nothing)
     if (tail0 + tid < rows.V) tail = Elem<T>::load1(row + (tail0 + tid) * kSize);
-    if (tid < kWave)
-      absorb<1>(st, mc, limit, odd, &tail, tail, c, lag,
-                [&](float* x, float shift) { *x = __builtin_fmaf(tail, c, shift); });
+    if (tid < kWave) absorb(st, mc, limit, odd, OneColumn{tail}, tail, c, lag);
   }
   move_max(st, fmaxf(tmax, tail), c);
   const Stats total = merge_stats(stat_lds, st, c);
@@ -578,7 +623,7 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_kernel(
     if (count > kListCap || lds.kept > kKeepCap)
       search_top<T>(lds, row, min(first, chunks) * N, has_tail ? rows.V : last * N, K);
     else
-      rank_list(lds.list + kListCap, lds.kept, K, lds.top);
+      rank_list(lds, lds.list + kListCap, lds.kept, K, lds.top);
     __syncthreads();
     if (tid < K) {
       const Cand e = lds.top[tid];
@@ -618,10 +663,11 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_join_kernel(
     const Cand* const all = part.cand + r * parts * K;
     const int n = parts * K;                       // <= 64 * 32
     if (tid == 0) lds.kept = 0;
+    constexpr int kOwn = kMaxParts * kMaxTop / kLpThreads;
     uint32_t best = 0;
-    Cand mine[kMaxParts * kMaxTop / kLpThreads];
+    Cand mine[kOwn];
 #pragma unroll
-    for (int u = 0; u < kMaxParts * kMaxTop / kLpThreads; ++u) {
+    for (int u = 0; u < kOwn; ++u) {
       const int i = u * kLpThreads + tid;
       mine[u] = i < n ? all[i] : Cand{0, kNoCol};
       if (mine[u].col != kNoCol) best = max(best, mine[u].key);
@@ -629,11 +675,11 @@ __global__ __launch_bounds__(kLpThreads) void token_logprobs_join_kernel(
     const uint32_t bound_key = raise_bound<C::kBits>(lds, best, K);
     static_assert(kMaxParts * kMaxTop <= kListCap + kKeepCap, "the list holds every candidate");
 #pragma unroll
-    for (int u = 0; u < kMaxParts * kMaxTop / kLpThreads; ++u)
+    for (int u = 0; u < kOwn; ++u)
       if (mine[u].col != kNoCol && mine[u].key >= bound_key)
         lds.list[atomicAdd(&lds.kept, 1)] = mine[u];
     __syncthreads();
-    rank_list(lds.list, lds.kept, K, lds.top);
+    rank_list(lds, lds.list, lds.kept, K, lds.top);
     __syncthreads();
     if (tid < K) {
       const Cand e = lds.top[tid];
@@ -751,10 +797,11 @@ int lp_parts(int64_t rows, int64_t V, int32_t dtype, int32_t top_k) {
   const int64_t chunks = V / (dtype == SOUPK_DTYPE_F32 ? 4 : 8);
   const int64_t steps = (chunks + kLpThreads - 1) / kLpThreads;
   const int64_t fill = int64_t{top_k > 0 ? kLpFillTop : kLpFill} * device_cu_count();
-  const int64_t want = rows > 0 ? (fill + rows - 1) / rows : 1;
+  const int64_t want = rows > 0 ? std::max<int64_t>(1, (fill + rows / 2) / rows) : 1;
   const int64_t least = steps * kLpThreads / (int64_t{1} << 27) + 1;   // (32-bit offsets in a part)
-  return static_cast<int>(
-      std::max<int64_t>(least, std::min<int64_t>({want, steps / 2, kMaxParts})));
+  const int64_t parts = std::max<int64_t>(1, std::min<int64_t>(want, kMaxParts));
+  const int64_t per = std::max<int64_t>(2, (steps + parts - 1) / parts);
+  return static_cast<int>(std::max<int64_t>(least, (steps + per - 1) / per));
 }
 
 bool bad_dtype(int32_t d) {
