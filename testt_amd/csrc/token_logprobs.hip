@@ -497,8 +497,8 @@ __device__ __forceinline__ void write_row(const RowOut& o, int64_t r, const Stat
 }
 
 // KEEP: the rows are read through the caches, for the backward that comes back to them (888 rows of
-// 151936 forward + backward 148.5 -> 137.9 us, 200 rows 45.5 -> 41.7, 2048 rows 322 -> 313); without one
-// they stream past (the forward of 888 rows alone 52.6 us, through the caches 59.1).
+// 151936 forward + backward 141.4 -> 131.4 us, 200 rows 41.4 -> 38.2, 2048 rows 312 -> 306); without one
+// they stream past (the forward of 888 rows alone 48.6 us, through the caches 53.8).
 // Eight workgroups a CU (registers by the launch bound, the lists below 20 KB): with the seven that fit
 // otherwise, eight alternatives of 1792 bf16 rows took 106.3 us instead of 95.6, of 2048 rows 113.8
 // instead of 106.4.
