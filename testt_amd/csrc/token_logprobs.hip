@@ -178,7 +178,9 @@ __device__ __forceinline__ void move_max(Stats& st, float m, float c) {
 
 // While a lane reads, its m may lag behind the largest value by kLag of x (2^8 in the terms): moving it
 // costs an exponential and a branch that some lane of 64 takes at nearly every chunk of a row of 40 or 80
-// chunks a lane.  The maximum itself is kept beside it, and the statistics are moved to it at the end.
+// chunks a lane.  The maximum itself is kept beside it, and the statistics are moved to it at the end. (A's terms
+// are then up to 8 larger, which adds 8 roundings of S, 2^-21 of the entropy's unit, at most.)  2048 rows of
+// 151936 bf16 102.7 -> 99.2 us.
 constexpr float kLag = 8.f;
 
 // A column by itself, as absorb takes them.
