@@ -216,3 +216,22 @@ def test_tangents_are_refused(grad):
                                                64)):
             with pytest.raises(RuntimeError, match="jvp"):
                 call()
+
+
+def test_second_derivatives_are_refused():
+    """A gradient taken with create_graph and differentiated again raises, also where the upstream
+    gradient is a constant (a gradient penalty would otherwise lose its second-order part in silence)."""
+    from testt_amd import dropout, embedding, head, rope
+    leaf = lambda *s: torch.randn(*s, device=DEV).requires_grad_(True)
+    tok = torch.arange(4, device=DEV)
+    cos, sin = (t.to(DEV) for t in workloads.rope_tables(16, 64))
+    w = torch.ones(64, device=DEV)
+    for x, call in (
+            (leaf(4, 200), lambda x: head.token_logprobs(x, tok, 2).entropy),
+            (leaf(4, 200), lambda x: dropout.dropout(x, 0.5, 1)),
+            (leaf(4, 200), lambda x: embedding.embedding(tok, x)),
+            (torch.randn(4, 192, device=DEV).half().requires_grad_(True),
+             lambda x: rope.qk_norm_rope(x, None, None, w, w, cos, sin, tok, 1, 16, 1, 1, 64))):
+        g, = torch.autograd.grad(call(x).sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            (call(x).float().sum() + g.float().pow(2).sum()).backward()

@@ -49,10 +49,11 @@ void check(const char* name, int rc) {
   throw std::move(err);
 }
 
-// Backwards are differentiable once: a gradient of theirs that is differentiated again raises (when it
-// is, as torch.autograd.function.once_differentiable).
+// Backwards are differentiable once: under create_graph a gradient of theirs that is differentiated again
+// raises when it is (also where only the saved inputs carry gradients, which
+// torch.autograd.function.once_differentiable does not see).
 struct Twice : Function<Twice> {
-  static variable_list forward(AutogradContext*, variable_list in) { return in; }
+  static Tensor forward(AutogradContext*, Tensor x) { return x; }
   static variable_list backward(AutogradContext*, variable_list) {
     throw std::runtime_error(
         "trying to differentiate twice an operator that is differentiable once");
@@ -60,10 +61,8 @@ struct Twice : Function<Twice> {
 };
 
 template <class F>
-variable_list once(const variable_list& grads, F&& f) {
-  bool again = false;
-  if (at::GradMode::is_enabled())
-    for (const Tensor& g : grads) again = again || (g.defined() && g.requires_grad());
+variable_list once(F&& f) {
+  const bool again = at::GradMode::is_enabled();
   variable_list out;
   {
     at::AutoGradMode off(false);
@@ -71,7 +70,7 @@ variable_list once(const variable_list& grads, F&& f) {
   }
   if (again)
     for (Tensor& o : out)
-      if (o.defined()) o = Twice::apply(variable_list{o.detach().requires_grad_(true)})[0];
+      if (o.defined()) o = Twice::apply(o.detach().requires_grad_(true));
   return out;
 }
 
@@ -189,7 +188,7 @@ struct Logprobs : Function<Logprobs> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     if (!g[0].defined() && !g[1].defined() && !g[2].defined()) return variable_list(4);
-    return once(g, [&]() -> variable_list {
+    return once([&]() -> variable_list {
       const variable_list s = ctx->get_saved_variables();
       const Tensor &z = s[0], &tok = s[1], &stats = s[2];
       const c10::DeviceGuard guard(z.device());
@@ -251,7 +250,7 @@ struct QkNorm : Function<QkNorm> {
     return qk_norm_forward(qkv, q, v, wq, wk, cos, sin, pos, n);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    return once(g, [&]() -> variable_list {
+    return once([&]() -> variable_list {
       const variable_list s = ctx->get_saved_variables();
       const Tensor &qkv = s[0], &lq = s[1], &wq = s[2], &wk = s[3];
       const c10::DeviceGuard guard(qkv.device());
@@ -330,7 +329,7 @@ struct Dropout : Function<Dropout> {
     return dropout_forward(x, r, r.defined() ? r.scalar_type() : x.scalar_type(), s, w, d);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    return once(g, [&]() -> variable_list {
+    return once([&]() -> variable_list {
       const variable_list s = ctx->get_saved_variables();
       const std::vector<int64_t> v = ctx->saved_data["d"].toIntVector();
       const Draws d{ctx->saved_data["p"].toDouble(), static_cast<uint64_t>(v[0]),
@@ -371,7 +370,7 @@ struct Embedding : Function<Embedding> {
     return embedding_forward(ids, table, scale, out_type);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    return once(g, [&]() -> variable_list {
+    return once([&]() -> variable_list {
       const Tensor ids = ctx->get_saved_variables()[0];
       const std::vector<int64_t> v = ctx->saved_data["v"].toIntVector();
       const int64_t vocab = v[0], width = v[1], tokens = ids.numel();
