@@ -152,23 +152,32 @@ struct Chunk {
 };
 
 // Running statistics: the maximum m, S = sum 2^x and A = sum 2^x x over x = z c - m c, c = log2(e) / T.
-// x is one fused multiply-add with the rounded m c, which every column of a row shares: its rounding
-// shifts all x alike and drops out of what is computed from them.  Where m c is out of that form's
-// range (rows of -inf, of the lowest value, with +inf) x is (z - m) c.
+// x is one fused multiply-add with the rounded m c: its rounding, the shift m c - round(m c), is in all x of
+// one m alike, so it drops out of differences and of ln S once it is taken off there.  Up to |m c| = 2^20 it
+// is 2^-5 at most; it grows with m c (to 2^7 from 2^31 on, where 2^x overflows).  Beyond that (rows far from
+// zero beside the temperature, masks of -1e9, of the lowest value or -inf alone, +inf) x is (z - m) c, with no
+// shift.
 struct Stats {
   float m, s, a;
 };
 
-__device__ __forceinline__ bool plain_form(float mc) { return fabsf(mc) < 1e30f; }
+__device__ __forceinline__ bool plain_form(float mc) { return fabsf(mc) < 0x1p20f; }
 __device__ __forceinline__ float exponent(float z, float m, float mc, float c) {
   return plain_form(mc) ? __builtin_fmaf(z, c, -mc) : (m == -INFINITY ? z : z - m) * c;
+}
+// What every x relative to m is above (z - m) c.
+__device__ __forceinline__ float shift_of(float m, float mc, float c) {
+  return plain_form(mc) ? __builtin_fmaf(m, c, -mc) : 0.f;
 }
 
 // The statistics relative to another maximum m >= st.m.
 __device__ __forceinline__ void move_max(Stats& st, float m, float c) {
   if (st.m == m) return;
   const float from = st.m * c, to = m * c;
-  float x = plain_form(from) && plain_form(to) ? from - to : (st.m - m) * c;
+  // (one of them out of the plain form: the shift of the other does not cancel)
+  float x = plain_form(from) && plain_form(to)
+                ? from - to
+                : (st.m - m) * c + (shift_of(m, to, c) - shift_of(st.m, from, c));
   x = fmaxf(x, kFloor);
   const float f = st.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x);   // (then s and a are 0)
   st.a = f * __builtin_fmaf(x, st.s, st.a);
@@ -201,10 +210,19 @@ __device__ __forceinline__ void absorb(Stats& st, float& mc, float& limit, bool&
                                        float bm, float c, float lag) {
   constexpr int N = W::N;
   if (__any(bm > limit)) {
-    if (bm > limit) move_max(st, bm, c);
-    mc = st.m * c;
-    limit = st.m + lag;
-    odd = __any(!plain_form(mc));
+    const float m = bm > limit ? bm : st.m, to = m * c;
+    const bool far = __any(!plain_form(to));
+    if (odd || far) {
+      move_max(st, m, c);
+    } else {                                       // (a lane that stays: times 1)
+      const float x = fmaxf(mc - to, kFloor), f = __builtin_amdgcn_exp2f(x);
+      st.a = f * __builtin_fmaf(x, st.s, st.a);
+      st.s = f * st.s;
+      st.m = m;
+    }
+    mc = to;
+    limit = m + lag;
+    odd = far;
   }
   float e[N], x[N];
   if (!odd) {
@@ -470,9 +488,7 @@ __device__ __forceinline__ Stats merge_stats(Stats* lds, Stats st, float c) {
 // exponents share (NaN for a row of -inf alone, as the formula gives); a column's log probability.
 __device__ __forceinline__ float log_sum(const Stats& st, float c) {
   if (!(st.m > -INFINITY)) return NAN;
-  const float mc = st.m * c;
-  const float shift = plain_form(mc) ? __builtin_fmaf(st.m, c, -mc) : 0.f;
-  return logf(st.s) - kLn2 * shift;
+  return logf(st.s) - kLn2 * shift_of(st.m, st.m * c, c);
 }
 template <typename T>
 __device__ __forceinline__ float column_lp(const char* row, int64_t col, const Stats& st,
