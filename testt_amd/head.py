@@ -490,16 +490,22 @@ class _HiddenLogprobs(torch.autograd.Function):
         if not ctx.needs_input_grad[0] or all(g is None for g in grads):
             return None, None, None, None, None
         hidden, weight, tokens, row_max, row_sum, ent, top_ids = ctx.saved_tensors
-        # The fp16 gradient of the logits is held at a power of two that brings the largest upstream
-        # gradient, over the temperature, to 32 .. 64 (as _grad_unit does for the loss): most of its entries are p * g, far
-        # below fp16's range otherwise.  Scaling by a power of two is exact.
-        tops = [g.detach().to(torch.float32).abs().amax().reshape(1) for g in grads
-                if g is not None and g.numel()]
-        top = torch.cat(tops).amax() if tops else hidden.new_ones((), dtype=torch.float32)
+        # A row's fp16 gradient of the logits is held at a power of two that brings its own largest
+        # upstream gradient, over the temperature, to 32 .. 64 (as _grad_unit does for the loss): most of
+        # its entries are p * g, far below fp16's range otherwise.  One scale for all rows leaves those with
+        # small gradients there: an entropy bonus at 1e-4 of another row's advantage, 151936 columns of
+        # standard deviation 2.4, 2e-2 off and of 0.05 all of it lost; 3e-4 and 2e-4 at the row's own.  A
+        # power of two is exact, and a row's divides out of its hidden gradient.
+        columns = [g if g.dim() == 2 else g[:, None] for g in grads if g is not None]
+        columns = [g.to(torch.float32).abs() for g in columns if g.shape[1]]
+        top = torch.cat(columns, 1).amax(1) if columns else \
+            hidden.new_zeros(hidden.shape[0], dtype=torch.float32)
         _, exponent = torch.frexp(torch.where(top > 0, top / ctx.args[1], 1.0))
         exponent = exponent.clamp(-100, 100)
         unit = torch.ldexp(torch.ones_like(top), 6 - exponent)
-        grads = [None if g is None else (g.to(torch.float32) * unit).contiguous() for g in grads]
+        grads = [None if g is None else
+                 (g.to(torch.float32) * (unit if g.dim() == 1 else unit[:, None])).contiguous()
+                 for g in grads]
         rows, width = hidden.shape
         vocab = weight.shape[0]
         dh = torch.empty_like(hidden)
@@ -513,7 +519,7 @@ class _HiddenLogprobs(torch.autograd.Function):
             del logits
             _hidden_grad(g, weight, dh[part])
             del g
-        return (dh.to(torch.float32) / unit).to(torch.float16), None, None, None, None
+        return (dh.to(torch.float32) / unit[:, None]).to(torch.float16), None, None, None, None
 
 
 def fused_token_logprobs(hidden16, weight16, tokens, top_k=0, temperature=1.0):
