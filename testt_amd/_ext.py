@@ -222,6 +222,16 @@ def dtype_code(tensor, name, allowed=(torch.float16, torch.bfloat16, torch.float
     return DTYPES[tensor.dtype]
 
 
+def refuse_dispatching(*args):
+    """Raises for a tensor subclass with a __torch_dispatch__ (a wrapper, a fake or distributed tensor):
+    the kernels read memory, which is not where such a tensor's values are."""
+    for t in args:
+        if isinstance(t, torch.Tensor) and \
+                type(t).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__:
+            raise TypeError(f"{type(t).__name__} implements __torch_dispatch__: the soupk kernels take "
+                            "tensors whose memory holds their values")
+
+
 def checked(result):
     """The result of a native operator (host()) for arguments that the caller has checked."""
     if result is None:

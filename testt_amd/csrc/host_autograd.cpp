@@ -89,9 +89,12 @@ int32_t code_of(at::ScalarType t) {
                                              : t == at::kFloat ? SOUPK_DTYPE_F32 : -1;
 }
 
-// A tensor argument, subclasses (Parameter) included; null for anything else.
+// A tensor argument, subclasses included (the Python caller has asked their __torch_function__); null for
+// anything else and for a subclass with a __torch_dispatch__, whose memory (if it has any) is not its values.
 const Tensor* tensor(PyObject* o) {
-  return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr;
+  if (!THPVariable_Check(o)) return nullptr;
+  const Tensor& t = THPVariable_Unpack(o);
+  return t.unsafeGetTensorImpl()->is_python_dispatch() ? nullptr : &t;
 }
 bool maybe(PyObject* o, Tensor& t) {
   if (o == Py_None) return true;

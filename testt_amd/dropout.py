@@ -12,6 +12,7 @@ and a step can be repeated.  torch's own dropout draws from the generator's stat
 per element (the reference's path, solution/model.py:195-206)."""
 
 import torch
+from torch.overrides import handle_torch_function, has_torch_function
 
 from . import _ext
 
@@ -49,9 +50,12 @@ def dropout(x, p, seed, call=0, rows=None, residual=None):
     step's or layer's number); rows: int64, the row number in [0, 2^32) that each row draws as;
     residual: x's shape, x's type or fp32.  The sum is rounded once.  p = 1 gives the residual (or
     zeros) exactly, whatever x holds."""
+    if has_torch_function((x, seed, rows, residual)):
+        return handle_torch_function(dropout, (x, seed, rows, residual), x, p, seed, call, rows, residual)
     done = _ext.host().dropout(x, p, seed, call, rows, residual)
     if done is not None:
         return done
+    _ext.refuse_dispatching(x, seed, rows, residual)
     if not isinstance(x, torch.Tensor):
         raise TypeError(f"x must be a tensor, got {type(x).__name__}")
     if not x.is_cuda:

@@ -9,6 +9,7 @@ tokens are sorted by id, stably, and every row's gradient is summed over its tok
 in fp32 and rounded once -- the same bits every time, unlike sums by atomics."""
 
 import torch
+from torch.overrides import handle_torch_function, has_torch_function
 
 from . import _ext
 
@@ -20,10 +21,13 @@ def embedding(ids, table, scale=1.0, out_dtype=None, padding_idx=None):
     ids: int64 or int32 of any shape; an id outside [0, V) gives a row of zeros and no gradient.
     table: contiguous fp16, bf16 or fp32 [V, H].  padding_idx: a row that gets no gradient (its
     values are looked up like any other's), as torch's."""
+    if has_torch_function((ids, table)):
+        return handle_torch_function(embedding, (ids, table), ids, table, scale, out_dtype, padding_idx)
     if padding_idx is None and (out_dtype is None or out_dtype is torch.float32):
         done = _ext.host().embedding(ids, table, scale, out_dtype is torch.float32, -1)
         if done is not None:
             return done
+    _ext.refuse_dispatching(ids, table)
     _ext.require(table, "table", ndim=2)
     _ext.dtype_code(table, "table")
     if not isinstance(ids, torch.Tensor):
@@ -46,6 +50,6 @@ def embedding(ids, table, scale=1.0, out_dtype=None, padding_idx=None):
 
 
 def supported(table):
-    """A table that embedding() takes."""
-    return (table.is_cuda and table.dim() == 2 and table.dtype in _ext.DTYPES
+    """A table that embedding() takes and no subclass has a say in."""
+    return (type(table) in (torch.Tensor, torch.nn.Parameter) and table.is_cuda and table.dim() == 2 and table.dtype in _ext.DTYPES
             and table.is_contiguous())

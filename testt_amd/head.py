@@ -36,6 +36,7 @@ import math
 from collections import namedtuple
 
 import torch
+from torch.overrides import handle_torch_function, has_torch_function
 
 from . import _ext
 from . import blas as _blas
@@ -378,7 +379,17 @@ def fused_head_loss(hidden16, weight16, targets, denominator):
 
 MAX_TOP = 32      # most alternatives per row
 
-TokenLogprobs = namedtuple("TokenLogprobs", "logprob entropy top_logprobs top_ids")
+
+class TokenLogprobs(namedtuple("TokenLogprobs", "logprob entropy top_logprobs top_ids")):
+    """The numbers of token_logprobs; also from one iterable of them, as torch builds a tuple again whose
+    tensors it has given a subclass's type."""
+
+    __slots__ = ()
+
+    def __new__(cls, logprob, entropy=None, top_logprobs=None, top_ids=None):
+        if entropy is None:
+            logprob, entropy, top_logprobs, top_ids = logprob
+        return super().__new__(cls, logprob, entropy, top_logprobs, top_ids)
 
 
 def _check_logprobs(top_k, temperature, vocab):
@@ -431,9 +442,12 @@ def token_logprobs(logits, tokens, top_k=0, temperature=1.0):
     gradient).  Masked logits may be -inf or the type's lowest value; a NaN or +inf in a row, or a
     row of -inf alone, makes the row's numbers NaN (its NaN logits rank with -inf among the
     alternatives).  A row without upstream gradient gets zeros."""
+    if has_torch_function((logits, tokens)):
+        return handle_torch_function(token_logprobs, (logits, tokens), logits, tokens, top_k, temperature)
     done = _ext.host().token_logprobs(logits, tokens, top_k, temperature)
     if done is not None:
         return TokenLogprobs(*done)
+    _ext.refuse_dispatching(logits, tokens)
     if not isinstance(logits, torch.Tensor) or not isinstance(tokens, torch.Tensor):
         raise TypeError("logits and tokens must be tensors")
     if not logits.is_cuda:
@@ -527,6 +541,7 @@ def fused_token_logprobs(hidden16, weight16, tokens, top_k=0, temperature=1.0):
     the full logits (chunks of CHUNK_ROWS rows), differentiable in hidden16: the log probabilities
     a policy-gradient or preference loss takes, where fused_head_loss gives the cross-entropy.
     The logits are fp16, as there."""
+    _ext.refuse_dispatching(hidden16, weight16, tokens)
     _ext.require(hidden16, "hidden16", dtype=torch.float16, ndim=2)
     _ext.require(weight16, "weight16", dtype=torch.float16, ndim=2, device=hidden16.device)
     _ext.require(tokens, "tokens", dtype=torch.int64, ndim=1, device=hidden16.device)

@@ -10,6 +10,7 @@ output; the LoRA branches get views of the same buffer.
 """
 
 import torch
+from torch.overrides import handle_torch_function, has_torch_function
 
 from . import _ext
 from ._common import next_pow2
@@ -177,10 +178,15 @@ def qk_norm_rope(qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx, bat
     lora_q [M, n_heads*head_dim] / lora_v [M, n_kv*head_dim]: None, the rows' type or fp32.  cos,
     sin, pos_idx, batch, seq as rope_pack_tokens; head_dim a multiple of 16 up to 256.  A token
     whose position lies outside [0, batch*seq) gets a row of zeros (and passes no gradient)."""
+    tensors = (qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx)
+    if has_torch_function(tensors):
+        return handle_torch_function(qk_norm_rope, tensors, *tensors, batch, seq, n_heads, n_kv, head_dim,
+                                     eps)
     done = _ext.host().qk_norm_rope(qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx, batch,
                                     seq, n_heads, n_kv, head_dim, eps)
     if done is not None:
         return done
+    _ext.refuse_dispatching(*tensors)
     _ext.require(qkv, "qkv", ndim=2)
     _ext.dtype_code(qkv, "qkv", (torch.float16, torch.bfloat16))
     rows, dev = qkv.shape[0], qkv.device
