@@ -396,6 +396,11 @@ def _forward(model, cos, sin, input_ids, attention_mask, labels, num_items_in_ba
     pos_idx = attention_mask.reshape(-1).nonzero().squeeze(1)
 
     ids = input_ids.reshape(-1).index_select(0, pos_idx)
+    # (embedding() gives an unknown id a row of zeros; in a training step it is a mistake of the data, and
+    # the device is waited for just above anyway)
+    if not torch.equal(ids.clamp(0, model.embed.shape[0] - 1), ids):
+        raise IndexError(f"input_ids of real tokens lie outside the embedding's {model.embed.shape[0]} "
+                         "rows")
     if _embedding.supported(model.embed):     # (the fp32 residual stream in one launch)
         s = _embedding.embedding(ids, model.embed, out_dtype=torch.float32)
     else:
