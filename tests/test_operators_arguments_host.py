@@ -1,4 +1,4 @@
-"""Arguments of the operators around the layer that are no plain tensors (CPU)."""
+"""Arguments of the operators around the layer that are no plain tensors, or are left out (CPU)."""
 
 import pytest
 import torch
@@ -67,3 +67,12 @@ def test_wrappers_without_memory_are_refused():
         with pytest.raises(TypeError, match="memory"):
             call()
     assert not embedding.supported(z)
+
+
+def test_counter_dropout_needs_a_seed():
+    """Modules left at one default seed would all draw the same mask."""
+    with pytest.raises(TypeError, match="seed"):
+        dropout.CounterDropout(0.1)
+    with pytest.raises(TypeError, match="seed"):
+        dropout.CounterDropout()
+    assert dropout.CounterDropout(0.1, 0).seed == 0

@@ -89,12 +89,16 @@ class CounterDropout(torch.nn.Dropout):
     itself.  As the LoRA dropout of a layer or model of this package (it is a torch.nn.Dropout) it
     runs on the real tokens' rows alone and draws at their padded positions.
 
-    Modules that are to draw independently (of two projections, of the layers) get seeds of their own.
+    The seed has no default: modules of one seed draw the same mask at the same positions, so those that
+    are to draw independently (of two projections, of the layers, of data-parallel ranks) get seeds of
+    their own.
     A forward that is run again inside a backward (activation checkpointing) raises: it would draw with
     another call number than the first run did; such a program calls dropout() with the step's number."""
 
-    def __init__(self, p=0.5, seed=0):
+    def __init__(self, p=0.5, seed=None):
         super().__init__(_check_p(p))
+        if seed is None:
+            raise TypeError("CounterDropout needs a seed of its own: modules of one seed draw the same mask")
         if not isinstance(seed, torch.Tensor):
             _check_word(seed, "seed")
         self.seed = seed
