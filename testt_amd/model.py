@@ -149,6 +149,12 @@ def _norm_weight(weight):
     return w if w.dtype == torch.float32 else w.float()
 
 
+def _head_norm_weight(weight):
+    """A query or key norm's weight as qk_norm_rope takes it: one that is trained as it is (its gradient
+    goes through the operator), a frozen one as _norm_weight gives it."""
+    return weight if weight.requires_grad else _norm_weight(weight)
+
+
 def _dropout_p(dropout):
     """The probability the dropout module applies now (0 for Identity or in eval mode)."""
     if isinstance(dropout, torch.nn.Dropout) and dropout.training:
@@ -267,7 +273,8 @@ class ModelPlan:
                 d is not None for d in drop) else 0.0,
             lora_dropout=tuple(drop), attn_scale=getattr(lp.attn, "scaling", None),
             **({} if lp.q_norm is None else dict(
-                q_norm=lp.q_norm.weight, k_norm=lp.k_norm.weight,
+                q_norm=_head_norm_weight(lp.q_norm.weight),
+                k_norm=_head_norm_weight(lp.k_norm.weight),
                 qk_eps=lp.q_norm.variance_epsilon)))
 
 
