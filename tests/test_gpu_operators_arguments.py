@@ -1,4 +1,4 @@
-"""Arguments of the operators around the layer that are no plain tensors."""
+"""Arguments of the operators around the layer that are no plain tensors or numbers."""
 
 import pytest
 import torch
@@ -47,3 +47,27 @@ def test_subclasses_come_back(i):
     first(got).float().sum().backward()
     assert torch.equal(sub.grad.as_subclass(torch.Tensor), plain.grad)
     assert type(call(torch.nn.Parameter(x))) is type(want)
+
+
+def test_numbers_that_want_a_gradient_are_refused():
+    """No gradient is given for a temperature, scale, probability or eps: a tensor that asks for one
+    raises instead of staying without in silence; other tensors of one number are taken."""
+    num = lambda v, grad: torch.tensor(v, device=DEV, requires_grad=grad)
+    (z, _), (x, _), (t, _), (q, _) = calls()
+    tok = torch.arange(6, device=DEV)
+    cos, sin = (c.to(DEV) for c in workloads.rope_tables(8, 64))
+    w = torch.ones(64, device=DEV)
+    weight = torch.randn(500, 64, device=DEV).half()
+    norm = lambda e: rope.qk_norm_rope(q, None, None, w, w, cos, sin, tok, 1, 8, 1, 1, 64, e)
+    for name, value, call in (
+            ("temperature", 0.5, lambda v: head.token_logprobs(z, tok, 0, v)),
+            ("temperature", 0.5, lambda v: head.fused_token_logprobs(x.half(), weight, tok, 0, v)),
+            ("p", 0.5, lambda v: dropout.dropout(x, v, 1)),
+            ("scale", 0.5, lambda v: embedding.embedding(tok, t, v)),
+            ("scale", 0.5, lambda v: embedding.embedding(tok, t, v, padding_idx=0)),
+            ("eps", 0.5, norm)):
+        with pytest.raises(TypeError, match=name):
+            call(num(value, True))
+        assert torch.equal(first(call(num(value, False))), first(call(value)))
+        with torch.no_grad():
+            assert torch.equal(first(call(num(value, True))), first(call(value)))

@@ -232,6 +232,14 @@ def refuse_dispatching(*args):
                             "tensors whose memory holds their values")
 
 
+def number(value, name):
+    """A number, from anything float() takes but a tensor that wants a gradient: the operators give none
+    for their numbers."""
+    if isinstance(value, torch.Tensor) and value.requires_grad and torch.is_grad_enabled():
+        raise TypeError(f"{name} wants a gradient, which is not given: pass a number (or {name}.detach())")
+    return float(value)
+
+
 def checked(result):
     """The result of a native operator (host()) for arguments that the caller has checked."""
     if result is None:

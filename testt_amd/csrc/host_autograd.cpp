@@ -126,7 +126,10 @@ bool integer(PyObject* o, int64_t& v) {
   PyErr_Clear();
   return false;
 }
+// A number, or a tensor of one that wants no gradient (none would be given; the Python caller says so).
 bool number(PyObject* o, double& v) {
+  if (THPVariable_Check(o) && at::GradMode::is_enabled() && THPVariable_Unpack(o).requires_grad())
+    return false;
   v = PyFloat_AsDouble(o);
   if (!PyErr_Occurred()) return true;
   PyErr_Clear();

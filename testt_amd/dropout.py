@@ -18,7 +18,7 @@ from . import _ext
 
 
 def _check_p(p):
-    p = float(p)
+    p = _ext.number(p, "p")
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout probability must lie in [0, 1], got {p}")
     return p

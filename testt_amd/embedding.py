@@ -45,7 +45,7 @@ def embedding(ids, table, scale=1.0, out_dtype=None, padding_idx=None):
                              f"{table.shape[0]} rows")
         padding_idx = int(padding_idx) % table.shape[0]
     return _ext.checked(_ext.host().embedding(
-        ids.to(torch.int64).contiguous(), table, float(scale), out_dtype is torch.float32,
+        ids.to(torch.int64).contiguous(), table, _ext.number(scale, "scale"), out_dtype is torch.float32,
         -1 if padding_idx is None else padding_idx))
 
 

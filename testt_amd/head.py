@@ -398,7 +398,7 @@ def _check_logprobs(top_k, temperature, vocab):
         raise TypeError(f"top_k must be an int, got {type(top_k).__name__}")
     if not 0 <= top_k <= min(MAX_TOP, vocab):
         raise ValueError(f"top_k must lie in [0, {min(MAX_TOP, vocab)}], got {top_k}")
-    temperature = float(temperature)
+    temperature = _ext.number(temperature, "temperature")
     # (an fp32 value with an fp32 reciprocal)
     if not 1e-30 <= temperature <= 1e30:
         raise ValueError(f"temperature must lie in [1e-30, 1e30], got {temperature}")

@@ -220,7 +220,7 @@ def qk_norm_rope(qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx, bat
         raise ValueError(f"pos_idx must be {rows} integer positions on {dev}")
     if batch < 0 or seq < 0 or batch * seq >= 1 << 31:
         raise ValueError(f"batch ({batch}) and seq ({seq}) must span fewer than 2^31 positions")
-    eps = float(eps)
+    eps = _ext.number(eps, "eps")
     if not 0.0 <= eps <= 3e38:
         raise ValueError(f"eps must be a non-negative number, got {eps}")
     return _ext.checked(_ext.host().qk_norm_rope(
