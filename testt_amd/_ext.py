@@ -23,7 +23,6 @@ LORA_SCRATCH_FLOATS = 4 << 20         # SOUPK_LORA_SCRATCH_FLOATS
 DTYPE_F16 = 0
 DTYPE_F32 = 1
 DTYPE_BF16 = 2
-QK_NORM_BLOCKS = 1024                 # SOUPK_QK_NORM_BLOCKS
 
 _p = ctypes.c_void_p
 _i32 = ctypes.c_int32
