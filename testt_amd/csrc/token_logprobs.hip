@@ -21,18 +21,19 @@
 // step's columns, those equal to its bound are listed by themselves, only as far as they can count (by
 // their order).  At the end the listed chunks that reach the last bound are read again, and their
 // columns ranked.  Where the list overflows (a row that rises from left to right) the row is read once
-// more by the last bound: 1030 rows of 40000 fp32 columns with 32 alternatives take 82 us instead of 39,
-// of 151936 columns 272 instead of 115 (K searches instead: 2118 and 10924).  Where even those columns do
+// more by the last bound: 1030 rows of 40000 fp32 columns with 32 alternatives take 83 us instead of 39,
+// of 151936 columns 271 instead of 115 (K searches instead: 2118 and 10924).  Where even those columns do
 // not fit (large ones that come back every 1024 columns, in some of the threads' places alone), the row
 // is ranked by K searches.
 //
 // Few rows are cut into parts, whose statistics and alternatives a second launch joins.
 //
-// Measured (MI355X): 2048 rows of 151936 bf16 (622 MB) 102 us without alternatives (6.1 TB/s; reading
-// alone 93), 115 with 8, 126 with 32: the bounds and lists are latency between barriers that all the
-// rows of a CU meet together, so 512 threads a row (127 us with 8) and 1024 are slower, and fewer or
-// more loads in flight change nothing.  The gradient of 888 rows fp16 reads and writes 540 MB in 91 us
-// (5.9 TB/s); one 16-byte store a thread 114, eight 99.
+// Measured (MI355X): 2048 rows of 151936 bf16 (622 MB) 100 us without alternatives (6.2 TB/s; reading
+// alone 93), 107 with 8, 118 with 32: the bounds and lists are latency between barriers that all the
+// rows of a CU meet together, so 512 threads a row (127 us with 8 where 256 took 115) and 1024 are slower, and
+// fewer or more loads in flight change nothing.  The gradient of 888 rows fp16 reads and writes 540 MB in
+// 77 us (7.0 TB/s, its reads in part from the Infinity Cache, where the forward left the rows; 91 behind a
+// forward that streams past them, where one 16-byte store a thread took 114 and eight 99).
 
 #include <algorithm>
 #include <type_traits>
