@@ -712,10 +712,10 @@ int soupk_gemm_nn_workspace(int64_t M, int32_t N, int32_t K, int64_t* floats);
  * beyond the reference's kernel set, next to soupk_head_stats_grad; the reference takes the loss and
  * the entropy only, solution/head.py:34-76).  logits: `rows` rows of V elements (dtype F16, BF16 or
  * F32), row r at (r / inner) * stride_outer + (r % inner) * stride_inner elements.  Over
- * d = (z - max z) / temperature, S = sum exp(d):
+ * d = (z - max z) / temperature (1e-30 to 1e30), S = sum exp(d):
  *   logprob = d[token] - ln S (0 for token -100; NaN for any other token outside [0, V))
- *   entropy = ln S - sum(exp(d) d) / S;  row_max = max z, row_sum = S (for the
- *   backward; both NULL: not wanted)
+ *   entropy = ln S - sum(exp(d) d) / S;  row_max = max z, row_sum = S as the kernel
+ *   holds it, a factor near 1 included (for the backward; both NULL: not wanted)
  *   top_id[r, k], top_lp[r, k] = d[top_id] - ln S: the top_k (0 .. 32, <= V) largest logits in
  *   decreasing order, equal ones by the lower column; a NaN ranks with -inf
  * NaN or +inf in a row, or a row of -inf alone, makes its numbers NaN.  top_lp and top_id are

@@ -52,6 +52,15 @@ def compare(z, tok, top_k, temperature, copies):
               2.0 ** -126 * factor + torch.finfo(z.dtype).smallest_normal * eps, "dlogits")
 
 
+@pytest.mark.parametrize("temperature", [1e-30, 9.9e29])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_ends_of_the_temperature_range(temperature, dtype):
+    z, tok = logits_of(5, 3001, dtype, 8)
+    tok = torch.where(tok < 0, 5, tok)
+    z[2] = 1.25
+    compare(z, tok, 4, temperature, 1)
+
+
 # rows cut into parts, and enough of them to stay whole
 @pytest.mark.parametrize("copies", [1, 150])
 @pytest.mark.parametrize("dtype", TYPES)

@@ -829,7 +829,8 @@ bool bad_dtype(int32_t d) {
 
 bool bad_lp(int32_t dtype, int64_t rows, int64_t inner, int64_t V, float temperature) {
   return bad_dtype(dtype) || rows < 0 || rows > 0x7fffffff / kMaxParts || inner < 1 || V < 1 ||
-         V >= (int64_t{1} << 31) - 16 || !(temperature > 0.f) || temperature > 3e38f;
+         V >= (int64_t{1} << 31) - 16 ||
+         !(temperature >= 1e-30f && temperature <= 1e30f);   // (1 / T and log2(e) / T are fp32 numbers)
 }
 
 }  // namespace
