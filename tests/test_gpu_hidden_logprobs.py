@@ -117,3 +117,43 @@ def test_no_rows():
     out = head.fused_token_logprobs(hidden, weight, torch.zeros(0, dtype=torch.int64, device=DEV), 3)
     grad, = torch.autograd.grad([out.logprob.sum() + out.top_logprobs.sum()], hidden)
     assert grad.shape == (0, 64) and out.top_ids.shape == (0, 3)
+
+
+@pytest.mark.parametrize("vocab,width", [(1017, 64), (1016, 36), (7, 8)])
+def test_sizes_that_the_split_product_does_not_take(vocab, width):
+    hidden, weight, tok, g = data(5, vocab, width, vocab)
+    leaf = hidden.clone().requires_grad_(True)
+    got = head.fused_token_logprobs(leaf, weight, tok, 3, 0.8)
+    ups = [torch.randn(o.shape, generator=g).to(DEV) for o in got[:3]]
+    grad, = torch.autograd.grad(got[:3], leaf, ups)
+    check_grad(grad, hidden, weight, tok, ups, 3, 0.8)
+
+
+def test_graph_replay():
+    """Forward and backward captured and replayed on other rows, with eager work between."""
+    hidden, weight, tok, g = data(300, 5000, 64, 9)
+    ups = [torch.randn(300, generator=g).to(DEV) * 10.0 ** -(torch.arange(300, device=DEV) % 6)
+           for _ in range(2)]
+
+    def step(h):
+        leaf = h.detach().requires_grad_(True)
+        out = head.fused_token_logprobs(leaf, weight, tok, 4)
+        grad, = torch.autograd.grad([out.logprob, out.entropy], leaf, ups)
+        return [o.detach() for o in out] + [grad]
+
+    static = hidden.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step(static)
+    for i in range(4):
+        new = (hidden.float() * (1 - 0.2 * i)).half()
+        static.copy_(new)
+        graph.replay()
+        want = step(new)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
