@@ -25,16 +25,18 @@
 extern "C" {
 #endif
 
-/* ABI version of this header; soupk_abi_version() returns the library's.  6 adds
-   soupk_token_logprobs_fwd, soupk_token_logprobs_bwd, soupk_token_logprobs_workspace,
+/* ABI version of this header; soupk_abi_version() returns the library's.  7 adds
+   soupk_rotary_tables, soupk_rotary, soupk_rope_append, soupk_paged_attention,
+   soupk_paged_attention_workspace, soupk_verify_drafts and soupk_verify_drafts_workspace to version
+   6's entry points; 6 added soupk_token_logprobs_fwd, soupk_token_logprobs_bwd, soupk_token_logprobs_workspace,
    soupk_qk_norm_rope_fwd, soupk_qk_norm_rope_bwd, soupk_dropout, soupk_embedding_fwd,
-   soupk_embedding_bwd and soupk_embedding_bwd_workspace to version 5's; 5 added soupk_gemm_nn,
+   soupk_embedding_bwd and soupk_embedding_bwd_workspace to version 5's, 5 soupk_gemm_nn,
    soupk_gemm_nn_workspace, soupk_head_plan, soupk_head_stats_grad_planned, soupk_head_finish,
    soupk_head_dh and soupk_attention_wide to version 4's entry points, which had added
    soupk_lora_rope_fwd, soupk_gemm_nn_nf4, soupk_gemm_tn_nf4_split, soupk_gemm_nn_nf4_split,
    soupk_gemm_lt, soupk_gemm_lt_index, soupk_layer_fwd, soupk_layer_bwd (with the layer's
    products on NF4 weights: SoupkLayerNf4) and soupk_init_device to version 3's. */
-#define SOUPK_ABI_VERSION 6
+#define SOUPK_ABI_VERSION 7
 
 /* Status of soupk_lora_bwd_params_noalloc for a problem beyond its static scratch (no launch). */
 #define SOUPK_STATUS_SCRATCH_LIMIT 20001
@@ -804,6 +806,89 @@ int soupk_embedding_bwd_workspace(int64_t M, int64_t V, int64_t H, int64_t* byte
 int soupk_embedding_bwd(const void* dout, int32_t grad_dtype, const int64_t* ids, void* dtable,
                         int32_t dtype, float scale, int64_t padding_idx, void* workspace,
                         int64_t workspace_bytes, int64_t M, int64_t V, int64_t H, void* stream);
+
+/*
+ * Tables of rotary positions (the reference takes them from transformers' rotary embedding,
+ * solution/model.py:209-279): cos, sin fp32 [seq, dim / 2], of position * frequency, times gain.
+ * inv_freq: host memory, dim / 2 frequencies in radians a position (at most 1e6), or NULL: theta^(-2 i /
+ * dim), scaled.  scaling: LINEAR, frequencies / factor; DYNAMIC, theta (factor seq / original -
+ * (factor - 1))^(dim / (dim - 2)) in theta's place where seq > original; YARN, frequency / factor * r +
+ * frequency * (1 - r) with r rising over the pairs from the one of beta_fast turns within original to the
+ * one of beta_slow.  dim even, at most 256; 1 < theta <= 1e30; 1 <= factor <= 1e6.  cos and sin 16-byte
+ * aligned.
+ */
+#define SOUPK_ROPE_DEFAULT 0
+#define SOUPK_ROPE_LINEAR 1
+#define SOUPK_ROPE_DYNAMIC 2
+#define SOUPK_ROPE_YARN 3
+int soupk_rotary_tables(float* cos, float* sin, int64_t seq, int32_t dim, const double* inv_freq, double theta,
+                        int32_t scaling, double factor, double original, double beta_fast, double beta_slow,
+                        double gain, void* stream);
+
+/*
+ * Rotation of the leading R elements of every head (solution/rope.py:24-75 rotates whole heads by
+ * halves): x [rows, heads, D] of dtype F16, BF16 or F32 with the given strides (elements; a head's elements
+ * adjacent), out [rows, heads, D] contiguous.  Pairs (i, i + R/2), or (2 i, 2 i + 1) when interleaved, turn by
+ * row pos[r] of cos, sin (fp32, R/2 columns, rows table_stride apart); the others are copied.  inverse: by
+ * the opposite angle (the gradient).  A row whose pos lies outside [0, n_pos) gets zeros.
+ */
+int soupk_rotary(const void* x, int32_t dtype, int64_t row_stride, int64_t head_stride, const float* cos,
+                 const float* sin, int64_t n_pos, int64_t table_stride, const int64_t* pos, void* out,
+                 int64_t rows, int32_t heads, int32_t D, int32_t R, int32_t interleaved, int32_t inverse,
+                 void* stream);
+
+/*
+ * New tokens into a paged key-value cache.  qkv [rows, (NH + 2 NKV) D] of dtype F16 or BF16, lora_q
+ * [rows, NH D], lora_v [rows, NKV D] (nullable; lora_dtype F32 or dtype) as soupk_rope_pack_tokens;
+ * rotation as soupk_rotary (cos NULL: none).  k_pages, v_pages: [n_pages, NKV, page_size, D] of dtype, pages page_stride
+ * elements apart.  Tokens
+ * cu[b] .. cu[b + 1] of the rows (cu NULL: row b) are the last ones of sequence b, which has lengths[b]
+ * tokens with them: token i stands at t = lengths[b] - (cu[b + 1] - cu[b]) + i, in slot t % page_size
+ * of page block_table[b, t / page_size].  q_out [rows, NH D] gets q + lora_q rotated; the slot gets k
+ * rotated and v + lora_v.  A token without a place (no sequence, t < 0 or outside the tables or the block
+ * table, a page outside [0, n_pages)) gets zeros in q_out and is written nowhere.  D a multiple of 16,
+ * at most 256; max_pages * page_size < 2^31.
+ */
+int soupk_rope_append(const void* qkv, const void* lora_q, const void* lora_v, int32_t lora_dtype,
+                      const float* cos, const float* sin, int64_t n_pos, int64_t table_stride, int32_t R,
+                      int32_t interleaved, const int32_t* cu, const int32_t* lengths,
+                      const int32_t* block_table, int32_t B, int64_t max_pages, void* q_out, void* k_pages,
+                      void* v_pages, int64_t n_pages, int64_t page_stride, int32_t page_size, int32_t dtype,
+                      int64_t rows, int32_t NH, int32_t NKV, int32_t D, void* stream);
+
+/*
+ * Attention of new tokens over that cache (the reference generates nothing; the training form is
+ * soupk_attention_varlen_fwd): out [rows, NH D] = softmax(scale q . k_j) v_j over the keys j <= t of each
+ * token, at its place t as above; query head h reads key head h / (NH / NKV).  q rows are q_stride elements
+ * apart.  A token that sees no key gets zeros, and so do rows of no sequence; keys in pages outside
+ * [0, n_pages) are not seen.  lengths beyond the block table are cut to it.  k_pages and v_pages 16-byte
+ * aligned, max_pages * page_size at most 2^30, rows * NH at most 2^23.  workspace:
+ * soupk_paged_attention_workspace bytes on the current device, 16-byte aligned; a call that runs beside another needs its own.
+ */
+int soupk_paged_attention_workspace(int64_t rows, int32_t B, int32_t NH, int32_t NKV, int32_t D,
+                                    int64_t max_pages, int32_t page_size, int64_t* bytes);
+int soupk_paged_attention(const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
+                          int64_t n_pages, int64_t page_stride, int32_t page_size,
+                          const int32_t* block_table, int64_t max_pages, const int32_t* lengths,
+                          const int32_t* cu, int32_t B, void* out, int32_t dtype,
+                          int64_t rows, int32_t NH, int32_t NKV, int32_t D, float scale, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+
+/*
+ * Verification of drafted tokens (next to soupk_token_logprobs_fwd).  target [B, K + 1, V] and draft
+ * [B, K, V] (NULL: the drafts were certain) probabilities of dtype F16, BF16 or F32, tokens [B, K],
+ * uniforms fp32 [B, K + 1] in [0, 1), lengths int32 [B] (NULL: K) the drafted tokens of each sequence.
+ * accepted[b] = n, the leading tokens with uniforms[b, i] * draft[b, i, x_i] < target[b, i, x_i];
+ * out[b] = those n, then the lowest id whose prefix sum of w exceeds uniforms[b, K] * sum(w), then -1;
+ * w = max(target[b, n] - draft[b, n], 0) after a refusal (target[b, n] where that is 0 everywhere),
+ * target[b, n] otherwise.  -1 in the drawn token's place where w is 0 everywhere.  A negative,
+ * infinite or NaN probability counts as 0.  workspace: soupk_verify_drafts_workspace bytes, 8-byte aligned.
+ */
+int soupk_verify_drafts_workspace(int64_t B, int64_t V, int64_t* bytes);
+int soupk_verify_drafts(const void* target, const void* draft, int32_t dtype, const int64_t* tokens,
+                        const float* uniforms, const int32_t* lengths, int64_t* out, int32_t* accepted,
+                        int64_t B, int32_t K, int64_t V, void* workspace, int64_t workspace_bytes,
+                        void* stream);
 
 #ifdef __cplusplus
 }

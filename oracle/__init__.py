@@ -15,6 +15,8 @@ apply_rotary_pos_emb, SiLU * up, cross-entropy):
 - logprobs.py log probabilities, entropy and top alternatives in float64
 - qk_norm.py  per-head RMS norm of queries and keys + rotation in float64
 - dropout.py  Philox4x32-10 and the keep mask drawn from it
+- generate.py rotary tables and rotation, the paged cache and its attention, verification of drafts, in
+              float64
 
 Only tests/, __graft_entry__.smoke() and bench.py's CPU-baseline leg may import this package,
 and only as the checker or the timed CPU baseline; the product path (testt_amd) never does.

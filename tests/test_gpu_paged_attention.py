@@ -1,0 +1,259 @@
+"""Attention over a paged cache against 64 bits.
+
+Tolerance, per output element, with W = sum p |v| (the oracle's second result):
+  a score q.k: D products exact in fp32, their sum and the scaling rounded, at most (D + 4) 2^-23 of
+    scale * sum |q k|, which the exponential turns into that relative error of p, top and bottom: twice;
+  p rounded to the cache's type: eps / 2 of it (and 2^-25 absolute for an fp16 one below 2^-14, beside
+    a largest p of at least 1); exponentials 2^-22; the fp32 sums over n keys n 2^-24;
+  the output's rounding: eps / 2 of it."""
+
+import pytest
+import torch
+
+from oracle import generate as og
+from testt_amd import attention
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+H, B = torch.float16, torch.bfloat16
+I32 = torch.int32
+
+
+def make(lengths, news, page, nh, nkv, d, dtype, seed=0, width=None, junk=float("nan"), spread=1.0):
+    """Pages in random order, everything outside the sequences `junk`."""
+    gen = torch.Generator().manual_seed(seed)
+    need = [-(-max(n, 0) // page) for n in lengths]
+    width = max(need + [1]) if width is None else width
+    order = torch.randperm(sum(need) + 2, generator=gen).tolist()
+    table = [[order.pop() if i < n else (-1 if i % 2 else 1 << 30) for i in range(width)] for n in need]
+    pages = torch.full((2, sum(need) + 2, nkv, page, d), junk)
+    for b, n in enumerate(lengths):
+        for t in range(n):
+            pages[:, table[b][t // page], :, t % page] = torch.randn(2, nkv, d, generator=gen)
+    cu = [0]
+    for n in news:
+        cu.append(cu[-1] + n)
+    q = spread * torch.randn(cu[-1], nh * d, generator=gen)
+    return q.to(dtype), *pages.to(dtype), table, cu
+
+
+def seqs(table, lengths, cu):
+    return (torch.tensor(table, dtype=I32, device=DEV).reshape(len(lengths), len(table[0]) if table else 1),
+            torch.tensor(lengths, dtype=I32, device=DEV),
+            None if cu is None else torch.tensor(cu, dtype=I32, device=DEV))
+
+
+def check(got, q, k, v, table, lengths, cu, dtype, scale=None):
+    want, weight = og.paged_attention(q, k, v, table, lengths, cu, scale)
+    d, n = k.shape[-1], max(lengths + [1])
+    s = d ** -0.5 if scale is None else abs(scale)
+    # |q . k| summed in absolute values is at most |q| |k|
+    rows = q.double().view(q.shape[0], -1, d).norm(dim=-1).amax(1) if q.numel() else torch.zeros(q.shape[0])
+    top = float(k.double().nan_to_num(0, 0, 0).norm(dim=-1).max())
+    delta = (2 * (d + 4) * 2.0 ** -23 * s * top * rows)[:, None]
+    eps = torch.finfo(dtype).eps
+    tol = (delta + eps / 2 + 2.0 ** -21 + n * 2.0 ** -24) * weight + eps / 2 * want.abs()
+    if dtype == H:
+        vmax = float(v.double().nan_to_num(0, 0, 0).abs().max())
+        tol = tol + n * 2.0 ** -25 * vmax + 2.0 ** -25
+    got = got.cpu().double()
+    assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol.clamp_min(1e-30)).max())
+
+
+CASES = [
+    # lengths, page, heads, key heads, D
+    ([1], 16, 1, 1, 128), ([1, 2, 15, 16, 17, 31, 32, 33], 16, 12, 2, 128),
+    ([127, 128, 129, 255, 256, 257, 300], 16, 4, 4, 64), ([0, 5, 0, 40], 8, 8, 1, 80),
+    ([64, 63, 65], 64, 6, 3, 96), ([37, 200], 1, 2, 1, 16), ([45, 90], 7, 7, 1, 112),
+    ([1000, 3, 0, 517], 100, 12, 2, 128), ([260], 256, 4, 2, 256), ([33, 140], 24, 32, 2, 192),
+    ([150], 16, 24, 1, 128), ([90], 16, 40, 1, 64)]
+
+
+@pytest.mark.parametrize("dtype", [H, B])
+@pytest.mark.parametrize("lengths,page,nh,nkv,d", CASES)
+def test_one_new_token(lengths, page, nh, nkv, d, dtype):
+    q, k, v, table, _ = make(lengths, [1] * len(lengths), page, nh, nkv, d, dtype, 1)
+    got = attention.paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), *seqs(table, lengths, None))
+    check(got, q, k, v, table, lengths, None, dtype)
+    again = attention.paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), *seqs(table, lengths, None))
+    assert torch.equal(got, again)
+
+
+@pytest.mark.parametrize("dtype", [H, B])
+@pytest.mark.parametrize("lengths,news,page,nh,nkv,d", [
+    ([20, 9], [5, 2], 16, 12, 2, 128), ([7, 7, 30], [7, 0, 3], 4, 2, 2, 64), ([140, 300], [40, 1], 24, 4, 1, 96),
+    ([64, 1], [64, 1], 16, 6, 2, 80), ([3, 10], [5, 4], 16, 2, 1, 128), ([200, 180], [9, 9], 32, 8, 2, 256),
+    ([0, 0, 12], [2, 1, 12], 5, 3, 3, 48), ([260, 131], [33, 20], 16, 8, 2, 128)])
+def test_several_new_tokens(lengths, news, page, nh, nkv, d, dtype):
+    q, k, v, table, cu = make(lengths, news, page, nh, nkv, d, dtype, 2)
+    got = attention.paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), *seqs(table, lengths, cu))
+    check(got, q, k, v, table, lengths, cu, dtype)
+
+
+def test_long_among_short():
+    """One sequence cut over many workgroups beside sequences of a few keys, and more sequences than a
+    workgroup has threads."""
+    for lengths in ([9000, 1, 2, 300], [5] * 300 + [4000] + [0, 7]):
+        q, k, v, table, _ = make(lengths, [1] * len(lengths), 64, 4, 2, 64, H, 3)
+        got = attention.paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), *seqs(table, lengths, None))
+        check(got, q, k, v, table, lengths, None, H)
+
+
+@pytest.mark.parametrize("dtype", [H, B])
+def test_large_scores(dtype):
+    """A single key far above the others: its value; scores of hundreds, falling and rising with the position."""
+    d, n = 64, 400
+    q, k, v, table, _ = make([n, n], [1, 1], 16, 2, 1, d, dtype, 4)
+    for b, order in ((0, 1), (1, -1)):
+        for t in range(n):
+            step = t if order > 0 else n - 1 - t
+            k[table[b][t // 16], 0, t % 16] = 0
+            k[table[b][t // 16], 0, t % 16, 0] = step / 4
+    q.zero_()
+    q.view(2, 2, d)[:, :, 0] = 40.0
+    got = attention.paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), *seqs(table, [n, n], None))
+    check(got, q, k, v, table, [n, n], None, dtype)
+
+
+def test_scale():
+    q, k, v, table, _ = make([50], [1], 16, 4, 2, 32, B, 5)
+    for scale in (0.0, 1.0, -0.3):
+        got = attention.paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), *seqs(table, [50], None), scale=scale)
+        check(got, q, k, v, table, [50], None, B, scale)
+
+
+def test_bad_pages_are_not_seen():
+    lengths = [40, 40, 16]
+    q, k, v, table, _ = make(lengths, [1] * 3, 16, 4, 2, 64, H, 6)
+    table[0][1] = -1
+    table[1][0] = 1 << 20
+    table[2][0] = -(1 << 31)          # (all of its keys: zeros)
+    got = attention.paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), *seqs(table, lengths, None))
+    check(got, q, k, v, table, lengths, None, H)
+    assert not bool(got[2].any()) and bool(got[:2].any(1).all())
+
+
+def test_lengths_beyond_the_table_are_cut():
+    q, k, v, table, _ = make([32, 20], [1, 1], 16, 2, 1, 64, H, 7)
+    dev = [t.to(DEV) for t in (q, k, v)]
+    a = attention.paged_attention(*dev, *seqs(table, [32, 20], None))
+    b = attention.paged_attention(*dev, *seqs(table, [1 << 30, 20], None))
+    c = attention.paged_attention(*dev, *seqs(table, [32, -5], None))
+    assert torch.equal(a, b) and torch.equal(a[0], c[0]) and not bool(c[1].any())
+
+
+def test_rows_of_no_sequence_are_zeros():
+    q, k, v, table, cu = make([9, 30], [2, 4], 16, 4, 2, 64, B, 8)
+    rows = torch.cat([q[:1] * float("nan"), q, q])
+    got = attention.paged_attention(rows.to(DEV), k.to(DEV), v.to(DEV),
+                                    *seqs(table, [9, 30], [c + 1 for c in cu]))
+    check(got[1:7], q, k, v, table, [9, 30], cu, B)
+    assert not bool(got[0].any()) and not bool(got[7:].any())
+    none = attention.paged_attention(rows.to(DEV), k.to(DEV), v.to(DEV), *seqs([], [], [0]))
+    assert none.shape == rows.shape and not bool(none.any())
+
+
+@pytest.mark.parametrize("cu", [[0, 5, 3, 6], [-3, 2, 4, 6], [0, 2, 4, 99], [5, 4, 3, 2]])
+def test_impossible_bounds_stay_inside(cu):
+    q, k, v, table, _ = make([20, 9, 300], [2, 2, 2], 16, 4, 2, 64, H, 9)
+    got = attention.paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), *seqs(table, [20, 9, 300], cu))
+    assert got.shape == (6, 256)
+
+
+@pytest.mark.parametrize("dtype", [H, B])
+def test_not_finite(dtype):
+    """A NaN score makes its heads' outputs NaN, in its sequence alone; a score of -inf has no weight."""
+    lengths = [200, 200, 200, 150]
+    q, k, v, table, _ = make(lengths, [1] * 4, 16, 4, 2, 64, dtype, 10)
+    k[table[0][5], 1, 3, 7] = float("nan")
+    q.view(4, 4, 64)[1, 2] = float("nan")
+    q.view(4, 4, 64)[2, :, 0] = 1.0
+    k[table[2][2], :, 2] = 0
+    k[table[2][2], :, 2, 0] = float("-inf")
+    got = attention.paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), *seqs(table, lengths, None))
+    nan = got.view(4, 4, 64).isnan().cpu()
+    want = torch.zeros(4, 4, dtype=torch.bool)
+    want[0, 2:], want[1, 2] = True, True
+    assert torch.equal(nan.all(-1), want) and torch.equal(nan.any(-1), want)
+    # without that key: the other weights alone
+    keys = [(table[2][t // 16], t % 16) for t in range(200) if (t // 16, t % 16) != (2, 2)]
+    p, s = (torch.tensor([x[i] for x in keys]) for i in (0, 1))
+    for h in range(4):
+        w = torch.softmax(k[p, h // 2, s].double() @ q.view(4, 4, 64)[2, h].double() / 8, 0)
+        far = (got.view(4, 4, 64)[2, h].cpu().double() - w @ v[p, h // 2, s].double()).abs()
+        assert float(far.max()) < 4 * torch.finfo(dtype).eps * 4
+
+
+def test_shared_pages_and_strided_queries():
+    q, k, v, table, _ = make([48, 48], [1, 1], 16, 4, 2, 64, H, 11)
+    table[1][:2] = table[0][:2]
+    wide = torch.randn(2, 600, generator=torch.Generator().manual_seed(1)).to(H)
+    wide[:, 3:259] = q                       # (rows at an odd element)
+    got = attention.paged_attention(wide.to(DEV)[:, 3:259], k.to(DEV), v.to(DEV), *seqs(table, [48, 48], None))
+    check(got, q, k, v, table, [48, 48], None, H)
+    col = q.t().contiguous().t()             # (a column-major query is copied)
+    again = attention.paged_attention(col.to(DEV), k.to(DEV), v.to(DEV), *seqs(table, [48, 48], None))
+    assert torch.equal(got, again)
+
+
+def test_far_pages():
+    """Page numbers whose offsets pass 2^31 elements, keys and values of a page side by side."""
+    page, nkv, d = 64, 2, 128
+    n = (1 << 31) // (2 * nkv * page * d) + 3
+    both = torch.empty(n, 2, nkv, page, d, dtype=H, device=DEV)
+    q, k, v, table, _ = make([100, 64], [1, 1], page, 4, nkv, d, H, 12)
+    far = [[n - 1, n - 3], [n - 2, -1]]
+    for b in range(2):
+        for i in range(2 if b == 0 else 1):
+            both[far[b][i], 0], both[far[b][i], 1] = k[table[b][i]].to(DEV), v[table[b][i]].to(DEV)
+    got = attention.paged_attention(q.to(DEV), both[:, 0], both[:, 1], *seqs(far, [100, 64], None))
+    want = attention.paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), *seqs(table, [100, 64], None))
+    assert torch.equal(got, want)
+
+
+def test_replays_with_other_lengths():
+    """A captured call reads lengths, tables and bounds on each replay."""
+    page, nh, nkv, d = 16, 4, 2, 64
+    q, k, v, table, _ = make([400, 300, 500], [1] * 3, page, nh, nkv, d, H, 13)
+    dq, dk, dv = q.to(DEV), k.to(DEV), v.to(DEV)
+    dt, dl, _ = seqs(table, [400, 300, 500], None)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        attention.paged_attention(dq, dk, dv, dt, dl)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attention.paged_attention(dq, dk, dv, dt, dl)
+    for lengths in ([400, 300, 500], [1, 0, 17], [130, 300, 499], [400, 300, 500]):
+        dl.copy_(torch.tensor(lengths, dtype=I32))
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = attention.paged_attention(dq, dk, dv, dt, dl)
+        assert torch.equal(out, eager)
+        check(out, q, k, v, table, lengths, None, H)
+
+
+def test_refusals():
+    q, k, v, table, _ = make([9, 30], [1, 1], 16, 4, 2, 64, H, 14)
+    dt, dl, _ = seqs(table, [9, 30], None)
+    ok = dict(q=q.to(DEV), k_pages=k.to(DEV), v_pages=v.to(DEV), block_table=dt, lengths=dl)
+    attention.paged_attention(**ok)
+    for error, kw in [
+            (TypeError, dict(q=q.to(DEV).bfloat16())), (ValueError, dict(q=q)), (TypeError, dict(q=None)),
+            (ValueError, dict(q=q.to(DEV)[:, :192])), (ValueError, dict(q=q.to(DEV)[:, :100])),
+            (ValueError, dict(q=q.to(DEV)[:1])), (ValueError, dict(q=q.to(DEV)[0])),
+            (ValueError, dict(scale=float("nan"))), (ValueError, dict(scale=1e31)),
+            (TypeError, dict(lengths=dl.long())), (ValueError, dict(cu_seqlens=dl)),
+            (ValueError, dict(block_table=dt[:1])), (ValueError, dict(block_table=dt.t())),
+            (ValueError, dict(k_pages=k.to(DEV)[:2])), (ValueError, dict(k_pages=k.to(DEV)[0])),
+            (TypeError, dict(k_pages=k.to(DEV).bfloat16())),
+            (ValueError, dict(k_pages=k.to(DEV).flatten()[4:].new_zeros(4 + k.numel())[4:].view(k.shape),
+                              v_pages=v.to(DEV)))]:
+        with pytest.raises(error):
+            attention.paged_attention(**{**ok, **kw})
+    for name in ("q", "k_pages", "v_pages"):
+        with pytest.raises(RuntimeError, match=f"no backward for {name}"):
+            attention.paged_attention(**{**ok, name: ok[name].clone().requires_grad_(True)})
+    with torch.no_grad():
+        attention.paged_attention(**{**ok, "q": ok["q"].clone().requires_grad_(True)})

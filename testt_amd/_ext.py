@@ -17,7 +17,7 @@ _lock = threading.Lock()
 _lib = None
 _host = None     # the CPython extension (csrc/host_ops.cpp), bound to the library's entry points
 
-ABI_VERSION = 6
+ABI_VERSION = 7
 STATUS_SCRATCH_LIMIT = 20001          # SOUPK_STATUS_SCRATCH_LIMIT
 LORA_SCRATCH_FLOATS = 4 << 20         # SOUPK_LORA_SCRATCH_FLOATS
 DTYPE_F16 = 0
@@ -28,6 +28,7 @@ _p = ctypes.c_void_p
 _i32 = ctypes.c_int32
 _i64 = ctypes.c_int64
 _f32 = ctypes.c_float
+_f64 = ctypes.c_double
 
 # name -> argument types (every entry point returns int status)
 SIGNATURES = {
@@ -102,6 +103,16 @@ SIGNATURES = {
     "soupk_embedding_fwd": [_p, _i32, _p, _p, _i32, _f32, _i64, _i64, _i64, _p],
     "soupk_embedding_bwd_workspace": [_i64, _i64, _i64, _p],
     "soupk_embedding_bwd": [_p, _i32, _p, _p, _i32, _f32, _i64, _p, _i64, _i64, _i64, _i64, _p],
+    "soupk_rotary_tables": [_p, _p, _i64, _i32, _p, _f64, _i32, _f64, _f64, _f64, _f64, _f64, _p],
+    "soupk_rotary": [_p, _i32, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _i64, _i32, _i32, _i32, _i32,
+                     _i32, _p],
+    "soupk_rope_append": [_p, _p, _p, _i32, _p, _p, _i64, _i64, _i32, _i32, _p, _p, _p, _i32, _i64,
+                          _p, _p, _p, _i64, _i64, _i32, _i32, _i64, _i32, _i32, _i32, _p],
+    "soupk_paged_attention_workspace": [_i64, _i32, _i32, _i32, _i32, _i64, _i32, _p],
+    "soupk_paged_attention": [_p, _i64, _p, _p, _i64, _i64, _i32, _p, _i64, _p, _p, _i32, _p, _i32,
+                              _i64, _i32, _i32, _i32, _f32, _p, _i64, _p],
+    "soupk_verify_drafts_workspace": [_i64, _i64, _p],
+    "soupk_verify_drafts": [_p, _p, _i32, _p, _p, _p, _p, _p, _i64, _i32, _i64, _p, _i64, _p],
     "soupk_layer_fwd": [_p, _p, _p],
     "soupk_layer_bwd": [_p, _p, _p],
 }

@@ -15,11 +15,15 @@ Inputs are RopePack's outputs, q [B, NH, T, D] and k, v [B, NKV, T, D] fp16 (D =
 row b sees key j iff j <= i and attention_mask[b, j] == 1 (the causal + key-padding mask of
 transformers' create_causal_mask).  The output is token-major, [B*T, NH*D] fp16: the rows the
 o-projection reads, with no transpose copy.  Other head dims, or CPU tensors, are not handled
-here (the caller keeps torch's SDPA for them, as the reference does for every shape)."""
+here (the caller keeps torch's SDPA for them, as the reference does for every shape).
+
+New tokens of sequences whose keys and values are cached in pages: paged_attention()
+(testt_amd/csrc/paged_attention.hip)."""
 
 import math
 
 import torch
+from torch.overrides import handle_torch_function, has_torch_function
 
 from . import _ext
 
@@ -274,3 +278,58 @@ def causal_attention(q, k, v, key_valid=None, scale=None):
     """Differentiable causal GQA attention: out [B*T, NH*D] fp16 (token-major)."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
     return CausalAttention.apply(q, k, v, key_valid, scale)
+
+
+# --------------------------------------------------------------------------------------------
+# New tokens over a paged key-value cache (csrc/paged_attention.hip)
+
+def paged_attention(q, k_pages, v_pages, block_table, lengths, cu_seqlens=None, scale=None):
+    """Attention of a decoding step: out [M, n_heads * D] in q's type, the new tokens' queries over
+    their sequences' cached keys and values, which rope.rope_append wrote (the new ones' included).
+
+    q: fp16 or bf16 [M, n_heads * D], any row stride; head h reads key head h // (n_heads / n_kv).
+    k_pages, v_pages [pages, n_kv, page_size, D] (D a multiple of 16 up to 256), block_table,
+    lengths, cu_seqlens: as rope.rope_append.  Token i of a sequence's n new ones sees the keys
+    j <= length - n + i: one token each without cu_seqlens; a few with it (drafted tokens to be
+    verified) or a prompt's part (whole prompts run faster through the varlen attention).  scale:
+    1 / sqrt(D) unless given.  A token that sees no key gets zeros, and so does a row of no sequence;
+    keys in pages outside [0, pages) are not seen.  A key that holds a NaN or infinity reaches every
+    token of its sequence's new ones.
+
+    The lengths are read on the device: a captured graph's replays may change them, the block table
+    and the pages, up to the block table's width.  Scores, sums and products are fp32; the
+    probabilities are rounded to the cache's type for the product with the values.  No gradient is
+    given.  The result does not depend on the order of anything: the same bits every time."""
+    tensors = (q, k_pages, v_pages, block_table, lengths, cu_seqlens)
+    if has_torch_function(tensors):
+        return handle_torch_function(paged_attention, tensors, *tensors, scale)
+    if scale is None and isinstance(k_pages, torch.Tensor) and k_pages.dim() and k_pages.shape[-1]:
+        scale = 1.0 / math.sqrt(k_pages.shape[-1])
+    done = _ext.host().paged_attention(*tensors, scale)
+    if done is not None:
+        return done
+    from .rope import check_pages, refuse_grad
+
+    _ext.refuse_dispatching(*tensors)
+    refuse_grad("paged_attention", (q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages"))
+    if not isinstance(q, torch.Tensor):
+        raise TypeError(f"q must be a tensor, got {type(q).__name__}")
+    if not q.is_cuda:
+        raise ValueError(f"q must be a HIP device tensor (got device {q.device}); the soupk kernels "
+                         "have no CPU path")
+    if q.dim() != 2:
+        raise ValueError(f"q must be [tokens, n_heads * head_dim], got {tuple(q.shape)}")
+    n_kv, _, d = check_pages(k_pages, v_pages, block_table, lengths, cu_seqlens, q.shape[0])
+    if q.dtype != k_pages.dtype or q.device != k_pages.device:
+        raise TypeError(f"q ({q.dtype} on {q.device}) must have the pages' type and device "
+                        f"({k_pages.dtype} on {k_pages.device})")
+    n_heads = q.shape[1] // d
+    if q.shape[1] % d or n_heads < 1 or n_heads % n_kv or n_heads > 1 << 16:
+        raise ValueError(f"q width {q.shape[1]} is no multiple of {n_kv} key heads of {d}")
+    if q.shape[0] * n_heads > 1 << 23:
+        raise ValueError(f"{q.shape[0]} tokens of {n_heads} heads exceed 2^23 rows")
+    scale = _ext.number(scale, "scale")
+    if not -1e30 <= scale <= 1e30:
+        raise ValueError(f"scale must lie in [-1e30, 1e30], got {scale}")
+    return _ext.checked(_ext.host().paged_attention(q.contiguous(), k_pages, v_pages, block_table, lengths,
+                                                    cu_seqlens, scale))

@@ -18,7 +18,7 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB_NAME = "libsoupk.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
-HOST_SRCS = [os.path.join(CSRC, f) for f in ("host_ops.cpp", "host_autograd.cpp")]
+HOST_SRCS = [os.path.join(CSRC, f) for f in ("host_ops.cpp", "host_autograd.cpp", "host_generate.cpp")]
 HOST_NAME = "_soupk_host.so"       # the CPython extension of the operators' host side
 HOST_PATH = os.path.join(HERE, HOST_NAME)
 ARCH = "gfx950"

@@ -32,7 +32,9 @@ using at::Tensor;
   X(soupk_gemm_nn_nf4_split) X(soupk_gemm_lt) X(soupk_gemm_nn) X(soupk_gemm_nn_workspace)         \
   X(soupk_token_logprobs_fwd) X(soupk_token_logprobs_bwd) X(soupk_token_logprobs_workspace)      \
   X(soupk_qk_norm_rope_fwd) X(soupk_qk_norm_rope_bwd) X(soupk_dropout) X(soupk_embedding_fwd)     \
-  X(soupk_embedding_bwd) X(soupk_embedding_bwd_workspace) X(soupk_layer_fwd) X(soupk_layer_bwd)
+  X(soupk_embedding_bwd) X(soupk_embedding_bwd_workspace) X(soupk_layer_fwd) X(soupk_layer_bwd)    \
+  X(soupk_rotary_tables) X(soupk_rotary) X(soupk_rope_append) X(soupk_paged_attention)            \
+  X(soupk_paged_attention_workspace) X(soupk_verify_drafts) X(soupk_verify_drafts_workspace)
 
 #define X(name) inline decltype(&name) p_##name = nullptr;
 SOUPK_ENTRIES(X)

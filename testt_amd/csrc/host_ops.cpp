@@ -605,7 +605,8 @@ PyMethodDef methods[] = {
     SOUPK_ENTRIES(X) M(bind), M(set_status), M(rmsnorm_fwd), M(rmsnorm_bwd), M(rope_tokens),
     M(rope_fwd), M(rope_bwd), M(varlen_fwd), M(varlen_bwd), M(attn_fwd), M(attn_bwd),
     M(swiglu_fwd), M(gemm), M(nf4_key), M(nf4_keys), M(abi_version), M(token_logprobs),
-    M(qk_norm_rope), M(dropout), M(embedding), {nullptr, nullptr, 0, nullptr}};
+    M(qk_norm_rope), M(dropout), M(embedding), M(rotary_tables), M(rotary), M(rope_append),
+    M(paged_attention), M(verify_drafts), {nullptr, nullptr, 0, nullptr}};
 #undef X
 #undef M
 

@@ -1,0 +1,628 @@
+// Attention of new tokens over a paged key-value cache: split over the cache's length and joined.
+//
+// For token i of the n_b new ones of sequence b, whose keys and values (its own included) are the first
+// `length_b` positions of the cache, and query head h with key head h / G:
+//   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - m),  j <= length_b - n_b + i
+// m is a running reference value (raised when a score exceeds it by more than 2^8, as in the training
+// attention), sums and products in fp32; a token that sees no key gets zeros.
+//
+// What bounds it: the cache's bytes -- a key head's row is read once for the G query heads and the few new
+// tokens that share it.  So the query rows of a key head (row = token * G + head in the group, 16 * NB of
+// them a tile) are the 16 columns of v_mfma_f32_16x16x32 products, and keys its rows:
+//   S^T (32 keys x 16 rows) = K Q^T        A = K rows, read from memory in the operand's order
+//   O^T (D x 16 rows) += V^T P^T           A = V^T by transpose reads of rows staged in LDS
+// A wavefront is on its own inside a chunk: it owns 32 of the chunk's 128 keys, its own strip of LDS and its
+// own softmax state; the four are merged once, at the end of its part of a row of work.  No barrier is in
+// the loop.  Page numbers are read two chunks ahead and rows one chunk ahead of their use.
+//
+// Split: the work is the list of all chunks of all (sequence, key head, row tile), in that order, cut into
+// equal parts, one a workgroup: a long sequence among short ones, or one alone, fills the chip the same
+// way, whatever the lengths are (they are in device memory: a captured graph's replays may change
+// them).  A workgroup writes what lies whole inside its part; of rows that reach across an end it leaves the
+// unnormalised sum, its reference value and its weight, two at most, and a second launch joins those in
+// workgroup order: the same bits every time.
+
+#include <algorithm>
+#include <type_traits>
+
+#include "elem.hpp"
+#include "fastdiv.hpp"
+
+namespace soupk {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / kWave;
+constexpr int kWaveKeys = 32;
+constexpr int kChunk = kWaves * kWaveKeys;
+constexpr float kMargin = 8.f;       // log2 of the largest unnormalised probability
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4 lds_s4;
+
+template <typename T>
+struct Ops;
+template <>
+struct Ops<f16> {
+  typedef f16 v8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f4 mfma(u32x4 a, u32x4 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0,
+                                                  0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_h2(a, b); }
+};
+template <>
+struct Ops<bf16> {
+  typedef bf16 v8 __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ f4 mfma(u32x4 a, u32x4 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0,
+                                                   0, 0);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_b2(a, b); }
+};
+
+struct PagedArgs {
+  const uint16_t* q;
+  const uint16_t* k;
+  const uint16_t* v;
+  const int32_t* table;
+  const int32_t* lengths;
+  const int32_t* cu;          // null: one new token a sequence
+  uint16_t* out;
+  uint32_t* first;            // [B + 1]: first chunk of each sequence, and their number
+  float* part;                // two of a workgroup: rows x D sums, rows reference values, rows weights
+  int64_t rows, q_stride, max_pages, pages, page_stride;
+  int B, NKV, G, D, page_size, parts;
+  float scale_log2;
+  FastDiv by_page, by_group;
+};
+
+// Sequence b's rows and length; an impossible one has no rows.
+struct Seq {
+  int64_t start;
+  int news, len;
+};
+__device__ __forceinline__ Seq sequence(const PagedArgs& p, int b) {
+  int64_t s0 = b, s1 = b + 1;
+  if (p.cu != nullptr) {
+    s0 = p.cu[b];
+    s1 = p.cu[b + 1];
+  }
+  const bool ok = s0 >= 0 && s1 >= s0 && s1 <= p.rows;
+  const int64_t most = p.max_pages * p.page_size;
+  return {ok ? s0 : 0, ok ? static_cast<int>(s1 - s0) : 0,
+          static_cast<int>(min(max(static_cast<int64_t>(p.lengths[b]), int64_t{0}), most))};
+}
+// Chunks of a (key head, row tile) of a sequence (one at least, which writes the zeros of one without
+// keys), and its row tiles.
+__device__ __forceinline__ int chunks_of(const Seq& s) { return max((s.len + kChunk - 1) / kChunk, 1); }
+template <int R>
+__device__ __forceinline__ int tiles_of(const Seq& s, int G) { return (s.news * G + R - 1) / R; }
+
+// Max (of a NaN: NaN) / sum over the four lanes that share a row (lane % 16).
+__device__ __forceinline__ float column_max(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __builtin_elementwise_maximum(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __builtin_elementwise_maximum(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float column_sum(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Inclusive sum over the workgroup's threads, in thread order.
+__device__ __forceinline__ uint32_t scan_threads(uint32_t v, uint32_t* sums, uint32_t& total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) {
+    const uint32_t o = __shfl_up(v, d);
+    if (lane >= d) v += o;
+  }
+  if (lane == 63) sums[w] = v;
+  __syncthreads();
+  uint32_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    if (i < w) before += sums[i];
+    total += sums[i];
+  }
+  __syncthreads();
+  return before + v;
+}
+
+// A wavefront's 32 keys of a chunk: 16-byte pieces of K in the operand's order (lane: key 16 n + l % 16,
+// dims 32 s + 8 (l / 16)) and of V in the same places.
+template <int S>
+struct Rows {
+  u32x4 k[2][S], v[2][S];
+  bool ok[2];
+};
+struct Place {
+  int32_t page[2];
+};
+
+template <typename T, int DP, int NB>
+struct Tile {
+  static constexpr int S = DP / 32, DT = DP / 16, R = 16 * NB;
+  static constexpr int kLd = DP + 16;                        // V rows in LDS: 16 + 8-byte reads free of conflicts
+  static constexpr int kStrip = kWaveKeys * kLd;             // halves of a wavefront's strip
+};
+
+template <typename T, int DP, int NB, int MIN>
+__global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArgs p) {
+  using TL = Tile<T, DP, NB>;
+  constexpr int S = TL::S, DT = TL::DT, R = TL::R, kLd = TL::kLd;
+  // (the merge of the wavefronts takes the strips over: 16 rows x DP floats each)
+  static_assert(kWaveKeys * kLd * 2 >= 16 * DP * 4, "");
+  __shared__ __align__(16) uint16_t strips[kWaves * TL::kStrip];
+  __shared__ float stats[kWaves][2][16 * NB];
+  __shared__ uint32_t sums[kWaves];
+  __shared__ uint32_t found[2];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, ql = lane & 15, gr = lane >> 4;
+  const int D = p.D;
+
+  // ---- this workgroup's part of the list, and the sequence that it begins in
+  if (threadIdx.x == 0) found[0] = p.B;
+  uint32_t total = 0;
+  auto part_of = [&](uint32_t& begin, uint32_t& end) {
+    const uint32_t per = (total + p.parts - 1) / p.parts;
+    begin = min(blockIdx.x * per, total);
+    end = min(begin + per, total);
+  };
+  uint32_t c_begin, c_end;
+  for (int pass = 0;; ++pass) {
+    uint32_t before = 0;
+    for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+      const int b = b0 + static_cast<int>(threadIdx.x);
+      uint32_t n = 0;
+      if (b < p.B) {
+        const Seq s = sequence(p, b);
+        n = static_cast<uint32_t>(tiles_of<R>(s, p.G)) * p.NKV * chunks_of(s);
+      }
+      uint32_t all;
+      const uint32_t upto = before + scan_threads(n, sums, all);
+      before += all;
+      if (pass == 0 && blockIdx.x == 0 && b < p.B) p.first[b] = upto - n;
+      if (p.B <= kThreads) total = before;
+      part_of(c_begin, c_end);
+      if (c_begin >= upto - n && c_begin < upto) {
+        found[0] = b;
+        found[1] = upto - n;
+      }
+    }
+    total = before;
+    if (p.B <= kThreads || pass == 1) break;     // (more sequences than threads: once the total is known)
+  }
+  part_of(c_begin, c_end);
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.first[p.B] = total;
+  __syncthreads();
+  // rows that belong to no sequence
+  if (p.cu != nullptr) {
+    const int64_t lead = min(max(static_cast<int64_t>(p.cu[0]), int64_t{0}), p.rows);
+    const int64_t tail = min(max(static_cast<int64_t>(p.cu[p.B]), lead), p.rows);
+    const int64_t width = static_cast<int64_t>(p.NKV) * p.G * D;
+    for (int64_t r = blockIdx.x; r < lead + p.rows - tail; r += gridDim.x) {
+      uint16_t* o = p.out + (r < lead ? r : tail + r - lead) * width;
+      for (int64_t c = threadIdx.x; c < width; c += kThreads) o[c] = 0;
+    }
+  }
+  int b = static_cast<int>(found[0]);
+  uint32_t seq0 = found[1];
+  uint16_t* const strip = strips + w * TL::kStrip;
+  uint32_t c = c_begin;
+  while (c < c_end && b < p.B) {
+    const Seq sq = sequence(p, b);
+    const uint32_t chunks = chunks_of(sq), tiles = tiles_of<R>(sq, p.G);
+    const uint32_t seq_chunks = chunks * tiles * p.NKV;
+    if (c >= seq0 + seq_chunks) {         // (the sequence is done, or has no rows)
+      seq0 += seq_chunks;
+      ++b;
+      continue;
+    }
+    const uint32_t item = (c - seq0) / chunks;
+    const int h = item / tiles, tile = item - h * tiles;
+    const uint32_t item0 = seq0 + item * chunks;
+    const int j_begin = c - item0;
+    const int j_end = min(chunks, c_end - item0);
+
+    // ---- the query rows
+    u32x4 qf[NB][S];
+    int limit[NB];                        // keys that this lane's row sees
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      const int rr = tile * R + 16 * u + ql;
+      const bool real = rr < sq.news * p.G;
+      const int i = p.by_group.div(real ? rr : 0), g = (real ? rr : 0) - i * p.G;
+      limit[u] = real ? max(sq.len - sq.news + i + 1, 0) : 0;
+      const uint16_t* row = p.q + (sq.start + i) * p.q_stride + static_cast<int64_t>(h * p.G + g) * D;
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const int d = 32 * s + 8 * gr;
+        qf[u][s] = real && d < D ? ld16<false>(row + d) : u32x4{0, 0, 0, 0};
+      }
+    }
+    // (the first row of the tile sees the fewest keys, the last one the most)
+    const int rr0 = tile * R, rr1 = min(rr0 + R, sq.news * p.G) - 1;
+    const int seen_all = max(sq.len - sq.news + static_cast<int>(p.by_group.div(rr0)) + 1, 0);
+    const int seen_any = max(sq.len - sq.news + static_cast<int>(p.by_group.div(rr1)) + 1, 0);
+    f4 acc[NB][DT];
+    float m_ref[NB], lsum[NB];
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      m_ref[u] = -INFINITY;
+      lsum[u] = 0.f;
+#pragma unroll
+      for (int t = 0; t < DT; ++t) acc[u][t] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+
+    const int32_t* pages = p.table + static_cast<int64_t>(b) * p.max_pages;
+    auto find = [&](int j) {
+      Place pl;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int key = j * kChunk + w * kWaveKeys + 16 * n + ql;
+        pl.page[n] = key < seen_any ? pages[p.by_page.div(key)] : -1;
+      }
+      return pl;
+    };
+    auto load = [&](Rows<S>& r, const Place& pl, int j) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int key = j * kChunk + w * kWaveKeys + 16 * n + ql;
+        const int slot = key - p.by_page.div(key) * p.page_size;
+        r.ok[n] = pl.page[n] >= 0 && pl.page[n] < p.pages;
+        // (a key without a place reads the first row of the cache: masked, and its value zeroed, below)
+        const int64_t at = r.ok[n] ? static_cast<int64_t>(pl.page[n]) * p.page_stride + (static_cast<int64_t>(h) * p.page_size + slot) * D
+                                    : 0;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          // (dims past D: the row's first again, which meet zeros of Q and columns that are not written)
+          const int d = 32 * s + 8 * gr;
+          const int64_t to = at + (d < D ? d : 0);
+          r.k[n][s] = *reinterpret_cast<const u32x4*>(p.k + to);
+          r.v[n][s] = *reinterpret_cast<const u32x4*>(p.v + to);
+        }
+      }
+    };
+    // (chunks in which this wavefront has keys that the tile sees)
+    const int j_mine = min(j_end, (seen_any - w * kWaveKeys + kChunk - 1) / kChunk);
+    Rows<S> r;
+    Place next;
+    if (j_begin < j_mine) {
+      next = find(j_begin);
+      load(r, next, j_begin);
+      next = find(j_begin + 1);
+    }
+    for (int j = j_begin; j < j_mine; ++j) {
+      const int key0 = j * kChunk + w * kWaveKeys;
+      const bool okay[2] = {r.ok[0], r.ok[1]};
+      const uint64_t all0 = __ballot(okay[0]), all1 = __ballot(okay[1]);
+      const bool whole = (all0 & all1) == ~uint64_t{0};
+      if (!whole) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int s = 0; s < S; ++s)
+            if (!okay[n]) r.v[n][s] = u32x4{0, 0, 0, 0};
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+          *reinterpret_cast<u32x4*>(strip + (16 * n + ql) * kLd + 32 * s + 8 * gr) = r.v[n][s];
+      f4 sc[NB][2];
+#pragma unroll
+      for (int u = 0; u < NB; ++u) sc[u][0] = sc[u][1] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int u = 0; u < NB; ++u) sc[u][n] = Ops<T>::mfma(r.k[n][s], qf[u][s], sc[u][n]);
+      // the next chunk's rows, and the page numbers of the one after it
+      if (j + 1 < j_mine) {
+        load(r, next, j + 1);
+        next = find(j + 2);
+      }
+      __asm__ volatile("" ::: "memory");
+      u32x4 pb[NB];
+      bool any = false;
+#pragma unroll
+      for (int u = 0; u < NB; ++u) {
+        sc[u][0] = sc[u][0] * p.scale_log2;
+        sc[u][1] = sc[u][1] * p.scale_log2;
+        if (!whole || key0 + kWaveKeys > seen_all) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int at = 4 * gr + (e & 3), n = e >> 2;
+            const bool seen = key0 + 16 * n + at < limit[u] && (((n ? all1 : all0) >> at) & 1);
+            sc[u][n][e & 3] = seen ? sc[u][n][e & 3] : -INFINITY;
+          }
+        }
+        float mx = sc[u][0][0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) mx = __builtin_elementwise_maximum(mx, sc[u][e >> 2][e & 3]);
+        if (__any(!(mx <= m_ref[u] + kMargin))) {       // (a NaN raises it to NaN)
+          const float m_new = __builtin_elementwise_maximum(m_ref[u], column_max(mx));
+          const float alpha = m_ref[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_ref[u] - m_new);
+          lsum[u] *= alpha;
+#pragma unroll
+          for (int t = 0; t < DT; ++t) acc[u][t] = acc[u][t] * alpha;
+          m_ref[u] = m_new;
+        }
+        const float m_use = m_ref[u] == -INFINITY ? 0.f : m_ref[u];
+        float pr[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          pr[e] = __builtin_amdgcn_exp2f(sc[u][e >> 2][e & 3] - m_use);
+          lsum[u] += pr[e];
+        }
+        pb[u] = u32x4{Ops<T>::pack(pr[0], pr[1]), Ops<T>::pack(pr[2], pr[3]), Ops<T>::pack(pr[4], pr[5]),
+                      Ops<T>::pack(pr[6], pr[7])};
+      }
+      // O^T += V^T P^T: transpose reads (lane k of a 16-lane group reads 8 bytes of row 4 gr + k / 4 at
+      // column 4 (k % 4); lane i gets column i of the four rows), rows 4 gr .. + 3 and 16 more
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+        const uint16_t* at = strip + (4 * gr + (ql >> 2)) * kLd + 16 * t + 4 * (ql & 3);
+        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at));
+        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + 16 * kLd));
+        const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
+        const u32x4 vf = {l2.x, l2.y, h2.x, h2.y};
+#pragma unroll
+        for (int u = 0; u < NB; ++u) acc[u][t] = Ops<T>::mfma(vf, pb[u], acc[u][t]);
+      }
+    }
+
+    // ---- the four wavefronts' sums into one
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      lsum[u] = column_sum(lsum[u]);
+      if (gr == 0) {
+        stats[w][0][16 * u + ql] = m_ref[u];
+        stats[w][1][16 * u + ql] = lsum[u];
+      }
+    }
+    const bool complete = j_begin == 0 && j_end == static_cast<int>(chunks);
+    float* const part = p.part + (2 * static_cast<int64_t>(blockIdx.x) + (j_begin == 0 ? 1 : 0)) * (R * (D + 2));
+    const int real_rows = min(R, sq.news * p.G - tile * R);
+    float* const mine = reinterpret_cast<float*>(strip);
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      __syncthreads();                    // (stats are written; the strips' last readers are done)
+      float m_all = stats[0][0][16 * u + ql];
+#pragma unroll
+      for (int i = 1; i < kWaves; ++i) m_all = fmaxf(m_all, stats[i][0][16 * u + ql]);
+      const float f = m_ref[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_ref[u] - m_all);
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+        *reinterpret_cast<f4*>(mine + ql * DP + 16 * t + 4 * gr) = acc[u][t] * f;
+      __syncthreads();
+      // thread: two neighbouring columns of a row
+      for (int e = threadIdx.x; e < 16 * (D / 2); e += kThreads) {
+        const int row = e / (D / 2), col = 2 * (e - row * (D / 2)), rt = 16 * u + row;
+        if (rt >= real_rows) break;
+        float x = 0.f, y = 0.f, l = 0.f, m = stats[0][0][rt];
+#pragma unroll
+        for (int i = 1; i < kWaves; ++i) m = fmaxf(m, stats[i][0][rt]);
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+          const float* src = reinterpret_cast<const float*>(strips + i * TL::kStrip) + row * DP + col;
+          x += src[0];
+          y += src[1];
+          const float mi = stats[i][0][rt];
+          l += mi == -INFINITY ? 0.f : stats[i][1][rt] * __builtin_amdgcn_exp2f(mi - m);
+        }
+        if (complete) {
+          const int rr = tile * R + rt, i = p.by_group.div(rr), g = rr - i * p.G;
+          const float inv = m == -INFINITY ? 0.f : 1.f / l;
+          uint16_t* o = p.out + ((sq.start + i) * p.NKV + h) * static_cast<int64_t>(p.G) * D + g * D + col;
+          *reinterpret_cast<uint32_t*>(o) = Ops<T>::pack(x * inv, y * inv);
+        } else {
+          part[rt * D + col] = x;
+          part[rt * D + col + 1] = y;
+          if (col == 0) {
+            part[R * D + rt] = m;
+            part[R * D + R + rt] = l;
+          }
+        }
+      }
+    }
+    __syncthreads();                      // (the strips and stats are free again)
+    c = item0 + j_end;
+  }
+}
+
+// Joins the parts of the rows that reach across workgroups: one workgroup a (token, query head).
+template <typename T, int R, int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedArgs p) {
+  __shared__ float best[THREADS / kWave];
+  __shared__ float2 cols[THREADS];
+  __shared__ float weights[THREADS];
+  const int heads = p.NKV * p.G;
+  const int64_t row = blockIdx.x / heads;
+  const int head = static_cast<int>(blockIdx.x - row * heads), h = head / p.G, g = head - h * p.G;
+  int b = static_cast<int>(row);
+  if (p.cu != nullptr) {
+    int hi = p.B;                          // the last sequence that starts at or before the row
+    b = 0;
+    while (hi - b > 1) {
+      const int mid = (b + hi) / 2;
+      if (p.cu[mid] <= row) b = mid;
+      else hi = mid;
+    }
+  }
+  const Seq s = sequence(p, b);
+  const uint32_t total = p.first[p.B];
+  if (row < s.start || row >= s.start + s.news || total == 0) return;
+  const uint32_t per = (total + p.parts - 1) / p.parts;
+  const int rr = static_cast<int>(row - s.start) * p.G + g;
+  const uint32_t chunks = chunks_of(s), tiles = tiles_of<R>(s, p.G);
+  const uint32_t c0 = p.first[b] + (h * tiles + rr / R) * chunks, c1 = c0 + chunks - 1;
+  const uint32_t w0 = c0 / per, w1 = c1 / per;
+  if (w0 == w1 || w1 >= static_cast<uint32_t>(p.parts)) return;      // (written whole)
+  const int rt = rr % R, D = p.D;
+  const int n = static_cast<int>(w1 - w0) + 1;
+  auto part = [&](int i) {
+    return p.part + (2 * static_cast<int64_t>(w0 + i) + (i == 0 ? 1 : 0)) * (R * (D + 2));
+  };
+  const int lane = threadIdx.x & 63;
+  float m = -INFINITY;
+  for (int i = threadIdx.x; i < n; i += THREADS) m = fmaxf(m, part(i)[R * D + rt]);
+#pragma unroll
+  for (int d = 32; d >= 1; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
+  if (lane == 0) best[threadIdx.x >> 6] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < THREADS / kWave; ++i) m = fmaxf(m, best[i]);
+  // columns 2 c, 2 c + 1 of every `by`-th part
+  const int half = D / 2, by = THREADS / half;
+  const int first = threadIdx.x / half, c = threadIdx.x - first * half;
+  float x = 0.f, y = 0.f, l = 0.f;
+  if (first < by) {
+#pragma unroll 4
+    for (int i = first; i < n; i += by) {
+      const float* src = part(i);
+      const float mi = src[R * D + rt];
+      const float f = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - m);
+      const float2 v = *reinterpret_cast<const float2*>(src + rt * D + 2 * c);
+      x += v.x * f;
+      y += v.y * f;
+      l += src[R * D + R + rt] * f;
+    }
+  }
+  cols[threadIdx.x] = float2{x, y};
+  weights[threadIdx.x] = l;
+  __syncthreads();
+  if (first != 0) return;
+  for (int i = 1; i < by; ++i) {
+    const float2 o = cols[i * half + c];
+    x += o.x;
+    y += o.y;
+    l += weights[i * half + c];
+  }
+  const float inv = m == -INFINITY ? 0.f : 1.f / l;
+  *reinterpret_cast<uint32_t*>(p.out + (row * heads + head) * D + 2 * c) = Ops<T>::pack(x * inv, y * inv);
+}
+
+// ---- host ---------------------------------------------------------------------------------------
+
+bool bad_ptr(const void* p, uintptr_t mask) {
+  return p == nullptr || (reinterpret_cast<uintptr_t>(p) & mask) != 0;
+}
+
+constexpr int kPartsPerCu = 2;
+constexpr int64_t kWideJoin = 256;       // rows up to which a join has 1024 threads
+constexpr int64_t kMostKeys = int64_t{1} << 30;
+
+// Row blocks of 16 a tile: what a sequence's rows fill on average.
+int blocks_of(int64_t rows, int32_t B, int32_t G, int32_t D) {
+  const int64_t of_seq = B > 0 ? (rows * G + B - 1) / B : 0;
+  if (of_seq <= 16) return 1;
+  if (of_seq <= 32 || D > 128) return 2;
+  return 4;
+}
+
+struct Plan {
+  int nb, parts;
+  bool join;
+  int64_t first_bytes, bytes;
+};
+
+// false: more chunks than 32 bits count.
+bool plan_of(int64_t rows, int32_t B, int32_t G, int32_t NKV, int32_t D, int64_t most_keys, Plan& pl) {
+  pl.nb = blocks_of(rows, B, G, D);
+  const int R = 16 * pl.nb;
+  const int64_t chunks = std::max<int64_t>((most_keys + kChunk - 1) / kChunk, 1);
+  const int64_t items = (rows * G / R + B) * NKV;
+  if (items > 0 && chunks > ((int64_t{1} << 31) - 1) / items) return false;
+  const int64_t list = items * chunks;
+  pl.parts = static_cast<int>(std::max<int64_t>(std::min<int64_t>(list, int64_t{kPartsPerCu} * device_cu_count()), 1));
+  pl.join = chunks > 1;
+  pl.first_bytes = (4 * (int64_t{B} + 1) + 15) / 16 * 16;
+  pl.bytes = pl.first_bytes + 2 * int64_t{pl.parts} * R * (D + 2) * 4;
+  return true;
+}
+
+template <typename T, int DP>
+int launch_paged(const PagedArgs& a, const Plan& pl, hipStream_t s) {
+  const dim3 grid(pl.parts), block(kThreads);
+  auto run = [&](auto nb, auto min_waves) -> int {
+    constexpr int NB = decltype(nb)::value;
+    int rc = launch_kernel(paged_attention_kernel<T, DP, NB, decltype(min_waves)::value>, grid, block, s, a);
+    if (rc != kOk || !pl.join) return rc;
+    const int64_t outs = a.rows * a.NKV * a.G;
+    const dim3 join(static_cast<unsigned>(outs));
+    // (few rows have many parts each)
+    if (outs <= kWideJoin) return launch_kernel(paged_join_kernel<T, 16 * NB, 1024>, join, dim3(1024), s, a);
+    return launch_kernel(paged_join_kernel<T, 16 * NB, 256>, join, dim3(256), s, a);
+  };
+  using std::integral_constant;
+  if (pl.nb == 1) return run(integral_constant<int, 1>{}, integral_constant<int, DP <= 128 ? 2 : 1>{});
+  if (pl.nb == 2) return run(integral_constant<int, 2>{}, integral_constant<int, DP <= 128 ? 2 : 1>{});
+  if constexpr (DP <= 128) return run(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+  else return kInvalid;
+}
+
+}  // namespace
+}  // namespace soupk
+
+using namespace soupk;
+
+extern "C" __attribute__((visibility("default"))) int soupk_paged_attention_workspace(
+    int64_t rows, int32_t B, int32_t NH, int32_t NKV, int32_t D, int64_t max_pages, int32_t page_size,
+    int64_t* bytes) {
+  Plan pl;
+  if (bytes == nullptr || rows < 0 || B < 0 || NKV < 1 || NH < NKV || NH % NKV || D < 16 || D % 16 || D > 256 ||
+      page_size < 1 || max_pages < 0 || max_pages > kMostKeys / page_size ||
+      !plan_of(rows, B, NH / NKV, NKV, D, max_pages * page_size, pl))
+    return kInvalid;
+  *bytes = pl.bytes;
+  return kOk;
+}
+
+extern "C" __attribute__((visibility("default"))) int soupk_paged_attention(
+    const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, int64_t n_pages,
+    int64_t page_stride, int32_t page_size, const int32_t* block_table, int64_t max_pages,
+    const int32_t* lengths, const int32_t* cu, int32_t B, void* out, int32_t dtype, int64_t rows, int32_t NH, int32_t NKV, int32_t D, float scale,
+    void* workspace, int64_t workspace_bytes, void* stream) {
+  Plan pl;
+  if (rows < 0 || B < 0 || NKV < 1 || NH < NKV || NH > (1 << 16) || NH % NKV || D < 16 || D % 16 || D > 256 ||
+      page_size < 1 || n_pages < 1 || n_pages >= (int64_t{1} << 31) || max_pages < 0 ||
+      max_pages > kMostKeys / page_size || q_stride < 0 ||
+      (n_pages > 1 && (page_stride < static_cast<int64_t>(NKV) * page_size * D || page_stride % 8)) ||
+      rows > kMaxGrid / NH || (cu == nullptr && rows != B) ||
+      !(scale >= -1e30f && scale <= 1e30f) ||
+      (dtype != SOUPK_DTYPE_F16 && dtype != SOUPK_DTYPE_BF16) ||
+      !plan_of(rows, B, NH / NKV, NKV, D, max_pages * page_size, pl))
+    return kInvalid;
+  if (rows == 0) return kOk;
+  if (bad_elem_ptr(q, dtype) || bad_ptr(out, 3) || bad_ptr(workspace, 15) || workspace_bytes < pl.bytes)
+    return kInvalid;
+  if (B < 1 || bad_ptr(lengths, 3) || (cu != nullptr && bad_ptr(cu, 3))) return kInvalid;
+  if (max_pages > 0 && bad_ptr(block_table, 3)) return kInvalid;
+  if (bad_ptr(k_pages, 15) || bad_ptr(v_pages, 15)) return kInvalid;
+  PagedArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k_pages),
+              static_cast<const uint16_t*>(v_pages), block_table, lengths, cu, static_cast<uint16_t*>(out),
+              static_cast<uint32_t*>(workspace),
+              reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.first_bytes), rows, q_stride,
+              max_pages, n_pages, page_stride, B, NKV, NH / NKV, D, page_size, pl.parts, scale * kLog2e,
+              FastDiv(static_cast<uint32_t>(page_size)), FastDiv(static_cast<uint32_t>(NH / NKV))};
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  return with_type(dtype, [&](auto tag) -> int {
+    using E = typename decltype(tag)::type;
+    if constexpr (std::is_same_v<E, float>) {
+      return kInvalid;
+    } else {
+      if (D <= 64) return launch_paged<E, 64>(a, pl, s);
+      if (D <= 96) return launch_paged<E, 96>(a, pl, s);
+      if (D <= 128) return launch_paged<E, 128>(a, pl, s);
+      return launch_paged<E, 256>(a, pl, s);
+    }
+  });
+}

@@ -552,3 +552,78 @@ def fused_token_logprobs(hidden16, weight16, tokens, top_k=0, temperature=1.0):
         raise ValueError(f"{tokens.numel()} tokens for {hidden16.shape[0]} rows")
     top_k, temperature = _check_logprobs(top_k, temperature, weight16.shape[0])
     return TokenLogprobs(*_HiddenLogprobs.apply(hidden16, weight16, tokens, top_k, temperature))
+
+
+# --------------------------------------------------------------------------------------------
+# Verification of drafted tokens (csrc/verify_drafts.hip)
+
+class DraftVerdict(namedtuple("DraftVerdict", "tokens accepted")):
+    """What verify_drafts says; also from one iterable of both, as torch builds a tuple again whose tensors
+    it has given a subclass's type."""
+
+    __slots__ = ()
+
+    def __new__(cls, tokens, accepted=None):
+        if accepted is None:
+            tokens, accepted = tokens
+        return super().__new__(cls, tokens, accepted)
+
+
+def verify_drafts(target_probs, drafts, uniforms, draft_probs=None, lengths=None):
+    """DraftVerdict(tokens int64 [B, K + 1], accepted int32 [B]): how many of each sequence's drafted
+    tokens stand, those tokens and one more, then -1.  The tokens kept are distributed as the target's
+    own would be, whatever the draft is (speculative sampling).
+
+    target_probs: [B, K + 1, V], the target's probabilities where each draft stands and after the last.
+    drafts: int64 [B, K].  draft_probs: [B, K, V], the distributions that the drafts were drawn from; None:
+    they were chosen, not drawn (greedy, or from an n-gram table).  Both fp16, bf16 or fp32, of one
+    type.  uniforms: fp32 [B, K + 1] in [0, 1), made by the caller; the same ones give the same
+    tokens.  lengths: int32 [B], how many of a sequence's K drafts count (None: all; 0: one token is
+    drawn from its first row).
+
+    Draft i stands while uniforms[i] * draft_probs[i, x_i] < target_probs[i, x_i].  The added token
+    is the lowest id whose prefix sum of w exceeds uniforms[K] * sum(w): w = max(target - draft, 0)
+    at the first refusal (the target's row where that is 0 everywhere), the target's next row if none
+    was refused; -1 where w is 0 everywhere.  Sums and products are 64-bit.  The rows need not sum to
+    one (a cut-off distribution may stay unnormalised in both); negative, infinite and NaN
+    probabilities count as 0; a draft outside the vocabulary is refused.  Greedy verification:
+    target_probs with a 1 at each row's best token and no draft_probs.  No gradient is given."""
+    tensors = (target_probs, drafts, uniforms, draft_probs, lengths)
+    if has_torch_function(tensors):
+        return handle_torch_function(verify_drafts, tensors, *tensors)
+    done = _ext.host().verify_drafts(*tensors)
+    if done is not None:
+        return DraftVerdict(*done)
+    from .rope import refuse_grad
+
+    _ext.refuse_dispatching(*tensors)
+    refuse_grad("verify_drafts", (target_probs, "target_probs"), (uniforms, "uniforms"),
+                (draft_probs, "draft_probs"))
+    if not isinstance(target_probs, torch.Tensor):
+        raise TypeError(f"target_probs must be a tensor, got {type(target_probs).__name__}")
+    if not target_probs.is_cuda:
+        raise ValueError(f"target_probs must be a HIP device tensor (got device {target_probs.device}); "
+                         "the soupk kernels have no CPU path")
+    _ext.dtype_code(target_probs, "target_probs")
+    if target_probs.dim() != 3 or target_probs.shape[1] < 1 or target_probs.shape[2] < 1:
+        raise ValueError(f"target_probs must be [B, K + 1, V] with V > 0, got {tuple(target_probs.shape)}")
+    batch, k, vocab = target_probs.shape[0], target_probs.shape[1] - 1, target_probs.shape[2]
+    dev = target_probs.device
+    if batch > 1 << 14 or k > 1 << 20 or vocab >= 1 << 40:
+        raise ValueError(f"at most 2^14 sequences of 2^20 drafts are taken, got {tuple(target_probs.shape)}")
+    for t, name, dtype, shape in ((drafts, "drafts", torch.int64, (batch, k)),
+                                  (uniforms, "uniforms", torch.float32, (batch, k + 1)),
+                                  (draft_probs, "draft_probs", target_probs.dtype, (batch, k, vocab)),
+                                  (lengths, "lengths", torch.int32, (batch,))):
+        if t is None and name in ("draft_probs", "lengths"):
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+        if t.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+        if t.device != dev or tuple(t.shape) != shape:
+            raise ValueError(f"{name} must be {shape} on {dev}, got {tuple(t.shape)} on {t.device}")
+    return DraftVerdict(*_ext.checked(_ext.host().verify_drafts(
+        target_probs.contiguous(), drafts.contiguous(), uniforms.contiguous(),
+        None if draft_probs is None else draft_probs.contiguous(),
+        None if lengths is None else lengths.contiguous())))

@@ -7,7 +7,13 @@ writes fp16 q/k/v directly into [batch, heads, seq, head_dim] at the token's pad
 the layout SDPA takes; padded positions with no token are zeroed by the same launch.  Backward
 is the transposed rotation, gathering per token and writing the fp16 gradient of the q/k/v GEMM
 output; the LoRA branches get views of the same buffer.
+
+For generation: tables scaled for long contexts (rotary_tables), the rotation by itself, of part of a
+head and in either layout (rotary), and the same step as above into a paged key-value cache
+(rope_append), in testt_amd/csrc/rotary.hip.
 """
+
+import math
 
 import torch
 from torch.overrides import handle_torch_function, has_torch_function
@@ -227,3 +233,263 @@ def qk_norm_rope(qkv, lora_q, lora_v, q_weight, k_weight, cos, sin, pos_idx, bat
         qkv, *deltas, *weights, _table(cos, seq, head_dim, "cos", dev),
         _table(sin, seq, head_dim, "sin", dev), as_index(pos_idx), batch, seq, n_heads, n_kv,
         head_dim, eps))
+
+
+# --------------------------------------------------------------------------------------------
+# Rotary positions in either layout, of part of a head, scaled for long contexts; new tokens into
+# a paged cache (csrc/rotary.hip)
+
+_SCALINGS = {"default": 0, "linear": 1, "dynamic": 2, "yarn": 3}     # SOUPK_ROPE_*
+_NO_GRAD = ("{} has no backward for {}: call it under torch.no_grad(), or detach what wants a "
+            "gradient")
+
+
+def refuse_grad(operator, *named):
+    """Raises for a tensor that would want a gradient of an operator that gives none."""
+    for t, name in named:
+        if isinstance(t, torch.Tensor) and \
+                (torch.is_grad_enabled() and t.requires_grad
+                 or torch.autograd.forward_ad.unpack_dual(t).tangent is not None):
+            raise RuntimeError(_NO_GRAD.format(operator, name))
+
+
+def _positive(scaling, key, default=None):
+    value = scaling.get(key)
+    if value is None:
+        value = default
+    if value is None:
+        raise ValueError(f"rope scaling {scaling.get('rope_type')!r} needs {key!r}")
+    return _ext.number(value, key)
+
+
+def rotary_tables(seq, rotary_dim, theta=10000.0, scaling=None, inv_freq=None, device="cuda"):
+    """(cos, sin) fp32 [seq, rotary_dim / 2] of positions 0 .. seq - 1, for rotary() and
+    rope_append(): pair i turns by theta^(-2 i / rotary_dim) a position.  The angles are formed in
+    64 bits, so far positions keep their places (in fp32 an angle at position 2^20 is 0.03 rad off).
+
+    scaling: None or a dict in transformers' `rope_scaling` form, for contexts longer than the
+    trained one -- rope_type "default", "linear" (factor), "dynamic" (factor,
+    original_max_position_embeddings; takes effect where seq exceeds it) or "yarn" (those two and,
+    optionally, beta_fast, beta_slow, attention_factor, mscale, mscale_all_dim).  inv_freq:
+    rotary_dim / 2 frequencies on the host (numbers, or a CPU tensor) in place of theta and scaling.
+    rotary_dim: even, at most 256.  The layer's own tables [seq, head_dim] hold every column twice:
+    their first half (cos[:, :head_dim // 2]) is this form."""
+    device = torch.device(device)
+    if device.type != "cuda":
+        raise ValueError(f"rotary tables are made on a HIP device (got {device}); the soupk kernels "
+                         "have no CPU path")
+    for v, name in ((seq, "seq"), (rotary_dim, "rotary_dim")):
+        if isinstance(v, bool) or not isinstance(v, int):
+            raise TypeError(f"{name} must be an int, got {type(v).__name__}")
+    if not 0 <= seq < 1 << 31:
+        raise ValueError(f"seq must lie in [0, 2^31), got {seq}")
+    if not 2 <= rotary_dim <= 256 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even and lie in [2, 256], got {rotary_dim}")
+    theta = _ext.number(theta, "theta")
+    if not 1.0 < theta <= 1e30:
+        raise ValueError(f"theta must lie in (1, 1e30], got {theta}")
+    kind, factor, original, fast, slow, gain = "default", 1.0, 1.0, 32.0, 1.0, 1.0
+    if inv_freq is not None:
+        if scaling is not None:
+            raise ValueError("inv_freq takes the place of theta and scaling: pass one of them")
+        if isinstance(inv_freq, torch.Tensor):
+            if inv_freq.device.type != "cpu":
+                raise ValueError(f"inv_freq must be on the host, got {inv_freq.device}")
+            inv_freq = inv_freq.detach().double().tolist()
+        inv_freq = tuple(float(f) for f in inv_freq)
+        if len(inv_freq) != rotary_dim // 2 or not all(abs(f) <= 1e6 for f in inv_freq):
+            raise ValueError(f"inv_freq must hold {rotary_dim // 2} frequencies of at most 1e6 rad")
+    elif scaling is not None:
+        kind = scaling.get("rope_type", scaling.get("type"))
+        if kind not in _SCALINGS:
+            raise ValueError(f"rope scaling must be one of {', '.join(_SCALINGS)}, got {kind!r} (other "
+                             "schemes: pass their frequencies as inv_freq)")
+        if kind != "default":
+            factor = _positive(scaling, "factor")
+            if not 1.0 <= factor <= 1e6:
+                raise ValueError(f"factor must lie in [1, 1e6], got {factor}")
+        if kind in ("dynamic", "yarn"):
+            original = _positive(scaling, "original_max_position_embeddings")
+            if not 1.0 <= original <= 1 << 31:
+                raise ValueError(f"original_max_position_embeddings must lie in [1, 2^31], got {original}")
+        if kind == "yarn":
+            fast, slow = _positive(scaling, "beta_fast", 32.0), _positive(scaling, "beta_slow", 1.0)
+            if not 0.0 < slow <= fast <= 1e6:
+                raise ValueError(f"0 < beta_slow <= beta_fast <= 1e6 is needed, got {slow}, {fast}")
+            gain = _yarn_gain(scaling, factor)
+    index = device.index if device.index is not None else torch.cuda.current_device()
+    return _ext.checked(_ext.host().rotary_tables(seq, rotary_dim, theta, _SCALINGS[kind], factor,
+                                                  original, fast, slow, gain, inv_freq, index))
+
+
+def _yarn_gain(scaling, factor):
+    """What the cosines and sines are multiplied by: attention_factor, or 0.1 m ln(factor) + 1 of
+    mscale over that of mscale_all_dim, or of m = 1."""
+    def of(m):
+        return 0.1 * m * math.log(factor) + 1.0
+
+    gain = scaling.get("attention_factor")
+    if gain is None:
+        m, every = scaling.get("mscale"), scaling.get("mscale_all_dim")
+        gain = of(float(m)) / of(float(every)) if m and every else of(1.0)
+    gain = _ext.number(gain, "attention_factor")
+    if not abs(gain) <= 1e30:
+        raise ValueError(f"attention_factor must be a number of at most 1e30, got {gain}")
+    return gain
+
+
+def _half_table(t, name, head_dim, device):
+    if not isinstance(t, torch.Tensor) or t.device != device:
+        raise ValueError(f"{name} must be a tensor on {device}")
+    if t.dtype != torch.float32:
+        raise TypeError(f"{name} must be torch.float32, got {t.dtype}")
+    if t.dim() != 2 or t.shape[1] < 1 or 2 * t.shape[1] > head_dim:
+        raise ValueError(f"{name} must be [positions, R / 2] with R at most the head dim {head_dim}, "
+                         f"got {tuple(t.shape)}")
+
+
+def _half_tables(cos, sin, head_dim, device):
+    _half_table(cos, "cos", head_dim, device)
+    _half_table(sin, "sin", head_dim, device)
+    if cos.shape != sin.shape:
+        raise ValueError(f"cos {tuple(cos.shape)} and sin {tuple(sin.shape)} differ")
+    if cos.stride() != sin.stride() or (cos.stride(1) != 1 and cos.shape[1] > 1):
+        cos, sin = cos.contiguous(), sin.contiguous()
+    return cos, sin
+
+
+def rotary(x, cos, sin, pos, interleaved=False):
+    """x [M, heads, D] with the leading R = 2 * cos.shape[1] elements of every head turned by the angles
+    of position pos[m], the others as they are; in x's type (fp16, bf16 or fp32), fp32 inside,
+    differentiable in x.
+
+    Pairs are (i, i + R/2) (transformers' rotate_half) or, interleaved, (2 i, 2 i + 1).  x: any token
+    and head strides, a head's elements adjacent (query columns of q|k|v rows, viewed as heads).
+    cos, sin: fp32 [positions, R/2] (rotary_tables(), or the first half of the layer's tables), any
+    row stride.  pos: int64 or int32 [M]; a token whose position lies outside the tables gets zeros
+    (and passes no gradient)."""
+    tensors = (x, cos, sin, pos)
+    if has_torch_function(tensors):
+        return handle_torch_function(rotary, tensors, *tensors, interleaved)
+    done = _ext.host().rotary(x, cos, sin, pos, interleaved)
+    if done is not None:
+        return done
+    _ext.refuse_dispatching(*tensors)
+    if not isinstance(x, torch.Tensor):
+        raise TypeError(f"x must be a tensor, got {type(x).__name__}")
+    if not x.is_cuda:
+        raise ValueError(f"x must be a HIP device tensor (got device {x.device}); the soupk kernels "
+                         "have no CPU path")
+    _ext.dtype_code(x, "x")
+    if x.dim() != 3 or not 1 <= x.shape[1] <= 1 << 16 or not 2 <= x.shape[2] <= 1 << 16:
+        raise ValueError(f"x must be [tokens, heads, head_dim], got {tuple(x.shape)}")
+    cos, sin = _half_tables(cos, sin, x.shape[2], x.device)
+    refuse_grad("rotary", (cos, "cos"), (sin, "sin"))
+    if not isinstance(pos, torch.Tensor) or pos.device != x.device or pos.dim() != 1 or \
+            pos.numel() != x.shape[0] or pos.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"pos must be {x.shape[0]} integer positions on {x.device}")
+    if x.stride(2) != 1:
+        x = x.contiguous()
+    return _ext.checked(_ext.host().rotary(x, cos, sin, as_index(pos), bool(interleaved)))
+
+
+def check_pages(k_pages, v_pages, block_table, lengths, cu_seqlens, rows):
+    """(n_kv, page_size, head_dim) of a paged cache and its sequences' int32 tensors, or an error."""
+    _ext.refuse_dispatching(k_pages, v_pages, block_table, lengths, cu_seqlens)
+    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a HIP device tensor (got device {t.device}); the soupk "
+                             "kernels have no CPU path")
+        _ext.dtype_code(t, name, (torch.float16, torch.bfloat16))
+        if t.dim() != 4 or 0 in t.shape:
+            raise ValueError(f"{name} must be [pages, n_kv, page_size, head_dim], got {tuple(t.shape)}")
+        _, n_kv, page, d = t.shape
+        if t.stride()[1:] != (page * d, d, 1) or (t.shape[0] > 1 and t.stride(0) < n_kv * page * d):
+            raise ValueError(f"{name} must hold each page's elements adjacent, got strides {t.stride()}")
+        if t.data_ptr() % 16 or (t.shape[0] > 1 and t.stride(0) % 8):
+            raise ValueError(f"{name}'s pages must be aligned to 16 bytes")
+    if v_pages.dtype != k_pages.dtype:
+        raise TypeError(f"v_pages must be {k_pages.dtype} as k_pages, got {v_pages.dtype}")
+    if v_pages.shape != k_pages.shape or \
+            v_pages.device != k_pages.device or \
+            (k_pages.shape[0] > 1 and v_pages.stride(0) != k_pages.stride(0)):
+        raise ValueError(f"k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must agree in "
+                         "shape, strides and device")
+    if d % 16 or d > 256:
+        raise ValueError(f"head_dim must be a multiple of 16 up to 256, got {d}")
+    if n_kv > 1 << 16 or page >= 1 << 31 or k_pages.shape[0] >= 1 << 31:
+        raise ValueError(f"too many pages, key heads or slots: {tuple(k_pages.shape)}")
+    dev = k_pages.device
+    _ext.require(lengths, "lengths", dtype=torch.int32, ndim=1, device=dev)
+    _ext.require(block_table, "block_table", dtype=torch.int32, ndim=2, device=dev)
+    batch = lengths.numel()
+    if block_table.shape[0] != batch:
+        raise ValueError(f"block_table has {block_table.shape[0]} rows for {batch} lengths")
+    if block_table.shape[1] * page > 1 << 30:
+        raise ValueError(f"block_table spans {block_table.shape[1]} pages of {page}, over 2^30 positions")
+    if cu_seqlens is not None:
+        _ext.require(cu_seqlens, "cu_seqlens", dtype=torch.int32, ndim=1, device=dev)
+        if cu_seqlens.numel() != batch + 1:
+            raise ValueError(f"cu_seqlens must hold {batch + 1} bounds, got {cu_seqlens.numel()}")
+    elif rows != batch:
+        raise ValueError(f"{rows} rows for {batch} sequences: without cu_seqlens each has one new token")
+    return n_kv, page, d
+
+
+def rope_append(qkv, lora_q, lora_v, cos, sin, k_pages, v_pages, block_table, lengths,
+                cu_seqlens=None, interleaved=False):
+    """The new tokens' step between the q|k|v projection and the attention of a decoding layer:
+    returns the queries [M, n_heads * D], rotated with their LoRA delta, and writes the rotated keys
+    and the values with theirs into a paged cache (attention.paged_attention reads it).
+
+    qkv: fp16 or bf16 [M, (n_heads + 2 * n_kv) * D] in the token-major layout of rope_pack_tokens
+    (whose bits the queries, keys and values have); lora_q, lora_v: None, the rows' type or fp32.
+    cos, sin: as rotary(), or None where the rows are rotated already (qk_norm_rope's).
+    k_pages, v_pages: [pages, n_kv, page_size, D] of qkv's type, written in place.  block_table:
+    int32 [batch, pages of a sequence]; lengths: int32 [batch], each sequence's tokens with the new
+    ones; cu_seqlens: int32 [batch + 1], where each one's new tokens start in qkv (None: one each).
+    Token i of a sequence's n new ones stands at t = length - n + i: its angle, and slot
+    t % page_size of page block_table[b, t // page_size].  A token without a place -- no sequence, t
+    outside [0, positions) or the block table, a page outside [0, pages) -- gets a row of zeros and is
+    written nowhere, so a captured graph's padding costs nothing: give it length 0.
+
+    No gradient is given.  Two sequences may share pages that neither writes."""
+    tensors = (qkv, lora_q, lora_v, cos, sin, k_pages, v_pages, block_table, lengths, cu_seqlens)
+    if has_torch_function(tensors):
+        return handle_torch_function(rope_append, tensors, *tensors, interleaved)
+    done = _ext.host().rope_append(*tensors, interleaved)
+    if done is not None:
+        return done
+    _ext.refuse_dispatching(*tensors)
+    refuse_grad("rope_append", (qkv, "qkv"), (lora_q, "lora_q"), (lora_v, "lora_v"), (cos, "cos"),
+                (sin, "sin"), (k_pages, "k_pages"), (v_pages, "v_pages"))
+    _ext.require(qkv, "qkv", ndim=2)
+    rows, dev = qkv.shape[0], qkv.device
+    n_kv, _, d = check_pages(k_pages, v_pages, block_table, lengths, cu_seqlens, rows)
+    if qkv.dtype != k_pages.dtype or k_pages.device != dev:
+        raise TypeError(f"qkv ({qkv.dtype} on {dev}) must have the pages' type and device "
+                        f"({k_pages.dtype} on {k_pages.device})")
+    n_heads = qkv.shape[1] // d - 2 * n_kv
+    if qkv.shape[1] % d or not 1 <= n_heads <= 1 << 16:
+        raise ValueError(f"qkv width {qkv.shape[1]} is no (n_heads + 2 * {n_kv}) * {d}")
+    deltas = []
+    for t, name, heads in ((lora_q, "lora_q", n_heads), (lora_v, "lora_v", n_kv)):
+        if t is not None:
+            if not isinstance(t, torch.Tensor) or t.device != dev:
+                raise ValueError(f"{name} must be a tensor on {dev}")
+            if t.dtype not in (qkv.dtype, torch.float32):
+                raise TypeError(f"{name} must be {qkv.dtype} or torch.float32, got {t.dtype}")
+            if tuple(t.shape) != (rows, heads * d):
+                raise ValueError(f"{name} shape {tuple(t.shape)} != {(rows, heads * d)}")
+            t = t.contiguous()
+        deltas.append(t)
+    if any(t is not None and t.dtype == torch.float32 for t in deltas):
+        deltas = [None if t is None else t.float() for t in deltas]     # (one type for both)
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin are given together, or neither")
+    if cos is not None:
+        cos, sin = _half_tables(cos, sin, d, dev)
+    return _ext.checked(_ext.host().rope_append(qkv, *deltas, cos, sin, k_pages, v_pages, block_table,
+                                                lengths, cu_seqlens, bool(interleaved)))
