@@ -9,18 +9,20 @@
 // What bounds it: the cache's bytes -- a key head's row is read once for the G query heads and the few new
 // tokens that share it.  So the query rows of a key head (row = token * G + head in the group, 16 * NB of
 // them a tile) are the 16 columns of v_mfma_f32_16x16x32 products, and keys its rows:
-//   S^T (32 keys x 16 rows) = K Q^T        A = K rows, read from memory in the operand's order
+//   S^T (32 keys x 16 rows) = K Q^T        A = K rows staged in LDS
 //   O^T (D x 16 rows) += V^T P^T           A = V^T by transpose reads of rows staged in LDS
 // A wavefront is on its own inside a chunk: it owns 32 of the chunk's 128 keys, its own strip of LDS and its
-// own softmax state; the four are merged once, at the end of its part of a row of work.  No barrier is in
-// the loop.  Page numbers are read two chunks ahead and rows one chunk ahead of their use.
+// own softmax state; the four are merged once, at the end of an item or part.  No barrier is in the
+// loop.  Page numbers are read two chunks ahead and rows one chunk ahead of their use.
 //
-// Split: the work is the list of all chunks of all (sequence, key head, row tile), in that order, cut into
-// equal parts, one a workgroup: a long sequence among short ones, or one alone, fills the chip the same
+// Split: the work is the list of all chunks of all items -- (sequence, key head, row tile) -- in that order,
+// cut into equal parts, one a workgroup: a long sequence among short ones, or one alone, fills the chip the same
 // way, whatever the lengths are (they are in device memory: a captured graph's replays may change
-// them).  A workgroup writes what lies whole inside its part; of rows that reach across an end it leaves the
-// unnormalised sum, its reference value and its weight, two at most, and a second launch joins those in
-// workgroup order: the same bits every time.
+// them).  Where the items are few, each is cut for itself (a workgroup that crosses into another item waits
+// for queries, page numbers and rows once more); where they are many, a part may end one item and
+// begin others.  A workgroup writes what lies whole inside its part; of an item that reaches across an end it
+// leaves the unnormalised sum, its reference value and its weight, two at most, and a second launch
+// joins those in workgroup order: the same bits every time.
 
 #include <algorithm>
 #include <type_traits>
@@ -70,7 +72,7 @@ struct PagedArgs {
   const int32_t* lengths;
   const int32_t* cu;          // null: one new token a sequence
   uint16_t* out;
-  uint32_t* first;            // [B + 1]: first chunk of each sequence, and their number
+  uint32_t* first;            // [B + 3]: first chunk of each sequence, their number, a part's, an item's multiple
   float* part;                // two of a workgroup: rows x D sums, rows reference values, rows weights
   int64_t rows, q_stride, max_pages, pages, page_stride;
   int B, NKV, G, D, page_size, parts;
@@ -80,8 +82,7 @@ struct PagedArgs {
 
 // Sequence b's rows and length; an impossible one has no rows.
 struct Seq {
-  int64_t start;
-  int news, len;
+  int start, news, len;
 };
 __device__ __forceinline__ Seq sequence(const PagedArgs& p, int b) {
   int64_t s0 = b, s1 = b + 1;
@@ -91,7 +92,7 @@ __device__ __forceinline__ Seq sequence(const PagedArgs& p, int b) {
   }
   const bool ok = s0 >= 0 && s1 >= s0 && s1 <= p.rows;
   const int64_t most = p.max_pages * p.page_size;
-  return {ok ? s0 : 0, ok ? static_cast<int>(s1 - s0) : 0,
+  return {ok ? static_cast<int>(s0) : 0, ok ? static_cast<int>(s1 - s0) : 0,
           static_cast<int>(min(max(static_cast<int64_t>(p.lengths[b]), int64_t{0}), most))};
 }
 // Chunks of a (key head, row tile) of a sequence (one at least, which writes the zeros of one without
@@ -114,15 +115,20 @@ __device__ __forceinline__ float column_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Inclusive sum over the workgroup's threads, in thread order.
-__device__ __forceinline__ uint32_t scan_threads(uint32_t v, uint32_t* sums, uint32_t& total) {
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+// Inclusive sum over the wavefront's lanes, and over the workgroup's threads, in order.
+__device__ __forceinline__ uint32_t scan_lanes(uint32_t v) {
+  const int lane = threadIdx.x & 63;
 #pragma unroll
   for (int d = 1; d < kWave; d *= 2) {
     const uint32_t o = __shfl_up(v, d);
     if (lane >= d) v += o;
   }
-  if (lane == 63) sums[w] = v;
+  return v;
+}
+__device__ __forceinline__ uint32_t scan_threads(uint32_t v, uint32_t* sums, uint32_t& total) {
+  const int w = threadIdx.x >> 6;
+  v = scan_lanes(v);
+  if ((threadIdx.x & 63) == 63) sums[w] = v;
   __syncthreads();
   uint32_t before = 0;
   total = 0;
@@ -134,31 +140,53 @@ __device__ __forceinline__ uint32_t scan_threads(uint32_t v, uint32_t* sums, uin
   __syncthreads();
   return before + v;
 }
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int l) { return __builtin_amdgcn_readlane(v, l); }
 
-// A wavefront's 32 keys of a chunk: 16-byte pieces of K in the operand's order (lane: key 16 n + l % 16,
-// dims 32 s + 8 (l / 16)) and of V in the same places.
-template <int S>
-struct Rows {
-  u32x4 k[2][S], v[2][S];
-  bool ok[2];
+// A barrier of the workgroup for what is in LDS (global stores stay in flight).
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// How the list is cut: chunks of a part, and what an item's chunks are rounded up to.
+struct Cut {
+  uint32_t per, unit;
 };
-struct Place {
-  int32_t page[2];
+__device__ __forceinline__ Cut cut_of(uint32_t chunks, uint32_t items, uint32_t parts) {
+  if (2 * items <= parts) {       // each item for itself: sum of ceil(chunks / per) <= chunks / per + items
+    const uint32_t per = max((chunks + (parts - items) - 1) / (parts - items), 1u);
+    return {per, per};
+  }
+  return {max((chunks + parts - 1) / parts, 1u), 1};
+}
+__device__ __forceinline__ uint32_t rounded(uint32_t n, uint32_t unit) { return (n + unit - 1) / unit * unit; }
+
+// A wavefront's 32 keys of a chunk, as loaded: 16-byte pieces of whole rows (a cache line at once: in the
+// operands' own order an instruction would touch half a line of 16 rows), and which keys have a place.
+template <int N>
+struct Rows {
+  u32x4 k[N], v[N];
+  uint32_t ok;
 };
 
 template <typename T, int DP, int NB>
 struct Tile {
   static constexpr int S = DP / 32, DT = DP / 16, R = 16 * NB;
-  static constexpr int kLd = DP + 16;                        // V rows in LDS: 16 + 8-byte reads free of conflicts
-  static constexpr int kStrip = kWaveKeys * kLd;             // halves of a wavefront's strip
+  static constexpr int kLd = DP + 16;                        // rows in LDS: reads of 16 and 8 bytes free of conflicts
+  static constexpr int kStrip = 2 * kWaveKeys * kLd;         // halves of a wavefront's strip: K, then V
+  // a load instruction takes kPer whole rows, kLanes lanes each (of them D / 8 with pieces of their own)
+  static constexpr int kLanes = DP / 8, kPer = kWave / kLanes, kLoads = (kWaveKeys + kPer - 1) / kPer;
 };
 
-template <typename T, int DP, int NB, int MIN>
+// PAST: keys and values are read past the caches.
+template <typename T, int DP, int NB, int MIN, bool PAST>
 __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArgs p) {
   using TL = Tile<T, DP, NB>;
   constexpr int S = TL::S, DT = TL::DT, R = TL::R, kLd = TL::kLd;
-  // (the merge of the wavefronts takes the strips over: 16 rows x DP floats each)
-  static_assert(kWaveKeys * kLd * 2 >= 16 * DP * 4, "");
+  constexpr int kSumLd = DP + 4;          // floats of a row of the merge
+  // (the merge of the wavefronts takes the strips over)
+  static_assert(TL::kStrip * 2 >= 16 * kSumLd * 4, "");
   __shared__ __align__(16) uint16_t strips[kWaves * TL::kStrip];
   __shared__ float stats[kWaves][2][16 * NB];
   __shared__ uint32_t sums[kWaves];
@@ -167,40 +195,81 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
   const int D = p.D;
 
   // ---- this workgroup's part of the list, and the sequence that it begins in
-  if (threadIdx.x == 0) found[0] = p.B;
-  uint32_t total = 0;
-  auto part_of = [&](uint32_t& begin, uint32_t& end) {
-    const uint32_t per = (total + p.parts - 1) / p.parts;
-    begin = min(blockIdx.x * per, total);
-    end = min(begin + per, total);
+  Cut cut;
+  uint32_t c_begin, c_end, seq0 = 0;
+  int b = p.B;
+  auto part_of = [&](uint32_t total) {
+    c_begin = min(blockIdx.x * cut.per, total);
+    c_end = min(c_begin + cut.per, total);
   };
-  uint32_t c_begin, c_end;
-  for (int pass = 0;; ++pass) {
-    uint32_t before = 0;
-    for (int b0 = 0; b0 < p.B; b0 += kThreads) {
-      const int b = b0 + static_cast<int>(threadIdx.x);
-      uint32_t n = 0;
-      if (b < p.B) {
-        const Seq s = sequence(p, b);
-        n = static_cast<uint32_t>(tiles_of<R>(s, p.G)) * p.NKV * chunks_of(s);
-      }
-      uint32_t all;
-      const uint32_t upto = before + scan_threads(n, sums, all);
-      before += all;
-      if (pass == 0 && blockIdx.x == 0 && b < p.B) p.first[b] = upto - n;
-      if (p.B <= kThreads) total = before;
-      part_of(c_begin, c_end);
-      if (c_begin >= upto - n && c_begin < upto) {
-        found[0] = b;
-        found[1] = upto - n;
+  Seq lane_seq{0, 0, 0};          // (up to 64 sequences: each lane has one)
+  if (p.B <= kWave) {             // every wavefront for itself
+    uint32_t items = 0, chunks = 0;
+    if (lane < p.B) {
+      const Seq s = sequence(p, lane);
+      lane_seq = s;
+      items = static_cast<uint32_t>(tiles_of<R>(s, p.G)) * p.NKV;
+      chunks = chunks_of(s);
+    }
+    cut = cut_of(lane_of(scan_lanes(items * chunks), 63), lane_of(scan_lanes(items), 63), p.parts);
+    const uint32_t n = items * rounded(chunks, cut.unit), upto = scan_lanes(n), total = lane_of(upto, 63);
+    part_of(total);
+    const uint64_t at = __ballot(c_begin >= upto - n && c_begin < upto);
+    if (at != 0) {
+      b = __ffsll(static_cast<unsigned long long>(at)) - 1;
+      seq0 = lane_of(upto - n, b);
+    }
+    if (blockIdx.x == 0 && w == 0) {
+      if (lane < p.B) p.first[lane] = upto - n;
+      if (lane == 0) {
+        p.first[p.B] = total;
+        p.first[p.B + 1] = cut.per;
+        p.first[p.B + 2] = cut.unit;
       }
     }
-    total = before;
-    if (p.B <= kThreads || pass == 1) break;     // (more sequences than threads: once the total is known)
+  } else {
+    uint32_t total = 0, all_chunks = 0, all_items = 0;
+    if (threadIdx.x == 0) found[0] = p.B;
+    for (int pass = 0; pass < 3; ++pass) {      // the list's sizes; its number of chunks; this part's begin
+      if (pass == 1) cut = cut_of(all_chunks, all_items, p.parts);
+      if (pass == 2) part_of(total);
+      uint32_t before = 0;
+      for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+        const int q = b0 + static_cast<int>(threadIdx.x);
+        uint32_t items = 0, chunks = 0;
+        if (q < p.B) {
+          const Seq s = sequence(p, q);
+          items = static_cast<uint32_t>(tiles_of<R>(s, p.G)) * p.NKV;
+          chunks = chunks_of(s);
+        }
+        uint32_t sum;
+        if (pass == 0) {
+          scan_threads(items * chunks, sums, sum);
+          all_chunks += sum;
+          scan_threads(items, sums, sum);
+          all_items += sum;
+        } else {
+          const uint32_t n = items * rounded(chunks, cut.unit);
+          const uint32_t upto = before + scan_threads(n, sums, sum);
+          before += sum;
+          if (pass == 1 && blockIdx.x == 0 && q < p.B) p.first[q] = upto - n;
+          if (pass == 2 && c_begin >= upto - n && c_begin < upto) {
+            found[0] = q;
+            found[1] = upto - n;
+          }
+        }
+      }
+      if (pass == 1) total = before;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      p.first[p.B] = total;
+      p.first[p.B + 1] = cut.per;
+      p.first[p.B + 2] = cut.unit;
+    }
+    __syncthreads();
+    b = static_cast<int>(found[0]);
+    seq0 = found[1];
   }
-  part_of(c_begin, c_end);
-  if (blockIdx.x == 0 && threadIdx.x == 0) p.first[p.B] = total;
-  __syncthreads();
   // rows that belong to no sequence
   if (p.cu != nullptr) {
     const int64_t lead = min(max(static_cast<int64_t>(p.cu[0]), int64_t{0}), p.rows);
@@ -211,24 +280,35 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
       for (int64_t c = threadIdx.x; c < width; c += kThreads) o[c] = 0;
     }
   }
-  int b = static_cast<int>(found[0]);
-  uint32_t seq0 = found[1];
   uint16_t* const strip = strips + w * TL::kStrip;
+  // this lane's piece of a row, and its row of load i (lanes and rows too many repeat the last ones)
+  const int lane_row = min(lane / TL::kLanes, TL::kPer - 1);
+  const int piece = 8 * min(lane - lane / TL::kLanes * TL::kLanes, D / 8 - 1);
+  auto row_of = [&](int i) {
+    const int row = i * TL::kPer + lane_row;
+    return kWaveKeys % TL::kPer ? min(row, kWaveKeys - 1) : row;
+  };
+  // of the sums of the merge: this thread's columns, first row and rows at a time
+  const int pairs = D / 2, sum_row = threadIdx.x / pairs, sum_col = 2 * (threadIdx.x - sum_row * pairs);
+  const int sum_rows = kThreads / pairs;
   uint32_t c = c_begin;
   while (c < c_end && b < p.B) {
-    const Seq sq = sequence(p, b);
-    const uint32_t chunks = chunks_of(sq), tiles = tiles_of<R>(sq, p.G);
-    const uint32_t seq_chunks = chunks * tiles * p.NKV;
+    const Seq sq = p.B <= kWave ? Seq{__builtin_amdgcn_readlane(lane_seq.start, b), __builtin_amdgcn_readlane(lane_seq.news, b),
+                                     __builtin_amdgcn_readlane(lane_seq.len, b)}
+                                : sequence(p, b);
+    const uint32_t chunks = chunks_of(sq), tiles = tiles_of<R>(sq, p.G), span = rounded(chunks, cut.unit);
+    const uint32_t seq_chunks = span * tiles * p.NKV;
     if (c >= seq0 + seq_chunks) {         // (the sequence is done, or has no rows)
       seq0 += seq_chunks;
       ++b;
       continue;
     }
-    const uint32_t item = (c - seq0) / chunks;
+    const uint32_t item = (c - seq0) / span;
     const int h = item / tiles, tile = item - h * tiles;
-    const uint32_t item0 = seq0 + item * chunks;
+    const uint32_t item0 = seq0 + item * span;
     const int j_begin = c - item0;
     const int j_end = min(chunks, c_end - item0);
+    c = item0 + span;                     // (what is left of it, if anything, is the next workgroup's)
 
     // ---- the query rows
     u32x4 qf[NB][S];
@@ -239,7 +319,7 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
       const bool real = rr < sq.news * p.G;
       const int i = p.by_group.div(real ? rr : 0), g = (real ? rr : 0) - i * p.G;
       limit[u] = real ? max(sq.len - sq.news + i + 1, 0) : 0;
-      const uint16_t* row = p.q + (sq.start + i) * p.q_stride + static_cast<int64_t>(h * p.G + g) * D;
+      const uint16_t* row = p.q + static_cast<int64_t>(sq.start + i) * p.q_stride + static_cast<int64_t>(h * p.G + g) * D;
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         const int d = 32 * s + 8 * gr;
@@ -261,38 +341,40 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
     }
 
     const int32_t* pages = p.table + static_cast<int64_t>(b) * p.max_pages;
+    // the page of key `lane % 32` of this wavefront's in chunk j (-1: none)
     auto find = [&](int j) {
-      Place pl;
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int key = j * kChunk + w * kWaveKeys + 16 * n + ql;
-        pl.page[n] = key < seen_any ? pages[p.by_page.div(key)] : -1;
-      }
-      return pl;
+      const int key = j * kChunk + w * kWaveKeys + (lane & 31);
+      const int page = key < seen_any ? pages[p.by_page.div(key)] : -1;
+      return page >= 0 && page < p.pages ? page : -1;
     };
-    auto load = [&](Rows<S>& r, const Place& pl, int j) {
+    const uint16_t* const k_lane = p.k + static_cast<int64_t>(h) * p.page_size * D + piece;
+    const uint16_t* const v_lane = p.v + static_cast<int64_t>(h) * p.page_size * D + piece;
+    auto load = [&](Rows<TL::kLoads>& r, int found_page, int j) {
+      r.ok = static_cast<uint32_t>(__ballot(found_page >= 0));
+      // (a key without a place reads a row of page 0: masked, and its value zeroed, below)
+      const int key = j * kChunk + w * kWaveKeys + (lane & 31);
+      const int slot = key - static_cast<int>(p.by_page.div(key)) * p.page_size;
+      const int64_t at = static_cast<int64_t>(max(found_page, 0)) * p.page_stride + slot * D;
+      const int at_lo = static_cast<int>(at), at_hi = static_cast<int>(at >> 32);
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        const int key = j * kChunk + w * kWaveKeys + 16 * n + ql;
-        const int slot = key - p.by_page.div(key) * p.page_size;
-        r.ok[n] = pl.page[n] >= 0 && pl.page[n] < p.pages;
-        // (a key without a place reads the first row of the cache: masked, and its value zeroed, below)
-        const int64_t at = r.ok[n] ? static_cast<int64_t>(pl.page[n]) * p.page_stride + (static_cast<int64_t>(h) * p.page_size + slot) * D
-                                    : 0;
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-          // (dims past D: the row's first again, which meet zeros of Q and columns that are not written)
-          const int d = 32 * s + 8 * gr;
-          const int64_t to = at + (d < D ? d : 0);
-          r.k[n][s] = *reinterpret_cast<const u32x4*>(p.k + to);
-          r.v[n][s] = *reinterpret_cast<const u32x4*>(p.v + to);
-        }
+      for (int i = 0; i < TL::kLoads; ++i) {
+        const int row = row_of(i);
+        const uint32_t lo = __shfl(at_lo, row), hi = __shfl(at_hi, row);
+        const int64_t to = static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+        r.k[i] = ld<PAST>(reinterpret_cast<const u32x4*>(k_lane + to));
+        r.v[i] = ld<PAST>(reinterpret_cast<const u32x4*>(v_lane + to));
       }
     };
+    if (D < DP) {                         // columns past D meet zeros of Q: no NaN may be there
+      for (int e = lane; e < kWaveKeys * (DP - D) / 8; e += kWave) {
+        const int row = e & (kWaveKeys - 1);
+        *reinterpret_cast<u32x4*>(strip + row * kLd + D + 8 * (e / kWaveKeys)) = u32x4{0, 0, 0, 0};
+      }
+    }
     // (chunks in which this wavefront has keys that the tile sees)
     const int j_mine = min(j_end, (seen_any - w * kWaveKeys + kChunk - 1) / kChunk);
-    Rows<S> r;
-    Place next;
+    Rows<TL::kLoads> r;
+    int next = -1;
     if (j_begin < j_mine) {
       next = find(j_begin);
       load(r, next, j_begin);
@@ -300,36 +382,36 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
     }
     for (int j = j_begin; j < j_mine; ++j) {
       const int key0 = j * kChunk + w * kWaveKeys;
-      const bool okay[2] = {r.ok[0], r.ok[1]};
-      const uint64_t all0 = __ballot(okay[0]), all1 = __ballot(okay[1]);
-      const bool whole = (all0 & all1) == ~uint64_t{0};
+      const uint32_t ok = r.ok;
+      const bool whole = ok == ~0u;
       if (!whole) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int s = 0; s < S; ++s)
-            if (!okay[n]) r.v[n][s] = u32x4{0, 0, 0, 0};
+        for (int i = 0; i < TL::kLoads; ++i) r.v[i] = r.v[i] & (0u - ((ok >> row_of(i)) & 1));
       }
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int s = 0; s < S; ++s)
-          *reinterpret_cast<u32x4*>(strip + (16 * n + ql) * kLd + 32 * s + 8 * gr) = r.v[n][s];
-      f4 sc[NB][2];
-#pragma unroll
-      for (int u = 0; u < NB; ++u) sc[u][0] = sc[u][1] = f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = 0; s < S; ++s)
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int u = 0; u < NB; ++u) sc[u][n] = Ops<T>::mfma(r.k[n][s], qf[u][s], sc[u][n]);
+      for (int i = 0; i < TL::kLoads; ++i) {
+        const int row = row_of(i);
+        *reinterpret_cast<u32x4*>(strip + row * kLd + piece) = r.k[i];
+        *reinterpret_cast<u32x4*>(strip + (kWaveKeys + row) * kLd + piece) = r.v[i];
+      }
       // the next chunk's rows, and the page numbers of the one after it
       if (j + 1 < j_mine) {
         load(r, next, j + 1);
         next = find(j + 2);
       }
       __asm__ volatile("" ::: "memory");
+      f4 sc[NB][2];
+#pragma unroll
+      for (int u = 0; u < NB; ++u) sc[u][0] = sc[u][1] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          const u32x4 kf = *reinterpret_cast<const u32x4*>(strip + (16 * n + ql) * kLd + 32 * s + 8 * gr);
+#pragma unroll
+          for (int u = 0; u < NB; ++u) sc[u][n] = Ops<T>::mfma(kf, qf[u][s], sc[u][n]);
+        }
+      }
       u32x4 pb[NB];
       bool any = false;
 #pragma unroll
@@ -340,7 +422,7 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int at = 4 * gr + (e & 3), n = e >> 2;
-            const bool seen = key0 + 16 * n + at < limit[u] && (((n ? all1 : all0) >> at) & 1);
+            const bool seen = key0 + 16 * n + at < limit[u] && ((ok >> (16 * n + at)) & 1);
             sc[u][n][e & 3] = seen ? sc[u][n][e & 3] : -INFINITY;
           }
         }
@@ -365,11 +447,12 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
         pb[u] = u32x4{Ops<T>::pack(pr[0], pr[1]), Ops<T>::pack(pr[2], pr[3]), Ops<T>::pack(pr[4], pr[5]),
                       Ops<T>::pack(pr[6], pr[7])};
       }
+      __asm__ volatile("" ::: "memory");      // (no reads of V before their time: registers)
       // O^T += V^T P^T: transpose reads (lane k of a 16-lane group reads 8 bytes of row 4 gr + k / 4 at
       // column 4 (k % 4); lane i gets column i of the four rows), rows 4 gr .. + 3 and 16 more
 #pragma unroll
       for (int t = 0; t < DT; ++t) {
-        const uint16_t* at = strip + (4 * gr + (ql >> 2)) * kLd + 16 * t + 4 * (ql & 3);
+        const uint16_t* at = strip + (kWaveKeys + 4 * gr + (ql >> 2)) * kLd + 16 * t + 4 * (ql & 3);
         const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at));
         const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + 16 * kLd));
         const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
@@ -380,6 +463,7 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
     }
 
     // ---- the four wavefronts' sums into one
+    const int real_rows = min(R, sq.news * p.G - tile * R);
 #pragma unroll
     for (int u = 0; u < NB; ++u) {
       lsum[u] = column_sum(lsum[u]);
@@ -390,60 +474,62 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
     }
     const bool complete = j_begin == 0 && j_end == static_cast<int>(chunks);
     float* const part = p.part + (2 * static_cast<int64_t>(blockIdx.x) + (j_begin == 0 ? 1 : 0)) * (R * (D + 2));
-    const int real_rows = min(R, sq.news * p.G - tile * R);
     float* const mine = reinterpret_cast<float*>(strip);
 #pragma unroll
     for (int u = 0; u < NB; ++u) {
-      __syncthreads();                    // (stats are written; the strips' last readers are done)
-      float m_all = stats[0][0][16 * u + ql];
+      if (16 * u >= real_rows) break;
+      lds_barrier();                      // (stats are written; the strips' last readers are done)
+      if (16 * u + ql < real_rows) {
+        float m_all = stats[0][0][16 * u + ql];
 #pragma unroll
-      for (int i = 1; i < kWaves; ++i) m_all = fmaxf(m_all, stats[i][0][16 * u + ql]);
-      const float f = m_ref[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_ref[u] - m_all);
+        for (int i = 1; i < kWaves; ++i) m_all = fmaxf(m_all, stats[i][0][16 * u + ql]);
+        const float f = m_ref[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_ref[u] - m_all);
 #pragma unroll
-      for (int t = 0; t < DT; ++t)
-        *reinterpret_cast<f4*>(mine + ql * DP + 16 * t + 4 * gr) = acc[u][t] * f;
-      __syncthreads();
-      // thread: two neighbouring columns of a row
-      for (int e = threadIdx.x; e < 16 * (D / 2); e += kThreads) {
-        const int row = e / (D / 2), col = 2 * (e - row * (D / 2)), rt = 16 * u + row;
+        for (int t = 0; t < DT; ++t)
+          *reinterpret_cast<f4*>(mine + ql * kSumLd + 16 * t + 4 * gr) = acc[u][t] * f;
+      }
+      lds_barrier();
+      // a thread: two neighbouring columns of a row
+      for (int row = sum_row; row < 16 && sum_row < sum_rows; row += sum_rows) {
+        const int rt = 16 * u + row;
         if (rt >= real_rows) break;
         float x = 0.f, y = 0.f, l = 0.f, m = stats[0][0][rt];
 #pragma unroll
         for (int i = 1; i < kWaves; ++i) m = fmaxf(m, stats[i][0][rt]);
 #pragma unroll
         for (int i = 0; i < kWaves; ++i) {
-          const float* src = reinterpret_cast<const float*>(strips + i * TL::kStrip) + row * DP + col;
-          x += src[0];
-          y += src[1];
+          const float2 v = *reinterpret_cast<const float2*>(
+              reinterpret_cast<const float*>(strips + i * TL::kStrip) + row * kSumLd + sum_col);
+          x += v.x;
+          y += v.y;
           const float mi = stats[i][0][rt];
           l += mi == -INFINITY ? 0.f : stats[i][1][rt] * __builtin_amdgcn_exp2f(mi - m);
         }
         if (complete) {
           const int rr = tile * R + rt, i = p.by_group.div(rr), g = rr - i * p.G;
           const float inv = m == -INFINITY ? 0.f : 1.f / l;
-          uint16_t* o = p.out + ((sq.start + i) * p.NKV + h) * static_cast<int64_t>(p.G) * D + g * D + col;
+          uint16_t* o = p.out + (static_cast<int64_t>(sq.start + i) * p.NKV + h) * p.G * D + g * D + sum_col;
           *reinterpret_cast<uint32_t*>(o) = Ops<T>::pack(x * inv, y * inv);
         } else {
-          part[rt * D + col] = x;
-          part[rt * D + col + 1] = y;
-          if (col == 0) {
+          *reinterpret_cast<float2*>(part + rt * D + sum_col) = float2{x, y};
+          if (sum_col == 0) {
             part[R * D + rt] = m;
             part[R * D + R + rt] = l;
           }
         }
       }
     }
-    __syncthreads();                      // (the strips and stats are free again)
-    c = item0 + j_end;
+    if (c < c_end) lds_barrier();         // (the strips and stats are free again)
   }
 }
 
-// Joins the parts of the rows that reach across workgroups: one workgroup a (token, query head).
+// Joins the parts of the rows that reach across workgroups: one workgroup a (token, query head) and 32
+// columns, 16 lanes a part.
+constexpr int kJoinCols = 32;
 template <typename T, int R, int THREADS>
 __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedArgs p) {
-  __shared__ float best[THREADS / kWave];
-  __shared__ float2 cols[THREADS];
-  __shared__ float weights[THREADS];
+  constexpr int kJoinWaves = THREADS / kWave;
+  __shared__ f4 sums[kJoinWaves * 16];      // of a wavefront: two columns' sums, weight, reference value
   const int heads = p.NKV * p.G;
   const int64_t row = blockIdx.x / heads;
   const int head = static_cast<int>(blockIdx.x - row * heads), h = head / p.G, g = head - h * p.G;
@@ -458,56 +544,62 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedArgs p) {
     }
   }
   const Seq s = sequence(p, b);
-  const uint32_t total = p.first[p.B];
+  const uint32_t first = p.first[b], total = p.first[p.B], per = p.first[p.B + 1], unit = p.first[p.B + 2];
   if (row < s.start || row >= s.start + s.news || total == 0) return;
-  const uint32_t per = (total + p.parts - 1) / p.parts;
   const int rr = static_cast<int>(row - s.start) * p.G + g;
   const uint32_t chunks = chunks_of(s), tiles = tiles_of<R>(s, p.G);
-  const uint32_t c0 = p.first[b] + (h * tiles + rr / R) * chunks, c1 = c0 + chunks - 1;
+  const uint32_t c0 = first + (h * tiles + rr / R) * rounded(chunks, unit), c1 = c0 + chunks - 1;
   const uint32_t w0 = c0 / per, w1 = c1 / per;
   if (w0 == w1 || w1 >= static_cast<uint32_t>(p.parts)) return;      // (written whole)
-  const int rt = rr % R, D = p.D;
-  const int n = static_cast<int>(w1 - w0) + 1;
-  auto part = [&](int i) {
-    return p.part + (2 * static_cast<int64_t>(w0 + i) + (i == 0 ? 1 : 0)) * (R * (D + 2));
-  };
-  const int lane = threadIdx.x & 63;
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += THREADS) m = fmaxf(m, part(i)[R * D + rt]);
-#pragma unroll
-  for (int d = 32; d >= 1; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
-  if (lane == 0) best[threadIdx.x >> 6] = m;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < THREADS / kWave; ++i) m = fmaxf(m, best[i]);
-  // columns 2 c, 2 c + 1 of every `by`-th part
-  const int half = D / 2, by = THREADS / half;
-  const int first = threadIdx.x / half, c = threadIdx.x - first * half;
-  float x = 0.f, y = 0.f, l = 0.f;
-  if (first < by) {
+  const int rt = rr % R, D = p.D, lane = threadIdx.x & 63, w = threadIdx.x >> 6, ql = lane & 15;
+  const int n = static_cast<int>(w1 - w0) + 1, col = blockIdx.y * kJoinCols + 2 * ql;
+  const int at = min(col, D - 2);
+  // every (THREADS / 16)-th part, under a reference value of the lane's own
+  float x = 0.f, y = 0.f, l = 0.f, m = -INFINITY;
 #pragma unroll 4
-    for (int i = first; i < n; i += by) {
-      const float* src = part(i);
-      const float mi = src[R * D + rt];
-      const float f = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - m);
-      const float2 v = *reinterpret_cast<const float2*>(src + rt * D + 2 * c);
-      x += v.x * f;
-      y += v.y * f;
-      l += src[R * D + R + rt] * f;
+  for (int i = threadIdx.x / 16; i < n; i += THREADS / 16) {
+    const float* src = p.part + (2 * static_cast<int64_t>(w0 + i) + (i == 0 ? 1 : 0)) * (R * (D + 2));
+    const float mi = src[R * D + rt], li = src[R * D + R + rt];
+    const float2 v = *reinterpret_cast<const float2*>(src + rt * D + at);
+    const float m_new = __builtin_elementwise_maximum(m, mi);
+    const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+    const float f = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - m_new);
+    x = x * a + v.x * f;
+    y = y * a + v.y * f;
+    l = l * a + li * f;
+    m = m_new;
+  }
+  auto join = [&] {                        // the four lanes of a column pair into one
+    const float m_new = column_max(m);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+    x = column_sum(x * f);
+    y = column_sum(y * f);
+    l = column_sum(l * f);
+    m = m_new;
+  };
+  join();
+  if constexpr (kJoinWaves > 1) {
+    if (lane < 16) sums[w * 16 + ql] = f4{x, y, l, m};
+    __syncthreads();
+    if (w != 0) return;
+    x = y = l = 0.f;
+    m = -INFINITY;
+#pragma unroll
+    for (int i = lane / 16; i < kJoinWaves; i += 4) {
+      const f4 o = sums[i * 16 + ql];
+      const float m_new = __builtin_elementwise_maximum(m, o.w);
+      const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+      const float f = o.w == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(o.w - m_new);
+      x = x * a + o.x * f;
+      y = y * a + o.y * f;
+      l = l * a + o.z * f;
+      m = m_new;
     }
+    join();
   }
-  cols[threadIdx.x] = float2{x, y};
-  weights[threadIdx.x] = l;
-  __syncthreads();
-  if (first != 0) return;
-  for (int i = 1; i < by; ++i) {
-    const float2 o = cols[i * half + c];
-    x += o.x;
-    y += o.y;
-    l += weights[i * half + c];
-  }
+  if (lane >= 16 || col >= D) return;
   const float inv = m == -INFINITY ? 0.f : 1.f / l;
-  *reinterpret_cast<uint32_t*>(p.out + (row * heads + head) * D + 2 * c) = Ops<T>::pack(x * inv, y * inv);
+  *reinterpret_cast<uint32_t*>(p.out + (row * heads + head) * D + col) = Ops<T>::pack(x * inv, y * inv);
 }
 
 // ---- host ---------------------------------------------------------------------------------------
@@ -516,8 +608,14 @@ bool bad_ptr(const void* p, uintptr_t mask) {
   return p == nullptr || (reinterpret_cast<uintptr_t>(p) & mask) != 0;
 }
 
-constexpr int kPartsPerCu = 2;
-constexpr int64_t kWideJoin = 256;       // rows up to which a join has 1024 threads
+// Workgroups that a CU holds, and that the list is cut for (more of them would wait for a place and begin
+// anew): by their LDS two, and one where registers (64 rows) or LDS (heads over 128) allow no more.
+int held(int nb, int32_t D) { return nb == 4 || D > 128 ? 1 : 2; }
+// Bytes of keys and values that the block tables can hold from which they are read past the caches: what the
+// Infinity Cache (256 MB) does not keep for a next call.  MI355X, past / through the caches: 64 sequences of
+// up to 8192 keys, 8 heads of 128, 198 / 216 us; 16 of up to 4096, 4 of 256, 49.9 / 53.5; within it,
+// 16 of 4096, 4 of 96, 26.6 / 24.4; 8 of 4096, 16 of 64, 22.8 / 21.8.
+constexpr int64_t kPastFrom = int64_t{256} << 20;
 constexpr int64_t kMostKeys = int64_t{1} << 30;
 
 // Row blocks of 16 a tile: what a sequence's rows fill on average.
@@ -529,7 +627,7 @@ int blocks_of(int64_t rows, int32_t B, int32_t G, int32_t D) {
 }
 
 struct Plan {
-  int nb, parts;
+  int nb, parts, parts_of_item;
   bool join;
   int64_t first_bytes, bytes;
 };
@@ -541,26 +639,31 @@ bool plan_of(int64_t rows, int32_t B, int32_t G, int32_t NKV, int32_t D, int64_t
   const int64_t chunks = std::max<int64_t>((most_keys + kChunk - 1) / kChunk, 1);
   const int64_t items = (rows * G / R + B) * NKV;
   if (items > 0 && chunks > ((int64_t{1} << 31) - 1) / items) return false;
-  const int64_t list = items * chunks;
-  pl.parts = static_cast<int>(std::max<int64_t>(std::min<int64_t>(list, int64_t{kPartsPerCu} * device_cu_count()), 1));
+  const int64_t list = items * chunks + items;      // (each item's rounding included)
+  pl.parts = static_cast<int>(std::max<int64_t>(std::min<int64_t>(list, int64_t{held(pl.nb, D)} * device_cu_count()), 1));
   pl.join = chunks > 1;
-  pl.first_bytes = (4 * (int64_t{B} + 1) + 15) / 16 * 16;
+  pl.parts_of_item = static_cast<int>(std::min<int64_t>(pl.parts / std::max<int64_t>(items, 1), chunks));
+  pl.first_bytes = (4 * (int64_t{B} + 3) + 15) / 16 * 16;
   pl.bytes = pl.first_bytes + 2 * int64_t{pl.parts} * R * (D + 2) * 4;
   return true;
 }
 
 template <typename T, int DP>
 int launch_paged(const PagedArgs& a, const Plan& pl, hipStream_t s) {
+  const bool past = a.max_pages * a.page_size * a.B > kPastFrom / (int64_t{4} * a.NKV * a.D);
   const dim3 grid(pl.parts), block(kThreads);
   auto run = [&](auto nb, auto min_waves) -> int {
     constexpr int NB = decltype(nb)::value;
-    int rc = launch_kernel(paged_attention_kernel<T, DP, NB, decltype(min_waves)::value>, grid, block, s, a);
+    constexpr int MIN = decltype(min_waves)::value;
+    // (64 rows: a prompt's part, whose tiles read the same keys one after another)
+    int rc = NB < 4 && past ? launch_kernel(paged_attention_kernel<T, DP, NB, MIN, NB < 4>, grid, block, s, a)
+                            : launch_kernel(paged_attention_kernel<T, DP, NB, MIN, false>, grid, block, s, a);
     if (rc != kOk || !pl.join) return rc;
-    const int64_t outs = a.rows * a.NKV * a.G;
-    const dim3 join(static_cast<unsigned>(outs));
-    // (few rows have many parts each)
-    if (outs <= kWideJoin) return launch_kernel(paged_join_kernel<T, 16 * NB, 1024>, join, dim3(1024), s, a);
-    return launch_kernel(paged_join_kernel<T, 16 * NB, 256>, join, dim3(256), s, a);
+    const dim3 join(static_cast<unsigned>(a.rows * a.NKV * a.G), static_cast<unsigned>((a.D + kJoinCols - 1) / kJoinCols));
+    // (by the parts that a row can have, when every item is one of equals)
+    if (pl.parts_of_item > 64) return launch_kernel(paged_join_kernel<T, 16 * NB, 1024>, join, dim3(1024), s, a);
+    if (pl.parts_of_item > 8) return launch_kernel(paged_join_kernel<T, 16 * NB, 256>, join, dim3(256), s, a);
+    return launch_kernel(paged_join_kernel<T, 16 * NB, 64>, join, dim3(64), s, a);
   };
   using std::integral_constant;
   if (pl.nb == 1) return run(integral_constant<int, 1>{}, integral_constant<int, DP <= 128 ? 2 : 1>{});
