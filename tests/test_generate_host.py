@@ -155,7 +155,7 @@ def test_empty_work_is_a_no_op(name, args):
 def test_workspaces():
     need = ctypes.c_int64()
     _ext.call("soupk_verify_drafts_workspace", 2, 151936, ctypes.addressof(need))
-    assert need.value == 2 * 16 * -(-151936 // 4096)
+    assert need.value == 2 * 16 * -(-151936 // 1024)
     _ext.call("soupk_verify_drafts_workspace", 1, 1 << 24, ctypes.addressof(need))
     assert need.value <= 16 * 256
     _ext.call("soupk_paged_attention_workspace", 1, 1, 12, 2, 128, 8, 16, ctypes.addressof(need))

@@ -8,6 +8,8 @@
 
 #include <vector>
 
+#include <c10/hip/HIPFunctions.h>
+
 #include "host_args.hpp"
 #include "host_autograd.hpp"
 
@@ -92,7 +94,7 @@ void written(const Tensor& t) {
 }  // namespace
 
 // rotary_tables(seq, dim, theta, scaling code, factor, original, beta_fast, beta_slow, gain, frequencies (a
-// tuple, or None), device index) -> (cos, sin)
+// tuple, or None), device index (-1: the current one)) -> (cos, sin)
 OP(rotary_tables) {
   HANDLE_TH_ERRORS
   ARGS(11);
@@ -103,7 +105,8 @@ OP(rotary_tables) {
   const int at_arg[6] = {2, 4, 5, 6, 7, 8};
   for (int i = 0; i < 6; ++i)
     if (!number(a[at_arg[i]], v[i])) ELSE_PYTHON;
-  if (seq < 0 || seq >= (int64_t{1} << 31) || dim < 2 || dim > 256 || dim % 2) ELSE_PYTHON;
+  if (seq < 0 || seq >= (int64_t{1} << 31) || dim < 2 || dim > 256 || dim % 2 || !(v[0] > 1.0 && v[0] <= 1e30))
+    ELSE_PYTHON;
   std::vector<double> freq;
   if (a[9] != Py_None) {
     if (!PyTuple_Check(a[9]) || PyTuple_GET_SIZE(a[9]) != dim / 2) ELSE_PYTHON;
@@ -114,7 +117,8 @@ OP(rotary_tables) {
   Tensor cos, sin;
   {
     const NoGil released;
-    const at::Device dev(at::kCUDA, static_cast<c10::DeviceIndex>(device));
+    const at::Device dev(at::kCUDA, device < 0 ? c10::hip::current_device()
+                                               : static_cast<c10::DeviceIndex>(device));
     const c10::DeviceGuard guard(dev);
     cos = empty({seq, dim / 2}, at::kFloat, dev);
     sin = empty({seq, dim / 2}, at::kFloat, dev);

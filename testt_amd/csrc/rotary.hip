@@ -13,7 +13,7 @@
 //            0.1 ln(factor) + 1
 // An angle is held in turns in 64 bits and reduced to the nearest quarter before its cosine and sine are
 // summed from their Taylor series: at position 2^20 an angle in fp32 would be 0.03 rad off, here the
-// error is 1e-9.
+// error is below 1e-9.
 //
 // Rotation: (a, b) -> (a c - b s, b c + a s) for the pairs (x[i], x[i + R/2]) or, interleaved,
 // (x[2 i], x[2 i + 1]) of the leading R = dim elements of a head; the others are copied.  Products and
@@ -21,8 +21,7 @@
 // that a token appended to the cache has the bits that the training path gives it.  The gradient is the same
 // with -s.
 //
-// Mapping: an item is 16 elements of a head (two runs of 8 that rotate against each other, or 16
-// neighbours); a wavefront takes the items of 64 / (D / 16) neighbouring heads of one token, PER times
+// Mapping: an item is 16 elements of a head, two runs of 8 (by halves they rotate against each other); a wavefront takes the items of 64 / (D / 16) neighbouring heads of one token, PER times
 // over, so that one read of the token's table row serves PER heads.  A head that cannot be cut so
 // (D or the rotated part no multiple of 16, or R/2 no multiple of 8) takes a pair per lane instead.
 
@@ -42,26 +41,29 @@ constexpr int kWaves = kThreads / kWave;
 // ---- tables -------------------------------------------------------------------------------------
 
 constexpr int kMaxPairs = 128;
+// Positions of a thread where there are many, whose first sum serves the others: 131072 positions of 128 in 15.0
+// us with one, 15.4 with two, 12.4 with four, 12.2 with eight (12.1 with nothing but the stores); 4096 positions
+// 6.9 -> 6.5.
+constexpr int kPositions = 8;
+constexpr int64_t kManyThreads = 16384;
 struct Turns {
   double per_pos[kMaxPairs];      // of a turn
 };
 
 // cos and sin of 2 pi r for r in [-1/2, 1/2]: quarter turns split off, then the series of the remaining
-// |x| <= pi / 4 (first terms left out: x^15 / 15! < 3e-14, x^16 / 16! < 2e-15).
+// |x| <= pi / 4 (first terms left out: x^13 / 13! < 7e-12, x^12 / 12! < 2e-10; an fp32 number near 1 is
+// rounded by up to 3e-8).
 __device__ __forceinline__ void cos_sin_turns(double r, double& c, double& s) {
   const double q = __builtin_rint(4.0 * r);
   const double x = __builtin_fma(q, -0.25, r) * 6.283185307179586476925;
   const double y = x * x;
-  double sn = 1.0 / 6227020800.0;
-  sn = __builtin_fma(sn, y, -1.0 / 39916800.0);
+  double sn = -1.0 / 39916800.0;
   sn = __builtin_fma(sn, y, 1.0 / 362880.0);
   sn = __builtin_fma(sn, y, -1.0 / 5040.0);
   sn = __builtin_fma(sn, y, 1.0 / 120.0);
   sn = __builtin_fma(sn, y, -1.0 / 6.0);
   sn = __builtin_fma(sn * y, x, x);
-  double cs = -1.0 / 87178291200.0;
-  cs = __builtin_fma(cs, y, 1.0 / 479001600.0);
-  cs = __builtin_fma(cs, y, -1.0 / 3628800.0);
+  double cs = -1.0 / 3628800.0;
   cs = __builtin_fma(cs, y, 1.0 / 40320.0);
   cs = __builtin_fma(cs, y, -1.0 / 720.0);
   cs = __builtin_fma(cs, y, 1.0 / 24.0);
@@ -73,41 +75,66 @@ __device__ __forceinline__ void cos_sin_turns(double r, double& c, double& s) {
   s = quarter >= 2 ? -b : b;
 }
 
-// N pairs a thread.
-template <int N>
+// N pairs of every `step`-th position a thread, P of them: the first angle's cosine and sine are summed, and
+// turned on by the step's (each turn rounds 1e-16) to the next ones.
+template <int N, int P>
 __global__ __launch_bounds__(kThreads) void rotary_tables_kernel(Turns turns, float* __restrict__ cos_t,
                                                                  float* __restrict__ sin_t, double gain,
-                                                                 uint32_t pos0, uint32_t items,
+                                                                 uint32_t step, uint32_t seq,
                                                                  FastDiv per_pos, int half) {
   const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
-  if (i >= items) return;
-  const uint32_t p = per_pos.div(i), g = i - p * per_pos.d;
-  const double pos = static_cast<double>(pos0 + p);
-  const int64_t at = static_cast<int64_t>(pos0 + p) * half + g * N;
-  float c[N], s[N];
+  const uint32_t q = per_pos.div(i), g = i - q * per_pos.d;
+  // (positions in blocks of P * step, a thread's `step` apart)
+  const uint32_t first = P == 1 ? q : q / step * (P * step) + q % step;
+  if (first >= seq) return;
+  double c[N], s[N], cs[N], ss[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const double t = pos * turns.per_pos[g * N + j];
-    double cd, sd;
-    cos_sin_turns(t - __builtin_rint(t), cd, sd);
-    c[j] = static_cast<float>(cd * gain);
-    s[j] = static_cast<float>(sd * gain);
+    const double f = turns.per_pos[g * N + j];
+    const double t = static_cast<double>(first) * f;
+    cos_sin_turns(t - __builtin_rint(t), c[j], s[j]);
+    c[j] *= gain;
+    s[j] *= gain;
+    if constexpr (P > 1) {
+      const double d = static_cast<double>(step) * f;
+      cos_sin_turns(d - __builtin_rint(d), cs[j], ss[j]);
+    }
   }
-  if constexpr (N == 4) {
-    st<true>(reinterpret_cast<f32x4*>(cos_t + at), f32x4{c[0], c[1], c[2], c[3]});
-    st<true>(reinterpret_cast<f32x4*>(sin_t + at), f32x4{s[0], s[1], s[2], s[3]});
-  } else {
-    cos_t[at] = c[0];
-    sin_t[at] = s[0];
+#pragma unroll
+  for (int k = 0; k < P; ++k) {
+    const uint32_t pos = first + k * step;
+    if (P > 1 && pos >= seq) return;
+    const int64_t at = static_cast<int64_t>(pos) * half + g * N;
+    if constexpr (N == 4) {
+      f32x4 a, b;
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        a[j] = static_cast<float>(c[j]);
+        b[j] = static_cast<float>(s[j]);
+      }
+      *reinterpret_cast<f32x4*>(cos_t + at) = a;
+      *reinterpret_cast<f32x4*>(sin_t + at) = b;
+    } else {
+      cos_t[at] = static_cast<float>(c[0]);
+      sin_t[at] = static_cast<float>(s[0]);
+    }
+    if (k + 1 < P) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const double x = __builtin_fma(c[j], cs[j], -(s[j] * ss[j]));
+        s[j] = __builtin_fma(s[j], cs[j], c[j] * ss[j]);
+        c[j] = x;
+      }
+    }
   }
 }
 
 // ---- the rotation of an item --------------------------------------------------------------------
 
-// What part of a head an item covers: N elements from `a` and N from `b` (in elements of the head); `turn`:
-// the first of its pairs in the tables, or -1 where the elements are copied.
+// What part of a head an item covers: N elements from `a` and N from `b` (in elements of the head); the first
+// pairs of both in the tables, or -1 where a run's elements are copied.
 struct Item {
-  int a, b, turn;
+  int a, b, turn_a, turn_b;
   bool two;           // (N = 1) there is a second element
 };
 
@@ -117,30 +144,45 @@ struct Layout {
   bool interleaved;
 };
 
+// (Neighbouring items are neighbours in memory, run by run, so that a wavefront's access covers whole lines
+// where it can.  Interleaved pairs lie within a run, and the runs of an item are the same place of both halves
+// of the head; as 16 neighbouring elements an access touched every other 16 bytes: 8192 tokens of 40
+// heads, half of each rotated, both ways 74 us instead of 57.)
 template <int N>
 __device__ __forceinline__ Item item_of(const Layout& l, int i) {
+  if constexpr (N > 1) {
+    if (l.interleaved) {
+      const int a = N * i, b = l.D / 2 + N * i;
+      return {a, b, a < 2 * l.half ? a / 2 : -1, b < 2 * l.half ? b / 2 : -1, true};
+    }
+  }
   const int turned = l.half / N;
-  if (i < turned)
-    return l.interleaved ? Item{2 * N * i, 2 * N * i + N, N * i, true}
-                         : Item{N * i, l.half + N * i, N * i, true};
-  const int at = 2 * l.half + 2 * N * (i - turned);
-  return Item{at, at + N, -1, at + N < l.D};
+  if (i < turned) {
+    if (N == 1 && l.interleaved) return {2 * i, 2 * i + 1, i, i, true};
+    return {N * i, l.half + N * i, N * i, N * i, true};
+  }
+  const int at = 2 * l.half + N * (i - turned), next = at + N * (l.items - turned);
+  return {at, next, -1, -1, next < l.D};
 }
 
-// x, y: the item's two runs, c, s: its pairs' cosines and sines.
+// x, y: the item's two runs, c, s: the cosines and sines of their pairs (interleaved: of x's N / 2, then of
+// y's).
 template <int N>
 __device__ __forceinline__ void turn(float (&x)[N], float (&y)[N], const float (&c)[N], const float (&s)[N],
-                                     bool interleaved) {
+                                     const Item& it, bool interleaved) {
   if (N > 1 && interleaved) {
+    auto pairs = [&](float (&v)[N], int first) {
 #pragma unroll
-    for (int j = 0; j < N; j += 2) {
-      const int u = j / 2, w = (N + j) / 2;
-      const float a = x[j] * c[u] - x[j + 1] * s[u], b = x[j + 1] * c[u] + x[j] * s[u];
-      const float d = y[j] * c[w] - y[j + 1] * s[w], e = y[j + 1] * c[w] + y[j] * s[w];
-      x[j] = a; x[j + 1] = b;
-      y[j] = d; y[j + 1] = e;
-    }
-  } else {
+      for (int j = 0; j < N; j += 2) {
+        const int u = first + j / 2;
+        const float a = v[j] * c[u] - v[j + 1] * s[u], b = v[j + 1] * c[u] + v[j] * s[u];
+        v[j] = a;
+        v[j + 1] = b;
+      }
+    };
+    if (it.turn_a >= 0) pairs(x, 0);
+    if (it.turn_b >= 0) pairs(y, N / 2);
+  } else if (it.turn_a >= 0) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const float a = x[j] * c[j] - y[j] * s[j], b = y[j] * c[j] + x[j] * s[j];
@@ -165,16 +207,27 @@ __device__ __forceinline__ void store_run(char* base, int64_t at, const float (&
     Elem<T>::store1(base + at * Elem<T>::kBytes, v[0]);
 }
 
-// The cosines and (times `sign`) sines of an item; an item that is copied turns by nothing.
+// The cosines and (times `sign`) sines of an item's pairs, in the order of turn(); nothing for a run that is
+// copied.
 template <int N>
-__device__ __forceinline__ void load_turns(const float* cos_t, const float* sin_t, int64_t row, int first,
-                                           float sign, float (&c)[N], float (&s)[N]) {
-  if (first >= 0) {
-    load_run<float, N, false>(reinterpret_cast<const char*>(cos_t), row + first, c);
-    load_run<float, N, false>(reinterpret_cast<const char*>(sin_t), row + first, s);
-#pragma unroll
-    for (int j = 0; j < N; ++j) s[j] = s[j] * sign;
+__device__ __forceinline__ void load_turns(const float* cos_t, const float* sin_t, int64_t row, const Item& it,
+                                           float sign, bool interleaved, float (&c)[N], float (&s)[N]) {
+  if constexpr (N == 8) {
+    const int second = interleaved ? it.turn_b : it.turn_a >= 0 ? it.turn_a + 4 : -1;
+    if (it.turn_a >= 0) {
+      load_n<float, 4, false>(reinterpret_cast<const char*>(cos_t + row + it.turn_a), c);
+      load_n<float, 4, false>(reinterpret_cast<const char*>(sin_t + row + it.turn_a), s);
+    }
+    if (second >= 0) {
+      load_n<float, 4, false>(reinterpret_cast<const char*>(cos_t + row + second), c + 4);
+      load_n<float, 4, false>(reinterpret_cast<const char*>(sin_t + row + second), s + 4);
+    }
+  } else if (it.turn_a >= 0) {
+    c[0] = cos_t[row + it.turn_a];
+    s[0] = sin_t[row + it.turn_a];
   }
+#pragma unroll
+  for (int j = 0; j < N; ++j) s[j] = s[j] * sign;
 }
 
 // ---- the rotation -------------------------------------------------------------------------------
@@ -213,14 +266,12 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs p, int64_t 
     const int h0 = group * PER * slots + slot;
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-      const int h = h0 + u * slots;
-      if (h < p.heads && placed) {
-        const int64_t at = row * p.row_stride + h * p.head_stride;
-        load_run<T, N, true>(p.x, at + it.a, x[u]);
-        if (N > 1 || it.two) load_run<T, N, true>(p.x, at + it.b, y[u]);
-      }
+      // (heads too many read the last one again)
+      const int64_t at = row * p.row_stride + min(h0 + u * slots, p.heads - 1) * p.head_stride;
+      load_run<T, N, true>(p.x, at + it.a, x[u]);
+      if (N > 1 || it.two) load_run<T, N, true>(p.x, at + it.b, y[u]);
     }
-    if (placed) load_turns<N>(p.cos_t, p.sin_t, t * p.table_stride, it.turn, p.sign, c, s);
+    if (placed) load_turns<N>(p.cos_t, p.sin_t, t * p.table_stride, it, p.sign, p.l.interleaved, c, s);
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
       const int h = h0 + u * slots;
@@ -228,13 +279,104 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryArgs p, int64_t 
       if (!placed) {
 #pragma unroll
         for (int j = 0; j < N; ++j) x[u][j] = y[u][j] = 0.f;
-      } else if (it.turn >= 0) {
-        turn<N>(x[u], y[u], c, s, p.l.interleaved);
+      } else {
+        turn<N>(x[u], y[u], c, s, it, p.l.interleaved);
       }
       const int64_t at = (row * p.heads + h) * p.l.D;
       store_run<T, N, true>(p.out, at + it.a, x[u]);
       if (N > 1 || it.two) store_run<T, N, true>(p.out, at + it.b, y[u]);
     }
+  }
+}
+
+// The same with one run of N elements a lane, in the order of memory; by halves, a run's partner is in another
+// lane of its head.  Every access covers whole lines, where runs of R / 2 elements would not be ones.
+template <typename T, int N, bool NT>
+__device__ __forceinline__ void load_some(const char* base, int64_t at, float (&v)[N]) {
+  const char* p = base + at * Elem<T>::kBytes;
+  if constexpr (N >= 4) {
+    load_n<T, N, NT>(p, v);
+  } else {
+    static_assert(N == 2, "");
+    v[0] = Elem<T>::load1(p);
+    v[1] = Elem<T>::load1(p + Elem<T>::kBytes);
+  }
+}
+template <typename T, int N, bool NT>
+__device__ __forceinline__ void store_some(char* base, int64_t at, const float (&v)[N]) {
+  char* p = base + at * Elem<T>::kBytes;
+  if constexpr (N >= 4) {
+    store_n<T, N, NT>(p, v);
+  } else if constexpr (std::is_same_v<T, float>) {
+    *reinterpret_cast<float*>(p) = v[0];
+    *reinterpret_cast<float*>(p + 4) = v[1];
+  } else {
+    typedef uint32_t word __attribute__((aligned(2)));
+    *reinterpret_cast<word*>(p) = std::is_same_v<T, f16> ? pack_h2(v[0], v[1]) : pack_b2(v[0], v[1]);
+  }
+}
+
+template <typename T, int N, int PER>
+__global__ __launch_bounds__(kThreads) void rotary_lines_kernel(RotaryArgs p, int64_t row0, uint32_t waves) {
+  const uint32_t wi = blockIdx.x * kWaves + (threadIdx.x >> 6);
+  if (wi >= waves) return;
+  const uint32_t tok = p.per_tok.div(wi);
+  const int group = static_cast<int>(wi - tok * p.per_tok.d);
+  const int64_t row = row0 + tok;
+  const int lane = threadIdx.x & 63, items = p.l.items, slots = kWave / items;
+  const int64_t t = p.pos[row];
+  const bool placed = t >= 0 && t < p.n_pos;
+  // (lanes too many repeat the last head's)
+  const int slot = min(lane / items, slots - 1), i = lane - lane / items * items;
+  const int a = N * i, h0 = group * PER * slots + slot;
+  const bool turned = a < 2 * p.l.half && placed, second = a >= p.l.half;
+  float x[PER][N], c[N], s[N];
+#pragma unroll
+  for (int u = 0; u < PER; ++u)
+    load_some<T, N, true>(p.x, row * p.row_stride + min(h0 + u * slots, p.heads - 1) * p.head_stride + a, x[u]);
+  if (turned) {
+    if (p.l.interleaved) {
+      const int64_t at = t * p.table_stride + a / 2;
+#pragma unroll
+      for (int j = 0; j < N / 2; ++j) {
+        c[j] = p.cos_t[at + j];
+        s[j] = p.sin_t[at + j] * p.sign;
+      }
+    } else {
+      const int64_t at = t * p.table_stride + (second ? a - p.l.half : a);
+      load_some<float, N, false>(reinterpret_cast<const char*>(p.cos_t), at, c);
+      load_some<float, N, false>(reinterpret_cast<const char*>(p.sin_t), at, s);
+#pragma unroll
+      for (int j = 0; j < N; ++j) s[j] = s[j] * (second ? p.sign : -p.sign);
+    }
+  }
+  const int partner = lane + (second ? -1 : 1) * (p.l.half / N);
+#pragma unroll
+  for (int u = 0; u < PER; ++u) {
+    float y[N];
+    if (!p.l.interleaved) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) y[j] = __shfl(x[u][j], partner);
+    }
+    if (!placed) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) x[u][j] = 0.f;
+    } else if (turned) {
+      if (p.l.interleaved) {
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+          const float v = x[u][j] * c[j / 2] - x[u][j + 1] * s[j / 2];
+          x[u][j + 1] = x[u][j + 1] * c[j / 2] + x[u][j] * s[j / 2];
+          x[u][j] = v;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[u][j] = x[u][j] * c[j] + y[j] * s[j];
+      }
+    }
+    const int h = h0 + u * slots;
+    if (h < p.heads && lane < slots * items)
+      store_some<T, N, true>(p.out, (row * p.heads + h) * p.l.D + a, x[u]);
   }
 }
 
@@ -317,15 +459,12 @@ __global__ __launch_bounds__(kThreads) void rope_append_kernel(AppendArgs p, int
     const int h0 = group * PER * slots + slot;
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
-      const int h = h0 + u * slots;
-      if (h < heads && placed) {
-        const int64_t at = (row * heads + h) * D;
-        load_run<T, N, true>(p.qkv, at + it.a, x[u]);
-        if (N > 1 || it.two) load_run<T, N, true>(p.qkv, at + it.b, y[u]);
-      }
+      const int64_t at = (row * heads + min(h0 + u * slots, heads - 1)) * D;
+      load_run<T, N, true>(p.qkv, at + it.a, x[u]);
+      if (N > 1 || it.two) load_run<T, N, true>(p.qkv, at + it.b, y[u]);
     }
     if (placed && p.cos_t != nullptr)
-      load_turns<N>(p.cos_t, p.sin_t, t * p.table_stride, it.turn, 1.f, c, s);
+      load_turns<N>(p.cos_t, p.sin_t, t * p.table_stride, it, 1.f, p.l.interleaved, c, s);
 #pragma unroll
     for (int u = 0; u < PER; ++u) {
       const int h = h0 + u * slots;
@@ -353,7 +492,7 @@ __global__ __launch_bounds__(kThreads) void rope_append_kernel(AppendArgs p, int
             if (N > 1 || it.two) y[u][j] = y[u][j] + dy[j];
           }
         }
-        if (!is_v && it.turn >= 0 && p.cos_t != nullptr) turn<N>(x[u], y[u], c, s, p.l.interleaved);
+        if (!is_v && p.cos_t != nullptr) turn<N>(x[u], y[u], c, s, it, p.l.interleaved);
       }
       if (is_q) {
         const int64_t at = (row * p.NH + h) * D;
@@ -398,8 +537,9 @@ int over_rows(int64_t rows, int64_t per_tok, F&& run) {
   return kOk;
 }
 
-// Wavefront items from which a wavefront takes two groups of heads (the second reuses the token's
-// tables), below which one fills the chip sooner.
+// Wavefront items from which a wavefront takes two groups of heads, or three where they divide a token's (they
+// share the token's place and tables), below which one fills the chip sooner.  MI355X: 8192 tokens of 40 heads
+// both ways 58.5 us with one, 57.7 with two, 58.4 with three; 8192 tokens of 48 heads appended 36.6, 33.8, 33.1.
 constexpr int64_t kTwoFrom = 4096;
 
 // Calls run(tag of <N>, tag of <PER>, groups of a token) for `heads` heads of layout l.
@@ -410,6 +550,8 @@ int with_items(Layout& l, int64_t rows, int heads, F&& run) {
   const int groups = (heads + slots - 1) / slots;
   using std::integral_constant;
   if (!runs) return run(integral_constant<int, 1>{}, integral_constant<int, 1>{}, groups);
+  if (rows * groups >= kTwoFrom && groups % 3 == 0)
+    return run(integral_constant<int, 8>{}, integral_constant<int, 3>{}, groups / 3);
   if (rows * groups >= kTwoFrom)
     return run(integral_constant<int, 8>{}, integral_constant<int, 2>{}, (groups + 1) / 2);
   return run(integral_constant<int, 8>{}, integral_constant<int, 1>{}, groups);
@@ -450,8 +592,9 @@ extern "C" __attribute__((visibility("default"))) int soupk_rotary_tables(
       const double high = std::fmin(std::ceil(pair(beta_slow)), dim - 1.0);
       width = std::fmax(high - low, 0.001);
     }
+    const double decay = 2.0 * std::log(theta) / dim;
     for (int i = 0; i < half; ++i) {
-      double f = std::pow(theta, -2.0 * i / dim);
+      double f = std::exp(-i * decay);
       if (scaling == SOUPK_ROPE_LINEAR) f /= factor;
       if (scaling == SOUPK_ROPE_YARN) {
         const double ramp = std::fmin(std::fmax((i - low) / width, 0.0), 1.0);
@@ -464,19 +607,17 @@ extern "C" __attribute__((visibility("default"))) int soupk_rotary_tables(
   if (seq == 0) return kOk;
   if (bad_ptr(cos, 15) || bad_ptr(sin, 15)) return kInvalid;
   const int n = half % 4 == 0 ? 4 : 1, per = half / n;
-  const int64_t step = std::max<int64_t>(1, std::min<int64_t>(kMaxGrid * kThreads, (int64_t{1} << 31) - 1) / per);
-  for (int64_t p = 0; p < seq; p += step) {
-    const int64_t items = std::min(step, seq - p) * per;
-    auto run = [&](auto kernel) {
-      return launch_kernel(kernel, dim3(static_cast<unsigned>((items + kThreads - 1) / kThreads)),
-                           dim3(kThreads), static_cast<hipStream_t>(stream), turns, cos, sin, gain,
-                           static_cast<uint32_t>(p), static_cast<uint32_t>(items),
-                           FastDiv(static_cast<uint32_t>(per)), half);
-    };
-    const int rc = n == 4 ? run(rotary_tables_kernel<4>) : run(rotary_tables_kernel<1>);
-    if (rc != kOk) return rc;
-  }
-  return kOk;
+  const int ps = seq * per >= kManyThreads ? kPositions : 1;
+  const uint32_t step = kThreads / 16;
+  const int64_t rows = ps == 1 ? seq : (seq + ps * step - 1) / (ps * step) * step, items = rows * per;
+  if (items > kMaxGrid * kThreads - kThreads) return kInvalid;
+  auto run = [&](auto kernel) {
+    return launch_kernel(kernel, dim3(static_cast<unsigned>((items + kThreads - 1) / kThreads)), dim3(kThreads),
+                         static_cast<hipStream_t>(stream), turns, cos, sin, gain, step,
+                         static_cast<uint32_t>(seq), FastDiv(static_cast<uint32_t>(per)), half);
+  };
+  if (ps == 1) return n == 4 ? run(rotary_tables_kernel<4, 1>) : run(rotary_tables_kernel<1, 1>);
+  return n == 4 ? run(rotary_tables_kernel<4, kPositions>) : run(rotary_tables_kernel<1, kPositions>);
 }
 
 extern "C" __attribute__((visibility("default"))) int soupk_rotary(
@@ -496,13 +637,32 @@ extern "C" __attribute__((visibility("default"))) int soupk_rotary(
                inverse ? -1.f : 1.f};
   return with_type(dtype, [&](auto tag) -> int {
     using E = typename decltype(tag)::type;
-    return with_items(a.l, rows, heads, [&](auto n, auto per, int groups) {
+    auto launch = [&](auto kernel, int groups) {
       a.groups = groups;
       a.per_tok = FastDiv(static_cast<uint32_t>(groups));
       return over_rows(rows, groups, [&](int64_t r, uint32_t waves, dim3 grid) {
-        return launch_kernel(rotary_kernel<E, decltype(n)::value, decltype(per)::value>, grid, dim3(kThreads),
-                             static_cast<hipStream_t>(stream), a, r, waves);
+        return launch_kernel(kernel, grid, dim3(kThreads), static_cast<hipStream_t>(stream), a, r, waves);
       });
+    };
+    // Runs in the order of memory, of 16 bytes or of two elements; where pairs of runs are whole lines too, in
+    // those, which need no exchange.
+    constexpr int kBytes = Elem<E>::kBytes, kRun = 16 / kBytes;
+    auto in_lines = [&](int n) {
+      return D % n == 0 && (interleaved ? R % n == 0 : R / 2 % n == 0) && D / n <= kWave;
+    };
+    const bool pairs = kBytes == 2 && D % 16 == 0 && D <= 16 * kWave && R % 16 == 0 &&
+                       (interleaved ? D / 2 * kBytes % 128 == 0
+                                    : R / 2 * kBytes % 128 == 0 && (D - R) / 2 * kBytes % 128 == 0);
+    if (!pairs && (in_lines(kRun) || in_lines(2))) {
+      const int n = in_lines(kRun) ? kRun : 2;
+      a.l.items = D / n;
+      const int slots = kWave / a.l.items, groups = (heads + slots - 1) / slots;
+      if (n == 2) return launch(rotary_lines_kernel<E, 2, 2>, (groups + 1) / 2);
+      if (rows * groups >= kTwoFrom) return launch(rotary_lines_kernel<E, kRun, 2>, (groups + 1) / 2);
+      return launch(rotary_lines_kernel<E, kRun, 1>, groups);
+    }
+    return with_items(a.l, rows, heads, [&](auto n, auto per, int groups) {
+      return launch(rotary_kernel<E, decltype(n)::value, decltype(per)::value>, groups);
     });
   });
 }

@@ -274,6 +274,10 @@ def rotary_tables(seq, rotary_dim, theta=10000.0, scaling=None, inv_freq=None, d
     rotary_dim / 2 frequencies on the host (numbers, or a CPU tensor) in place of theta and scaling.
     rotary_dim: even, at most 256.  The layer's own tables [seq, head_dim] hold every column twice:
     their first half (cos[:, :head_dim // 2]) is this form."""
+    if scaling is None and inv_freq is None and isinstance(device, str) and device == "cuda":
+        done = _ext.host().rotary_tables(seq, rotary_dim, theta, 0, 1.0, 1.0, 32.0, 1.0, 1.0, None, -1)
+        if done is not None:
+            return done
     device = torch.device(device)
     if device.type != "cuda":
         raise ValueError(f"rotary tables are made on a HIP device (got {device}); the soupk kernels "
