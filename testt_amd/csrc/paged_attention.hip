@@ -173,7 +173,13 @@ struct Rows {
 template <typename T, int DP, int NB>
 struct Tile {
   static constexpr int S = DP / 32, DT = DP / 16, R = 16 * NB;
-  static constexpr int kLd = DP + 16;                        // rows in LDS: reads of 16 and 8 bytes free of conflicts
+  // Queries in LDS for 32 rows of a wide head, whose accumulators leave them no registers (with the queries in
+  // registers, 53 others were kept in memory: 5 new tokens of 32 sequences of up to 8192 keys 80.4 us instead of
+  // 69.6, of 8 sequences of up to 4096 25.8 / 20.9).
+  static constexpr bool kQueriesInLds = NB == 2 && (DP == 96 || DP == 128);
+  // Rows in LDS: reads of 16 and 8 bytes free of conflicts with 16 halves between them, and two workgroups a CU
+  // beside the queries with 8.
+  static constexpr int kLd = kQueriesInLds && DP == 128 ? DP + 8 : DP + 16;
   static constexpr int kStrip = 2 * kWaveKeys * kLd;         // halves of a wavefront's strip: K, then V
   // a load instruction takes kPer whole rows, kLanes lanes each (of them D / 8 with pieces of their own)
   static constexpr int kLanes = DP / 8, kPer = kWave / kLanes, kLoads = (kWaveKeys + kPer - 1) / kPer;
@@ -189,6 +195,7 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
   static_assert(TL::kStrip * 2 >= 16 * kSumLd * 4, "");
   __shared__ __align__(16) uint16_t strips[kWaves * TL::kStrip];
   __shared__ float stats[kWaves][2][16 * NB];
+  __shared__ __align__(16) uint16_t q_rows[TL::kQueriesInLds ? R * kLd : 8];
   __shared__ uint32_t sums[kWaves];
   __shared__ uint32_t found[2];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, ql = lane & 15, gr = lane >> 4;
@@ -310,35 +317,10 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
     const int j_end = min(chunks, c_end - item0);
     c = item0 + span;                     // (what is left of it, if anything, is the next workgroup's)
 
-    // ---- the query rows
-    u32x4 qf[NB][S];
-    int limit[NB];                        // keys that this lane's row sees
-#pragma unroll
-    for (int u = 0; u < NB; ++u) {
-      const int rr = tile * R + 16 * u + ql;
-      const bool real = rr < sq.news * p.G;
-      const int i = p.by_group.div(real ? rr : 0), g = (real ? rr : 0) - i * p.G;
-      limit[u] = real ? max(sq.len - sq.news + i + 1, 0) : 0;
-      const uint16_t* row = p.q + static_cast<int64_t>(sq.start + i) * p.q_stride + static_cast<int64_t>(h * p.G + g) * D;
-#pragma unroll
-      for (int s = 0; s < S; ++s) {
-        const int d = 32 * s + 8 * gr;
-        qf[u][s] = real && d < D ? ld16<false>(row + d) : u32x4{0, 0, 0, 0};
-      }
-    }
     // (the first row of the tile sees the fewest keys, the last one the most)
     const int rr0 = tile * R, rr1 = min(rr0 + R, sq.news * p.G) - 1;
     const int seen_all = max(sq.len - sq.news + static_cast<int>(p.by_group.div(rr0)) + 1, 0);
     const int seen_any = max(sq.len - sq.news + static_cast<int>(p.by_group.div(rr1)) + 1, 0);
-    f4 acc[NB][DT];
-    float m_ref[NB], lsum[NB];
-#pragma unroll
-    for (int u = 0; u < NB; ++u) {
-      m_ref[u] = -INFINITY;
-      lsum[u] = 0.f;
-#pragma unroll
-      for (int t = 0; t < DT; ++t) acc[u][t] = f4{0.f, 0.f, 0.f, 0.f};
-    }
 
     const int32_t* pages = p.table + static_cast<int64_t>(b) * p.max_pages;
     // the page of key `lane % 32` of this wavefront's in chunk j (-1: none)
@@ -354,7 +336,7 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
       // (a key without a place reads a row of page 0: masked, and its value zeroed, below)
       const int key = j * kChunk + w * kWaveKeys + (lane & 31);
       const int slot = key - static_cast<int>(p.by_page.div(key)) * p.page_size;
-      const int64_t at = static_cast<int64_t>(max(found_page, 0)) * p.page_stride + slot * D;
+      const int64_t at = static_cast<int64_t>(max(found_page, 0)) * p.page_stride + static_cast<int64_t>(slot) * D;
       const int at_lo = static_cast<int>(at), at_hi = static_cast<int>(at >> 32);
 #pragma unroll
       for (int i = 0; i < TL::kLoads; ++i) {
@@ -365,7 +347,7 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
         r.v[i] = ld<PAST>(reinterpret_cast<const u32x4*>(v_lane + to));
       }
     };
-    if (D < DP) {                         // columns past D meet zeros of Q: no NaN may be there
+    if (D < DP) {                         // columns past D: zeros of K, which meet any of Q
       for (int e = lane; e < kWaveKeys * (DP - D) / 8; e += kWave) {
         const int row = e & (kWaveKeys - 1);
         *reinterpret_cast<u32x4*>(strip + row * kLd + D + 8 * (e / kWaveKeys)) = u32x4{0, 0, 0, 0};
@@ -379,6 +361,37 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
       next = find(j_begin);
       load(r, next, j_begin);
       next = find(j_begin + 1);
+    }
+    // ---- the query rows (after the first keys are on their way)
+    u32x4 qf[NB][S];
+    int limit[NB];                        // keys that this lane's row sees
+    // (rows too many repeat the last one, and columns past D the first, which meet zeros of K)
+    auto query = [&](int u, int s) {
+      const int rr = min(rr0 + 16 * u + ql, rr1), i = p.by_group.div(rr), g = rr - i * p.G, d = 32 * s + 8 * gr;
+      const uint16_t* row = p.q + static_cast<int64_t>(sq.start + i) * p.q_stride + static_cast<int64_t>(h * p.G + g) * D;
+      return ld16<false>(row + (d < D ? d : 0));
+    };
+#pragma unroll
+    for (int u = 0; u < NB; ++u)
+      limit[u] = max(sq.len - sq.news + static_cast<int>(p.by_group.div(min(rr0 + 16 * u + ql, rr1))) + 1, 0);
+    if constexpr (TL::kQueriesInLds) {
+      for (int f = w; f < NB * S; f += kWaves)
+        *reinterpret_cast<u32x4*>(q_rows + (16 * (f / S) + ql) * kLd + 32 * (f % S) + 8 * gr) = query(f / S, f % S);
+      lds_barrier();
+    } else {
+#pragma unroll
+      for (int u = 0; u < NB; ++u)
+#pragma unroll
+        for (int s = 0; s < S; ++s) qf[u][s] = query(u, s);
+    }
+    f4 acc[NB][DT];
+    float m_ref[NB], lsum[NB];
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+      m_ref[u] = -INFINITY;
+      lsum[u] = 0.f;
+#pragma unroll
+      for (int t = 0; t < DT; ++t) acc[u][t] = f4{0.f, 0.f, 0.f, 0.f};
     }
     for (int j = j_begin; j < j_mine; ++j) {
       const int key0 = j * kChunk + w * kWaveKeys;
@@ -409,7 +422,12 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
         for (int n = 0; n < 2; ++n) {
           const u32x4 kf = *reinterpret_cast<const u32x4*>(strip + (16 * n + ql) * kLd + 32 * s + 8 * gr);
 #pragma unroll
-          for (int u = 0; u < NB; ++u) sc[u][n] = Ops<T>::mfma(kf, qf[u][s], sc[u][n]);
+          for (int u = 0; u < NB; ++u) {
+            u32x4 q = qf[u][s];
+            if constexpr (TL::kQueriesInLds)
+              q = *reinterpret_cast<const u32x4*>(q_rows + (16 * u + ql) * kLd + 32 * s + 8 * gr);
+            sc[u][n] = Ops<T>::mfma(kf, q, sc[u][n]);
+          }
         }
       }
       u32x4 pb[NB];
