@@ -99,6 +99,16 @@ def test_long_among_short():
         check(got, q, k, v, table, lengths, None, H)
 
 
+@pytest.mark.parametrize("batch,news,nh,nkv,d", [(100, 1, 8, 4, 64), (64, 1, 8, 8, 128), (70, 3, 8, 4, 32),
+                                                 (300, 1, 4, 2, 16)])
+def test_many_items(batch, news, nh, nkv, d):
+    """More items than workgroups take one each: parts that end one item and begin another."""
+    lengths = [(i * 173) % 640 for i in range(batch)]
+    q, k, v, table, cu = make(lengths, [news] * batch, 32, nh, nkv, d, H, batch)
+    got = attention.paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), *seqs(table, lengths, None if news == 1 else cu))
+    check(got, q, k, v, table, lengths, cu, H)
+
+
 @pytest.mark.parametrize("dtype", [H, B])
 def test_large_scores(dtype):
     """A single key far above the others: its value; scores of hundreds, falling and rising with the position."""

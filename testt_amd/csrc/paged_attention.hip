@@ -237,37 +237,42 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
   } else {
     uint32_t total = 0, all_chunks = 0, all_items = 0;
     if (threadIdx.x == 0) found[0] = p.B;
-    for (int pass = 0; pass < 3; ++pass) {      // the list's sizes; its number of chunks; this part's begin
-      if (pass == 1) cut = cut_of(all_chunks, all_items, p.parts);
-      if (pass == 2) part_of(total);
+    auto look = [&](int q, uint32_t& items, uint32_t& chunks) {
+      items = chunks = 0;
+      if (q >= p.B) return;
+      const Seq s = sequence(p, q);
+      items = static_cast<uint32_t>(tiles_of<R>(s, p.G)) * p.NKV;
+      chunks = chunks_of(s);
+    };
+    uint32_t items, chunks;
+    for (int q = threadIdx.x; q < p.B; q += kThreads) {
+      look(q, items, chunks);
+      all_chunks += items * chunks;
+      all_items += items;
+    }
+    scan_threads(all_chunks, sums, all_chunks);
+    scan_threads(all_items, sums, all_items);
+    cut = cut_of(all_chunks, all_items, p.parts);
+    for (int pass = 0;; ++pass) {
       uint32_t before = 0;
       for (int b0 = 0; b0 < p.B; b0 += kThreads) {
         const int q = b0 + static_cast<int>(threadIdx.x);
-        uint32_t items = 0, chunks = 0;
-        if (q < p.B) {
-          const Seq s = sequence(p, q);
-          items = static_cast<uint32_t>(tiles_of<R>(s, p.G)) * p.NKV;
-          chunks = chunks_of(s);
-        }
+        look(q, items, chunks);
         uint32_t sum;
-        if (pass == 0) {
-          scan_threads(items * chunks, sums, sum);
-          all_chunks += sum;
-          scan_threads(items, sums, sum);
-          all_items += sum;
-        } else {
-          const uint32_t n = items * rounded(chunks, cut.unit);
-          const uint32_t upto = before + scan_threads(n, sums, sum);
-          before += sum;
-          if (pass == 1 && blockIdx.x == 0 && q < p.B) p.first[q] = upto - n;
-          if (pass == 2 && c_begin >= upto - n && c_begin < upto) {
-            found[0] = q;
-            found[1] = upto - n;
-          }
+        const uint32_t n = items * rounded(chunks, cut.unit), upto = before + scan_threads(n, sums, sum);
+        before += sum;
+        if (pass == 0 && blockIdx.x == 0 && q < p.B) p.first[q] = upto - n;
+        if (p.B <= kThreads) total = sum;
+        part_of(total);
+        if (c_begin >= upto - n && c_begin < upto) {
+          found[0] = q;
+          found[1] = upto - n;
         }
       }
-      if (pass == 1) total = before;
+      total = before;
+      if (p.B <= kThreads || pass == 1) break;      // (more sequences than threads: once the total is known)
     }
+    part_of(total);
     if (blockIdx.x == 0 && threadIdx.x == 0) {
       p.first[p.B] = total;
       p.first[p.B + 1] = cut.per;
@@ -431,7 +436,6 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
         }
       }
       u32x4 pb[NB];
-      bool any = false;
 #pragma unroll
       for (int u = 0; u < NB; ++u) {
         sc[u][0] = sc[u][0] * p.scale_log2;
@@ -620,6 +624,54 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedArgs p) {
   *reinterpret_cast<uint32_t*>(p.out + (row * heads + head) * D + col) = Ops<T>::pack(x * inv, y * inv);
 }
 
+// The same where items are many and few of them reach across a workgroup's end: a workgroup joins the item that
+// begins in the part of the main launch's workgroup of its number, if that one did not finish it.
+template <typename T, int R>
+__global__ __launch_bounds__(kThreads) void paged_join_last_kernel(PagedArgs p) {
+  const uint32_t total = p.first[p.B], per = p.first[p.B + 1], unit = p.first[p.B + 2];
+  const uint32_t c0 = blockIdx.x * per, c1 = c0 + per;
+  if (c1 >= total) return;
+  // the sequence of chunk c1 - 1: the last one whose first chunk is not behind it, 64 at a time
+  const int lane = threadIdx.x & 63;
+  int b = 0, n_left = p.B;
+  while (n_left > 1) {
+    const int step = (n_left + kWave - 1) / kWave, at = b + lane * step;
+    const int count = __popcll(__ballot(lane * step < n_left && at < p.B && p.first[at] <= c1 - 1));
+    b += (max(count, 1) - 1) * step;
+    n_left = min(step, p.B - b);
+    if (step == 1) break;
+  }
+  const Seq s = sequence(p, b);
+  const uint32_t chunks = chunks_of(s), tiles = tiles_of<R>(s, p.G), span = rounded(chunks, unit);
+  const uint32_t seq0 = p.first[b], item = (c1 - 1 - seq0) / span, item0 = seq0 + item * span;
+  if (item0 < c0 || item0 + chunks <= c1 || item >= tiles * p.NKV) return;
+  const uint32_t w1 = (item0 + chunks - 1) / per;
+  if (w1 >= static_cast<uint32_t>(p.parts)) return;
+  const int h = item / tiles, tile = item - h * tiles, n = static_cast<int>(w1 - blockIdx.x) + 1, D = p.D;
+  const int rows = min(R, s.news * p.G - tile * R), pairs = D / 2;
+  for (int e = threadIdx.x; e < rows * pairs; e += kThreads) {
+    const int rt = e / pairs, col = 2 * (e - rt * pairs);
+    float x = 0.f, y = 0.f, l = 0.f, m = -INFINITY;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float* src = p.part + (2 * static_cast<int64_t>(blockIdx.x + i) + (i == 0 ? 1 : 0)) * (R * (D + 2));
+      const float mi = src[R * D + rt], li = src[R * D + R + rt];
+      const float2 v = *reinterpret_cast<const float2*>(src + rt * D + col);
+      const float m_new = __builtin_elementwise_maximum(m, mi);
+      const float a = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+      const float f = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - m_new);
+      x = x * a + v.x * f;
+      y = y * a + v.y * f;
+      l = l * a + li * f;
+      m = m_new;
+    }
+    const int rr = tile * R + rt, i = p.by_group.div(rr), g = rr - i * p.G;
+    const float inv = m == -INFINITY ? 0.f : 1.f / l;
+    uint16_t* o = p.out + (static_cast<int64_t>(s.start + i) * p.NKV + h) * p.G * D + g * D + col;
+    *reinterpret_cast<uint32_t*>(o) = Ops<T>::pack(x * inv, y * inv);
+  }
+}
+
 // ---- host ---------------------------------------------------------------------------------------
 
 bool bad_ptr(const void* p, uintptr_t mask) {
@@ -646,7 +698,7 @@ int blocks_of(int64_t rows, int32_t B, int32_t G, int32_t D) {
 
 struct Plan {
   int nb, parts, parts_of_item;
-  bool join;
+  bool join, many;            // something to join; of many items
   int64_t first_bytes, bytes;
 };
 
@@ -660,6 +712,7 @@ bool plan_of(int64_t rows, int32_t B, int32_t G, int32_t NKV, int32_t D, int64_t
   const int64_t list = items * chunks + items;      // (each item's rounding included)
   pl.parts = static_cast<int>(std::max<int64_t>(std::min<int64_t>(list, int64_t{held(pl.nb, D)} * device_cu_count()), 1));
   pl.join = chunks > 1;
+  pl.many = 2 * items > pl.parts;
   pl.parts_of_item = static_cast<int>(std::min<int64_t>(pl.parts / std::max<int64_t>(items, 1), chunks));
   pl.first_bytes = (4 * (int64_t{B} + 3) + 15) / 16 * 16;
   pl.bytes = pl.first_bytes + 2 * int64_t{pl.parts} * R * (D + 2) * 4;
@@ -677,6 +730,7 @@ int launch_paged(const PagedArgs& a, const Plan& pl, hipStream_t s) {
     int rc = NB < 4 && past ? launch_kernel(paged_attention_kernel<T, DP, NB, MIN, NB < 4>, grid, block, s, a)
                             : launch_kernel(paged_attention_kernel<T, DP, NB, MIN, false>, grid, block, s, a);
     if (rc != kOk || !pl.join) return rc;
+    if (pl.many) return launch_kernel(paged_join_last_kernel<T, 16 * NB>, grid, block, s, a);
     const dim3 join(static_cast<unsigned>(a.rows * a.NKV * a.G), static_cast<unsigned>((a.D + kJoinCols - 1) / kJoinCols));
     // (by the parts that a row can have, when every item is one of equals)
     if (pl.parts_of_item > 64) return launch_kernel(paged_join_kernel<T, 16 * NB, 1024>, join, dim3(1024), s, a);
