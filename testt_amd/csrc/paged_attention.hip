@@ -11,6 +11,8 @@
 // them a tile) are the 16 columns of v_mfma_f32_16x16x32 products, and keys its rows:
 //   S^T (32 keys x 16 rows) = K Q^T        A = K rows staged in LDS
 //   O^T (D x 16 rows) += V^T P^T           A = V^T by transpose reads of rows staged in LDS
+// P is rounded to the cache's type, as the operand has to be: to the output's own rounding (a relative error of
+// 0.0017 in bf16, 0.0002 in fp16 over the timed cases) this adds as much again in squares (0.0022, 0.00025).
 // A wavefront is on its own inside a chunk: it owns 32 of the chunk's 128 keys, its own strip of LDS and its
 // own softmax state; the four are merged once, at the end of an item or part.  No barrier is in the
 // loop.  Page numbers are read two chunks ahead and rows one chunk ahead of their use.
@@ -23,6 +25,10 @@
 // begin others.  A workgroup writes what lies whole inside its part; of an item that reaches across an end it
 // leaves the unnormalised sum, its reference value and its weight, two at most, and a second launch
 // joins those in workgroup order: the same bits every time.
+//
+// MI355X: 64 sequences of up to 8192 keys, 8 heads of 128 in bf16 (1.09 GB) 178 us and a join of 4.7: 6.1 TB/s.  A
+// single step is latency: launch, lengths and schedule 2 us, page numbers 0.5, rows 2, a wavefront's 32 keys
+// 1.5, merge 1.4; the join 4 and the gap before it 1.5 (8 sequences of up to 4096 keys 13.4 us in all).
 
 #include <algorithm>
 #include <type_traits>

@@ -16,6 +16,11 @@
 // Only the row that the token is drawn from is read (and the draft's): V elements a sequence.  Two
 // launches: parts of a row are summed by a wavefront each, which finds n for itself (K reads); then one
 // workgroup a sequence picks the part that holds the number and goes through its 1024 columns alone.
+//
+// MI355X, 64 sequences of 8 drafts and 151936 fp32 columns: 18.4 us, of which the sums (63 MB, half the rows
+// refused) 14.5 and the pick 4.0.  One sequence: 4.7 and 3.4, latency (tokens, their probabilities, the row,
+// one after another).  A wavefront's row in flight 512 columns at a time: eight wavefronts a SIMD; 1024 at a
+// time 18.9 us, and 16.5 instead of 15.0 for bf16.
 
 #include <algorithm>
 #include <type_traits>
@@ -109,30 +114,22 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
   const Row r = row_of<T>(a, b, n, refused);
   const int64_t c0 = part * a.part, c1 = min(c0 + a.part, a.V);
   double w = 0.0, p = 0.0;
-  for (int64_t at = c0; at < c1; at += kPart) {
-    constexpr int kSteps = kPart / (8 * kWave);
-    float pv[kSteps][8], qv[kSteps][8];
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      const int64_t c = at + 8 * (kWave * i + lane);
-      if (c + 8 <= c1) {
-        Elem<T>::unpack8(Elem<T>::template load8<false>(r.p + c * E), pv[i]);
-        if (r.q != nullptr) Elem<T>::unpack8(Elem<T>::template load8<false>(r.q + c * E), qv[i]);
-      } else {
-        for (int j = 0; j < 8; ++j) {
-          pv[i][j] = c + j < c1 ? Elem<T>::load1(r.p + (c + j) * E) : 0.f;
-          if (r.q != nullptr) qv[i][j] = c + j < c1 ? Elem<T>::load1(r.q + (c + j) * E) : 0.f;
-        }
+#pragma unroll 1
+  for (int64_t c = c0 + 8 * lane; c < c1; c += 8 * kWave) {
+    float pv[8], qv[8];
+    if (c + 8 <= c1) {
+      Elem<T>::unpack8(Elem<T>::template load8<false>(r.p + c * E), pv);
+      if (r.q != nullptr) Elem<T>::unpack8(Elem<T>::template load8<false>(r.q + c * E), qv);
+    } else {
+      for (int j = 0; j < 8; ++j) {
+        pv[j] = c + j < c1 ? Elem<T>::load1(r.p + (c + j) * E) : 0.f;
+        if (r.q != nullptr) qv[j] = c + j < c1 ? Elem<T>::load1(r.q + (c + j) * E) : 0.f;
       }
     }
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      const int64_t c = at + 8 * (kWave * i + lane);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p += mass(pv[i][j]);
-        w += weight(pv[i][j], r.q != nullptr ? qv[i][j] : 0.f, c + j == r.one);
-      }
+    for (int j = 0; j < 8; ++j) {
+      p += mass(pv[j]);
+      w += weight(pv[j], r.q != nullptr ? qv[j] : 0.f, c + j == r.one);
     }
   }
 #pragma unroll
