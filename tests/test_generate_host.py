@@ -36,6 +36,7 @@ def test_cpu_tensors_are_refused():
     (dict(rotary_dim=258), ValueError, "even"), (dict(rotary_dim=0), ValueError, "even"),
     (dict(theta=1.0), ValueError, "theta"), (dict(theta=float("nan")), ValueError, "theta"),
     (dict(scaling={"rope_type": "other"}), ValueError, "inv_freq"),
+    (dict(scaling="linear"), TypeError, "dict"),
     (dict(scaling={"rope_type": "linear"}), ValueError, "factor"),
     (dict(scaling={"rope_type": "linear", "factor": 0.5}), ValueError, "factor"),
     (dict(scaling={"rope_type": "yarn", "factor": 2.0}), ValueError, "original"),

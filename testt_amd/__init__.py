@@ -10,7 +10,8 @@ functions, autograd.Function signatures and constants):
 - attention.py causal GQA flash attention (head dim 128), forward and backward
 - mlp.py      gate/up GEMM + SwiGLU in fp16, gate/up kept (or recomputed) for backward
 - head.py     fused head + loss + entropy + accuracy + per-row loss, no full logits; log
-              probabilities of given tokens with entropy and top alternatives
+              probabilities of given tokens with entropy and top alternatives; verification of
+              drafted tokens
 - dropout.py  dropout drawn from a counter, with no mask stored
 - embedding.py scaled lookup and its gradient by sorted tokens
 - warmup.py   start/wait hooks (the kernels are prebuilt, nothing compiles at run time)

@@ -14,6 +14,7 @@ head and in either layout (rotary), and the same step as above into a paged key-
 """
 
 import math
+from collections.abc import Mapping
 
 import torch
 from torch.overrides import handle_torch_function, has_torch_function
@@ -304,6 +305,8 @@ def rotary_tables(seq, rotary_dim, theta=10000.0, scaling=None, inv_freq=None, d
         if len(inv_freq) != rotary_dim // 2 or not all(abs(f) <= 1e6 for f in inv_freq):
             raise ValueError(f"inv_freq must hold {rotary_dim // 2} frequencies of at most 1e6 rad")
     elif scaling is not None:
+        if not isinstance(scaling, Mapping):
+            raise TypeError(f"scaling must be None or a dict, got {type(scaling).__name__}")
         kind = scaling.get("rope_type", scaling.get("type"))
         if kind not in _SCALINGS:
             raise ValueError(f"rope scaling must be one of {', '.join(_SCALINGS)}, got {kind!r} (other "
