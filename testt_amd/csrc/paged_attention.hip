@@ -334,18 +334,16 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
     const int seen_any = max(sq.len - sq.news + static_cast<int>(p.by_group.div(rr1)) + 1, 0);
 
     const int32_t* pages = p.table + static_cast<int64_t>(b) * p.max_pages;
-    // the page of key `lane % 32` of this wavefront's in chunk j (-1: none)
-    auto find = [&](int j) {
-      const int key = j * kChunk + w * kWaveKeys + (lane & 31);
-      const int page = key < seen_any ? pages[p.by_page.div(key)] : -1;
-      return page >= 0 && page < p.pages ? page : -1;
-    };
+    // the page of key `lane % 32` of this wavefront's in chunk j (of the last key for those behind it), as it is in
+    // the table: looked at when its rows are loaded, as a wait for it is one for all loads before it
+    auto find = [&](int j) { return pages[p.by_page.div(min(j * kChunk + w * kWaveKeys + (lane & 31), seen_any - 1))]; };
     const uint16_t* const k_lane = p.k + static_cast<int64_t>(h) * p.page_size * D + piece;
     const uint16_t* const v_lane = p.v + static_cast<int64_t>(h) * p.page_size * D + piece;
     auto load = [&](Rows<TL::kLoads>& r, int found_page, int j) {
+      const int key = j * kChunk + w * kWaveKeys + (lane & 31);
+      if (found_page >= p.pages || key >= seen_any) found_page = -1;
       r.ok = static_cast<uint32_t>(__ballot(found_page >= 0));
       // (a key without a place reads a row of page 0: masked, and its value zeroed, below)
-      const int key = j * kChunk + w * kWaveKeys + (lane & 31);
       const int slot = key - static_cast<int>(p.by_page.div(key)) * p.page_size;
       const int64_t at = static_cast<int64_t>(max(found_page, 0)) * p.page_stride + static_cast<int64_t>(slot) * D;
       const int at_lo = static_cast<int>(at), at_hi = static_cast<int>(at >> 32);
@@ -368,13 +366,12 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
     const int j_mine = min(j_end, (seen_any - w * kWaveKeys + kChunk - 1) / kChunk);
     Rows<TL::kLoads> r;
     int next = -1;
-    if (j_begin < j_mine) {
-      next = find(j_begin);
-      load(r, next, j_begin);
-      next = find(j_begin + 1);
-    }
-    // ---- the query rows (after the first keys are on their way)
-    u32x4 qf[NB][S];
+    if (j_begin < j_mine) next = find(j_begin);
+    // ---- the query rows, on their way while the page numbers are
+    // (for LDS, a wavefront loads every fourth piece; pieces too many repeat the last one)
+    constexpr int kParts = (NB * S + kWaves - 1) / kWaves;
+    u32x4 qf[NB][S], q_part[kParts];
+    auto part_at = [&](int i) { return min(w + i * kWaves, NB * S - 1); };
     int limit[NB];                        // keys that this lane's row sees
     // (rows too many repeat the last one, and columns past D the first, which meet zeros of K)
     auto query = [&](int u, int s) {
@@ -386,14 +383,25 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
     for (int u = 0; u < NB; ++u)
       limit[u] = max(sq.len - sq.news + static_cast<int>(p.by_group.div(min(rr0 + 16 * u + ql, rr1))) + 1, 0);
     if constexpr (TL::kQueriesInLds) {
-      for (int f = w; f < NB * S; f += kWaves)
-        *reinterpret_cast<u32x4*>(q_rows + (16 * (f / S) + ql) * kLd + 32 * (f % S) + 8 * gr) = query(f / S, f % S);
-      lds_barrier();
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) q_part[i] = query(part_at(i) / S, part_at(i) % S);
     } else {
 #pragma unroll
       for (int u = 0; u < NB; ++u)
 #pragma unroll
         for (int s = 0; s < S; ++s) qf[u][s] = query(u, s);
+    }
+    if (j_begin < j_mine) {
+      load(r, next, j_begin);
+      if (j_begin + 1 < j_mine) next = find(j_begin + 1);
+    }
+    if constexpr (TL::kQueriesInLds) {
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) {
+        const int f = part_at(i);
+        *reinterpret_cast<u32x4*>(q_rows + (16 * (f / S) + ql) * kLd + 32 * (f % S) + 8 * gr) = q_part[i];
+      }
+      lds_barrier();
     }
     f4 acc[NB][DT];
     float m_ref[NB], lsum[NB];
@@ -403,6 +411,13 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
       lsum[u] = 0.f;
 #pragma unroll
       for (int t = 0; t < DT; ++t) acc[u][t] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    // (wait for the queries here: the loop would wait for them, and for the rows that it loads, in every step)
+    if constexpr (!TL::kQueriesInLds) {
+#pragma unroll
+      for (int u = 0; u < NB; ++u)
+#pragma unroll
+        for (int s = 0; s < S; ++s) __asm__ volatile("" : "+v"(qf[u][s]));
     }
     for (int j = j_begin; j < j_mine; ++j) {
       const int key0 = j * kChunk + w * kWaveKeys;
@@ -421,7 +436,7 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
       // the next chunk's rows, and the page numbers of the one after it
       if (j + 1 < j_mine) {
         load(r, next, j + 1);
-        next = find(j + 2);
+        if (j + 2 < j_mine) next = find(j + 2);
       }
       __asm__ volatile("" ::: "memory");
       f4 sc[NB][2];
