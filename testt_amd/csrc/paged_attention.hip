@@ -122,13 +122,20 @@ __device__ __forceinline__ float column_sum(float v) {
 }
 
 // Inclusive sum over the wavefront's lanes, and over the workgroup's threads, in order.
+// (Of lanes by DPP: within rows of 16 from 1, 2, 4 and 8 lanes before, then the last lane of a row for the next
+// one and of the first half for the second.)
 __device__ __forceinline__ uint32_t scan_lanes(uint32_t v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const uint32_t o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
+  auto add = [&](auto ctrl, auto rows) {
+    v += __builtin_amdgcn_update_dpp(0, v, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+  };
+  using std::integral_constant;
+  constexpr integral_constant<int, 0xf> all;
+  add(integral_constant<int, 0x111>{}, all);
+  add(integral_constant<int, 0x112>{}, all);
+  add(integral_constant<int, 0x114>{}, all);
+  add(integral_constant<int, 0x118>{}, all);
+  add(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});
+  add(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
   return v;
 }
 __device__ __forceinline__ uint32_t scan_threads(uint32_t v, uint32_t* sums, uint32_t& total) {
@@ -365,7 +372,7 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
     // (chunks in which this wavefront has keys that the tile sees)
     const int j_mine = min(j_end, (seen_any - w * kWaveKeys + kChunk - 1) / kChunk);
     Rows<TL::kLoads> r;
-    int next = -1;
+    int next;                             // (not set before: that would wait for the last item's stores)
     if (j_begin < j_mine) next = find(j_begin);
     // ---- the query rows, on their way while the page numbers are
     // (for LDS, a wavefront loads every fourth piece; pieces too many repeat the last one)
