@@ -83,7 +83,7 @@ struct PagedArgs {
   int64_t rows, q_stride, max_pages, pages, page_stride;
   int B, NKV, G, D, page_size, parts;
   float scale_log2;
-  FastDiv by_page, by_group;
+  FastDiv by_page, by_group, by_quad;
 };
 
 // Sequence b's rows and length; an impossible one has no rows.
@@ -173,7 +173,9 @@ __device__ __forceinline__ Cut cut_of(uint32_t chunks, uint32_t items, uint32_t 
   }
   return {max((chunks + parts - 1) / parts, 1u), 1};
 }
-__device__ __forceinline__ uint32_t rounded(uint32_t n, uint32_t unit) { return (n + unit - 1) / unit * unit; }
+__device__ __forceinline__ uint32_t rounded(uint32_t n, uint32_t unit) {
+  return unit == 1 ? n : (n + unit - 1) / unit * unit;
+}
 
 // A wavefront's 32 keys of a chunk, as loaded: 16-byte pieces of whole rows (a cache line at once: in the
 // operands' own order an instruction would touch half a line of 16 rows), and which keys have a place.
@@ -204,8 +206,9 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
   using TL = Tile<T, DP, NB>;
   constexpr int S = TL::S, DT = TL::DT, R = TL::R, kLd = TL::kLd;
   constexpr int kSumLd = DP + 4;          // floats of a row of the merge
-  // (the merge of the wavefronts takes the strips over)
-  static_assert(TL::kStrip * 2 >= 16 * kSumLd * 4, "");
+  // (the merge of the wavefronts takes the strips over, kMerged row blocks at a time)
+  constexpr int kMerged = NB < 2 ? NB : 2;
+  static_assert(TL::kStrip * 2 >= 16 * kMerged * kSumLd * 4 && NB % kMerged == 0, "");
   __shared__ __align__(16) uint16_t strips[kWaves * TL::kStrip];
   __shared__ float stats[kWaves][2][16 * NB];
   __shared__ __align__(16) uint16_t q_rows[TL::kQueriesInLds ? R * kLd : 8];
@@ -314,8 +317,8 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
     return kWaveKeys % TL::kPer ? min(row, kWaveKeys - 1) : row;
   };
   // of the sums of the merge: this thread's columns, first row and rows at a time
-  const int pairs = D / 2, sum_row = threadIdx.x / pairs, sum_col = 2 * (threadIdx.x - sum_row * pairs);
-  const int sum_rows = kThreads / pairs;
+  const int sum_row = p.by_quad.div(threadIdx.x), sum_col = 4 * (threadIdx.x - sum_row * p.by_quad.d);
+  const int sum_rows = p.by_quad.div(kThreads);
   uint32_t c = c_begin;
   while (c < c_end && b < p.B) {
     const Seq sq = p.B <= kWave ? Seq{__builtin_amdgcn_readlane(lane_seq.start, b), __builtin_amdgcn_readlane(lane_seq.news, b),
@@ -329,7 +332,7 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
       continue;
     }
     const uint32_t item = (c - seq0) / span;
-    const int h = item / tiles, tile = item - h * tiles;
+    const int h = tiles == 1 ? item : item / tiles, tile = item - h * tiles;
     const uint32_t item0 = seq0 + item * span;
     const int j_begin = c - item0;
     const int j_end = min(chunks, c_end - item0);
@@ -526,43 +529,45 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
     float* const part = p.part + (2 * static_cast<int64_t>(blockIdx.x) + (j_begin == 0 ? 1 : 0)) * (R * (D + 2));
     float* const mine = reinterpret_cast<float*>(strip);
 #pragma unroll
-    for (int u = 0; u < NB; ++u) {
-      if (16 * u >= real_rows) break;
+    for (int u0 = 0; u0 < NB; u0 += kMerged) {
+      if (16 * u0 >= real_rows) break;
       lds_barrier();                      // (stats are written; the strips' last readers are done)
-      if (16 * u + ql < real_rows) {
+#pragma unroll
+      for (int u = u0; u < u0 + kMerged; ++u) {
+        if (16 * u + ql >= real_rows) break;
         float m_all = stats[0][0][16 * u + ql];
 #pragma unroll
         for (int i = 1; i < kWaves; ++i) m_all = fmaxf(m_all, stats[i][0][16 * u + ql]);
         const float f = m_ref[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_ref[u] - m_all);
+        if (gr == 0) stats[w][1][16 * u + ql] = lsum[u] * f;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
-          *reinterpret_cast<f4*>(mine + ql * kSumLd + 16 * t + 4 * gr) = acc[u][t] * f;
+          *reinterpret_cast<f4*>(mine + (16 * (u - u0) + ql) * kSumLd + 16 * t + 4 * gr) = acc[u][t] * f;
       }
       lds_barrier();
-      // a thread: two neighbouring columns of a row
-      for (int row = sum_row; row < 16 && sum_row < sum_rows; row += sum_rows) {
-        const int rt = 16 * u + row;
+      // a thread: four neighbouring columns of a row
+      for (int row = sum_row; row < 16 * kMerged && sum_row < sum_rows; row += sum_rows) {
+        const int rt = 16 * u0 + row;
         if (rt >= real_rows) break;
-        float x = 0.f, y = 0.f, l = 0.f, m = stats[0][0][rt];
-#pragma unroll
-        for (int i = 1; i < kWaves; ++i) m = fmaxf(m, stats[i][0][rt]);
+        f4 x = f4{0.f, 0.f, 0.f, 0.f};
+        float l = 0.f;
 #pragma unroll
         for (int i = 0; i < kWaves; ++i) {
-          const float2 v = *reinterpret_cast<const float2*>(
-              reinterpret_cast<const float*>(strips + i * TL::kStrip) + row * kSumLd + sum_col);
-          x += v.x;
-          y += v.y;
-          const float mi = stats[i][0][rt];
-          l += mi == -INFINITY ? 0.f : stats[i][1][rt] * __builtin_amdgcn_exp2f(mi - m);
+          x = x + *reinterpret_cast<const f4*>(reinterpret_cast<const float*>(strips + i * TL::kStrip) + row * kSumLd +
+                                               sum_col);
+          l += stats[i][1][rt];
         }
         if (complete) {
           const int rr = tile * R + rt, i = p.by_group.div(rr), g = rr - i * p.G;
-          const float inv = m == -INFINITY ? 0.f : 1.f / l;
+          const float inv = l == 0.f ? 0.f : 1.f / l;       // (no key: no weight)
           uint16_t* o = p.out + (static_cast<int64_t>(sq.start + i) * p.NKV + h) * p.G * D + g * D + sum_col;
-          *reinterpret_cast<uint32_t*>(o) = Ops<T>::pack(x * inv, y * inv);
+          *reinterpret_cast<u32x2_a2*>(o) = u32x2{Ops<T>::pack(x[0] * inv, x[1] * inv), Ops<T>::pack(x[2] * inv, x[3] * inv)};
         } else {
-          *reinterpret_cast<float2*>(part + rt * D + sum_col) = float2{x, y};
+          *reinterpret_cast<f4*>(part + rt * D + sum_col) = x;
           if (sum_col == 0) {
+            float m = stats[0][0][rt];
+#pragma unroll
+            for (int i = 1; i < kWaves; ++i) m = fmaxf(m, stats[i][0][rt]);
             part[R * D + rt] = m;
             part[R * D + R + rt] = l;
           }
@@ -815,7 +820,7 @@ extern "C" __attribute__((visibility("default"))) int soupk_paged_attention(
               static_cast<uint32_t*>(workspace),
               reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.first_bytes), rows, q_stride,
               max_pages, n_pages, page_stride, B, NKV, NH / NKV, D, page_size, pl.parts, scale * kLog2e,
-              FastDiv(static_cast<uint32_t>(page_size)), FastDiv(static_cast<uint32_t>(NH / NKV))};
+              FastDiv(static_cast<uint32_t>(page_size)), FastDiv(static_cast<uint32_t>(NH / NKV)), FastDiv(static_cast<uint32_t>(D / 4))};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return with_type(dtype, [&](auto tag) -> int {
     using E = typename decltype(tag)::type;
