@@ -82,6 +82,7 @@ struct PagedArgs {
   float* part;                // two of a workgroup: rows x D sums, rows reference values, rows weights
   int64_t rows, q_stride, max_pages, pages, page_stride;
   int B, NKV, G, D, page_size, parts;
+  bool tiled;                 // more than one row tile a sequence
   float scale_log2;
   FastDiv by_page, by_group, by_quad;
 };
@@ -188,27 +189,25 @@ struct Rows {
 template <typename T, int DP, int NB>
 struct Tile {
   static constexpr int S = DP / 32, DT = DP / 16, R = 16 * NB;
-  // Queries in LDS for 32 rows of a wide head, whose accumulators leave them no registers (with the queries in
-  // registers, 53 others were kept in memory: 5 new tokens of 32 sequences of up to 8192 keys 80.4 us instead of
-  // 69.6, of 8 sequences of up to 4096 25.8 / 20.9).
-  static constexpr bool kQueriesInLds = NB == 2 && (DP == 96 || DP == 128);
+  // Queries in LDS for 32 rows of a wide head, whose accumulators leave them no registers (in registers, 5 new
+  // tokens of 32 sequences of up to 8192 keys took 71.7 us instead of 60.5, of 8 sequences of up to 4096 17.9 / 16.5).
+  static constexpr bool kQueriesInLds = NB == 2 && DP == 128;
   // Rows in LDS: reads of 16 and 8 bytes free of conflicts with 16 halves between them, and two workgroups a CU
   // beside the queries with 8.
-  static constexpr int kLd = kQueriesInLds && DP == 128 ? DP + 8 : DP + 16;
+  static constexpr int kLd = kQueriesInLds ? DP + 8 : DP + 16;
   static constexpr int kStrip = 2 * kWaveKeys * kLd;         // halves of a wavefront's strip: K, then V
   // a load instruction takes kPer whole rows, kLanes lanes each (of them D / 8 with pieces of their own)
   static constexpr int kLanes = DP / 8, kPer = kWave / kLanes, kLoads = (kWaveKeys + kPer - 1) / kPer;
 };
 
 // PAST: keys and values are read past the caches.
-template <typename T, int DP, int NB, int MIN, bool PAST>
-__global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArgs p) {
+template <typename T, int DP, int NB, bool PAST>
+__global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_kernel(PagedArgs p) {
   using TL = Tile<T, DP, NB>;
   constexpr int S = TL::S, DT = TL::DT, R = TL::R, kLd = TL::kLd;
   constexpr int kSumLd = DP + 4;          // floats of a row of the merge
-  // (the merge of the wavefronts takes the strips over, kMerged row blocks at a time)
-  constexpr int kMerged = NB < 2 ? NB : 2;
-  static_assert(TL::kStrip * 2 >= 16 * kMerged * kSumLd * 4 && NB % kMerged == 0, "");
+  // (the merge of the wavefronts takes the strips over)
+  static_assert(TL::kStrip * 2 >= R * kSumLd * 4, "");
   __shared__ __align__(16) uint16_t strips[kWaves * TL::kStrip];
   __shared__ float stats[kWaves][2][16 * NB];
   __shared__ __align__(16) uint16_t q_rows[TL::kQueriesInLds ? R * kLd : 8];
@@ -221,8 +220,15 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
   Cut cut;
   uint32_t c_begin, c_end, seq0 = 0;
   int b = p.B;
+  // (Workgroups go round the eight XCDs.  Row tiles of a sequence, which stand next to each other in the list and
+  // read the same keys, go to one of them: 8 sequences' 64 new tokens of 32 heads over 4096 keys 83 us instead of
+  // 157.  Items that are cut for themselves are many parts apart: there it cost more than it gave.)
+  uint32_t me = blockIdx.x;
   auto part_of = [&](uint32_t total) {
-    c_begin = min(blockIdx.x * cut.per, total);
+    const uint32_t used = p.tiled && cut.unit == 1 ? (total + cut.per - 1) / cut.per : 0;
+    const uint32_t xcd = blockIdx.x & 7;
+    me = blockIdx.x < used ? xcd * (used >> 3) + min(xcd, used & 7) + (blockIdx.x >> 3) : blockIdx.x;
+    c_begin = min(me * cut.per, total);
     c_end = min(c_begin + cut.per, total);
   };
   Seq lane_seq{0, 0, 0};          // (up to 64 sequences: each lane has one)
@@ -526,51 +532,45 @@ __global__ __launch_bounds__(kThreads, MIN) void paged_attention_kernel(PagedArg
       }
     }
     const bool complete = j_begin == 0 && j_end == static_cast<int>(chunks);
-    float* const part = p.part + (2 * static_cast<int64_t>(blockIdx.x) + (j_begin == 0 ? 1 : 0)) * (R * (D + 2));
+    float* const part = p.part + (2 * static_cast<int64_t>(me) + (j_begin == 0 ? 1 : 0)) * (R * (D + 2));
     float* const mine = reinterpret_cast<float*>(strip);
+    lds_barrier();                      // (stats are written; the strips' last readers are done)
 #pragma unroll
-    for (int u0 = 0; u0 < NB; u0 += kMerged) {
-      if (16 * u0 >= real_rows) break;
-      lds_barrier();                      // (stats are written; the strips' last readers are done)
+    for (int u = 0; u < NB; ++u) {
+      if (16 * u + ql >= real_rows) break;
+      float m_all = stats[0][0][16 * u + ql];
 #pragma unroll
-      for (int u = u0; u < u0 + kMerged; ++u) {
-        if (16 * u + ql >= real_rows) break;
-        float m_all = stats[0][0][16 * u + ql];
+      for (int i = 1; i < kWaves; ++i) m_all = fmaxf(m_all, stats[i][0][16 * u + ql]);
+      const float f = m_ref[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_ref[u] - m_all);
+      if (gr == 0) stats[w][1][16 * u + ql] = lsum[u] * f;
 #pragma unroll
-        for (int i = 1; i < kWaves; ++i) m_all = fmaxf(m_all, stats[i][0][16 * u + ql]);
-        const float f = m_ref[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_ref[u] - m_all);
-        if (gr == 0) stats[w][1][16 * u + ql] = lsum[u] * f;
+      for (int t = 0; t < DT; ++t)
+        *reinterpret_cast<f4*>(mine + (16 * u + ql) * kSumLd + 16 * t + 4 * gr) = acc[u][t] * f;
+    }
+    lds_barrier();
+    // a thread: four neighbouring columns of a row
+    for (int rt = sum_row; rt < real_rows && sum_row < sum_rows; rt += sum_rows) {
+      f4 x = f4{0.f, 0.f, 0.f, 0.f};
+      float l = 0.f;
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
-          *reinterpret_cast<f4*>(mine + (16 * (u - u0) + ql) * kSumLd + 16 * t + 4 * gr) = acc[u][t] * f;
+      for (int i = 0; i < kWaves; ++i) {
+        x = x + *reinterpret_cast<const f4*>(reinterpret_cast<const float*>(strips + i * TL::kStrip) + rt * kSumLd +
+                                             sum_col);
+        l += stats[i][1][rt];
       }
-      lds_barrier();
-      // a thread: four neighbouring columns of a row
-      for (int row = sum_row; row < 16 * kMerged && sum_row < sum_rows; row += sum_rows) {
-        const int rt = 16 * u0 + row;
-        if (rt >= real_rows) break;
-        f4 x = f4{0.f, 0.f, 0.f, 0.f};
-        float l = 0.f;
+      if (complete) {
+        const int rr = tile * R + rt, i = p.by_group.div(rr), g = rr - i * p.G;
+        const float inv = l == 0.f ? 0.f : 1.f / l;       // (no key: no weight)
+        uint16_t* o = p.out + (static_cast<int64_t>(sq.start + i) * p.NKV + h) * p.G * D + g * D + sum_col;
+        *reinterpret_cast<u32x2_a2*>(o) = u32x2{Ops<T>::pack(x[0] * inv, x[1] * inv), Ops<T>::pack(x[2] * inv, x[3] * inv)};
+      } else {
+        *reinterpret_cast<f4*>(part + rt * D + sum_col) = x;
+        if (sum_col == 0) {
+          float m = stats[0][0][rt];
 #pragma unroll
-        for (int i = 0; i < kWaves; ++i) {
-          x = x + *reinterpret_cast<const f4*>(reinterpret_cast<const float*>(strips + i * TL::kStrip) + row * kSumLd +
-                                               sum_col);
-          l += stats[i][1][rt];
-        }
-        if (complete) {
-          const int rr = tile * R + rt, i = p.by_group.div(rr), g = rr - i * p.G;
-          const float inv = l == 0.f ? 0.f : 1.f / l;       // (no key: no weight)
-          uint16_t* o = p.out + (static_cast<int64_t>(sq.start + i) * p.NKV + h) * p.G * D + g * D + sum_col;
-          *reinterpret_cast<u32x2_a2*>(o) = u32x2{Ops<T>::pack(x[0] * inv, x[1] * inv), Ops<T>::pack(x[2] * inv, x[3] * inv)};
-        } else {
-          *reinterpret_cast<f4*>(part + rt * D + sum_col) = x;
-          if (sum_col == 0) {
-            float m = stats[0][0][rt];
-#pragma unroll
-            for (int i = 1; i < kWaves; ++i) m = fmaxf(m, stats[i][0][rt]);
-            part[R * D + rt] = m;
-            part[R * D + R + rt] = l;
-          }
+          for (int i = 1; i < kWaves; ++i) m = fmaxf(m, stats[i][0][rt]);
+          part[R * D + rt] = m;
+          part[R * D + R + rt] = l;
         }
       }
     }
@@ -712,39 +712,39 @@ bool bad_ptr(const void* p, uintptr_t mask) {
 }
 
 // Workgroups that a CU holds, and that the list is cut for (more of them would wait for a place and begin
-// anew): by their LDS two, and one where registers (64 rows) or LDS (heads over 128) allow no more.
-int held(int nb, int32_t D) { return nb == 4 || D > 128 ? 1 : 2; }
+// anew): by their LDS two, and one of heads over 128.
+int held(int32_t D) { return D > 128 ? 1 : 2; }
 // Bytes of keys and values that the block tables can hold from which they are read past the caches: what the
-// Infinity Cache (256 MB) does not keep for a next call.  MI355X, past / through the caches: 64 sequences of
-// up to 8192 keys, 8 heads of 128, 198 / 216 us; 16 of up to 4096, 4 of 256, 49.9 / 53.5; within it,
-// 16 of 4096, 4 of 96, 26.6 / 24.4; 8 of 4096, 16 of 64, 22.8 / 21.8.
-constexpr int64_t kPastFrom = int64_t{256} << 20;
+// Infinity Cache (256 MB, other tensors in it too) does not keep for a next call.  MI355X, past / through the caches:
+// 64 sequences of up to 8192 keys, 8 heads of 128 (1 GB) 172 / 192 us; 14 of up to 4096, 4 of 256 (224 MB) 32.0 / 34.5;
+// 12 of 4096, 16 of 64 (192 MB) 26.3 / 26.8; 10 of them (160 MB) 23.0 / 22.7; 8 (128 MB) 19.4 / 18.6; 16 of 4096, 4 of 96
+// (96 MB) 21.5 / 20.2.  Not where several row tiles of a sequence read the same keys (16 sequences' 16 tokens of 32
+// heads over 8192 keys 120 instead of 114).
+constexpr int64_t kPastFrom = int64_t{176} << 20;
 constexpr int64_t kMostKeys = int64_t{1} << 30;
 
-// Row blocks of 16 a tile: what a sequence's rows fill on average.
-int blocks_of(int64_t rows, int32_t B, int32_t G, int32_t D) {
-  const int64_t of_seq = B > 0 ? (rows * G + B - 1) / B : 0;
-  if (of_seq <= 16) return 1;
-  if (of_seq <= 32 || D > 128) return 2;
-  return 4;
-}
+// Row blocks of 16 a tile: what a sequence's rows fill on average, two at most.  (Four, whose sums leave a CU one
+// workgroup: 8 sequences of up to 4096 keys with 54 rows 22.0 us instead of 18.4, 2 x 512 tokens of 12 heads over 2048
+// keys 59 / 49, 8 x 64 of 32 heads over 4096 78 / 83.)
+int blocks_of(int64_t rows, int32_t B, int32_t G) { return B > 0 && rows * G > int64_t{16} * B ? 2 : 1; }
 
 struct Plan {
   int nb, parts, parts_of_item;
-  bool join, many;            // something to join; of many items
+  bool join, many, tiled;     // something to join; of many items; of several of a sequence's rows
   int64_t first_bytes, bytes;
 };
 
 // false: more chunks than 32 bits count.
 bool plan_of(int64_t rows, int32_t B, int32_t G, int32_t NKV, int32_t D, int64_t most_keys, Plan& pl) {
-  pl.nb = blocks_of(rows, B, G, D);
+  pl.nb = blocks_of(rows, B, G);
   const int R = 16 * pl.nb;
   const int64_t chunks = std::max<int64_t>((most_keys + kChunk - 1) / kChunk, 1);
   const int64_t items = (rows * G / R + B) * NKV;
   if (items > 0 && chunks > ((int64_t{1} << 31) - 1) / items) return false;
   const int64_t list = items * chunks + items;      // (each item's rounding included)
-  pl.parts = static_cast<int>(std::max<int64_t>(std::min<int64_t>(list, int64_t{held(pl.nb, D)} * device_cu_count()), 1));
+  pl.parts = static_cast<int>(std::max<int64_t>(std::min<int64_t>(list, int64_t{held(D)} * device_cu_count()), 1));
   pl.join = chunks > 1;
+  pl.tiled = rows * G > int64_t{R} * B;
   pl.many = 2 * items > pl.parts;
   pl.parts_of_item = static_cast<int>(std::min<int64_t>(pl.parts / std::max<int64_t>(items, 1), chunks));
   pl.first_bytes = (4 * (int64_t{B} + 3) + 15) / 16 * 16;
@@ -754,14 +754,12 @@ bool plan_of(int64_t rows, int32_t B, int32_t G, int32_t NKV, int32_t D, int64_t
 
 template <typename T, int DP>
 int launch_paged(const PagedArgs& a, const Plan& pl, hipStream_t s) {
-  const bool past = a.max_pages * a.page_size * a.B > kPastFrom / (int64_t{4} * a.NKV * a.D);
+  const bool past = !pl.tiled && a.max_pages * a.page_size * a.B > kPastFrom / (int64_t{4} * a.NKV * a.D);
   const dim3 grid(pl.parts), block(kThreads);
-  auto run = [&](auto nb, auto min_waves) -> int {
+  auto run = [&](auto nb) -> int {
     constexpr int NB = decltype(nb)::value;
-    constexpr int MIN = decltype(min_waves)::value;
-    // (64 rows: a prompt's part, whose tiles read the same keys one after another)
-    int rc = NB < 4 && past ? launch_kernel(paged_attention_kernel<T, DP, NB, MIN, NB < 4>, grid, block, s, a)
-                            : launch_kernel(paged_attention_kernel<T, DP, NB, MIN, false>, grid, block, s, a);
+    const int rc = past ? launch_kernel(paged_attention_kernel<T, DP, NB, true>, grid, block, s, a)
+                        : launch_kernel(paged_attention_kernel<T, DP, NB, false>, grid, block, s, a);
     if (rc != kOk || !pl.join) return rc;
     if (pl.many) return launch_kernel(paged_join_last_kernel<T, 16 * NB>, grid, block, s, a);
     const dim3 join(static_cast<unsigned>(a.rows * a.NKV * a.G), static_cast<unsigned>((a.D + kJoinCols - 1) / kJoinCols));
@@ -771,10 +769,8 @@ int launch_paged(const PagedArgs& a, const Plan& pl, hipStream_t s) {
     return launch_kernel(paged_join_kernel<T, 16 * NB, 64>, join, dim3(64), s, a);
   };
   using std::integral_constant;
-  if (pl.nb == 1) return run(integral_constant<int, 1>{}, integral_constant<int, DP <= 128 ? 2 : 1>{});
-  if (pl.nb == 2) return run(integral_constant<int, 2>{}, integral_constant<int, DP <= 128 ? 2 : 1>{});
-  if constexpr (DP <= 128) return run(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-  else return kInvalid;
+  if (pl.nb == 1) return run(integral_constant<int, 1>{});
+  return run(integral_constant<int, 2>{});
 }
 
 }  // namespace
@@ -819,7 +815,7 @@ extern "C" __attribute__((visibility("default"))) int soupk_paged_attention(
               static_cast<const uint16_t*>(v_pages), block_table, lengths, cu, static_cast<uint16_t*>(out),
               static_cast<uint32_t*>(workspace),
               reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.first_bytes), rows, q_stride,
-              max_pages, n_pages, page_stride, B, NKV, NH / NKV, D, page_size, pl.parts, scale * kLog2e,
+              max_pages, n_pages, page_stride, B, NKV, NH / NKV, D, page_size, pl.parts, pl.tiled, scale * kLog2e,
               FastDiv(static_cast<uint32_t>(page_size)), FastDiv(static_cast<uint32_t>(NH / NKV)), FastDiv(static_cast<uint32_t>(D / 4))};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return with_type(dtype, [&](auto tag) -> int {
