@@ -100,6 +100,26 @@ __device__ __forceinline__ double weight(float pv, float qv, bool one) {
   return one || w < 0.0 ? 0.0 : w;
 }
 
+// v of another lane, by DPP (0 in rows of 16 outside ROWS, and where there is no such lane).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double v) {
+  const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits), CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+// Inclusive prefix sum over the wavefront's lanes: within rows of 16 from 1, 2, 4 and 8 lanes before, then the last
+// lane of a row for the next one and of the first half for the second.
+__device__ __forceinline__ double scan_lanes(double v) {
+  v += moved<0x111, 0xf>(v);
+  v += moved<0x112, 0xf>(v);
+  v += moved<0x114, 0xf>(v);
+  v += moved<0x118, 0xf>(v);
+  v += moved<0x142, 0xa>(v);
+  v += moved<0x143, 0xc>(v);
+  return v;
+}
+
 // A wavefront a part.  (One of a workgroup's finding n for all: 16.6 to 19.5 us instead of 16.6 for 64 bf16
 // rows, with 4 to 16 wavefronts.)
 template <typename T>
@@ -132,12 +152,9 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
       w += weight(pv[j], r.q != nullptr ? qv[j] : 0.f, c + j == r.one);
     }
   }
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    w += __shfl_xor(w, d);
-    p += __shfl_xor(p, d);
-  }
-  if (lane == 0) {
+  w = scan_lanes(w);
+  p = scan_lanes(p);
+  if (lane == kWave - 1) {
     double* out = a.sums + 2 * (static_cast<int64_t>(b) * a.parts + part);
     out[0] = w;
     out[1] = p;
@@ -148,14 +165,7 @@ __global__ __launch_bounds__(kThreads) void verify_sums_kernel(VerifyArgs a) {
 // Inclusive prefix sum over the workgroup's threads; `before`: the sum of the threads before, `all`: of all.
 __device__ __forceinline__ double scan_threads(double v, double* scratch, double& before, double& all) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  double x = v;
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const double o = __shfl_up(x, d);
-    if (lane >= d) x += o;
-  }
-  double up = __shfl_up(x, 1);
-  if (lane == 0) up = 0.0;
+  const double x = scan_lanes(v), up = moved<0x138, 0xf>(x);
   __syncthreads();
   if (lane == 63) scratch[w] = x;
   __syncthreads();
