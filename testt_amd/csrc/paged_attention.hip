@@ -26,9 +26,9 @@
 // leaves the unnormalised sum, its reference value and its weight, two at most, and a second launch
 // joins those in workgroup order: the same bits every time.
 //
-// MI355X: 64 sequences of up to 8192 keys, 8 heads of 128 in bf16 (1.09 GB) 178 us and a join of 4.7: 6.1 TB/s.  A
-// single step is latency: launch, lengths and schedule 2 us, page numbers 0.5, rows 2, a wavefront's 32 keys
-// 1.5, merge 1.4; the join 4 and the gap before it 1.5 (8 sequences of up to 4096 keys 13.4 us in all).
+// MI355X: 64 sequences of up to 8192 keys, 8 heads of 128 in bf16 (1.09 GB) 168 us and a join of 4.7: 6.5 TB/s.  A
+// single step is latency: lengths and schedule 1.2 us, page numbers and queries 1, rows 2.4, a wavefront's 32 keys
+// 0.9, merge 1; the join 4 (8 sequences of up to 4096 keys 12.0 us in all).
 
 #include <algorithm>
 #include <type_traits>

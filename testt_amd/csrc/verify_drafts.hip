@@ -17,10 +17,10 @@
 // launches: parts of a row are summed by a wavefront each, which finds n for itself (K reads); then one
 // workgroup a sequence picks the part that holds the number and goes through its 1024 columns alone.
 //
-// MI355X, 64 sequences of 8 drafts and 151936 fp32 columns: 18.4 us, of which the sums (63 MB, half the rows
-// refused) 14.5 and the pick 4.0.  One sequence: 4.7 and 3.4, latency (tokens, their probabilities, the row,
+// MI355X, 64 sequences of 8 drafts and 151936 fp32 columns: 17.1 us, of which the sums (63 MB, half the rows
+// refused) 14.1 and the pick 3.9.  One sequence: 4.4 and 3.0, latency (tokens, their probabilities, the row,
 // one after another).  A wavefront's row in flight 512 columns at a time: eight wavefronts a SIMD; 1024 at a
-// time 18.9 us, and 16.5 instead of 15.0 for bf16.
+// time 18.9 instead of 18.4 us then, and 16.5 instead of 15.0 for bf16; parts of 2048 columns 20.0 / 18.2.
 
 #include <algorithm>
 #include <type_traits>
