@@ -100,13 +100,26 @@ def test_long_among_short():
 
 
 @pytest.mark.parametrize("batch,news,nh,nkv,d", [(100, 1, 8, 4, 64), (64, 1, 8, 8, 128), (70, 3, 8, 4, 32),
-                                                 (300, 1, 4, 2, 16)])
+                                                 (300, 1, 4, 2, 16), (64, 20, 8, 4, 128), (90, 21, 8, 4, 96),
+                                                 (270, 12, 6, 2, 32)])
 def test_many_items(batch, news, nh, nkv, d):
     """More items than workgroups take one each: parts that end one item and begin another."""
     lengths = [(i * 173) % 640 for i in range(batch)]
     q, k, v, table, cu = make(lengths, [news] * batch, 32, nh, nkv, d, H, batch)
     got = attention.paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), *seqs(table, lengths, None if news == 1 else cu))
     check(got, q, k, v, table, lengths, cu, H)
+
+
+@pytest.mark.parametrize("dtype", [H, B])
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+@pytest.mark.parametrize("news", [1, 5, 13])
+def test_wide_tables(news, d, dtype):
+    """Block tables that could hold over 176 MB: keys and values are read past the caches (rows of one tile)."""
+    lengths, page, nh, nkv = [700, 0, 131], 64, 16, 4
+    width = -(-(200 << 20) // (4 * nkv * d * page * len(lengths)))
+    q, k, v, table, cu = make(lengths, [news] * 3, page, nh, nkv, d, dtype, 6, width)
+    got = attention.paged_attention(q.to(DEV), k.to(DEV), v.to(DEV), *seqs(table, lengths, None if news == 1 else cu))
+    check(got, q, k, v, table, lengths, cu, dtype)
 
 
 @pytest.mark.parametrize("dtype", [H, B])

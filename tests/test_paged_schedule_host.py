@@ -89,3 +89,14 @@ def test_items_cut_for_themselves_fit_the_parts():
             for chunks in (items, items + 1, 10 * items + 3, 997 * items):
                 per, unit = cut_of(chunks, items, parts)
                 assert unit == per and chunks // per + items <= parts
+
+
+def test_parts_are_dealt_to_xcds_in_runs():
+    """The order of the parts where sequences have several row tiles: each taken once, and the workgroups of an XCD
+    (every eighth) take neighbouring ones."""
+    for used in list(range(1, 70)) + [255, 256, 509, 512]:
+        part = [(w & 7) * (used >> 3) + min(w & 7, used & 7) + (w >> 3) for w in range(used)]
+        assert sorted(part) == list(range(used))
+        for x in range(8):
+            mine = part[x::8]
+            assert mine == list(range(mine[0], mine[0] + len(mine))) if mine else True
