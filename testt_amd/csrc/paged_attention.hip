@@ -327,9 +327,10 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
   const int sum_rows = p.by_quad.div(kThreads);
   uint32_t c = c_begin;
   while (c < c_end && b < p.B) {
-    const Seq sq = p.B <= kWave ? Seq{__builtin_amdgcn_readlane(lane_seq.start, b), __builtin_amdgcn_readlane(lane_seq.news, b),
-                                     __builtin_amdgcn_readlane(lane_seq.len, b)}
-                                : sequence(p, b);
+    const Seq sq = p.B > kWave ? sequence(p, b)
+                               : Seq{__builtin_amdgcn_readlane(lane_seq.start, b),
+                                     __builtin_amdgcn_readlane(lane_seq.news, b),
+                                     __builtin_amdgcn_readlane(lane_seq.len, b)};
     const uint32_t chunks = chunks_of(sq), tiles = tiles_of<R>(sq, p.G), span = rounded(chunks, cut.unit);
     const uint32_t seq_chunks = span * tiles * p.NKV;
     if (c >= seq0 + seq_chunks) {         // (the sequence is done, or has no rows)
@@ -793,8 +794,8 @@ extern "C" __attribute__((visibility("default"))) int soupk_paged_attention_work
 extern "C" __attribute__((visibility("default"))) int soupk_paged_attention(
     const void* q, int64_t q_stride, const void* k_pages, const void* v_pages, int64_t n_pages,
     int64_t page_stride, int32_t page_size, const int32_t* block_table, int64_t max_pages,
-    const int32_t* lengths, const int32_t* cu, int32_t B, void* out, int32_t dtype, int64_t rows, int32_t NH, int32_t NKV, int32_t D, float scale,
-    void* workspace, int64_t workspace_bytes, void* stream) {
+    const int32_t* lengths, const int32_t* cu, int32_t B, void* out, int32_t dtype, int64_t rows, int32_t NH,
+    int32_t NKV, int32_t D, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
   Plan pl;
   if (rows < 0 || B < 0 || NKV < 1 || NH < NKV || NH > (1 << 16) || NH % NKV || D < 16 || D % 16 || D > 256 ||
       page_size < 1 || n_pages < 1 || n_pages >= (int64_t{1} << 31) || max_pages < 0 ||
@@ -816,7 +817,8 @@ extern "C" __attribute__((visibility("default"))) int soupk_paged_attention(
               static_cast<uint32_t*>(workspace),
               reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.first_bytes), rows, q_stride,
               max_pages, n_pages, page_stride, B, NKV, NH / NKV, D, page_size, pl.parts, pl.tiled, scale * kLog2e,
-              FastDiv(static_cast<uint32_t>(page_size)), FastDiv(static_cast<uint32_t>(NH / NKV)), FastDiv(static_cast<uint32_t>(D / 4))};
+              FastDiv(static_cast<uint32_t>(page_size)), FastDiv(static_cast<uint32_t>(NH / NKV)),
+              FastDiv(static_cast<uint32_t>(D / 4))};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   return with_type(dtype, [&](auto tag) -> int {
     using E = typename decltype(tag)::type;

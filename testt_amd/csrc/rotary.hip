@@ -25,9 +25,10 @@
 // interleaved, 29 us each way (5.9 TB/s); 8192 tokens of 48 heads appended 33 us (5.4 TB/s); tables of 131072
 // positions of 128 12.2 us (67 MB of stores; the angles hide behind them).  A few tokens are bound by the host.
 //
-// Mapping: an item is 16 elements of a head, two runs of 8 (by halves they rotate against each other); a wavefront takes the items of 64 / (D / 16) neighbouring heads of one token, PER times
-// over, so that one read of the token's table row serves PER heads.  A head that cannot be cut so
-// (D or the rotated part no multiple of 16, or R/2 no multiple of 8) takes a pair per lane instead.
+// Mapping: an item is 16 elements of a head, two runs of 8 (by halves they rotate against each other); a
+// wavefront takes the items of 64 / (D / 16) neighbouring heads of one token, PER times over, so that one read
+// of the token's table row serves PER heads.  A head that cannot be cut so (D or the rotated part no multiple
+// of 16) takes a pair per lane instead.
 
 #include <algorithm>
 #include <cmath>
