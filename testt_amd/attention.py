@@ -297,9 +297,9 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, cu_seqlens=None, 
     token of its sequence's new ones.
 
     The lengths are read on the device: a captured graph's replays may change them, the block table
-    and the pages, up to the block table's width.  Scores, sums and products are fp32; the
-    probabilities are rounded to the cache's type for the product with the values.  No gradient is
-    given.  The result does not depend on the order of anything: the same bits every time."""
+    and the pages, up to the block table's width.  Scores, sums and products are fp32; a
+    probability meets the values as two numbers of the cache's type, off by 2^-16 of itself at most.  No
+    gradient is given.  The result does not depend on the order of anything: the same bits every time."""
     tensors = (q, k_pages, v_pages, block_table, lengths, cu_seqlens)
     if has_torch_function(tensors):
         return handle_torch_function(paged_attention, tensors, *tensors, scale)

@@ -11,8 +11,11 @@
 // them a tile) are the 16 columns of v_mfma_f32_16x16x32 products, and keys its rows:
 //   S^T (32 keys x 16 rows) = K Q^T        A = K rows staged in LDS
 //   O^T (D x 16 rows) += V^T P^T           A = V^T by transpose reads of rows staged in LDS
-// P is rounded to the cache's type, as the operand has to be: to the output's own rounding (a relative error of
-// 0.0017 in bf16, 0.0002 in fp16 over the timed cases) this adds as much again in squares (0.0022, 0.00025).
+// An operand is of the cache's type, so P goes in as two: rounded, and what that left, rounded again (a relative
+// error of 2^-16 in bf16, 2^-22 in fp16).  Rounded alone it added as much error again, in squares, as the output's own
+// rounding.  MI355X, with the second product / without: 64 sequences of up to 8192 keys 172.0 / 171.5 us, one
+// token over 32768 keys 14.1 / 14.0, 5 new tokens of 16 sequences 20.8 / 19.9, of 32 of up to 8192 keys 64.4 / 60.8, 64
+// tokens of 8 sequences 93 / 82.
 // A wavefront is on its own inside a chunk: it owns 32 of the chunk's 128 keys, its own strip of LDS and its
 // own softmax state; the four are merged once, at the end of an item or part.  No barrier is in the
 // loop.  Page numbers are read two chunks ahead and rows one chunk ahead of their use.
@@ -59,6 +62,8 @@ struct Ops<f16> {
                                                   0, 0);
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_h2(a, b); }
+  static __device__ __forceinline__ float first(uint32_t w) { return lo_h(w); }
+  static __device__ __forceinline__ float second(uint32_t w) { return hi_h(w); }
 };
 template <>
 struct Ops<bf16> {
@@ -68,6 +73,8 @@ struct Ops<bf16> {
                                                    0, 0);
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_b2(a, b); }
+  static __device__ __forceinline__ float first(uint32_t w) { return __uint_as_float(w << 16); }
+  static __device__ __forceinline__ float second(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 };
 
 struct PagedArgs {
@@ -473,7 +480,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
           }
         }
       }
-      u32x4 pb[NB];
+      u32x4 pb[NB], rest[NB];               // the weights rounded, and what is left of them
 #pragma unroll
       for (int u = 0; u < NB; ++u) {
         sc[u][0] = sc[u][0] * p.scale_log2;
@@ -504,8 +511,12 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
           pr[e] = __builtin_amdgcn_exp2f(sc[u][e >> 2][e & 3] - m_use);
           lsum[u] += pr[e];
         }
-        pb[u] = u32x4{Ops<T>::pack(pr[0], pr[1]), Ops<T>::pack(pr[2], pr[3]), Ops<T>::pack(pr[4], pr[5]),
-                      Ops<T>::pack(pr[6], pr[7])};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t two = Ops<T>::pack(pr[2 * e], pr[2 * e + 1]);
+          pb[u][e] = two;
+          rest[u][e] = Ops<T>::pack(pr[2 * e] - Ops<T>::first(two), pr[2 * e + 1] - Ops<T>::second(two));
+        }
       }
       __asm__ volatile("" ::: "memory");      // (no reads of V before their time: registers)
       // O^T += V^T P^T: transpose reads (lane k of a 16-lane group reads 8 bytes of row 4 gr + k / 4 at
@@ -518,7 +529,10 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
         const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
         const u32x4 vf = {l2.x, l2.y, h2.x, h2.y};
 #pragma unroll
-        for (int u = 0; u < NB; ++u) acc[u][t] = Ops<T>::mfma(vf, pb[u], acc[u][t]);
+        for (int u = 0; u < NB; ++u) {
+          acc[u][t] = Ops<T>::mfma(vf, pb[u], acc[u][t]);
+          acc[u][t] = Ops<T>::mfma(vf, rest[u], acc[u][t]);
+        }
       }
     }
 
