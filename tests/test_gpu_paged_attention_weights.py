@@ -54,3 +54,30 @@ def test_weights_hold_more_bits_than_the_cache(lengths, news, page, nh, nkv, d, 
     if dtype == H:
         tol = tol + n * 2.0 ** -25 * float(v.double().abs().max()) + 2.0 ** -25
     assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("dtype", [H, B])
+@pytest.mark.parametrize("news", [1, 3])
+@pytest.mark.parametrize("score", [-10.0, -14.0, -17.625])
+@pytest.mark.parametrize("top", [0, 8190])
+def test_many_small_weights_beside_a_large_one(top, score, news, dtype):
+    """One key's weight is 1 and its value 0; thousands weigh e^score and have values of 1.  600 sequences of the
+    same pages, so that a workgroup takes many chunks of one.  The exponent is at most 26: its roundings change a
+    weight by 2^-17; 600 additions of a lane, 2^-14; an fp16 weight's absolute error is 2^-38 of the largest."""
+    n, d, page, batch, nh = 8192, 16, 256, 600, 16
+    k, v = torch.zeros(2, n // page, 1, page, d)
+    k[..., 0], v[..., 1] = score, 1.0
+    k[top // page, 0, top % page] = 0
+    v[top // page, 0, top % page] = 0
+    q = torch.zeros(batch * news, nh, d)
+    q[..., 0] = 1
+    got = run(q.view(batch * news, -1).to(dtype), k.to(dtype), v.to(dtype), [list(range(n // page))] * batch,
+              [n] * batch, list(range(0, batch * news + 1, news)))
+    got = got.cpu().double().view(batch, news, nh, d)
+    p = torch.tensor(score, dtype=torch.float64).exp()
+    for i in range(news):
+        m = n - news + i                     # keys beside the large one, if the token sees it
+        want = m * p / (1 + m * p) if top <= m else torch.ones((), dtype=torch.float64)
+        tol = (2.0 ** -14 + 2.0 ** -17 + 2.0 ** -16 + torch.finfo(dtype).eps / 2) * want + n * 2.0 ** -38
+        assert bool(((got[:, i, :, 1] - want).abs() <= tol).all()), float((got[:, i, :, 1] / want - 1).abs().max())
+    assert not bool(got[..., 2:].any())

@@ -3,8 +3,8 @@
 // For token i of the n_b new ones of sequence b, whose keys and values (its own included) are the first
 // `length_b` positions of the cache, and query head h with key head h / G:
 //   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - m),  j <= length_b - n_b + i
-// m is a running reference value (raised when a score exceeds it by more than 2^8, as in the training
-// attention), sums and products in fp32; a token that sees no key gets zeros.
+// m is a running reference value (raised when a score exceeds it by more than a margin, 2^8 in bf16 as in the
+// training attention), sums and products in fp32; a token that sees no key gets zeros.
 //
 // What bounds it: the cache's bytes -- a key head's row is read once for the G query heads and the few new
 // tokens that share it.  So the query rows of a key head (row = token * G + head in the group, 16 * NB of
@@ -46,16 +46,19 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / kWave;
 constexpr int kWaveKeys = 32;
 constexpr int kChunk = kWaves * kWaveKeys;
-constexpr float kMargin = 8.f;       // log2 of the largest unnormalised probability
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4 lds_s4;
 
+// kRaise: log2 of the weight of a score equal to the reference value; kMargin: by how much a score may exceed it.
+// fp16 weights lie below 2^15, not below 1, so that those without all bits begin at 2^-27 of the reference's (with 0
+// and 8: at 2^-14, and 8000 weights of 2^-25 beside one of 1 were lost).
 template <typename T>
 struct Ops;
 template <>
 struct Ops<f16> {
+  static constexpr float kRaise = 13.f, kMargin = 2.f;
   typedef f16 v8 __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ f4 mfma(u32x4 a, u32x4 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0,
@@ -67,6 +70,7 @@ struct Ops<f16> {
 };
 template <>
 struct Ops<bf16> {
+  static constexpr float kRaise = 0.f, kMargin = 8.f;
   typedef bf16 v8 __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ f4 mfma(u32x4 a, u32x4 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0,
@@ -496,7 +500,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
         float mx = sc[u][0][0];
 #pragma unroll
         for (int e = 1; e < 8; ++e) mx = __builtin_elementwise_maximum(mx, sc[u][e >> 2][e & 3]);
-        if (__any(!(mx <= m_ref[u] + kMargin))) {       // (a NaN raises it to NaN)
+        if (__any(!(mx <= m_ref[u] + Ops<T>::kMargin))) {       // (a NaN raises it to NaN)
           const float m_new = __builtin_elementwise_maximum(m_ref[u], column_max(mx));
           const float alpha = m_ref[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_ref[u] - m_new);
           lsum[u] *= alpha;
@@ -504,7 +508,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
           for (int t = 0; t < DT; ++t) acc[u][t] = acc[u][t] * alpha;
           m_ref[u] = m_new;
         }
-        const float m_use = m_ref[u] == -INFINITY ? 0.f : m_ref[u];
+        const float m_use = m_ref[u] == -INFINITY ? 0.f : m_ref[u] - Ops<T>::kRaise;
         float pr[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
