@@ -292,8 +292,9 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, cu_seqlens=None, 
     lengths, cu_seqlens: as rope.rope_append.  Token i of a sequence's n new ones sees the keys
     j <= length - n + i: one token each without cu_seqlens; a few with it (drafted tokens to be
     verified) or a prompt's part (whole prompts run faster through the varlen attention).  scale:
-    1 / sqrt(D) unless given.  A token that sees no key gets zeros, and so does a row of no sequence;
-    keys in pages outside [0, pages) are not seen.  A key that holds a NaN or infinity reaches every
+    1 / sqrt(D) unless given.  A token that sees no key gets zeros, and so does a row of no sequence
+    or of one whose bounds leave the rows (cu_seqlens ascends: where it does not, nothing else is
+    promised than that no memory but out's is written); keys in pages outside [0, pages) are not seen.  A key that holds a NaN or infinity reaches every
     token of its sequence's new ones.
 
     The lengths are read on the device: a captured graph's replays may change them, the block table

@@ -98,20 +98,23 @@ struct PagedArgs {
   FastDiv by_page, by_group, by_quad;
 };
 
-// Sequence b's rows and length; an impossible one has no rows.
+// Sequence b's rows and length.  One whose bounds leave the rows has no keys, so that the rows which it
+// spans get their zeros as any row without keys does.
 struct Seq {
   int start, news, len;
 };
 __device__ __forceinline__ Seq sequence(const PagedArgs& p, int b) {
-  int64_t s0 = b, s1 = b + 1;
+  int s0 = b, s1 = b + 1;
   if (p.cu != nullptr) {
     s0 = p.cu[b];
     s1 = p.cu[b + 1];
   }
-  const bool ok = s0 >= 0 && s1 >= s0 && s1 <= p.rows;
-  const int64_t most = p.max_pages * p.page_size;
-  return {ok ? static_cast<int>(s0) : 0, ok ? static_cast<int>(s1 - s0) : 0,
-          static_cast<int>(min(max(static_cast<int64_t>(p.lengths[b]), int64_t{0}), most))};
+  // (at most 2^23 rows and 2^30 keys)
+  const int rows = static_cast<int>(p.rows), most = static_cast<int>(p.max_pages) * p.page_size;
+  const bool ok = s0 >= 0 && s1 <= rows;
+  s0 = min(max(s0, 0), rows);
+  s1 = min(max(s1, s0), rows);
+  return {s0, s1 - s0, min(max(p.lengths[b], 0), ok ? most : 0)};
 }
 // Chunks of a (key head, row tile) of a sequence (one at least, which writes the zeros of one without
 // keys), and its row tiles.
