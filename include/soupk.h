@@ -860,10 +860,11 @@ int soupk_rope_append(const void* qkv, const void* lora_q, const void* lora_v, i
  * Attention of new tokens over that cache (the reference generates nothing; the training form is
  * soupk_attention_varlen_fwd): out [rows, NH D] = softmax(scale q . k_j) v_j over the keys j <= t of each
  * token, at its place t as above; query head h reads key head h / (NH / NKV).  q rows are q_stride elements
- * apart.  A token that sees no key gets zeros, and so do rows of no sequence and of one whose bounds
- * leave the rows (cu ascends; where it does not, only out is written, with what is not said); keys in pages outside
- * [0, n_pages) are not seen.  lengths beyond the block table are cut to it.  k_pages and v_pages 16-byte
- * aligned, max_pages * page_size at most 2^30, rows * NH at most 2^23.  workspace:
+ * apart.  A token that sees no key gets zeros, and so do rows of no sequence and of one whose bounds leave the
+ * rows (cu ascends; where it does not, only out is written, with what is not said); keys in pages outside
+ * [0, n_pages) are not seen.  A length may pass the block table: places count from it all the same, and keys
+ * behind the table are not seen.  k_pages and v_pages 16-byte aligned, max_pages * page_size at most 2^30,
+ * rows * NH at most 2^23.  workspace:
  * soupk_paged_attention_workspace bytes on the current device, 16-byte aligned; a call that runs beside another needs its own.
  */
 int soupk_paged_attention_workspace(int64_t rows, int32_t B, int32_t NH, int32_t NKV, int32_t D,

@@ -101,10 +101,10 @@ def paged_attention(q, k, v, table, lengths, cu=None, scale=None):
     weight = torch.zeros_like(out)
     bounds = [(b, b + 1) for b in range(len(lengths))] if cu is None else list(zip(cu[:-1], cu[1:]))
     for b, (lo, hi) in enumerate(bounds):
-        length = min(max(lengths[b], 0), len(table[b]) * page)
+        length, held = lengths[b], max(min(lengths[b], len(table[b]) * page), 0)
         keys = [(table[b][t // page], t % page) if 0 <= table[b][t // page] < n_pages else None
-                for t in range(length)]
-        seen = [t for t in range(length) if keys[t] is not None]
+                for t in range(held)]
+        seen = [t for t in range(held) if keys[t] is not None]
         if not seen:
             continue
         p, s = (torch.tensor([keys[t][i] for t in seen]) for i in (0, 1))

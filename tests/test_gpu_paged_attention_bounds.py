@@ -44,3 +44,21 @@ def test_the_last_of_many_sequences_passes_the_rows(nh, nkv, d, over):
     got = over_nan(q.to(DEV), k.to(DEV), v.to(DEV), *seqs(table, lengths, cu[:-1] + [cu[-1] + over]))
     check(got[:267], q[:267], k, v, table[:-1], lengths[:-1], cu[:-1], torch.float16)
     assert not bool(got[267:].any())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("beyond", [1, 2, 4, 9, (1 << 31) - 1 - 64])
+@pytest.mark.parametrize("news", [1, 5, 24])
+def test_tokens_stand_where_the_append_puts_them_beyond_the_table(news, beyond, dtype):
+    """Lengths that pass the block table: token i stands at length - news + i all the same, and sees the keys up to
+    there that the table holds."""
+    cap = 64
+    q, k, v, table, _ = make([cap, 30], [news, news], 16, 4, 2, 64, dtype, 5)
+    args = q.to(DEV), k.to(DEV), v.to(DEV)
+    lengths = [cap + beyond, 30]
+    got = attention.paged_attention(*args, *seqs(table, lengths, [0, news, 2 * news]))
+    # each token by itself, at its place
+    rows = torch.cat([q[i:i + 1] for i in range(2 * news)])
+    alone = [min(max(n - news + i + 1, 0), cap) for n in lengths for i in range(news)]
+    check(got, rows, k, v, [table[b] for b in (0, 1) for _ in range(news)], alone, None, dtype)
+    check(got, q, k, v, table, lengths, [0, news, 2 * news], dtype)

@@ -93,13 +93,15 @@ struct PagedArgs {
   float* part;                // two of a workgroup: rows x D sums, rows reference values, rows weights
   int64_t rows, q_stride, max_pages, pages, page_stride;
   int B, NKV, G, D, page_size, parts;
+  int held;                   // keys that a row of the block table holds (at most 2^30)
   bool tiled;                 // more than one row tile a sequence
   float scale_log2;
   FastDiv by_page, by_group, by_quad;
 };
 
-// Sequence b's rows and length.  One whose bounds leave the rows has no keys, so that the rows which it
-// spans get their zeros as any row without keys does.
+// Sequence b's rows and length, which may pass its block table: its tokens' places count from it all the same.
+// One whose bounds leave the rows has no keys, so that the rows which it spans get their zeros as any row
+// without keys does.
 struct Seq {
   int start, news, len;
 };
@@ -109,16 +111,17 @@ __device__ __forceinline__ Seq sequence(const PagedArgs& p, int b) {
     s0 = p.cu[b];
     s1 = p.cu[b + 1];
   }
-  // (at most 2^23 rows and 2^30 keys)
-  const int rows = static_cast<int>(p.rows), most = static_cast<int>(p.max_pages) * p.page_size;
+  const int rows = static_cast<int>(p.rows);      // (at most 2^23)
   const bool ok = s0 >= 0 && s1 <= rows;
   s0 = min(max(s0, 0), rows);
   s1 = min(max(s1, s0), rows);
-  return {s0, s1 - s0, min(max(p.lengths[b], 0), ok ? most : 0)};
+  return {s0, s1 - s0, ok ? max(p.lengths[b], 0) : 0};
 }
 // Chunks of a (key head, row tile) of a sequence (one at least, which writes the zeros of one without
 // keys), and its row tiles.
-__device__ __forceinline__ int chunks_of(const Seq& s) { return max((s.len + kChunk - 1) / kChunk, 1); }
+__device__ __forceinline__ int chunks_of(const Seq& s, int held) {
+  return max((min(s.len, held) + kChunk - 1) / kChunk, 1);
+}
 template <int R>
 __device__ __forceinline__ int tiles_of(const Seq& s, int G) { return (s.news * G + R - 1) / R; }
 
@@ -252,7 +255,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
       const Seq s = sequence(p, lane);
       lane_seq = s;
       items = static_cast<uint32_t>(tiles_of<R>(s, p.G)) * p.NKV;
-      chunks = chunks_of(s);
+      chunks = chunks_of(s, p.held);
     }
     cut = cut_of(lane_of(scan_lanes(items * chunks), 63), lane_of(scan_lanes(items), 63), p.parts);
     const uint32_t n = items * rounded(chunks, cut.unit), upto = scan_lanes(n), total = lane_of(upto, 63);
@@ -278,7 +281,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
       if (q >= p.B) return;
       const Seq s = sequence(p, q);
       items = static_cast<uint32_t>(tiles_of<R>(s, p.G)) * p.NKV;
-      chunks = chunks_of(s);
+      chunks = chunks_of(s, p.held);
     };
     uint32_t items, chunks;
     for (int q = threadIdx.x; q < p.B; q += kThreads) {
@@ -345,7 +348,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
                                : Seq{__builtin_amdgcn_readlane(lane_seq.start, b),
                                      __builtin_amdgcn_readlane(lane_seq.news, b),
                                      __builtin_amdgcn_readlane(lane_seq.len, b)};
-    const uint32_t chunks = chunks_of(sq), tiles = tiles_of<R>(sq, p.G), span = rounded(chunks, cut.unit);
+    const uint32_t chunks = chunks_of(sq, p.held), tiles = tiles_of<R>(sq, p.G), span = rounded(chunks, cut.unit);
     const uint32_t seq_chunks = span * tiles * p.NKV;
     if (c >= seq0 + seq_chunks) {         // (the sequence is done, or has no rows)
       seq0 += seq_chunks;
@@ -361,8 +364,10 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
 
     // (the first row of the tile sees the fewest keys, the last one the most)
     const int rr0 = tile * R, rr1 = min(rr0 + R, sq.news * p.G) - 1;
-    const int seen_all = max(sq.len - sq.news + static_cast<int>(p.by_group.div(rr0)) + 1, 0);
-    const int seen_any = max(sq.len - sq.news + static_cast<int>(p.by_group.div(rr1)) + 1, 0);
+    auto seen_by = [&](int rr) {
+      return min(max(sq.len - sq.news + static_cast<int>(p.by_group.div(rr)) + 1, 0), p.held);
+    };
+    const int seen_all = seen_by(rr0), seen_any = seen_by(rr1);
 
     const int32_t* pages = p.table + static_cast<int64_t>(b) * p.max_pages;
     // the page of key `lane % 32` of this wavefront's in chunk j (of the last key for those behind it), as it is in
@@ -412,7 +417,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
     };
 #pragma unroll
     for (int u = 0; u < NB; ++u)
-      limit[u] = max(sq.len - sq.news + static_cast<int>(p.by_group.div(min(rr0 + 16 * u + ql, rr1))) + 1, 0);
+      limit[u] = seen_by(min(rr0 + 16 * u + ql, rr1));
     if constexpr (TL::kQueriesInLds) {
 #pragma unroll
       for (int i = 0; i < kParts; ++i) q_part[i] = query(part_at(i) / S, part_at(i) % S);
@@ -624,7 +629,7 @@ __global__ __launch_bounds__(THREADS) void paged_join_kernel(PagedArgs p) {
   const uint32_t first = p.first[b], total = p.first[p.B], per = p.first[p.B + 1], unit = p.first[p.B + 2];
   if (row < s.start || row >= s.start + s.news || total == 0) return;
   const int rr = static_cast<int>(row - s.start) * p.G + g;
-  const uint32_t chunks = chunks_of(s), tiles = tiles_of<R>(s, p.G);
+  const uint32_t chunks = chunks_of(s, p.held), tiles = tiles_of<R>(s, p.G);
   const uint32_t c0 = first + (h * tiles + rr / R) * rounded(chunks, unit), c1 = c0 + chunks - 1;
   const uint32_t w0 = c0 / per, w1 = c1 / per;
   if (w0 == w1 || w1 >= static_cast<uint32_t>(p.parts)) return;      // (written whole)
@@ -697,7 +702,7 @@ __global__ __launch_bounds__(kThreads) void paged_join_last_kernel(PagedArgs p) 
     if (step == 1) break;
   }
   const Seq s = sequence(p, b);
-  const uint32_t chunks = chunks_of(s), tiles = tiles_of<R>(s, p.G), span = rounded(chunks, unit);
+  const uint32_t chunks = chunks_of(s, p.held), tiles = tiles_of<R>(s, p.G), span = rounded(chunks, unit);
   const uint32_t seq0 = p.first[b], item = (c1 - 1 - seq0) / span, item0 = seq0 + item * span;
   if (item0 < c0 || item0 + chunks <= c1 || item >= tiles * p.NKV) return;
   const uint32_t w1 = (item0 + chunks - 1) / per;
@@ -837,7 +842,8 @@ extern "C" __attribute__((visibility("default"))) int soupk_paged_attention(
               static_cast<const uint16_t*>(v_pages), block_table, lengths, cu, static_cast<uint16_t*>(out),
               static_cast<uint32_t*>(workspace),
               reinterpret_cast<float*>(static_cast<char*>(workspace) + pl.first_bytes), rows, q_stride,
-              max_pages, n_pages, page_stride, B, NKV, NH / NKV, D, page_size, pl.parts, pl.tiled, scale * kLog2e,
+              max_pages, n_pages, page_stride, B, NKV, NH / NKV, D, page_size, pl.parts,
+              static_cast<int>(max_pages * page_size), pl.tiled, scale * kLog2e,
               FastDiv(static_cast<uint32_t>(page_size)), FastDiv(static_cast<uint32_t>(NH / NKV)),
               FastDiv(static_cast<uint32_t>(D / 4))};
   const hipStream_t s = static_cast<hipStream_t>(stream);
