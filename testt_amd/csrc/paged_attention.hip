@@ -59,6 +59,7 @@ struct Ops;
 template <>
 struct Ops<f16> {
   static constexpr float kRaise = 13.f, kMargin = 2.f;
+  static constexpr uint16_t kNoNumber = 0x7c00;     // (bits of infinities and NaN)
   typedef f16 v8 __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ f4 mfma(u32x4 a, u32x4 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0,
@@ -71,6 +72,7 @@ struct Ops<f16> {
 template <>
 struct Ops<bf16> {
   static constexpr float kRaise = 0.f, kMargin = 8.f;
+  static constexpr uint16_t kNoNumber = 0x7f80;
   typedef bf16 v8 __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ f4 mfma(u32x4 a, u32x4 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0,
@@ -334,7 +336,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
   uint16_t* const strip = strips + w * TL::kStrip;
   // this lane's piece of a row, and its row of load i (lanes and rows too many repeat the last ones)
   const int lane_row = min(lane / TL::kLanes, TL::kPer - 1);
-  const int piece = 8 * min(lane - lane / TL::kLanes * TL::kLanes, D / 8 - 1);
+  auto piece_of = [&](int l) { return 8 * min(l - l / TL::kLanes * TL::kLanes, D / 8 - 1); };
+  const int piece = piece_of(lane);
   auto row_of = [&](int i) {
     const int row = i * TL::kPer + lane_row;
     return kWaveKeys % TL::kPer ? min(row, kWaveKeys - 1) : row;
@@ -373,8 +376,13 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
     // the page of key `lane % 32` of this wavefront's in chunk j (of the last key for those behind it), as it is in
     // the table: looked at when its rows are loaded, as a wait for it is one for all loads before it
     auto find = [&](int j) { return pages[p.by_page.div(min(j * kChunk + w * kWaveKeys + (lane & 31), seen_any - 1))]; };
-    const uint16_t* const k_lane = p.k + static_cast<int64_t>(h) * p.page_size * D + piece;
-    const uint16_t* const v_lane = p.v + static_cast<int64_t>(h) * p.page_size * D + piece;
+    // (Places worked out here: kept over all items, they would be kept in memory, and a wait for one is a wait for
+    // all loads before it.)
+    int here = lane;
+    __asm__ volatile("" : "+v"(here));
+    const int64_t lane_at = static_cast<int64_t>(h) * p.page_size * D + piece_of(here);
+    const uint16_t* const k_lane = p.k + lane_at;
+    const uint16_t* const v_lane = p.v + lane_at;
     auto load = [&](Rows<TL::kLoads>& r, int found_page, int j) {
       const int key = j * kChunk + w * kWaveKeys + (lane & 31);
       if (found_page >= p.pages || key >= seen_any) found_page = -1;
@@ -392,10 +400,10 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
         r.v[i] = ld<PAST>(reinterpret_cast<const u32x4*>(v_lane + to));
       }
     };
-    if (D < DP) {                         // columns past D: zeros of K, which meet any of Q
-      for (int e = lane; e < kWaveKeys * (DP - D) / 8; e += kWave) {
-        const int row = e & (kWaveKeys - 1);
-        *reinterpret_cast<u32x4*>(strip + row * kLd + D + 8 * (e / kWaveKeys)) = u32x4{0, 0, 0, 0};
+    if (D < DP) {                         // columns past D: zeros of K, which meet any of Q, and of V
+      for (int e = lane; e < 2 * kWaveKeys * (DP - D) / 8; e += kWave) {
+        const int row = e & (2 * kWaveKeys - 1);
+        *reinterpret_cast<u32x4*>(strip + row * kLd + D + 8 * (e / (2 * kWaveKeys))) = u32x4{0, 0, 0, 0};
       }
     }
     // (chunks in which this wavefront has keys that the tile sees)
@@ -409,9 +417,10 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
     u32x4 qf[NB][S], q_part[kParts];
     auto part_at = [&](int i) { return min(w + i * kWaves, NB * S - 1); };
     int limit[NB];                        // keys that this lane's row sees
+    const int q_row = here & 15, q_col = 8 * (here >> 4);
     // (rows too many repeat the last one, and columns past D the first, which meet zeros of K)
     auto query = [&](int u, int s) {
-      const int rr = min(rr0 + 16 * u + ql, rr1), i = p.by_group.div(rr), g = rr - i * p.G, d = 32 * s + 8 * gr;
+      const int rr = min(rr0 + 16 * u + q_row, rr1), i = p.by_group.div(rr), g = rr - i * p.G, d = 32 * s + q_col;
       const uint16_t* row = p.q + static_cast<int64_t>(sq.start + i) * p.q_stride + static_cast<int64_t>(h * p.G + g) * D;
       return ld16<false>(row + (d < D ? d : 0));
     };
@@ -435,19 +444,22 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
 #pragma unroll
       for (int i = 0; i < kParts; ++i) {
         const int f = part_at(i);
-        *reinterpret_cast<u32x4*>(q_rows + (16 * (f / S) + ql) * kLd + 32 * (f % S) + 8 * gr) = q_part[i];
+        *reinterpret_cast<u32x4*>(q_rows + (16 * (f / S) + q_row) * kLd + 32 * (f % S) + q_col) = q_part[i];
       }
       lds_barrier();
     }
     f4 acc[NB][DT];
     float m_ref[NB], lsum[NB];
+    auto begin = [&] {
 #pragma unroll
-    for (int u = 0; u < NB; ++u) {
-      m_ref[u] = -INFINITY;
-      lsum[u] = 0.f;
+      for (int u = 0; u < NB; ++u) {
+        m_ref[u] = -INFINITY;
+        lsum[u] = 0.f;
 #pragma unroll
-      for (int t = 0; t < DT; ++t) acc[u][t] = f4{0.f, 0.f, 0.f, 0.f};
-    }
+        for (int t = 0; t < DT; ++t) acc[u][t] = f4{0.f, 0.f, 0.f, 0.f};
+      }
+    };
+    begin();
     // (wait for the queries here: the loop would wait for them, and for the rows that it loads, in every step)
     if constexpr (!TL::kQueriesInLds) {
 #pragma unroll
@@ -455,7 +467,7 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
 #pragma unroll
         for (int s = 0; s < S; ++s) __asm__ volatile("" : "+v"(qf[u][s]));
     }
-    for (int j = j_begin; j < j_mine; ++j) {
+    auto chunk = [&](auto careful, int j) {
       const int key0 = j * kChunk + w * kWaveKeys;
       const uint32_t ok = r.ok;
       const bool whole = ok == ~0u;
@@ -530,6 +542,24 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
           rest[u][e] = Ops<T>::pack(pr[2 * e] - Ops<T>::first(two), pr[2 * e + 1] - Ops<T>::second(two));
         }
       }
+      if constexpr (decltype(careful)::value) {      // (such values are added to the rows that see them)
+#pragma unroll 1
+        for (int key = 0; key < kWaveKeys; ++key) {
+#pragma unroll
+          for (int t = 0; t < DT; ++t) {
+            uint16_t* at = strip + (kWaveKeys + key) * kLd + 16 * t + 4 * gr;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint16_t v = at[e];
+              if ((v & Ops<T>::kNoNumber) != Ops<T>::kNoNumber) continue;
+#pragma unroll
+              for (int u = 0; u < NB; ++u)
+                if (key0 + key < limit[u]) acc[u][t][e] += Ops<T>::first(v);
+              at[e] = 0;
+            }
+          }
+        }
+      }
       __asm__ volatile("" ::: "memory");      // (no reads of V before their time: registers)
       // O^T += V^T P^T: transpose reads (lane k of a 16-lane group reads 8 bytes of row 4 gr + k / 4 at
       // column 4 (k % 4); lane i gets column i of the four rows), rows 4 gr .. + 3 and 16 more
@@ -546,6 +576,22 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
           acc[u][t] = Ops<T>::mfma(vf, rest[u], acc[u][t]);
         }
       }
+    };
+    for (int j = j_begin; j < j_mine; ++j) chunk(std::false_type{}, j);
+    // Sums that are no numbers are made again without the values that are none: 0 times one would reach the rows that
+    // do not see its key, and what rounding left of a weight would turn an infinity into a NaN.
+    float zero = 0.f;
+#pragma unroll
+    for (int u = 0; u < NB; ++u)
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) zero = __builtin_fmaf(acc[u][t][e], 0.f, zero);
+    if (__any(!(zero == 0.f))) {
+      begin();
+      load(r, find(j_begin), j_begin);
+      if (j_begin + 1 < j_mine) next = find(j_begin + 1);
+      for (int j = j_begin; j < j_mine; ++j) chunk(std::true_type{}, j);
     }
 
     // ---- the four wavefronts' sums into one
