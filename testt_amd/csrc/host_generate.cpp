@@ -188,10 +188,14 @@ OP(rope_append) {
     const NoGil released;
     const c10::DeviceGuard guard(dev);
     q = empty({rows, nh * D}, t, dev);
+    // (tables of no positions have no address, which would mean no rotation: any other, as none is read)
+    auto table_at = [&](const Tensor& c) {
+      return c.defined() && c.size(0) == 0 ? reinterpret_cast<const float*>(address(*lengths)) : address<float>(c);
+    };
     if (rows > 0) {
       check("soupk_rope_append",
             p_soupk_rope_append(
-                address(*qkv), address(lq), address(lv), code_of(dt), address<float>(cos), address<float>(sin),
+                address(*qkv), address(lq), address(lv), code_of(dt), table_at(cos), table_at(sin),
                 cos.defined() ? cos.size(0) : 0, cos.defined() ? cos.stride(0) : 0,
                 cos.defined() ? static_cast<int32_t>(2 * cos.size(1)) : 0, a[10] == Py_True,
                 address<int32_t>(cu), address<int32_t>(*lengths), address<int32_t>(*table),
