@@ -23,7 +23,9 @@ def frequencies(dim, theta, scaling=None, seq=0):
         # pair i turns n0 theta^(-2 i / dim) / (2 pi) times within n0
         at = [dim / 2 * math.log(n0 / (2 * math.pi * turns)) / math.log(theta)
               for turns in (scaling.get("beta_fast", 32), scaling.get("beta_slow", 1))]
-        low, high = max(math.floor(at[0]), 0), min(math.ceil(at[1]), dim - 1)
+        if scaling.get("truncate", True):
+            at = [math.floor(at[0]), math.ceil(at[1])]
+        low, high = max(at[0], 0), min(at[1], dim - 1)
         r = [min(max((i - low) / max(high - low, 0.001), 0.0), 1.0) for i in range(dim // 2)]
         freq = [f * (1 - x) + f / scaling["factor"] * x for f, x in zip(freq, r)]
         gain = scaling.get("attention_factor", 0.1 * math.log(scaling["factor"]) + 1)

@@ -1,0 +1,27 @@
+"""Tables from a model's rope_scaling on the GPU, against 64 bits; tolerances as in test_gpu_rotary.py."""
+
+import pytest
+import torch
+
+from oracle import generate as og
+from testt_amd import rope
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def same(got, want):
+    for a, b in zip(got, want):
+        assert bool(((a.cpu().double() - b).abs() <= 2.0 ** -24 * b.abs() + 2e-9).all())
+
+
+@pytest.mark.parametrize("seq,dim,theta,kw", [
+    (4097, 64, 150000.0, dict(factor=32.0)), (300, 128, 1e6, {}), (65, 96, 5e5, dict(beta_fast=20.0, beta_slow=1.5)),
+    (33, 64, 1e4, dict(attention_factor=0.75))])
+def test_yarn_between_pairs(seq, dim, theta, kw):
+    scaling = {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096, "truncate": False, **kw}
+    same(rope.rotary_tables(seq, dim, theta, scaling, device=DEV), og.rotary_tables(seq, dim, theta, scaling))
+    scaling["truncate"] = True
+    whole = rope.rotary_tables(seq, dim, theta, scaling, device=DEV)
+    del scaling["truncate"]
+    assert all(torch.equal(a, b) for a, b in zip(whole, rope.rotary_tables(seq, dim, theta, scaling, device=DEV)))

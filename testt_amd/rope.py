@@ -271,7 +271,7 @@ def rotary_tables(seq, rotary_dim, theta=10000.0, scaling=None, inv_freq=None, d
     scaling: None or a dict in transformers' `rope_scaling` form, for contexts longer than the
     trained one -- rope_type "default", "linear" (factor), "dynamic" (factor,
     original_max_position_embeddings; takes effect where seq exceeds it) or "yarn" (those two and,
-    optionally, beta_fast, beta_slow, attention_factor, mscale, mscale_all_dim).  inv_freq:
+    optionally, beta_fast, beta_slow, attention_factor, mscale, mscale_all_dim, truncate).  inv_freq:
     rotary_dim / 2 frequencies on the host (numbers, or a CPU tensor) in place of theta and scaling.
     rotary_dim: even, at most 256.  The layer's own tables [seq, head_dim] hold every column twice:
     their first half (cos[:, :head_dim // 2]) is this form."""
@@ -324,9 +324,27 @@ def rotary_tables(seq, rotary_dim, theta=10000.0, scaling=None, inv_freq=None, d
             if not 0.0 < slow <= fast <= 1e6:
                 raise ValueError(f"0 < beta_slow <= beta_fast <= 1e6 is needed, got {slow}, {fast}")
             gain = _yarn_gain(scaling, factor)
+            truncate = scaling.get("truncate")
+            if not isinstance(truncate, (bool, type(None))):
+                raise TypeError(f"truncate must be True or False, got {truncate!r}")
+            if truncate is False:
+                inv_freq = _yarn_between(rotary_dim, theta, factor, original, fast, slow)
     index = device.index if device.index is not None else torch.cuda.current_device()
     return _ext.checked(_ext.host().rotary_tables(seq, rotary_dim, theta, _SCALINGS[kind], factor,
                                                   original, fast, slow, gain, inv_freq, index))
+
+
+def _yarn_between(dim, theta, factor, original, fast, slow):
+    """YaRN's frequencies where the ramp begins and ends between pairs (csrc/rotary.hip widens it to whole ones)."""
+    low, high = (dim * math.log(original / (2.0 * math.pi * turns)) / (2.0 * math.log(theta))
+                 for turns in (fast, slow))
+    low, high = max(low, 0.0), min(high, dim - 1.0)
+    freq = []
+    for i in range(dim // 2):
+        ramp = min(max((i - low) / max(high - low, 0.001), 0.0), 1.0)
+        f = theta ** (-2.0 * i / dim)
+        freq.append(f / factor * ramp + f * (1.0 - ramp))
+    return tuple(freq)
 
 
 def _yarn_gain(scaling, factor):
