@@ -25,3 +25,17 @@ def test_yarn_between_pairs(seq, dim, theta, kw):
     whole = rope.rotary_tables(seq, dim, theta, scaling, device=DEV)
     del scaling["truncate"]
     assert all(torch.equal(a, b) for a, b in zip(whole, rope.rotary_tables(seq, dim, theta, scaling, device=DEV)))
+
+
+@pytest.mark.parametrize("scaling", [
+    {"rope_type": "default", "rope_theta": 1e6}, {"rope_type": "linear", "factor": 2.0, "rope_theta": 5e5},
+    {"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096, "rope_theta": 150000.0}])
+def test_the_base_stands_in_the_scaling(scaling):
+    """transformers keeps rope_theta beside the scaling."""
+    theta = scaling["rope_theta"]
+    want = og.rotary_tables(300, 64, theta, scaling)
+    same(rope.rotary_tables(300, 64, scaling=scaling, device=DEV), want)
+    same(rope.rotary_tables(300, 64, theta, scaling, device=DEV), want)
+    same(rope.rotary_tables(300, 64, device=DEV), og.rotary_tables(300, 64, 1e4))
+    bare = {k: v for k, v in scaling.items() if k != "rope_theta"}
+    same(rope.rotary_tables(300, 64, scaling=bare, device=DEV), og.rotary_tables(300, 64, 1e4, bare))

@@ -58,3 +58,13 @@ def test_frequencies_between_pairs(dim, theta, scaling):
 def test_truncate_is_a_truth_value():
     with pytest.raises(TypeError, match="truncate"):
         rope.rotary_tables(8, 16, scaling=yarn(truncate="no"))
+
+
+def test_two_bases_are_refused():
+    for scaling in ({"rope_type": "default", "rope_theta": 1e6}, yarn(rope_theta=1e6)):
+        with pytest.raises(ValueError, match="rope_theta"):
+            rope.rotary_tables(8, 16, 1e4, scaling)
+    with pytest.raises(ValueError, match="theta"):
+        rope.rotary_tables(8, 16, scaling=yarn(rope_theta=0.5))
+    with pytest.raises(ValueError, match="theta"):
+        rope.rotary_tables(8, 16, 0.0)

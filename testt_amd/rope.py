@@ -263,9 +263,10 @@ def _positive(scaling, key, default=None):
     return _ext.number(value, key)
 
 
-def rotary_tables(seq, rotary_dim, theta=10000.0, scaling=None, inv_freq=None, device="cuda"):
+def rotary_tables(seq, rotary_dim, theta=None, scaling=None, inv_freq=None, device="cuda"):
     """(cos, sin) fp32 [seq, rotary_dim / 2] of positions 0 .. seq - 1, for rotary() and
-    rope_append(): pair i turns by theta^(-2 i / rotary_dim) a position.  The angles are formed in
+    rope_append(): pair i turns by theta^(-2 i / rotary_dim) a position (theta: scaling's rope_theta, or
+    10000, unless given).  The angles are formed in
     64 bits, so far positions keep their places (in fp32 an angle at position 2^20 is 0.03 rad off).
 
     scaling: None or a dict in transformers' `rope_scaling` form, for contexts longer than the
@@ -276,7 +277,8 @@ def rotary_tables(seq, rotary_dim, theta=10000.0, scaling=None, inv_freq=None, d
     rotary_dim: even, at most 256.  The layer's own tables [seq, head_dim] hold every column twice:
     their first half (cos[:, :head_dim // 2]) is this form."""
     if scaling is None and inv_freq is None and isinstance(device, str) and device == "cuda":
-        done = _ext.host().rotary_tables(seq, rotary_dim, theta, 0, 1.0, 1.0, 32.0, 1.0, 1.0, None, -1)
+        done = _ext.host().rotary_tables(seq, rotary_dim, 1e4 if theta is None else theta, 0, 1.0, 1.0, 32.0, 1.0,
+                                         1.0, None, -1)
         if done is not None:
             return done
     device = torch.device(device)
@@ -290,6 +292,13 @@ def rotary_tables(seq, rotary_dim, theta=10000.0, scaling=None, inv_freq=None, d
         raise ValueError(f"seq must lie in [0, 2^31), got {seq}")
     if not 2 <= rotary_dim <= 256 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be even and lie in [2, 256], got {rotary_dim}")
+    if scaling is not None and not isinstance(scaling, Mapping):
+        raise TypeError(f"scaling must be None or a dict, got {type(scaling).__name__}")
+    told = None if scaling is None else scaling.get("rope_theta")
+    if theta is None:
+        theta = 1e4 if told is None else told
+    elif told is not None and _ext.number(theta, "theta") != _ext.number(told, "rope_theta"):
+        raise ValueError(f"theta {theta} is not scaling's rope_theta {told}: pass one of them")
     theta = _ext.number(theta, "theta")
     if not 1.0 < theta <= 1e30:
         raise ValueError(f"theta must lie in (1, 1e30], got {theta}")
@@ -305,8 +314,6 @@ def rotary_tables(seq, rotary_dim, theta=10000.0, scaling=None, inv_freq=None, d
         if len(inv_freq) != rotary_dim // 2 or not all(abs(f) <= 1e6 for f in inv_freq):
             raise ValueError(f"inv_freq must hold {rotary_dim // 2} frequencies of at most 1e6 rad")
     elif scaling is not None:
-        if not isinstance(scaling, Mapping):
-            raise TypeError(f"scaling must be None or a dict, got {type(scaling).__name__}")
         kind = scaling.get("rope_type", scaling.get("type"))
         if kind not in _SCALINGS:
             raise ValueError(f"rope scaling must be one of {', '.join(_SCALINGS)}, got {kind!r} (other "
