@@ -68,3 +68,26 @@ def test_two_bases_are_refused():
         rope.rotary_tables(8, 16, scaling=yarn(rope_theta=0.5))
     with pytest.raises(ValueError, match="theta"):
         rope.rotary_tables(8, 16, 0.0)
+
+
+@pytest.mark.parametrize("scaling,match", [
+    (yarn(short_factor=[1.0]), "short_factor"), (yarn(low_freq_factor=1.0), "low_freq_factor"),
+    ({"rope_type": "linear", "factor": 2.0, "beta_fast": 32.0}, "beta_fast"),
+    ({"rope_type": "linear", "factor": 2.0, "attention_factor": 0.5}, "attention_factor"),
+    ({"rope_type": "dynamic", "factor": 2.0, "original_max_position_embeddings": 64, "alpha": 2.0}, "alpha"),
+    ({"rope_type": "default", "factor": 2.0}, "factor"), ({"rope_type": "default", "truncate": True}, "truncate"),
+    (yarn(partial_rotary_factor=0.5), "partial_rotary_factor"),
+    ({"rope_type": "default", "partial_rotary_factor": 0.25}, "partial_rotary_factor")])
+def test_keys_that_would_be_passed_over_are_refused(scaling, match):
+    with pytest.raises(ValueError, match=match):
+        rope.rotary_tables(8, 16, scaling=scaling)
+
+
+def test_scalings_of_configurations_are_read():
+    """What transformers' configurations hold comes as far as the device."""
+    for scaling in ({"rope_type": "default"}, {"rope_type": "linear", "factor": 2.0}, yarn(truncate=False), yarn()):
+        config = transformers.Qwen2Config(rope_parameters={**scaling, "rope_theta": 1e6})
+        with pytest.raises(ValueError, match="no CPU path"):
+            rope.rotary_tables(8, 16, scaling=config.rope_scaling, device="cpu")
+        rope._check_scaling({**config.rope_scaling, "partial_rotary_factor": 1.0, "beta_fast": None, "type": None})
+    rope._check_scaling({"rope_type": "linear", "factor": 2.0, "original_max_position_embeddings": 64})

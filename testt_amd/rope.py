@@ -263,19 +263,44 @@ def _positive(scaling, key, default=None):
     return _ext.number(value, key)
 
 
+# What a scaling of each kind may say: the kind, the base, and a model's trained length where it has no part in
+# the frequencies.
+_EVERY_SCALING = ("rope_type", "type", "rope_theta", "original_max_position_embeddings")
+_SCALING_KEYS = {"default": (), "linear": ("factor",), "dynamic": ("factor",),
+                 "yarn": ("factor", "beta_fast", "beta_slow", "attention_factor", "mscale", "mscale_all_dim",
+                          "truncate")}
+
+
+def _check_scaling(scaling):
+    """The kind of a rope scaling; raises for a key that would be passed over."""
+    kind = scaling.get("rope_type", scaling.get("type"))
+    if kind not in _SCALINGS:
+        raise ValueError(f"rope scaling must be one of {', '.join(_SCALINGS)}, got {kind!r} (other "
+                         "schemes: pass their frequencies as inv_freq)")
+    if scaling.get("partial_rotary_factor") not in (None, 1):
+        raise ValueError("partial_rotary_factor is not read: multiply the head dim by it for rotary_dim, and leave "
+                         "it out of scaling")
+    for key, value in scaling.items():
+        if value is not None and key not in (*_EVERY_SCALING, *_SCALING_KEYS[kind], "partial_rotary_factor"):
+            raise ValueError(f"rope scaling {kind!r} does not read {key!r}: leave it out, or pass frequencies "
+                             "as inv_freq")
+    return kind
+
+
 def rotary_tables(seq, rotary_dim, theta=None, scaling=None, inv_freq=None, device="cuda"):
     """(cos, sin) fp32 [seq, rotary_dim / 2] of positions 0 .. seq - 1, for rotary() and
     rope_append(): pair i turns by theta^(-2 i / rotary_dim) a position (theta: scaling's rope_theta, or
-    10000, unless given).  The angles are formed in
-    64 bits, so far positions keep their places (in fp32 an angle at position 2^20 is 0.03 rad off).
+    10000, unless given).  The angles are formed in 64 bits, so far positions keep their places (in
+    fp32 an angle at position 2^20 is 0.03 rad off).
 
-    scaling: None or a dict in transformers' `rope_scaling` form, for contexts longer than the
+    scaling: None or a dict in the form of transformers' `rope_scaling`, for contexts longer than the
     trained one -- rope_type "default", "linear" (factor), "dynamic" (factor,
-    original_max_position_embeddings; takes effect where seq exceeds it) or "yarn" (those two and,
-    optionally, beta_fast, beta_slow, attention_factor, mscale, mscale_all_dim, truncate).  inv_freq:
-    rotary_dim / 2 frequencies on the host (numbers, or a CPU tensor) in place of theta and scaling.
-    rotary_dim: even, at most 256.  The layer's own tables [seq, head_dim] hold every column twice:
-    their first half (cos[:, :head_dim // 2]) is this form."""
+    original_max_position_embeddings, which transformers leaves to the configuration's
+    max_position_embeddings; takes effect where seq exceeds it) or "yarn" (those two and, optionally,
+    beta_fast, beta_slow, attention_factor, mscale, mscale_all_dim, truncate).  A key that its kind does
+    not read raises.  inv_freq: rotary_dim / 2 frequencies on the host (numbers, or a CPU tensor) in
+    place of theta and scaling.  rotary_dim: even, at most 256.  The layer's own tables [seq, head_dim]
+    hold every column twice: their first half (cos[:, :head_dim // 2]) is this form."""
     if scaling is None and inv_freq is None and isinstance(device, str) and device == "cuda":
         done = _ext.host().rotary_tables(seq, rotary_dim, 1e4 if theta is None else theta, 0, 1.0, 1.0, 32.0, 1.0,
                                          1.0, None, -1)
@@ -314,10 +339,7 @@ def rotary_tables(seq, rotary_dim, theta=None, scaling=None, inv_freq=None, devi
         if len(inv_freq) != rotary_dim // 2 or not all(abs(f) <= 1e6 for f in inv_freq):
             raise ValueError(f"inv_freq must hold {rotary_dim // 2} frequencies of at most 1e6 rad")
     elif scaling is not None:
-        kind = scaling.get("rope_type", scaling.get("type"))
-        if kind not in _SCALINGS:
-            raise ValueError(f"rope scaling must be one of {', '.join(_SCALINGS)}, got {kind!r} (other "
-                             "schemes: pass their frequencies as inv_freq)")
+        kind = _check_scaling(scaling)
         if kind != "default":
             factor = _positive(scaling, "factor")
             if not 1.0 <= factor <= 1e6:
