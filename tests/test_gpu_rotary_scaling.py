@@ -1,5 +1,7 @@
 """Tables from a model's rope_scaling on the GPU, against 64 bits; tolerances as in test_gpu_rotary.py."""
 
+from fractions import Fraction
+
 import pytest
 import torch
 
@@ -39,3 +41,20 @@ def test_the_base_stands_in_the_scaling(scaling):
     same(rope.rotary_tables(300, 64, device=DEV), og.rotary_tables(300, 64, 1e4))
     bare = {k: v for k, v in scaling.items() if k != "rope_theta"}
     same(rope.rotary_tables(300, 64, scaling=bare, device=DEV), og.rotary_tables(300, 64, 1e4, bare))
+
+
+# pi, to 50 digits
+PI = Fraction("3.14159265358979323846264338327950288419716939937510")
+
+
+@pytest.mark.parametrize("seq,freq", [
+    ((1 << 21) + 5, [1e6, -999999.9, 123456.78901234567, 1.0]), ((1 << 24) + 1, [1e6]), (1 << 20, [1e6] * 4),
+    (700, [987654.321, 1e6, 0.3]), ((1 << 24) + 3, [0.1, 1.0, 700.7, 3e4])])
+def test_far_angles_of_given_frequencies(seq, freq):
+    """Angles of up to 10^13 rad, reduced by whole numbers here: a double's product with a position is not the
+    angle (2^21 * 10^6 rad in 64 bits is off by 1e-4)."""
+    cos, sin = rope.rotary_tables(seq, 2 * len(freq), inv_freq=freq, device=DEV)
+    rows = sorted({0, 1, 17, 127, seq // 3, seq // 2, *range(seq - 40, seq)})
+    at = [[float(Fraction(f) * t % (2 * PI)) for f in freq] for t in rows]
+    ang = torch.tensor(at, dtype=torch.float64)
+    same((cos[rows], sin[rows]), (ang.cos(), ang.sin()))

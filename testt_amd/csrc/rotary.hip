@@ -11,9 +11,10 @@
 //            inv_i (1 - r_i) + inv_i / factor * r_i, with a ramp r_i over the pair's number from the pair
 //            that turns beta_fast times within n0 to the one that turns beta_slow times; the gain is
 //            0.1 ln(factor) + 1
-// An angle is held in turns in 64 bits and reduced to the nearest quarter before its cosine and sine are
-// summed from their Taylor series: at position 2^20 an angle in fp32 would be 0.03 rad off, here the
-// error is below 1e-9.
+// An angle is held in turns, as two 64-bit numbers, and reduced to the nearest quarter before its cosine and
+// sine are summed from their Taylor series, which end 2e-10 early: at position 2^20 an angle in fp32 would be 0.03
+// rad off.  A frequency made from theta is rounded to 64 bits (1e-15 of the angle, 1e-9 rad at 10^6 rad);
+// a given one is taken exactly.
 //
 // Rotation: (a, b) -> (a c - b s, b c + a s) for the pairs (x[i], x[i + R/2]) or, interleaved,
 // (x[2 i], x[2 i + 1]) of the leading R = dim elements of a head; the others are copied.  Products and
@@ -51,9 +52,15 @@ constexpr int kMaxPairs = 128;
 // 6.9 -> 6.5.
 constexpr int kPositions = 8;
 constexpr int64_t kManyThreads = 16384;
-struct Turns {
-  double per_pos[kMaxPairs];      // of a turn
+struct Turns {                    // a position's part of a turn: a double, and what that left
+  double per_pos[kMaxPairs], rest[kMaxPairs];
 };
+// Position `pos`'s turns of frequency f + rest, whole ones taken off.  (The product's rounding is added back: at 10^13
+// rad it is 10^-3 rad.)
+__device__ __forceinline__ double turns_at(double pos, double f, double rest) {
+  const double t = pos * f;
+  return t - __builtin_rint(t) + __builtin_fma(pos, rest, __builtin_fma(pos, f, -t));
+}
 
 // cos and sin of 2 pi r for r in [-1/2, 1/2]: quarter turns split off, then the series of the remaining
 // |x| <= pi / 4 (first terms left out: x^13 / 13! < 7e-12, x^12 / 12! < 2e-10; an fp32 number near 1 is
@@ -95,14 +102,12 @@ __global__ __launch_bounds__(kThreads) void rotary_tables_kernel(Turns turns, fl
   double c[N], s[N], cs[N], ss[N];
 #pragma unroll
   for (int j = 0; j < N; ++j) {
-    const double f = turns.per_pos[g * N + j];
-    const double t = static_cast<double>(first) * f;
-    cos_sin_turns(t - __builtin_rint(t), c[j], s[j]);
+    const double f = turns.per_pos[g * N + j], rest = turns.rest[g * N + j];
+    cos_sin_turns(turns_at(first, f, rest), c[j], s[j]);
     c[j] *= gain;
     s[j] *= gain;
     if constexpr (P > 1) {
-      const double d = static_cast<double>(step) * f;
-      cos_sin_turns(d - __builtin_rint(d), cs[j], ss[j]);
+      cos_sin_turns(turns_at(step, f, rest), cs[j], ss[j]);
     }
   }
 #pragma unroll
@@ -575,11 +580,16 @@ extern "C" __attribute__((visibility("default"))) int soupk_rotary_tables(
   if (!(std::fabs(gain) <= 1e30)) return kInvalid;
   Turns turns;
   const int half = dim / 2;
+  auto set = [&](int i, double f) {         // f / (2 pi), of which the second number is below 2^-53 of the first
+    constexpr double kPerTurn = 0x1.45f306dc9c883p-3, kLeft = -0x1.6b01ec5417056p-57;
+    turns.per_pos[i] = f * kPerTurn;
+    turns.rest[i] = std::fma(f, kPerTurn, -turns.per_pos[i]) + f * kLeft;
+  };
   if (inv_freq != nullptr) {
     for (int i = 0; i < half; ++i) {
-      // (so that position 2^31 stays an exact number of quarters beside its angle)
+      // (2^31 positions of it are below 2^49 turns, whose parts a double and its rest hold)
       if (!(std::fabs(inv_freq[i]) <= 1e6)) return kInvalid;
-      turns.per_pos[i] = inv_freq[i] / kTwoPi;
+      set(i, inv_freq[i]);
     }
   } else {
     if (!(theta > 1.0 && theta <= 1e30)) return kInvalid;
@@ -605,10 +615,10 @@ extern "C" __attribute__((visibility("default"))) int soupk_rotary_tables(
         const double ramp = std::fmin(std::fmax((i - low) / width, 0.0), 1.0);
         f = f / factor * ramp + f * (1.0 - ramp);
       }
-      turns.per_pos[i] = f / kTwoPi;
+      set(i, f);
     }
   }
-  for (int i = half; i < kMaxPairs; ++i) turns.per_pos[i] = 0.0;
+  for (int i = half; i < kMaxPairs; ++i) turns.per_pos[i] = turns.rest[i] = 0.0;
   if (seq == 0) return kOk;
   if (bad_ptr(cos, 15) || bad_ptr(sin, 15)) return kInvalid;
   const int n = half % 4 == 0 ? 4 : 1, per = half / n;
