@@ -249,8 +249,8 @@ struct RotaryArgs {
   const int64_t* pos;
   char* out;
   int64_t n_pos, table_stride, row_stride, head_stride;
-  int heads, groups;      // heads of a token; wavefront items of a token
-  FastDiv per_tok;        // divides by groups
+  int heads;              // of a token
+  FastDiv per_tok;        // divides by the wavefront items of a token
   Layout l;
   float sign;
 };
@@ -406,9 +406,9 @@ struct AppendArgs {
   char* v_pages;
   int64_t n_pos, table_stride, pages, max_pages, page_stride, rows;
   int32_t B;
-  int NH, NKV, groups;
+  int NH, NKV;
   bool lora_f32;
-  FastDiv per_tok, per_page;
+  FastDiv per_tok, per_page;      // by the wavefront items of a token, by a page's slots
   Layout l;
 };
 
@@ -648,12 +648,11 @@ extern "C" __attribute__((visibility("default"))) int soupk_rotary(
       (n_pos > 0 && (bad_ptr(cos, 3) || bad_ptr(sin, 3))))
     return kInvalid;
   RotaryArgs a{static_cast<const char*>(x), cos, sin, pos, static_cast<char*>(out), n_pos, table_stride,
-               row_stride, head_stride, heads, 0, FastDiv(1), Layout{D, R / 2, 0, interleaved != 0},
+               row_stride, head_stride, heads, FastDiv(1), Layout{D, R / 2, 0, interleaved != 0},
                inverse ? -1.f : 1.f};
   return with_type(dtype, [&](auto tag) -> int {
     using E = typename decltype(tag)::type;
     auto launch = [&](auto kernel, int groups) {
-      a.groups = groups;
       a.per_tok = FastDiv(static_cast<uint32_t>(groups));
       return over_rows(rows, groups, [&](int64_t r, uint32_t waves, dim3 grid) {
         return launch_kernel(kernel, grid, dim3(kThreads), static_cast<hipStream_t>(stream), a, r, waves);
@@ -708,7 +707,7 @@ extern "C" __attribute__((visibility("default"))) int soupk_rope_append(
   AppendArgs a{static_cast<const char*>(qkv), static_cast<const char*>(lora_q),
                static_cast<const char*>(lora_v), cos, sin, cu, lengths, block_table,
                static_cast<char*>(q_out), static_cast<char*>(k_pages), static_cast<char*>(v_pages), n_pos,
-               table_stride, n_pages, max_pages, page_stride, rows, B, NH, NKV, 0,
+               table_stride, n_pages, max_pages, page_stride, rows, B, NH, NKV,
                lora_dtype == SOUPK_DTYPE_F32, FastDiv(1), FastDiv(static_cast<uint32_t>(page_size)),
                // (without tables every item is copied: cut as if all of the head were rotated)
                Layout{D, rotate ? R / 2 : D / 2, 0, interleaved != 0}};
@@ -718,7 +717,6 @@ extern "C" __attribute__((visibility("default"))) int soupk_rope_append(
       return kInvalid;
     } else {
       return with_items(a.l, rows, NH + 2 * NKV, [&](auto n, auto per, int groups) {
-        a.groups = groups;
         a.per_tok = FastDiv(static_cast<uint32_t>(groups));
         return over_rows(rows, groups, [&](int64_t r, uint32_t waves, dim3 grid) {
           return launch_kernel(rope_append_kernel<E, decltype(n)::value, decltype(per)::value>, grid,
