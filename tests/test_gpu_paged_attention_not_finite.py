@@ -1,5 +1,7 @@
-"""Keys and values that are no numbers, in the paged attention: they reach the tokens that see them, in their own
-columns, and no others.  Beside them the bits are those of the same call without them."""
+"""Keys and values that are no numbers, in the paged attention: they reach the tokens that see them, a value's in its
+own column, and no others.  A value leaves the other results' bits as they are without it; a key may raise the
+reference value of rows beside its own, so that their weights are rounded elsewhere: 2^-16 of each weight, both
+times, and the output's rounding eps / 2, both times."""
 
 import pytest
 import torch
@@ -42,14 +44,16 @@ def test_a_later_tokens_value(nh, nkv, d, news, what, dtype):
 @pytest.mark.parametrize("what", [NAN, INF, -INF])
 @pytest.mark.parametrize("nh,nkv,d,news", SHAPES)
 def test_a_later_tokens_key(nh, nkv, d, news, what, dtype):
-    """The key of the last new token: the others have the bits that they had."""
+    """The key of the last new token: the others are what they were."""
     lengths = [40, 131, 1000]
     q, k, v, table, cu = make(lengths, [news] * 3, 16, nh, nkv, d, dtype, 2)
     want = run(q, k, v, table, lengths, cu).view(3, news, -1)
     k[table[1][130 // 16], :, 130 % 16] = what
     got = run(q, k, v, table, lengths, cu).view(3, news, -1)
     got[1, -1] = want[1, -1] = 0
-    assert torch.equal(got, want)
+    tol = torch.finfo(dtype).eps * want.double().abs() + 4 * 2.0 ** -16 * float(v.double().nan_to_num(0).abs().max())
+    assert bool(((got.double() - want.double()).abs() <= tol).all())
+    assert torch.equal(got[[0, 2]], want[[0, 2]])
 
 
 @pytest.mark.parametrize("dtype", [H, B])

@@ -376,10 +376,10 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
     // the page of key `lane % 32` of this wavefront's in chunk j (of the last key for those behind it), as it is in
     // the table: looked at when its rows are loaded, as a wait for it is one for all loads before it
     auto find = [&](int j) { return pages[p.by_page.div(min(j * kChunk + w * kWaveKeys + (lane & 31), seen_any - 1))]; };
-    // (Places worked out here: kept over all items, they would be kept in memory, and a wait for one is a wait for
-    // all loads before it.)
+    // (Places worked out here where registers are few: kept over all items, they would be kept in memory, and a wait
+    // for one is a wait for all loads before it.)
     int here = lane;
-    __asm__ volatile("" : "+v"(here));
+    if constexpr (NB == 2) __asm__ volatile("" : "+v"(here));
     const int64_t lane_at = static_cast<int64_t>(h) * p.page_size * D + piece_of(here);
     const uint16_t* const k_lane = p.k + lane_at;
     const uint16_t* const v_lane = p.v + lane_at;
@@ -580,14 +580,15 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
     for (int j = j_begin; j < j_mine; ++j) chunk(std::false_type{}, j);
     // Sums that are no numbers are made again without the values that are none: 0 times one would reach the rows that
     // do not see its key, and what rounding left of a weight would turn an infinity into a NaN.
-    float zero = 0.f;
+    float top[2] = {0.f, 0.f};            // (of a NaN: NaN)
+    auto larger = [](float a, float b) { return __builtin_elementwise_maximum(a, __builtin_fabsf(b)); };
 #pragma unroll
     for (int u = 0; u < NB; ++u)
 #pragma unroll
       for (int t = 0; t < DT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) zero = __builtin_fmaf(acc[u][t][e], 0.f, zero);
-    if (__any(!(zero == 0.f))) {
+        for (int e = 0; e < 4; ++e) top[e >> 1] = larger(top[e >> 1], acc[u][t][e]);
+    if (__any(!(larger(top[0], top[1]) < INFINITY))) {
       begin();
       load(r, find(j_begin), j_begin);
       if (j_begin + 1 < j_mine) next = find(j_begin + 1);
