@@ -23,15 +23,15 @@
 // Split: the work is the list of all chunks of all items -- (sequence, key head, row tile) -- in that order,
 // cut into equal parts, one a workgroup: a long sequence among short ones, or one alone, fills the chip the same
 // way, whatever the lengths are (they are in device memory: a captured graph's replays may change
-// them).  Where the items are few, each is cut for itself (a workgroup that crosses into another item waits
+// them; cut_of() says where it does not).  Where the items are few, each is cut for itself (a workgroup that crosses into another item waits
 // for queries, page numbers and rows once more); where they are many, a part may end one item and
 // begin others.  A workgroup writes what lies whole inside its part; of an item that reaches across an end it
 // leaves the unnormalised sum, its reference value and its weight, two at most, and a second launch
 // joins those in workgroup order: the same bits every time.
 //
-// MI355X: 64 sequences of up to 8192 keys, 8 heads of 128 in bf16 (1.09 GB) 168 us and a join of 4.7: 6.5 TB/s.  A
+// MI355X: 64 sequences of up to 8192 keys, 8 heads of 128 in bf16 (1.09 GB) 169 us and a join of 4.7: 6.5 TB/s.  A
 // single step is latency: lengths and schedule 1.2 us, page numbers and queries 1, rows 2.4, a wavefront's 32 keys
-// 0.9, merge 1; the join 4 (8 sequences of up to 4096 keys 12.0 us in all).
+// 1, merge 1; the join 4 (8 sequences of up to 4096 keys 12.3 us in all).
 
 #include <algorithm>
 #include <type_traits>
@@ -183,6 +183,9 @@ __device__ __forceinline__ void lds_barrier() {
 }
 
 // How the list is cut: chunks of a part, and what an item's chunks are rounded up to.
+// (Cut for themselves, items are given a part more each, whether they fill it or not: close to half as many items as
+// parts, a part is up to twice the mean.  16 sequences of up to 16 tokens and 8192 keys, 32/8 heads: 240 items of 8032
+// chunks in all, 30 a part of 512, 15.7 their mean; 119 us, for 43 of memory.)
 struct Cut {
   uint32_t per, unit;
 };
@@ -209,7 +212,7 @@ template <typename T, int DP, int NB>
 struct Tile {
   static constexpr int S = DP / 32, DT = DP / 16, R = 16 * NB;
   // Queries in LDS for 32 rows of a wide head, whose accumulators leave them no registers (in registers, 5 new
-  // tokens of 32 sequences of up to 8192 keys took 71.7 us instead of 60.5, of 8 sequences of up to 4096 17.9 / 16.5).
+  // tokens of 32 sequences of up to 8192 keys took 73.2 us instead of 68.7, of 8 sequences of up to 4096 20.1 / 17.3).
   static constexpr bool kQueriesInLds = NB == 2 && DP == 128;
   // Rows in LDS: reads of 16 and 8 bytes free of conflicts with 16 halves between them, and two workgroups a CU
   // beside the queries with 8.
@@ -240,8 +243,8 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
   uint32_t c_begin, c_end, seq0 = 0;
   int b = p.B;
   // (Workgroups go round the eight XCDs.  Row tiles of a sequence, which stand next to each other in the list and
-  // read the same keys, go to one of them: 8 sequences' 64 new tokens of 32 heads over 4096 keys 83 us instead of
-  // 157.  Items that are cut for themselves are many parts apart: there it cost more than it gave.)
+  // read the same keys, go to one of them: 8 sequences' 64 new tokens of 32 heads over 4096 keys 99 us instead of
+  // 165.  Items that are cut for themselves are many parts apart: there it cost more than it gave.)
   uint32_t me = blockIdx.x;
   auto part_of = [&](uint32_t total) {
     const uint32_t used = p.tiled && cut.unit == 1 ? (total + cut.per - 1) / cut.per : 0;
@@ -790,16 +793,17 @@ bool bad_ptr(const void* p, uintptr_t mask) {
 int held(int32_t D) { return D > 128 ? 1 : 2; }
 // Bytes of keys and values that the block tables can hold from which they are read past the caches: what the
 // Infinity Cache (256 MB, other tensors in it too) does not keep for a next call.  MI355X, past / through the caches:
-// 64 sequences of up to 8192 keys, 8 heads of 128 (1 GB) 172 / 192 us; 14 of up to 4096, 4 of 256 (224 MB) 32.0 / 34.5;
-// 12 of 4096, 16 of 64 (192 MB) 26.3 / 26.8; 10 of them (160 MB) 23.0 / 22.7; 8 (128 MB) 19.4 / 18.6; 16 of 4096, 4 of 96
-// (96 MB) 21.5 / 20.2.  Not where several row tiles of a sequence read the same keys (16 sequences' 16 tokens of 32
-// heads over 8192 keys 120 instead of 114).
+// 64 sequences of up to 8192 keys, 8 heads of 128 (1 GB) 176 / 195 us; 14 of up to 4096, 4 of 256 (224 MB) 32.9 / 35.5;
+// 12 of 4096, 16 of 64 (192 MB) 26.0 / 26.9; 10 of them (160 MB) 23.0 / 22.8; 8 (128 MB) 19.4 / 19.3; 16 of 4096, 4 of 96
+// (96 MB) 18.0 / 17.3.  Not where several row tiles of a sequence read the same keys (16 sequences' 16 tokens of 32
+// heads over 8192 keys 126 instead of 118).  What the lengths hold of a table is known to the device alone: short
+// sequences in wide tables are read past the caches too.
 constexpr int64_t kPastFrom = int64_t{176} << 20;
 constexpr int64_t kMostKeys = int64_t{1} << 30;
 
 // Row blocks of 16 a tile: what a sequence's rows fill on average, two at most.  (Four, whose sums leave a CU one
-// workgroup: 8 sequences of up to 4096 keys with 54 rows 22.0 us instead of 18.4, 2 x 512 tokens of 12 heads over 2048
-// keys 59 / 49, 8 x 64 of 32 heads over 4096 78 / 83.)
+// workgroup, with one product of the weights: 8 sequences of up to 4096 keys with 54 rows 22.0 us instead of 18.4, 2 x
+// 512 tokens of 12 heads over 2048 keys 59 / 49, 8 x 64 of 32 heads over 4096 78 / 83.)
 int blocks_of(int64_t rows, int32_t B, int32_t G) { return B > 0 && rows * G > int64_t{16} * B ? 2 : 1; }
 
 struct Plan {
