@@ -81,3 +81,27 @@ def test_many_small_weights_beside_a_large_one(top, score, news, dtype):
         tol = (2.0 ** -14 + 2.0 ** -17 + 2.0 ** -16 + torch.finfo(dtype).eps / 2) * want + n * 2.0 ** -38
         assert bool(((got[:, i, :, 1] - want).abs() <= tol).all()), float((got[:, i, :, 1] / want - 1).abs().max())
     assert not bool(got[..., 2:].any())
+
+
+@pytest.mark.parametrize("dtype", [H, B])
+@pytest.mark.parametrize("news", [1, 20])
+@pytest.mark.parametrize("q_at", [2.0 ** e for e in (-2, 4, 8, 11, 12, 13, 14)] + [2.0 ** 15])
+@pytest.mark.parametrize("order", ["rising", "falling", "flat", "below zero"])
+def test_scores_of_any_size(order, q_at, news, dtype):
+    """Scores from hundreds to 2 * 10^9, steps of 512 q_at apart, so that the largest ones a token sees have all the
+    weight (its neighbours' is below 2^-180); equal ones share it.  Their values are one of 1 and 2: exact."""
+    n, d, page = 300, 32, 16
+    k, v = torch.zeros(2, 19, 1, page, d)
+    t = torch.arange(n)
+    step = {"rising": t // 3, "falling": (n - 1 - t) // 3, "flat": torch.full((n,), 50), "below zero": t // 3 - 101}[order]
+    k[t // page, 0, t % page, 3] = 512.0 * step
+    v[t // page, 0, t % page, 7] = 1.0 + t % 3 // 2
+    q = torch.zeros(news, 2, d)
+    q[..., 3] = q_at
+    got = run(q.view(news, -1).to(dtype), k.to(dtype), v.to(dtype), [list(range(19))], [n], [0, news])
+    for i in range(news):
+        seen = n - news + i + 1
+        best = (step[:seen] == step[:seen].max()).nonzero()[:, 0]
+        want = float((1.0 + best % 3 // 2).double().mean())
+        far = (got.cpu().view(news, 2, d)[i, :, 7].double() - want).abs().max()
+        assert float(far) <= want * (torch.finfo(dtype).eps / 2 + 2.0 ** -15), (i, float(far))

@@ -3,8 +3,8 @@
 // For token i of the n_b new ones of sequence b, whose keys and values (its own included) are the first
 // `length_b` positions of the cache, and query head h with key head h / G:
 //   out = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q . k_j - m),  j <= length_b - n_b + i
-// m is a running reference value (raised when a score exceeds it by more than a margin, 2^8 in bf16 as in the
-// training attention), sums and products in fp32; a token that sees no key gets zeros.
+// m is a running reference value (raised when a score exceeds it by more than a margin, 8 in bf16 as in the training
+// attention: weights of 2^8), sums and products in fp32; a token that sees no key gets zeros.
 //
 // What bounds it: the cache's bytes -- a key head's row is read once for the G query heads and the few new
 // tokens that share it.  So the query rows of a key head (row = token * G + head in the group, 16 * NB of
@@ -51,14 +51,14 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef short s4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4 lds_s4;
 
-// kRaise: log2 of the weight of a score equal to the reference value; kMargin: by how much a score may exceed it.
-// fp16 weights lie below 2^15, not below 1, so that those without all bits begin at 2^-27 of the reference's (with 0
-// and 8: at 2^-14, and 8000 weights of 2^-25 beside one of 1 were lost).
+// kRaise: how far below the largest score the reference value is set, kMost: by how much a score may exceed it (log2 of
+// a weight).  fp16 weights go up to 2^15, so that those without all bits begin at 2^-27 of the largest (with 0 and 8:
+// at 2^-14, and 8000 weights of 2^-25 beside one of 1 were lost).
 template <typename T>
 struct Ops;
 template <>
 struct Ops<f16> {
-  static constexpr float kRaise = 13.f, kMargin = 2.f;
+  static constexpr float kRaise = 13.f, kMost = 15.f;
   static constexpr uint16_t kNoNumber = 0x7c00;     // (bits of infinities and NaN)
   typedef f16 v8 __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ f4 mfma(u32x4 a, u32x4 b, f4 c) {
@@ -71,7 +71,7 @@ struct Ops<f16> {
 };
 template <>
 struct Ops<bf16> {
-  static constexpr float kRaise = 0.f, kMargin = 8.f;
+  static constexpr float kRaise = 0.f, kMost = 8.f;
   static constexpr uint16_t kNoNumber = 0x7f80;
   typedef bf16 v8 __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ f4 mfma(u32x4 a, u32x4 b, f4 c) {
@@ -523,15 +523,17 @@ __global__ __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) void paged_attention_k
         float mx = sc[u][0][0];
 #pragma unroll
         for (int e = 1; e < 8; ++e) mx = __builtin_elementwise_maximum(mx, sc[u][e >> 2][e & 3]);
-        if (__any(!(mx <= m_ref[u] + Ops<T>::kMargin))) {       // (a NaN raises it to NaN)
-          const float m_new = __builtin_elementwise_maximum(m_ref[u], column_max(mx));
+        if (__any(!(mx - m_ref[u] <= Ops<T>::kMost))) {         // (a NaN raises it to NaN)
+          // (from 2^22 on a score is no longer sure to hold the difference, and the reference value is the score)
+          const float top = column_max(mx), less = __builtin_fabsf(top) < 0x1p22f ? Ops<T>::kRaise : 0.f;
+          const float m_new = __builtin_elementwise_maximum(m_ref[u], top - less);
           const float alpha = m_ref[u] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m_ref[u] - m_new);
           lsum[u] *= alpha;
 #pragma unroll
           for (int t = 0; t < DT; ++t) acc[u][t] = acc[u][t] * alpha;
           m_ref[u] = m_new;
         }
-        const float m_use = m_ref[u] == -INFINITY ? 0.f : m_ref[u] - Ops<T>::kRaise;
+        const float m_use = m_ref[u] == -INFINITY ? 0.f : m_ref[u];
         float pr[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
