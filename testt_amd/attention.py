@@ -293,10 +293,10 @@ def paged_attention(q, k_pages, v_pages, block_table, lengths, cu_seqlens=None, 
     j <= length - n + i that the block table holds: one token each without cu_seqlens; a few with it
     (drafted tokens to be verified) or a prompt's part (whole fp16 prompts with heads of 128 run faster
     through the varlen attention).  scale: 1 / sqrt(D) unless given.  A token that sees no key gets
-    zeros, and so does a row of no sequence or of one whose bounds leave the rows (cu_seqlens ascends:
-    where it does not, nothing else is promised than that no memory but out's is written); keys in
-    pages outside [0, pages) are not seen.  A NaN or infinity in a key or value reaches the tokens that
-    see it alone; a value's stays in its column.
+    zeros (also where all of its scores are -inf), and so does a row of no sequence or of one whose
+    bounds leave the rows (cu_seqlens ascends: where it does not, nothing else is promised than that no
+    memory but out's is written); keys in pages outside [0, pages) are not seen.  A NaN or infinity in a
+    key or value reaches the tokens that see it alone; a value's stays in its column.
 
     The lengths are read on the device: a captured graph's replays may change them, the block table
     and the pages, up to the block table's width.  Scores, sums and products are fp32; a
